@@ -33,7 +33,8 @@ __all__ = [
     "FgpuError", "lib", "lib_path", "Index", "gen_gmm", "l2_topk", "kmeans_fit", "kmeans_update",
     "fixed_shift", "pq_train", "pq_encode", "build_ivfpq", "write_ivf_data", "read_ivf_data",
     "write_fvecs", "read_fvecs", "read_ivecs", "probe_counts", "rerank", "knn_exact", "graph_search",
-    "stream_read", "row_gather", "FAULT_ID", "prune_probes", "graph_add_reverse",
+    "stream_read", "row_gather", "FAULT_ID", "prune_probes", "graph_add_reverse", "linear", "linear_backward",
+    "layer_norm", "layer_norm_backward", "contrastive_loss", "contrastive_loss_backward",
 ]
 
 lib_path = os.path.join(os.path.dirname(os.path.abspath(__file__)), "_lib", "libfusiongpu.so")
@@ -121,6 +122,18 @@ _SIGS = {
     "fgpu_write_fvecs": (_i32, [_c.c_char_p, _vp, _i64, _i32]),
     "fgpu_read_fvecs": (_i32, [_c.c_char_p, _i32, _c.POINTER(_i64), _vp]),
     "fgpu_read_ivecs": (_i32, [_c.c_char_p, _c.POINTER(_i32), _c.POINTER(_i64), _vp]),
+    "fgpu_linear_workspace_bytes": (_sz, [_i64, _i32, _i32, _i32]),
+    "fgpu_linear": (_i32, [_vp, _vp, _vp, _vp, _i64, _i32, _i32, _i32, _i32, _vp, _vp, _vp, _sz, _vp]),
+    "fgpu_linear_backward_workspace_bytes": (_sz, [_i64, _i32, _i32, _i32]),
+    "fgpu_linear_backward": (_i32, [_vp, _vp, _vp, _vp, _i64, _i32, _i32, _i32, _i32, _vp, _vp, _vp, _vp, _sz, _vp]),
+    "fgpu_layer_norm": (_i32, [_vp, _vp, _vp, _i64, _i32, _i32, _f32, _vp, _vp, _vp, _vp]),
+    "fgpu_layer_norm_backward_workspace_bytes": (_sz, [_i64, _i32, _i32]),
+    "fgpu_layer_norm_backward": (_i32, [_vp, _vp, _vp, _vp, _vp, _i64, _i32, _i32, _vp, _vp, _vp, _vp, _sz, _vp]),
+    "fgpu_contrastive_loss_workspace_bytes": (_sz, [_i32, _i32, _i32, _i32]),
+    "fgpu_contrastive_loss": (_i32, [_vp, _vp, _vp, _vp, _vp, _i32, _i32, _i32, _i32, _f32, _vp, _vp, _vp, _sz, _vp]),
+    "fgpu_contrastive_loss_backward_workspace_bytes": (_sz, [_i32, _i32, _i32, _i32]),
+    "fgpu_contrastive_loss_backward": (_i32, [_vp, _vp, _vp, _vp, _vp, _vp, _vp, _i32, _i32, _i32, _i32, _f32, _vp, _vp,
+                                              _vp, _vp, _sz, _vp]),
     "fgpu_gen_gmm": (None, [_i64, _i32, _i32, _f64, _f64, _f64, _f64, _u64, _i32, _vp, _i32]),
 }
 
@@ -953,3 +966,191 @@ def build_ivfpq(x, nlist: int, pq_m: int, kmeans_iters: int = 20, init_mode: int
                                             seed, pq_iters, sample_size, _np_ptr(offs), _np_ptr(ids), _np_ptr(codes),
                                             _np_ptr(cent), _np_ptr(cb), _stream()))
     return offs, ids, codes, cent, cb
+
+
+# --------------------------------------------------------------------------- query head
+# The layers between an encoder and the index, and the loss they are trained by.  The first array decides the type:
+# bfloat16 stays, any other floating type is read as float32 (as everywhere in this package); the arrays beside it must
+# have that type already, so that no weight is converted anew at every call.
+ACTIVATIONS = {"none": 0, "relu": 1, "gelu": 2, "silu": 3}
+
+
+def _act_code(act):
+    if act not in ACTIVATIONS:
+        raise ValueError(f"act: {act!r} is none of {sorted(ACTIVATIONS)}")
+    return ACTIVATIONS[act]
+
+
+def _head_first(a, name):
+    """The array that decides a call's type, as a contiguous 16-byte-aligned device matrix."""
+    torch = _torch()
+    if not (torch.is_tensor(a) and a.dtype == torch.bfloat16):
+        a = _arg(a, torch.float32, name, (None, None))
+    return _head(a, a.dtype, name, (None, None))
+
+
+def _head(a, dtype, name, shape):
+    """`a` as a contiguous, 16-byte-aligned device tensor; its dtype must be `dtype`."""
+    torch = _torch()
+    if isinstance(a, np.ndarray):
+        a = torch.from_numpy(np.ascontiguousarray(a))
+    elif not torch.is_tensor(a):
+        raise TypeError(f"{name}: expected a numpy array or a torch tensor, got {type(a).__name__}")
+    if a.dtype != dtype:
+        raise TypeError(f"{name}: dtype {str(a.dtype).replace('torch.', '')}, expected "
+                        f"{str(dtype).replace('torch.', '')} as the call's other arrays have")
+    if a.dim() != len(shape) or any(w is not None and g != w for g, w in zip(a.shape, shape)):
+        want = ["any" if w is None else w for w in shape]
+        raise ValueError(f"{name}: shape {tuple(a.shape)}, expected {want}")
+    if not a.is_cuda:
+        a = a.to("cuda")
+    if not a.is_contiguous():
+        a = a.contiguous()
+    return a.clone() if a.data_ptr() % 16 else a
+
+
+def _head_opt(a, dtype, name, shape):
+    return None if a is None else _head(a, dtype, name, shape)
+
+
+def _ptr(t):
+    return None if t is None else t.data_ptr()
+
+
+def _head_out(out, like, shape, name="out"):
+    if out is None:
+        return _torch().empty(shape, dtype=like.dtype, device=like.device)
+    return _out(out, like.dtype, shape, name)
+
+
+def _dtype_code(t):
+    return int(t.dtype != _torch().float32)
+
+
+def linear(x, weight, bias=None, residual=None, act: str = "none", save_pre: bool = False, out=None, stream=None):
+    """act(x weight^T + bias) + residual (fgpu_linear): x [rows][in], weight [out][in], bias [out], residual
+    [rows][out], act one of none, relu, gelu, silu.  With save_pre also the value before act, which linear_backward
+    needs: (y, pre)."""
+    code = _act_code(act)
+    with _on(stream):
+        x = _head_first(x, "x")
+        (rows, k), t = x.shape, x.dtype
+        w = _head(weight, t, "weight", (None, k))
+        n = w.shape[0]
+        b = _head_opt(bias, t, "bias", (n,))
+        r = _head_opt(residual, t, "residual", (rows, n))
+        y = _head_out(out, x, (rows, n))
+        pre = _head_out(None, x, (rows, n)) if save_pre else None
+        dt = _dtype_code(x)
+        ws = _workspace(lib.fgpu_linear_workspace_bytes(rows, k, n, dt))
+        _check(lib.fgpu_linear(x.data_ptr(), w.data_ptr(), _ptr(b), _ptr(r), rows, k, n, dt, code, y.data_ptr(), _ptr(pre),
+                               ws.data_ptr(), ws.numel(), _stream()))
+    return (y, pre) if save_pre else y
+
+
+def linear_backward(dy, x, weight, pre=None, act: str = "none", want=("x", "weight", "bias"), stream=None):
+    """Gradients of linear (fgpu_linear_backward): (dx, dweight, dbias), None for those not in `want`.  pre: the value
+    before act that linear(save_pre=True) returned (not needed for act "none").  The residual's gradient is dy."""
+    code = _act_code(act)
+    if not set(want) <= {"x", "weight", "bias"}:
+        raise ValueError(f"want: {tuple(want)!r} names something other than x, weight and bias")
+    if code and pre is None:
+        raise ValueError(f"pre: act {act!r} needs the value before it")
+    with _on(stream):
+        dy = _head_first(dy, "dy")
+        (rows, n), t = dy.shape, dy.dtype
+        x = _head(x, t, "x", (rows, None))
+        k = x.shape[1]
+        w = _head(weight, t, "weight", (n, k))
+        z = _head_opt(pre, t, "pre", (rows, n)) if code else None
+        dx = _head_out(None, dy, (rows, k)) if "x" in want else None
+        dw = _head_out(None, dy, (n, k)) if "weight" in want else None
+        db = _head_out(None, dy, (n,)) if "bias" in want else None
+        dt = _dtype_code(dy)
+        ws = _workspace(lib.fgpu_linear_backward_workspace_bytes(rows, k, n, dt))
+        _check(lib.fgpu_linear_backward(dy.data_ptr(), x.data_ptr(), w.data_ptr(), _ptr(z), rows, k, n, dt, code, _ptr(dx),
+                                        _ptr(dw), _ptr(db), ws.data_ptr(), ws.numel(), _stream()))
+    return dx, dw, db
+
+
+def layer_norm(x, gamma=None, beta=None, eps: float = 1e-5, out=None, stream=None):
+    """Layer norm over the rows of x [rows][dim] (fgpu_layer_norm): (y, mean, rstd), the last two float32 [rows] for
+    layer_norm_backward."""
+    torch = _torch()
+    with _on(stream):
+        x = _head_first(x, "x")
+        (rows, dim), t = x.shape, x.dtype
+        g, b = _head_opt(gamma, t, "gamma", (dim,)), _head_opt(beta, t, "beta", (dim,))
+        y = _head_out(out, x, (rows, dim))
+        mean, rstd = torch.empty((2, rows), dtype=torch.float32, device=x.device).unbind()
+        _check(lib.fgpu_layer_norm(x.data_ptr(), _ptr(g), _ptr(b), rows, dim, _dtype_code(x), eps, y.data_ptr(),
+                                   mean.data_ptr(), rstd.data_ptr(), _stream()))
+    return y, mean, rstd
+
+
+def layer_norm_backward(dy, x, gamma, mean, rstd, want=("x", "gamma", "beta"), stream=None):
+    """Gradients of layer_norm (fgpu_layer_norm_backward): (dx, dgamma, dbeta), None for those not in `want`."""
+    torch = _torch()
+    if not set(want) <= {"x", "gamma", "beta"}:
+        raise ValueError(f"want: {tuple(want)!r} names something other than x, gamma and beta")
+    with _on(stream):
+        dy = _head_first(dy, "dy")
+        (rows, dim), t = dy.shape, dy.dtype
+        x = _head(x, t, "x", (rows, dim))
+        g = _head_opt(gamma, t, "gamma", (dim,))
+        mean, rstd = _dev(mean, torch.float32, "mean", (rows,)), _dev(rstd, torch.float32, "rstd", (rows,))
+        dx = _head_out(None, dy, (rows, dim)) if "x" in want else None
+        dg = _head_out(None, dy, (dim,)) if "gamma" in want else None
+        db = _head_out(None, dy, (dim,)) if "beta" in want else None
+        dt = _dtype_code(dy)
+        ws = _workspace(lib.fgpu_layer_norm_backward_workspace_bytes(rows, dim, dt))
+        _check(lib.fgpu_layer_norm_backward(dy.data_ptr(), x.data_ptr(), _ptr(g), mean.data_ptr(), rstd.data_ptr(), rows,
+                                            dim, dt, _ptr(dx), _ptr(dg), _ptr(db), ws.data_ptr(), ws.numel(), _stream()))
+    return dx, dg, db
+
+
+def _loss_args(queries, candidates, targets, bias, ids):
+    torch = _torch()
+    q = _head_first(queries, "queries")
+    nq, dim = q.shape
+    c = _head(candidates, q.dtype, "candidates", (None, dim))
+    nc = c.shape[0]
+    t = _dev(targets, torch.int32, "targets", (nq,))
+    b = None if bias is None else _dev(bias, torch.float32, "bias", (nc,))
+    i = None if ids is None else _dev(ids, torch.int32, "ids", (nc,))
+    return q, c, t, b, i, nq, nc, dim, _dtype_code(q)
+
+
+def contrastive_loss(queries, candidates, targets, scale: float = 1.0, bias=None, ids=None, stream=None):
+    """Softmax contrastive loss (fgpu_contrastive_loss): scores scale q.c + bias, loss_i = log sum_j exp s_ij - s_{i,
+    targets_i}.  queries [nq][dim], candidates [nc][dim], targets int32 [nq] (outside [0, nc): the row is ignored), bias
+    float32 [nc] (-inf masks a candidate; -scale |c|^2 / 2 makes the scores the index's L2 metric), ids int32 [nc]
+    (copies of the target's document are left out).  Returns (loss, lse), float32 [nq]."""
+    torch = _torch()
+    with _on(stream):
+        q, c, t, b, i, nq, nc, dim, dt = _loss_args(queries, candidates, targets, bias, ids)
+        loss, lse = torch.empty((2, nq), dtype=torch.float32, device=q.device).unbind()
+        ws = _workspace(lib.fgpu_contrastive_loss_workspace_bytes(nq, nc, dim, dt))
+        _check(lib.fgpu_contrastive_loss(q.data_ptr(), c.data_ptr(), t.data_ptr(), _ptr(b), _ptr(i), nq, nc, dim, dt, scale,
+                                         loss.data_ptr(), lse.data_ptr(), ws.data_ptr(), ws.numel(), _stream()))
+    return loss, lse
+
+
+def contrastive_loss_backward(dloss, queries, candidates, targets, lse, scale: float = 1.0, bias=None, ids=None,
+                              candidate_grads: bool = True, workspace=None, stream=None):
+    """Gradients of contrastive_loss (fgpu_contrastive_loss_backward) for dloss float32 [nq] and the forward call's
+    lse: (dqueries, dcandidates, dbias), the last two None without candidate_grads (fixed candidates).  dbias is float32
+    [nc]."""
+    torch = _torch()
+    with _on(stream):
+        q, c, t, b, i, nq, nc, dim, dt = _loss_args(queries, candidates, targets, bias, ids)
+        g, lse = _dev(dloss, torch.float32, "dloss", (nq,)), _dev(lse, torch.float32, "lse", (nq,))
+        dq = _head_out(None, q, (nq, dim))
+        dc = _head_out(None, q, (nc, dim)) if candidate_grads else None
+        db = torch.empty(nc, dtype=torch.float32, device=q.device) if candidate_grads else None
+        ws = workspace if workspace is not None else _workspace(
+            lib.fgpu_contrastive_loss_backward_workspace_bytes(nq, nc, dim, dt))
+        _check(lib.fgpu_contrastive_loss_backward(g.data_ptr(), q.data_ptr(), c.data_ptr(), t.data_ptr(), lse.data_ptr(),
+                                                  _ptr(b), _ptr(i), nq, nc, dim, dt, scale, dq.data_ptr(), _ptr(dc), _ptr(db),
+                                                  ws.data_ptr(), _ws_check(ws), _stream()))
+    return dq, dc, db

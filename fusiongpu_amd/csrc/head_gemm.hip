@@ -1,0 +1,202 @@
+// head_gemm.hip -- products with a fused epilogue, the packing of their operands and the last step of column sums.
+#include <algorithm>
+
+#include "head.hpp"
+
+namespace fgpu {
+namespace {
+
+// out = act(alpha D + bias) + residual for four consecutive columns n .. n + 3 of row m (cnt of them inside).
+template <class T>
+__device__ __forceinline__ void finish4(const Finish& f, f32x4 v, int64_t at, int n, int cnt) {
+  v *= f.alpha;
+  if (f.bias) v += load4_n((const T*)f.bias + n, cnt);
+  if (f.pre) store4_n((T*)f.pre + at, v, cnt);
+  if (f.act != FGPU_ACT_NONE) {
+#pragma unroll
+    for (int r = 0; r < 4; ++r) v[r] = act_value(v[r], f.act);
+  }
+  if (f.residual) v += load4_n((const T*)f.residual + at, cnt);
+  store4_n((T*)f.out + at, v, cnt);
+}
+
+template <class T>
+struct ProductEpi {
+  Finish f;
+  float* part;  // [split][m][n4] in place of the result, or NULL
+  int m, n;
+
+  template <class G>
+  __device__ __forceinline__ void finish(f32x4 (&acc)[G::FN][G::FM], int m0, int n0, int, int, int sp, int wm, int wn,
+                                         int lane, char*) const {
+    const int n4 = (n + 3) & ~3;
+#pragma unroll
+    for (int j = 0; j < G::FM; ++j) {
+      const int row = m0 + (wm * G::FM + j) * 16 + (lane & 15);
+      if (row >= m) continue;
+#pragma unroll
+      for (int i = 0; i < G::FN; ++i) {
+        const int col = n0 + (wn * G::FN + i) * 16 + (lane >> 4) * 4;
+        if (col >= n) continue;
+        if (part)
+          *reinterpret_cast<f32x4*>(part + ((int64_t)sp * m + row) * n4 + col) = acc[i][j];
+        else
+          finish4<T>(f, acc[i][j], (int64_t)row * n + col, col, n - col);
+      }
+    }
+  }
+};
+
+// Adds the parts of a split product in order and finishes it: one thread four columns.
+template <class T>
+__global__ __launch_bounds__(256) void split_finish_kernel(const float* part, int m, int n, int splits, Finish f) {
+  const int n4 = (n + 3) >> 2;
+  const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x, total = (int64_t)m * n4;
+  if (i >= total) return;
+  const int64_t row = i / n4;
+  const int col = (int)(i - row * n4) * 4;
+  f32x4 v = {0, 0, 0, 0};
+  if (f.add) v = *reinterpret_cast<const f32x4*>(f.add + i * 4);
+  for (int s = 0; s < splits; ++s) v += *reinterpret_cast<const f32x4*>(part + ((int64_t)s * total + i) * 4);
+  if (f.sum)
+    *reinterpret_cast<f32x4*>(f.sum + i * 4) = v;
+  else
+    finish4<T>(f, v, row * n + col, col, n - col);
+}
+
+struct Plan {
+  int tile, tiles_m, tiles_n, splits, k_per_split;
+};
+Plan plan_of(const Product& p) {
+  Plan q;
+  auto tiles = [&](int t) { return (int64_t)ceil_div(p.m, t) * ceil_div(p.n, t); };
+  q.tile = tiles(256) >= 192 ? 256 : tiles(128) >= 256 ? 128 : 64;
+  q.tiles_m = ceil_div(p.m, q.tile);
+  q.tiles_n = ceil_div(p.n, q.tile);
+  const int64_t t = (int64_t)q.tiles_m * q.tiles_n;
+  const int steps = ceil_div(p.k, kGemmBK);
+  int64_t want = q.tile == 256 ? 1 : std::max<int64_t>(1, 512 / t);
+  want = std::min<int64_t>(want, std::max(1, steps / 4));
+  q.k_per_split = ceil_div(steps, want) * kGemmBK;
+  q.splits = ceil_div(p.k, q.k_per_split);
+  return q;
+}
+
+template <class T, bool AKC, bool BKC, int PAIRS, class E>
+fgpu_status run(const GemmArgs& g, const E& e, hipStream_t s) {
+  gemm_kernel<T, AKC, BKC, PAIRS, E><<<g.tiles_m * g.tiles_n * g.splits, T::threads, 0, s>>>(g, e);
+  FGPU_HIP(hipGetLastError());
+  return FGPU_OK;
+}
+template <bool AKC, bool BKC, int PAIRS, class E>
+fgpu_status run_tile(int tile, const GemmArgs& g, const E& e, hipStream_t s) {
+  if (tile == 256) return run<Tile256, AKC, BKC, PAIRS>(g, e, s);
+  if (tile == 128) return run<Tile128, AKC, BKC, PAIRS>(g, e, s);
+  return run<Tile64, AKC, BKC, PAIRS>(g, e, s);
+}
+template <int PAIRS, class E>
+fgpu_status run_form(bool a_kc, bool b_kc, int tile, const GemmArgs& g, const E& e, hipStream_t s) {
+  if (a_kc && b_kc) return run_tile<true, true, PAIRS>(tile, g, e, s);
+  if (a_kc) return run_tile<true, false, PAIRS>(tile, g, e, s);
+  return run_tile<false, false, PAIRS>(tile, g, e, s);
+}
+
+template <class T>
+__device__ __forceinline__ bool row_is_zero(int64_t r, const float* zb, const int32_t* zt, int nc) {
+  return (zb && zb[r] <= FGPU_MASK_BIAS) || (zt && (uint32_t)zt[r] >= (uint32_t)nc);
+}
+
+// One thread four columns of a row.
+template <class T>
+__global__ __launch_bounds__(256) void pack_kernel(const T* src, int64_t rows, int64_t cols, int64_t ldp, int64_t plane,
+                                                   uint16_t* dst, const float* zb, const int32_t* zt, int nc) {
+  const int64_t per = ldp / 4, total = rows * per;
+  for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < total; i += (int64_t)gridDim.x * 256) {
+    const int64_t r = i / per, c = (i - r * per) * 4;
+    f32x4 v = {0, 0, 0, 0};
+    if (c < cols && !row_is_zero<T>(r, zb, zt, nc)) v = load4_n(src + r * cols + c, (int)min(cols - c, (int64_t)4));
+    if constexpr (sizeof(T) == 2) {
+      *reinterpret_cast<bf16x4*>(dst + r * ldp + c) = __builtin_convertvector(v, bf16x4);
+    } else {
+      bf16x4 h, m, l;
+#pragma unroll
+      for (int k = 0; k < 4; ++k) {
+        bf16 a, b, d;
+        split_f32(v[k], a, b, d);
+        h[k] = a, m[k] = b, l[k] = d;
+      }
+      *reinterpret_cast<bf16x4*>(dst + r * ldp + c) = h;
+      *reinterpret_cast<bf16x4*>(dst + plane + r * ldp + c) = m;
+      *reinterpret_cast<bf16x4*>(dst + 2 * plane + r * ldp + c) = l;
+    }
+  }
+}
+
+// 64 columns x 16 groups of parts a workgroup.
+template <class T>
+__global__ __launch_bounds__(1024) void column_finish_kernel(const float* part, int parts, int64_t stride, int64_t cols, T* out) {
+  __shared__ float sum[16][64];
+  const int64_t c = (int64_t)blockIdx.x * 64 + (threadIdx.x & 63);
+  const int g = threadIdx.x >> 6;
+  float v = 0;
+  if (c < cols)
+    for (int p = g; p < parts; p += 16) v += part[(int64_t)p * stride + c];
+  sum[g][threadIdx.x & 63] = v;
+  __syncthreads();
+  if (g == 0 && c < cols) {
+    for (int k = 1; k < 16; ++k) v += sum[k][threadIdx.x];
+    out[c] = (T)v;
+  }
+}
+
+}  // namespace
+
+size_t product_workspace_bytes(const Product& p) {
+  const Plan q = plan_of(p);
+  return q.splits > 1 || p.chunked ? carve_bytes<float>((size_t)q.splits * p.m * ((p.n + 3) & ~3)) : 0;
+}
+
+fgpu_status launch_product(const Product& p, const GemmOperand& a, bool a_kc, const GemmOperand& b, bool b_kc,
+                           const Finish& f, void* ws, hipStream_t s) {
+  const Plan q = plan_of(p);
+  const GemmArgs g{a, b, p.m, p.n, p.k, q.tiles_m, q.tiles_n, q.splits, q.k_per_split};
+  float* part = q.splits > 1 || p.chunked ? static_cast<float*>(ws) : nullptr;
+  if (p.f32)
+    FGPU_TRY((run_form<6>(a_kc, b_kc, q.tile, g, ProductEpi<float>{f, part, p.m, p.n}, s)));
+  else
+    FGPU_TRY((run_form<1>(a_kc, b_kc, q.tile, g, ProductEpi<bf16>{f, part, p.m, p.n}, s)));
+  if (part) {
+    const int64_t total = (int64_t)p.m * ((p.n + 3) / 4);
+    if (p.f32)
+      split_finish_kernel<float><<<ceil_div(total, 256), 256, 0, s>>>(part, p.m, p.n, q.splits, f);
+    else
+      split_finish_kernel<bf16><<<ceil_div(total, 256), 256, 0, s>>>(part, p.m, p.n, q.splits, f);
+    FGPU_HIP(hipGetLastError());
+  }
+  return FGPU_OK;
+}
+
+fgpu_status launch_pack(const void* src, int64_t rows, int64_t cols, bool f32, const GemmOperand& dst,
+                        const float* zero_bias, const int32_t* zero_target, int nc, hipStream_t s) {
+  const int64_t total = rows * (dst.ld / 4);
+  const int grid = (int)std::min<int64_t>(ceil_div(total, 256), 8192);
+  uint16_t* d = const_cast<uint16_t*>(dst.p);
+  if (f32)
+    pack_kernel<float><<<grid, 256, 0, s>>>((const float*)src, rows, cols, dst.ld, dst.plane, d, zero_bias, zero_target, nc);
+  else
+    pack_kernel<bf16><<<grid, 256, 0, s>>>((const bf16*)src, rows, cols, dst.ld, dst.plane, d, zero_bias, zero_target, nc);
+  FGPU_HIP(hipGetLastError());
+  return FGPU_OK;
+}
+
+fgpu_status launch_column_finish(const float* part, int parts, int64_t stride, int64_t cols, bool f32_out, void* out,
+                                 hipStream_t s) {
+  if (f32_out)
+    column_finish_kernel<float><<<ceil_div(cols, 64), 1024, 0, s>>>(part, parts, stride, cols, (float*)out);
+  else
+    column_finish_kernel<bf16><<<ceil_div(cols, 64), 1024, 0, s>>>(part, parts, stride, cols, (bf16*)out);
+  FGPU_HIP(hipGetLastError());
+  return FGPU_OK;
+}
+
+}  // namespace fgpu

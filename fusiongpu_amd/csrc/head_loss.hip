@@ -1,0 +1,408 @@
+// head_loss.hip -- the softmax contrastive loss of queries against candidate vectors, and its gradient.
+//
+// s_ij = scale q_i.c_j + bias_j over the candidates j that row i keeps; lse_i = log sum_j exp s_ij and
+// loss_i = lse_i - s_i,t(i).  Neither pass holds the score matrix: the forward pass keeps a running maximum and sum a
+// (row, column tile) in the product's epilogue and joins them; the backward pass forms the product again, turns it
+// into G_ij = g_i (exp(s_ij - lse_i) - [j = t(i)]) in the epilogue and takes dq = scale G c and dc = scale G^T q from it
+// in column chunks that bound the workspace.  Scores live in units of log 2 (s log2 e), so an exponential is one
+// instruction.
+#include <algorithm>
+
+#include "head.hpp"
+
+namespace fgpu {
+namespace {
+
+struct LossArgs {
+  const float* bias;       // [nc] or NULL
+  const int32_t* ids;      // [nc] or NULL
+  const int32_t* target;   // [nq]
+  float scale2;            // scale * log2(e)
+  int nq, nc;
+};
+
+__device__ __forceinline__ bool masked_bias(float b) { return b <= FGPU_MASK_BIAS; }
+
+// The scores of a lane's four columns n .. n + 3 at row m: s2 = scale2 acc + bias2, -inf where the column is masked, beyond the
+// candidates, or another copy of the row's document.
+struct ColumnSide {
+  f32x4 bias2;
+  int id[4];
+  __device__ __forceinline__ void load(const LossArgs& a, int n) {
+#pragma unroll
+    for (int r = 0; r < 4; ++r) {
+      const bool in = n + r < a.nc;
+      float b = in ? (a.bias ? a.bias[n + r] : 0.0f) : -INFINITY;
+      bias2[r] = masked_bias(b) ? -INFINITY : b * kLog2e;
+      id[r] = in && a.ids ? a.ids[n + r] : 0;
+    }
+  }
+};
+struct RowSide {
+  int t;       // target column, -1: none
+  int id;      // its document
+  bool dedup;  // copies of it are left out
+  __device__ __forceinline__ void load(const LossArgs& a, int m) {
+    t = m < a.nq ? a.target[m] : -1;
+    if ((uint32_t)t >= (uint32_t)a.nc) t = -1;
+    dedup = a.ids && t >= 0;
+    id = dedup ? a.ids[t] : 0;
+  }
+};
+__device__ __forceinline__ float score2(const LossArgs& a, float acc, const ColumnSide& c, const RowSide& w, int n, int r) {
+  float s = c.bias2[r] == -INFINITY ? -INFINITY : fmaf(a.scale2, acc, c.bias2[r]);
+  if (w.dedup && c.id[r] == w.id && n + r != w.t) s = -INFINITY;
+  return s;
+}
+
+// Forward: per row and column tile (maximum, sum of exp2(s - maximum)), and the target's score.
+struct StatsEpi {
+  LossArgs a;
+  f32x2* part;     // [tiles_n][nq]
+  float* target2;  // [nq]
+
+  template <class G>
+  __device__ __forceinline__ void finish(f32x4 (&acc)[G::FN][G::FM], int m0, int n0, int, int tn, int, int wm, int wn,
+                                         int lane, char* lds) const {
+    f32x2* sh = reinterpret_cast<f32x2*>(lds);  // [WN][BM]
+    ColumnSide cs[G::FN];
+#pragma unroll
+    for (int i = 0; i < G::FN; ++i) cs[i].load(a, n0 + (wn * G::FN + i) * 16 + (lane >> 4) * 4);
+#pragma unroll
+    for (int j = 0; j < G::FM; ++j) {
+      const int ml = (wm * G::FM + j) * 16 + (lane & 15), m = m0 + ml;
+      RowSide w;
+      w.load(a, m);
+      float top = -INFINITY;
+#pragma unroll
+      for (int i = 0; i < G::FN; ++i) {
+        const int n = n0 + (wn * G::FN + i) * 16 + (lane >> 4) * 4;
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {
+          const float s = score2(a, acc[i][j][r], cs[i], w, n, r);
+          acc[i][j][r] = s;
+          top = fmaxf(top, s);  // a NaN score makes the sum NaN
+          if (n + r == w.t) target2[m] = s;
+        }
+      }
+      top = fmaxf(top, shfl_xor_f(top, 16));
+      top = fmaxf(top, shfl_xor_f(top, 32));
+      const float base = top == -INFINITY ? 0.0f : top;
+      float sum = 0;
+#pragma unroll
+      for (int i = 0; i < G::FN; ++i)
+#pragma unroll
+        for (int r = 0; r < 4; ++r) sum += fast_exp2(acc[i][j][r] - base);
+      sum += shfl_xor_f(sum, 16);
+      sum += shfl_xor_f(sum, 32);
+      if (lane < 16) sh[wn * G::BM + ml] = f32x2{top, sum};
+    }
+    __syncthreads();
+    for (int ml = threadIdx.x; ml < G::BM; ml += G::threads) {
+      if (m0 + ml >= a.nq) continue;
+      float top = -INFINITY, sum = 0;
+#pragma unroll
+      for (int w = 0; w < G::WN; ++w) top = fmaxf(top, sh[w * G::BM + ml][0]);
+      const float base = top == -INFINITY ? 0.0f : top;
+#pragma unroll
+      for (int w = 0; w < G::WN; ++w) sum += sh[w * G::BM + ml][1] * fast_exp2(sh[w * G::BM + ml][0] - base);
+      part[(int64_t)tn * a.nq + m0 + ml] = f32x2{top, sum};
+    }
+  }
+};
+
+// Joins a row's parts: 64 rows a workgroup, sixteen groups of parts.
+__global__ __launch_bounds__(1024) void loss_join_kernel(LossArgs a, const f32x2* part, int parts, const float* target2,
+                                                         float* loss, float* lse) {
+  __shared__ f32x2 sh[16][64];
+  const int lane = threadIdx.x & 63, g = threadIdx.x >> 6, m = blockIdx.x * 64 + lane;
+  float top = -INFINITY, sum = 0;
+  if (m < a.nq)
+    for (int p = g; p < parts; p += 16) {
+      const f32x2 v = part[(int64_t)p * a.nq + m];
+      const float t = fmaxf(top, v[0]);
+      if (t != -INFINITY) sum = sum * fast_exp2(top - t) + v[1] * fast_exp2(v[0] - t);
+      else sum += v[1];  // zero, or NaN
+      top = t;
+    }
+  sh[g][lane] = f32x2{top, sum};
+  __syncthreads();
+  if (g || m >= a.nq) return;
+  float all = top;
+  for (int k = 1; k < 16; ++k) all = fmaxf(all, sh[k][lane][0]);
+  const float base = all == -INFINITY ? 0.0f : all;
+  sum = 0;
+  for (int k = 0; k < 16; ++k) sum += sh[k][lane][1] * fast_exp2(sh[k][lane][0] - base);
+  const float l2 = base + __builtin_amdgcn_logf(sum);  // log2; of 0: -inf
+  lse[m] = l2 * kLn2;
+  const int t = a.target[m];
+  const bool live = (uint32_t)t < (uint32_t)a.nc && l2 != -INFINITY;
+  loss[m] = live ? (l2 - target2[m]) * kLn2 : 0.0f;
+}
+
+// What the backward pass needs of each row: lse in units of log 2 and the row's weight; a row without a gradient has
+// weight 0 and an infinite lse, so its G is zero.
+__global__ __launch_bounds__(256) void loss_rows_kernel(LossArgs a, const float* dloss, const float* lse, f32x2* rows,
+                                                        int32_t* live_target) {
+  const int m = blockIdx.x * 256 + threadIdx.x;
+  if (m >= a.nq) return;
+  const int t = a.target[m];
+  const bool live = (uint32_t)t < (uint32_t)a.nc && lse[m] != -INFINITY && !(a.bias && masked_bias(a.bias[t]));
+  rows[m] = live ? f32x2{lse[m] * kLog2e, dloss[m]} : f32x2{INFINITY, 0.0f};
+  live_target[m] = live ? t : -1;
+}
+
+// Backward: G of the columns c0 .. c0 + n - 1, as an operand [nq][ldg], and its column sums a tile row.
+template <bool F32>
+struct GradEpi {
+  LossArgs a;         // target: live_target
+  const f32x2* rows;
+  uint16_t* g;
+  int64_t ldg, plane;
+  float* dbias_part;  // [tiles_m][n] or NULL
+  int c0, n;          // the chunk's columns
+
+  template <class G>
+  __device__ __forceinline__ void finish(f32x4 (&acc)[G::FN][G::FM], int m0, int n0, int tm, int, int, int wm, int wn,
+                                         int lane, char* lds) const {
+    ColumnSide cs[G::FN];
+    f32x4 col[G::FN];
+#pragma unroll
+    for (int i = 0; i < G::FN; ++i) {
+      cs[i].load(a, c0 + n0 + (wn * G::FN + i) * 16 + (lane >> 4) * 4);
+      col[i] = f32x4{0, 0, 0, 0};
+    }
+#pragma unroll
+    for (int j = 0; j < G::FM; ++j) {
+      const int m = m0 + (wm * G::FM + j) * 16 + (lane & 15);
+      RowSide w;
+      w.load(a, m);
+      const f32x2 row = m < a.nq ? rows[m] : f32x2{INFINITY, 0.0f};
+#pragma unroll
+      for (int i = 0; i < G::FN; ++i) {
+        const int nl = n0 + (wn * G::FN + i) * 16 + (lane >> 4) * 4;
+        f32x4 v;
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {
+          float p = fast_exp2(score2(a, acc[i][j][r], cs[i], w, c0 + nl, r) - row[0]);
+          if (c0 + nl + r == w.t) p -= 1.0f;
+          v[r] = p * row[1];
+        }
+        col[i] += v;
+        if (m < a.nq && nl < ldg) {  // the padding's columns are zero
+          uint16_t* d = g + (int64_t)m * ldg + nl;
+          if constexpr (!F32) {
+            *reinterpret_cast<bf16x4*>(d) = __builtin_convertvector(v, bf16x4);
+          } else {
+            bf16x4 h, mi, l;
+#pragma unroll
+            for (int r = 0; r < 4; ++r) {
+              bf16 x, y, z;
+              split_f32(v[r], x, y, z);
+              h[r] = x, mi[r] = y, l[r] = z;
+            }
+            *reinterpret_cast<bf16x4*>(d) = h;
+            *reinterpret_cast<bf16x4*>(d + plane) = mi;
+            *reinterpret_cast<bf16x4*>(d + 2 * plane) = l;
+          }
+        }
+      }
+    }
+    if (!dbias_part) return;
+    f32x4* sh = reinterpret_cast<f32x4*>(lds);  // [WM][BN / 4]
+#pragma unroll
+    for (int i = 0; i < G::FN; ++i) {
+#pragma unroll
+      for (int r = 0; r < 4; ++r) {
+        float v = col[i][r];
+        v += shfl_xor_f(v, 1);
+        v += shfl_xor_f(v, 2);
+        v += shfl_xor_f(v, 4);
+        v += shfl_xor_f(v, 8);
+        col[i][r] = v;
+      }
+      if ((lane & 15) == 0) sh[wm * (G::BN / 4) + (wn * G::FN + i) * 4 + (lane >> 4)] = col[i];
+    }
+    __syncthreads();
+    const float* flat = reinterpret_cast<const float*>(lds);
+    for (int c = threadIdx.x; c < G::BN; c += G::threads) {
+      if (n0 + c >= n) continue;
+      float v = 0;
+#pragma unroll
+      for (int w = 0; w < G::WM; ++w) v += flat[w * G::BN + c];
+      dbias_part[(int64_t)tm * n + n0 + c] = v;
+    }
+  }
+};
+
+struct ScorePlan {
+  int tile, tiles_m, tiles_n;
+};
+ScorePlan score_plan(int nq, int nc) {
+  auto tiles = [&](int t) { return (int64_t)ceil_div(nq, t) * ceil_div(nc, t); };
+  const int t = tiles(256) >= 192 ? 256 : tiles(128) >= 192 ? 128 : 64;
+  return {t, ceil_div(nq, t), ceil_div(nc, t)};
+}
+
+template <int PAIRS, class E>
+fgpu_status launch_scores(const ScorePlan& p, const GemmOperand& q, const GemmOperand& c, int nq, int nc, int dim, const E& e,
+                          hipStream_t s) {
+  const GemmArgs g{q, c, nq, nc, dim, p.tiles_m, p.tiles_n, 1, (dim + kGemmBK - 1) / kGemmBK * kGemmBK};
+  const int grid = p.tiles_m * p.tiles_n;
+  if (p.tile == 256)
+    gemm_kernel<Tile256, true, true, PAIRS, E><<<grid, Tile256::threads, 0, s>>>(g, e);
+  else if (p.tile == 128)
+    gemm_kernel<Tile128, true, true, PAIRS, E><<<grid, Tile128::threads, 0, s>>>(g, e);
+  else
+    gemm_kernel<Tile64, true, true, PAIRS, E><<<grid, Tile64::threads, 0, s>>>(g, e);
+  FGPU_HIP(hipGetLastError());
+  return FGPU_OK;
+}
+
+fgpu_status check_loss(int nq, int nc, int dim, int dtype) {
+  FGPU_CHECK(dtype == FGPU_DTYPE_F32 || dtype == FGPU_DTYPE_BF16, FGPU_ERR_ARG, "contrastive loss: unknown dtype");
+  FGPU_CHECK(nq >= 0 && nc >= 1 && dim >= 1, FGPU_ERR_ARG, "contrastive loss: nq >= 0, nc and dim >= 1");
+  FGPU_CHECK(nq <= FGPU_LOSS_MAX_QUERIES && nc <= FGPU_HEAD_MAX_ROWS && dim <= FGPU_HEAD_MAX_DIM, FGPU_ERR_UNSUPPORTED,
+             "contrastive loss: more than 2^20 queries, 2^30 candidates or 2^16 dims");
+  return FGPU_OK;
+}
+bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
+
+// Columns of G held at a time at most: 2^31 elements of G, whole tiles, and at most 2^20 columns, which keeps a tile's rows
+// within 32-bit offsets.
+int64_t most_columns(int nq, int nc) {
+  const int64_t most = std::min<int64_t>((int64_t)1 << 20, ((int64_t)1 << 31) / std::max(1, nq));
+  return std::min<int64_t>(nc, most / 256 * 256);
+}
+// The backward pass's workspace when it holds `step` columns of G.
+size_t backward_bytes(int nq, int nc, int dim, bool f32, int step) {
+  const bool chunked = step < nc;
+  size_t b = carve_bytes<f32x2>(nq) + carve_bytes<int32_t>(nq) + packed_bytes(nq, dim, f32) + packed_bytes(nc, dim, f32) +
+             packed_bytes(nq, step, f32) + carve_bytes<float>((size_t)ceil_div(nq, 64) * step);
+  if (chunked) b += carve_bytes<float>((size_t)nq * ((dim + 3) & ~3));
+  return b + std::max(product_workspace_bytes({nq, dim, step, f32, chunked}), product_workspace_bytes({step, dim, nq, f32}));
+}
+
+}  // namespace
+}  // namespace fgpu
+
+using namespace fgpu;
+
+extern "C" {
+
+size_t fgpu_contrastive_loss_workspace_bytes(int nq, int nc, int dim, int dtype) {
+  if (check_loss(nq, nc, dim, dtype) != FGPU_OK || nq == 0) return 0;
+  const bool f32 = dtype == FGPU_DTYPE_F32;
+  size_t b = carve_bytes<f32x2>((size_t)score_plan(nq, nc).tiles_n * nq) + carve_bytes<float>(nq);
+  if (needs_pack(dim, f32)) b += packed_bytes(nq, dim, f32) + packed_bytes(nc, dim, f32);
+  return b;
+}
+
+fgpu_status fgpu_contrastive_loss(const void* d_q, const void* d_c, const int32_t* d_target, const float* d_bias,
+                                  const int32_t* d_ids, int nq, int nc, int dim, int dtype, float scale, float* d_loss,
+                                  float* d_lse, void* d_workspace, size_t workspace_bytes, void* stream) {
+  FGPU_TRY(check_loss(nq, nc, dim, dtype));
+  if (nq == 0) return FGPU_OK;
+  FGPU_CHECK(d_q && d_c && d_target && d_loss && d_lse, FGPU_ERR_ARG, "contrastive loss: null argument");
+  FGPU_CHECK(aligned16(d_q) && aligned16(d_c) && aligned16(d_workspace), FGPU_ERR_ARG,
+             "contrastive loss: queries, candidates and workspace must be 16-byte aligned");
+  const bool f32 = dtype == FGPU_DTYPE_F32, pk = needs_pack(dim, f32);
+  const ScorePlan sp = score_plan(nq, nc);
+  Carve ws(d_workspace, workspace_bytes);
+  f32x2* part = ws.take<f32x2>((size_t)sp.tiles_n * nq);
+  float* target2 = ws.take<float>(nq);
+  char* qp = pk ? ws.take<char>(packed_bytes(nq, dim, f32)) : nullptr;
+  char* cp = pk ? ws.take<char>(packed_bytes(nc, dim, f32)) : nullptr;
+  FGPU_CHECK(ws.ok(), FGPU_ERR_WORKSPACE, "contrastive loss: workspace smaller than fgpu_contrastive_loss_workspace_bytes");
+  hipStream_t s = as_stream(stream);
+  GemmOperand q = as_is(d_q, dim), c = as_is(d_c, dim);
+  if (pk) {
+    q = packed(qp, nq, dim);
+    c = packed(cp, nc, dim);
+    FGPU_TRY(launch_pack(d_q, nq, dim, f32, q, nullptr, nullptr, 0, s));
+    FGPU_TRY(launch_pack(d_c, nc, dim, f32, c, nullptr, nullptr, 0, s));
+  }
+  const LossArgs a{d_bias, d_ids, d_target, scale * kLog2e, nq, nc};
+  const StatsEpi e{a, part, target2};
+  FGPU_TRY(f32 ? launch_scores<6>(sp, q, c, nq, nc, dim, e, s) : launch_scores<1>(sp, q, c, nq, nc, dim, e, s));
+  loss_join_kernel<<<ceil_div(nq, 64), 1024, 0, s>>>(a, part, sp.tiles_n, target2, d_loss, d_lse);
+  FGPU_HIP(hipGetLastError());
+  return FGPU_OK;
+}
+
+size_t fgpu_contrastive_loss_backward_workspace_bytes(int nq, int nc, int dim, int dtype) {
+  if (check_loss(nq, nc, dim, dtype) != FGPU_OK || nq == 0) return 0;
+  const bool f32 = dtype == FGPU_DTYPE_F32;
+  return backward_bytes(nq, nc, dim, f32, (int)most_columns(nq, nc));
+}
+
+fgpu_status fgpu_contrastive_loss_backward(const float* d_dloss, const void* d_q, const void* d_c, const int32_t* d_target,
+                                           const float* d_lse, const float* d_bias, const int32_t* d_ids, int nq, int nc,
+                                           int dim, int dtype, float scale, void* d_dq, void* d_dc, float* d_dbias,
+                                           void* d_workspace, size_t workspace_bytes, void* stream) {
+  FGPU_TRY(check_loss(nq, nc, dim, dtype));
+  const bool f32 = dtype == FGPU_DTYPE_F32;
+  hipStream_t s = as_stream(stream);
+  if (nq == 0) {
+    if (d_dc) FGPU_TRY(launch_column_finish(nullptr, 0, 0, (int64_t)nc * dim, f32, d_dc, s));
+    if (d_dbias) FGPU_TRY(launch_column_finish(nullptr, 0, 0, nc, true, d_dbias, s));
+    return FGPU_OK;
+  }
+  FGPU_CHECK(d_dloss && d_q && d_c && d_target && d_lse, FGPU_ERR_ARG, "contrastive loss backward: null argument");
+  FGPU_CHECK(aligned16(d_q) && aligned16(d_c) && aligned16(d_workspace), FGPU_ERR_ARG,
+             "contrastive loss backward: queries, candidates and workspace must be 16-byte aligned");
+  int step = (int)most_columns(nq, nc);
+  while (step > 256 && backward_bytes(nq, nc, dim, f32, step) > workspace_bytes) step = std::max(256, step / 2 / 256 * 256);
+  const bool copy_c = d_bias || needs_pack(dim, f32);
+  Carve ws(d_workspace, workspace_bytes);
+  f32x2* rows = ws.take<f32x2>(nq);
+  int32_t* live_target = ws.take<int32_t>(nq);
+  char* qp = ws.take<char>(packed_bytes(nq, dim, f32));
+  char* cp = copy_c ? ws.take<char>(packed_bytes(nc, dim, f32)) : nullptr;
+  char* gp = ws.take<char>(packed_bytes(nq, step, f32));
+  float* dbias_part = d_dbias ? ws.take<float>((size_t)ceil_div(nq, 64) * step) : nullptr;
+  float* dq_sum = step < nc && d_dq ? ws.take<float>((size_t)nq * ((dim + 3) & ~3)) : nullptr;
+  char* pw = ws.take<char>(std::max(d_dq ? product_workspace_bytes({nq, dim, step, f32, step < nc}) : 0,
+                                    d_dc ? product_workspace_bytes({step, dim, nq, f32}) : 0));
+  FGPU_CHECK(ws.ok(), FGPU_ERR_WORKSPACE,
+             "contrastive loss backward: workspace too small for 256 columns of the score gradient");
+  LossArgs a{d_bias, d_ids, d_target, scale * kLog2e, nq, nc};
+  loss_rows_kernel<<<ceil_div(nq, 256), 256, 0, s>>>(a, d_dloss, d_lse, rows, live_target);
+  FGPU_HIP(hipGetLastError());
+  a.target = live_target;
+  // Rows without a gradient and masked candidates become zero vectors: their G is zero, and what they hold (infinities
+  // and NaN included) must not reach the products.
+  const GemmOperand q = packed(qp, nq, dim);
+  FGPU_TRY(launch_pack(d_q, nq, dim, f32, q, nullptr, live_target, nc, s));
+  GemmOperand c = as_is(d_c, dim);
+  if (copy_c) {
+    c = packed(cp, nc, dim);
+    FGPU_TRY(launch_pack(d_c, nc, dim, f32, c, d_bias, nullptr, 0, s));
+  }
+  for (int c0 = 0; c0 < nc; c0 += step) {
+    const int n = std::min(step, nc - c0);
+    const GemmOperand g = packed(gp, nq, n), cc{c.p + (int64_t)c0 * c.ld, c.ld, c.plane};
+    const ScorePlan sp = score_plan(nq, n);
+    uint16_t* gw = const_cast<uint16_t*>(g.p);
+    if (f32)
+      FGPU_TRY(launch_scores<6>(sp, q, cc, nq, n, dim, GradEpi<true>{a, rows, gw, g.ld, g.plane, dbias_part, c0, n}, s));
+    else
+      FGPU_TRY(launch_scores<1>(sp, q, cc, nq, n, dim, GradEpi<false>{a, rows, gw, g.ld, g.plane, dbias_part, c0, n}, s));
+    if (d_dbias) FGPU_TRY(launch_column_finish(dbias_part, sp.tiles_m, n, n, true, d_dbias + c0, s));
+    if (d_dq) {
+      Finish f;
+      f.out = d_dq, f.alpha = scale;
+      f.add = c0 > 0 ? dq_sum : nullptr;
+      f.sum = c0 + n < nc ? dq_sum : nullptr;
+      FGPU_TRY(launch_product({nq, dim, n, f32, step < nc}, g, true, cc, false, f, pw, s));
+    }
+    if (d_dc) {
+      Finish f;
+      f.out = static_cast<char*>(d_dc) + (int64_t)c0 * dim * (f32 ? 4 : 2), f.alpha = scale;
+      FGPU_TRY(launch_product({n, dim, nq, f32}, g, false, q, false, f, pw, s));
+    }
+  }
+  return FGPU_OK;
+}
+
+}  // extern "C"

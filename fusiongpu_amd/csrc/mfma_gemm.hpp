@@ -1,0 +1,275 @@
+// mfma_gemm.hpp -- the matrix-product core of the query head's operators (head_linear.hip, head_loss.hip).
+//
+// D[m][n] = sum_k A(m, k) B(n, k) on bf16 MFMA with float32 accumulators.  Each operand is read either with k contiguous
+// (rows of k) or with k strided (rows of m or n, one row a k), so the forward product x W^T and both gradients dz W and
+// dz^T x come from one kernel without a transposed copy.  float32 operands are held as three bf16 planes (split_f32
+// below) and the k loop walks the six plane pairs whose product is above 2^-24 of the whole.
+#pragma once
+
+#include "common.hpp"
+
+namespace fgpu {
+
+typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
+typedef __bf16 bf16x4 __attribute__((ext_vector_type(4)));
+typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
+typedef float f32x2 __attribute__((ext_vector_type(2)));
+typedef float f32x4 __attribute__((ext_vector_type(4)));
+typedef short s16x4 __attribute__((ext_vector_type(4)));
+typedef short s16x8 __attribute__((ext_vector_type(8)));
+
+using bf16 = __bf16;
+
+__device__ __forceinline__ float to_f32(float v) { return v; }
+__device__ __forceinline__ float to_f32(bf16 v) { return (float)v; }
+
+// Four consecutive elements as float32, at any address an element may have (global memory takes unaligned vectors).
+typedef float f32x4u __attribute__((ext_vector_type(4), aligned(4)));
+typedef __bf16 bf16x4u __attribute__((ext_vector_type(4), aligned(2)));
+__device__ __forceinline__ f32x4 load4(const float* p) { return *reinterpret_cast<const f32x4u*>(p); }
+__device__ __forceinline__ f32x4 load4(const bf16* p) {
+  return __builtin_convertvector(*reinterpret_cast<const bf16x4u*>(p), f32x4);
+}
+__device__ __forceinline__ void store4(float* p, f32x4 v) { *reinterpret_cast<f32x4u*>(p) = v; }
+__device__ __forceinline__ void store4(bf16* p, f32x4 v) {
+  *reinterpret_cast<bf16x4u*>(p) = __builtin_convertvector(v, bf16x4);
+}
+// The first `n` (1 to 4) of them; the others read as zero and are not written.
+template <class T>
+__device__ __forceinline__ f32x4 load4_n(const T* p, int n) {
+  if (n >= 4) return load4(p);
+  f32x4 v = {0, 0, 0, 0};
+  for (int i = 0; i < n; ++i) v[i] = to_f32(p[i]);
+  return v;
+}
+template <class T>
+__device__ __forceinline__ void store4_n(T* p, f32x4 v, int n) {
+  if (n >= 4) {
+    store4(p, v);
+    return;
+  }
+  for (int i = 0; i < n; ++i) p[i] = (T)v[i];
+}
+
+// x = h + m + l exactly (24 significant bits in three bf16 of 8): the first cut off rather than rounded, so that no
+// finite x becomes infinite, the others rounded.  Of a value that is not finite only h is kept.
+__device__ __forceinline__ void split_f32(float x, bf16& h, bf16& m, bf16& l) {
+  const uint32_t u = __float_as_uint(x);
+  const float hf = __uint_as_float(u & 0xFFFF0000u);
+  const bool fin = (u & 0x7F800000u) != 0x7F800000u;
+  // A NaN whose payload lies in the low half would become infinite when cut.
+  h = fin ? (bf16)hf : (bf16)x;
+  const float r = fin ? x - hf : 0.0f;
+  m = (bf16)r;
+  l = (bf16)(r - (float)m);
+}
+
+// One operand of a product.  k_contig: element (r, k) at p[r ld + k]; k strided: at p[k ld + r].  p is 16-byte aligned
+// and ld a multiple of 8, plane (elements) the distance of the split planes.
+struct GemmOperand {
+  const uint16_t* p;
+  int64_t ld;
+  int64_t plane;
+};
+
+struct GemmArgs {
+  GemmOperand a, b;
+  int m, n, k;
+  int tiles_m, tiles_n;
+  int splits;       // workgroups a tile, each on its own part of k
+  int k_per_split;  // a multiple of kGemmBK
+};
+
+constexpr int kGemmBK = 64;
+
+// Plane pairs (a, b) in the order they are accumulated: the smallest products first.
+__device__ __forceinline__ int pair_a(int p) { return (0x201100 >> (4 * (5 - p))) & 0xF; }
+__device__ __forceinline__ int pair_b(int p) { return (0x021010 >> (4 * (5 - p))) & 0xF; }
+
+// Tiles: BM x BN a workgroup of WM x WN waves, each wave (BM / WM) x (BN / WN) in 16 x 16 MFMA tiles.
+template <int BM_, int BN_, int WM_, int WN_>
+struct GemmTile {
+  static constexpr int BM = BM_, BN = BN_, WM = WM_, WN = WN_;
+  static constexpr int waves = WM * WN, threads = waves * kWave;
+  static constexpr int FM = BM / WM / 16, FN = BN / WN / 16;
+  static constexpr int stage_bytes = (BM + BN) * kGemmBK * 2;
+};
+using Tile256 = GemmTile<256, 256, 2, 4>;
+using Tile128 = GemmTile<128, 128, 2, 2>;
+using Tile64 = GemmTile<64, 64, 2, 2>;
+
+typedef __attribute__((address_space(3))) void lds_void;
+typedef __attribute__((address_space(3))) char lds_char;
+
+// The part of an operand's LDS tile that one lane fills (16 bytes a load straight to LDS), and the addresses its
+// fragments are read from.  R: rows of m or n in the tile, NT: threads.
+//
+// k contiguous: R rows of 128 bytes (64 k), the row's eight 16-byte chunks permuted by chunk ^ (row & 7), so the 16
+// rows of a fragment read spread over the banks.  k strided: 64 rows of R elements, read with the transposing LDS load,
+// in which 16 lanes read four rows of 32 bytes; chunk pairs are permuted by the row's low bits so that those rows, and
+// the ones eight further that the next 16 lanes read, lie in different banks.
+template <bool KC, int CHUNKS>
+__device__ __forceinline__ int tile_swizzle(int row) {
+  if constexpr (KC) return row & 7;
+  return (2 * ((row & 3) | (((row >> 3) & 1) << 2))) & (CHUNKS - 1);
+}
+template <int R, int NT, bool KC>
+struct TileLoad {
+  static constexpr int row_bytes = KC ? kGemmBK * 2 : R * 2;
+  static constexpr int rows = KC ? R : kGemmBK;
+  static constexpr int rows_a_load = NT * 16 / row_bytes;
+  static constexpr int loads = rows / rows_a_load;
+  static constexpr int chunks = row_bytes / 16;
+  static_assert(KC || rows_a_load % 16 == 0, "the permutation must not depend on the load");
+  static_assert(rows % rows_a_load == 0, "whole loads");
+
+  uint32_t voff;   // byte offset of the lane's chunk in load 0, from the tile's first element
+  uint32_t vstep;  // byte distance of a lane's chunks in successive loads (uniform)
+  int kc;          // KC: first k of the lane's chunk
+
+  __device__ void init(int64_t ld, int tid) {
+    const int row = tid / chunks, slot = tid % chunks;
+    const int chunk = slot ^ tile_swizzle<KC, chunks>(row);
+    voff = (uint32_t)((int64_t)row * ld * 2) + chunk * 16;
+    vstep = (uint32_t)((int64_t)rows_a_load * ld * 2);
+    kc = chunk * 8;
+  }
+  // Issues the loads of k0 .. k0 + 63 into the tile at `lds`.  r0: the tile's first row (m or n) of nr.  Reads beyond the
+  // operand give zeros: the buffer ends with its last group of eight, and a chunk past the end of k is sent beyond it.
+  __device__ __forceinline__ void issue(const GemmOperand& o, int plane, int r0, int nr, int k0, int nk, lds_char* lds,
+                                        int wave) const {
+    const uint16_t* base = o.p + plane * o.plane;
+    int64_t last;  // elements from base to the end of the last one wanted
+    if constexpr (KC) {
+      base += (int64_t)r0 * o.ld + k0;
+      last = (int64_t)(min(nr - r0, R) - 1) * o.ld + min(((nk + 7) & ~7) - k0, kGemmBK);
+    } else {
+      base += (int64_t)k0 * o.ld + r0;
+      last = (int64_t)(min(nk - k0, kGemmBK) - 1) * o.ld + min(((nr + 7) & ~7) - r0, R);
+    }
+    auto rsrc = __builtin_amdgcn_make_buffer_rsrc(const_cast<uint16_t*>(base), 0, (int)(last * 2), 0x00027000);
+    const uint32_t off = (KC && kc >= nk - k0) ? 0x80000000u : voff;
+#pragma unroll
+    for (int i = 0; i < loads; ++i)
+      __builtin_amdgcn_raw_ptr_buffer_load_lds(rsrc, (lds_void*)(lds + i * (NT * 16) + wave * (kWave * 16)), 16,
+                                               off + i * vstep, 0, 0, 0);
+  }
+};
+
+// A lane's fragments of 16 rows x 32 k (k half kk of the 64) from the tile at `lds`.
+template <int R, bool KC>
+struct TileRead {
+  uint32_t base;  // k contiguous: address of (row l % 16, chunk l / 16); strided: in-row part and row part apart
+  uint32_t rowp;
+  __device__ void init(int lane, int first_row) {
+    if constexpr (KC) {
+      base = (first_row + (lane & 15)) * 128 + (((lane >> 4) ^ (lane & 7)) * 16);
+      rowp = 0;
+    } else {
+      const int i = lane & 15, g = lane >> 4;
+      const int s = tile_swizzle<KC, R / 8>((i >> 2) | (g << 3));
+      rowp = (g * 8 + (i >> 2)) * R * 2;
+      base = (first_row * 2) ^ (s * 16 + ((i & 3) >> 1) * 16 + (i & 1) * 8);
+    }
+  }
+  __device__ __forceinline__ bf16x8 get(const lds_char* lds, int f, int kk) const {
+    typedef __attribute__((address_space(3))) const bf16x8 lds_frag;
+    typedef __attribute__((address_space(3))) s16x4 lds_half;
+    if constexpr (KC) {
+      return *(lds_frag*)(lds + ((base ^ (kk * 64)) + f * 2048));
+    } else {
+      const uint32_t a = rowp + (base ^ (f * 32)) + kk * 32 * R * 2;
+      const s16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_half*)(lds + a));
+      const s16x4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_half*)(lds + a + 4 * R * 2));
+      s16x8 v = {lo[0], lo[1], lo[2], lo[3], hi[0], hi[1], hi[2], hi[3]};
+      return __builtin_bit_cast(bf16x8, v);
+    }
+  }
+};
+
+// Workgroup -> (tile_m, tile_n, split).  Consecutive workgroups go to the eight XCDs in turn; each XCD gets a contiguous
+// run of tiles, walked in groups of eight tile rows, so its L2 serves the operand rows that neighbouring tiles share.
+__device__ __forceinline__ void gemm_tile_of(const GemmArgs& g, int wg, int total, int& tm, int& tn, int& sp) {
+  constexpr int kXcd = 8, kGroup = 8;
+  const int per = total / kXcd, rest = total % kXcd, x = wg % kXcd;
+  int t = x * per + min(x, rest) + wg / kXcd;
+  sp = t % g.splits;
+  t /= g.splits;
+  const int group = kGroup * g.tiles_n, first = t / group * kGroup;
+  const int gm = min(g.tiles_m - first, kGroup), in = t % group;
+  tm = first + in % gm;
+  tn = in / gm;
+}
+
+// acc[fn][fm] element r of a lane: n = 16 fn + 4 (lane / 16) + r, m = 16 fm + lane % 16 of the wave's part.
+template <class T, bool AKC, bool BKC, int PAIRS, class Epi>
+__global__ __launch_bounds__(T::threads, T::threads == 512 ? 2 : 1) void gemm_kernel(GemmArgs g, Epi epi) {
+  __shared__ __attribute__((aligned(1024))) char s0[T::stage_bytes];
+  __shared__ __attribute__((aligned(1024))) char s1[T::stage_bytes];
+  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int wm = wave / T::WN, wn = wave % T::WN;
+  int tm, tn, sp;
+  gemm_tile_of(g, blockIdx.x, gridDim.x, tm, tn, sp);
+  const int m0 = tm * T::BM, n0 = tn * T::BN;
+  const int kbeg = sp * g.k_per_split, kend = min(g.k, kbeg + g.k_per_split);
+
+  TileLoad<T::BM, T::threads, AKC> la;
+  TileLoad<T::BN, T::threads, BKC> lb;
+  la.init(g.a.ld, tid);
+  lb.init(g.b.ld, tid);
+  TileRead<T::BM, AKC> ra;
+  TileRead<T::BN, BKC> rb;
+  ra.init(lane, wm * (T::BM / T::WM));
+  rb.init(lane, wn * (T::BN / T::WN));
+
+  f32x4 acc[T::FN][T::FM];
+#pragma unroll
+  for (int i = 0; i < T::FN; ++i)
+#pragma unroll
+    for (int j = 0; j < T::FM; ++j) acc[i][j] = f32x4{0, 0, 0, 0};
+
+  constexpr int boff = T::BM * kGemmBK * 2;
+  const int nk = max(0, (kend - kbeg + kGemmBK - 1) / kGemmBK), steps = nk * PAIRS;
+  int pk = kbeg, pp = 0;  // the next stage to load
+  auto issue = [&](char* s) {
+    const int qa = PAIRS == 1 ? 0 : pair_a(pp), qb = PAIRS == 1 ? 0 : pair_b(pp);
+    la.issue(g.a, qa, m0, g.m, pk, g.k, (lds_char*)s, wave);
+    lb.issue(g.b, qb, n0, g.n, pk, g.k, (lds_char*)s + boff, wave);
+    pk += kGemmBK;
+    if (PAIRS > 1 && pk >= kend) {
+      pk = kbeg;
+      ++pp;
+    }
+  };
+  auto compute = [&](char* s) {
+    const lds_char* sa = (const lds_char*)s;
+    const lds_char* sb = (const lds_char*)s + boff;
+#pragma unroll
+    for (int kk = 0; kk < 2; ++kk) {
+      bf16x8 fa[T::FM], fb[T::FN];
+#pragma unroll
+      for (int i = 0; i < T::FN; ++i) fb[i] = rb.get(sb, i, kk);
+#pragma unroll
+      for (int j = 0; j < T::FM; ++j) fa[j] = ra.get(sa, j, kk);
+#pragma unroll
+      for (int j = 0; j < T::FM; ++j)
+#pragma unroll
+        for (int i = 0; i < T::FN; ++i)
+          acc[i][j] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(fb[i], fa[j], acc[i][j], 0, 0, 0);
+    }
+  };
+  if (steps > 0) issue(s0);
+  for (int s = 0; s < steps; s += 2) {
+    __syncthreads();  // stage s has landed; nobody reads the other buffer any more
+    if (s + 1 < steps) issue(s1);
+    compute(s0);
+    if (s + 1 >= steps) break;
+    __syncthreads();
+    if (s + 2 < steps) issue(s0);
+    compute(s1);
+  }
+  __syncthreads();
+  epi.template finish<T>(acc, m0, n0, tm, tn, sp, wm, wn, lane, s0);
+}
+
+}  // namespace fgpu

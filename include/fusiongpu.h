@@ -598,6 +598,98 @@ float fgpu_tune_percentile(const float* values, int64_t n, float pct);
  * coarse rank; *coverage gets the cumulative coverage there.  Host only. */
 int fgpu_tune_elbow(const int32_t* hits_per_rank, int n, int64_t total_hits, float* coverage);
 
+/* ---- query head: the layers between an encoder and the index ------------ */
+
+/* No counterpart in the reference, whose queries arrive in the index's space.
+ * These are the operators of the small trained map that takes an encoder's
+ * hidden states there, forward for serving and backward for training it
+ * against the index's vectors.  Arrays are row-major and contiguous, all of
+ * one call's of one dtype unless said otherwise: FGPU_DTYPE_F32 or
+ * FGPU_DTYPE_BF16 (results are rounded once, to nearest even; every sum,
+ * softmax and statistic is held in float32).  float32 products are formed from
+ * bfloat16 triples that hold the operands exactly (six products, the dropped
+ * ones below 2^-24 of the result's terms); an operand that is not finite makes
+ * the float32 results it touches NaN.  Calls only enqueue kernels on `stream`
+ * (no allocation, no synchronisation; they can be captured), results do not
+ * depend on timing (no floating-point atomics), and rows = 0 is allowed.
+ * Workspaces, and the matrices that enter a product (x, w, dy, queries,
+ * candidates), must be 16-byte aligned; other arrays need their element's
+ * alignment. */
+#define FGPU_DTYPE_F32 0
+#define FGPU_DTYPE_BF16 1
+#define FGPU_ACT_NONE 0
+#define FGPU_ACT_RELU 1
+#define FGPU_ACT_GELU 2 /* z Phi(z), Phi the normal distribution function */
+#define FGPU_ACT_SILU 3
+#define FGPU_HEAD_MAX_ROWS (1 << 30)
+#define FGPU_HEAD_MAX_DIM (1 << 16)
+
+/* y [rows][out_dim] = act(z) + residual with z = x [rows][in_dim] w^T + bias,
+ * w [out_dim][in_dim].  d_bias [out_dim], d_residual [rows][out_dim] and d_pre
+ * [rows][out_dim] (gets z, which fgpu_linear_backward needs when act is not
+ * FGPU_ACT_NONE) may be NULL.  d_residual may be d_y itself. */
+size_t fgpu_linear_workspace_bytes(int64_t rows, int in_dim, int out_dim, int dtype);
+fgpu_status fgpu_linear(const void* d_x, const void* d_w, const void* d_bias, const void* d_residual, int64_t rows,
+                        int in_dim, int out_dim, int dtype, int act, void* d_y, void* d_pre, void* d_workspace,
+                        size_t workspace_bytes, void* stream);
+/* Gradients of fgpu_linear for dy [rows][out_dim], with dz = dy act'(pre):
+ * dx = dz w, dw = dz^T x, db = the column sums of dz; the residual's gradient
+ * is dy itself.  Each of d_dx, d_dw, d_db may be NULL (not wanted); d_w is read
+ * for dx, d_x for dw, d_pre when act is not FGPU_ACT_NONE.  In bfloat16, dz is
+ * rounded to bfloat16 before the two products (not before db). */
+size_t fgpu_linear_backward_workspace_bytes(int64_t rows, int in_dim, int out_dim, int dtype);
+fgpu_status fgpu_linear_backward(const void* d_dy, const void* d_x, const void* d_w, const void* d_pre, int64_t rows,
+                                 int in_dim, int out_dim, int dtype, int act, void* d_dx, void* d_dw, void* d_db,
+                                 void* d_workspace, size_t workspace_bytes, void* stream);
+
+/* y = (x - mean) rstd gamma + beta for each row of x [rows][dim], mean and
+ * rstd = 1 / sqrt(variance + eps) its own (biased variance, about the mean).
+ * d_gamma, d_beta [dim] may be NULL (one, zero); d_mean, d_rstd [rows] float32
+ * (what the backward pass needs) may be NULL.  d_y may be d_x.  dim <= 16384. */
+fgpu_status fgpu_layer_norm(const void* d_x, const void* d_gamma, const void* d_beta, int64_t rows, int dim, int dtype,
+                            float eps, void* d_y, float* d_mean, float* d_rstd, void* stream);
+/* Gradients of fgpu_layer_norm: with h = (x - mean) rstd and u = dy gamma,
+ * dx = rstd (u - mean(u) - h mean(u h)), dgamma = the column sums of dy h,
+ * dbeta those of dy.  Each of d_dx, d_dgamma, d_dbeta may be NULL; d_dx may be
+ * d_dy or d_x. */
+size_t fgpu_layer_norm_backward_workspace_bytes(int64_t rows, int dim, int dtype);
+fgpu_status fgpu_layer_norm_backward(const void* d_dy, const void* d_x, const void* d_gamma, const float* d_mean,
+                                     const float* d_rstd, int64_t rows, int dim, int dtype, void* d_dx, void* d_dgamma,
+                                     void* d_dbeta, void* d_workspace, size_t workspace_bytes, void* stream);
+
+/* Softmax contrastive loss of queries [nq][dim] against candidates [nc][dim]:
+ * with scores s_ij = scale q_i.c_j + bias_j,
+ *   lse_i = log sum_j exp s_ij,  loss_i = lse_i - s_{i, target_i}.
+ * d_bias [nc] float32 (may be NULL) carries the index's L2 metric (-scale
+ * |c_j|^2 / 2: then exp s_ij ~ exp(-scale |q_i - c_j|^2 / 2)), a sampled
+ * softmax's -log of the sampling probabilities, and masks: a candidate whose
+ * bias is at most FGPU_MASK_BIAS (-infinity, or the lowest finite value) is
+ * left out, whatever its vector holds.  d_ids [nc] (may be NULL) names each
+ * candidate's document: copies of the target's document other than the target
+ * are left out of that row.  A row whose target lies outside [0, nc) has loss 0
+ * and no gradient (its lse is over all unmasked candidates); a row with no
+ * candidate left has lse -infinity, loss 0 and no gradient; a row whose target
+ * is masked has an infinite loss and no gradient.  d_loss, d_lse [nq] float32.
+ * nq <= FGPU_LOSS_MAX_QUERIES. */
+#define FGPU_MASK_BIAS (-8.507059173023462e37f) /* -2^126 */
+#define FGPU_LOSS_MAX_QUERIES (1 << 20)
+size_t fgpu_contrastive_loss_workspace_bytes(int nq, int nc, int dim, int dtype);
+fgpu_status fgpu_contrastive_loss(const void* d_q, const void* d_c, const int32_t* d_target, const float* d_bias,
+                                  const int32_t* d_ids, int nq, int nc, int dim, int dtype, float scale, float* d_loss,
+                                  float* d_lse, void* d_workspace, size_t workspace_bytes, void* stream);
+/* Its gradients for dloss [nq] float32, from the lse of the forward call:
+ * G_ij = dloss_i (exp(s_ij - lse_i) - [j = target_i]); dq = scale G c, dc = scale
+ * G^T q, dbias_j = sum_i G_ij (float32).  Each of d_dq, d_dc, d_dbias may be
+ * NULL (fixed candidates need no dc).  In bfloat16, G is rounded to bfloat16
+ * before the two products (not before dbias).  G is held in the workspace, all
+ * columns at once in the returned size (up to 2^31 elements); a smaller
+ * workspace is used in chunks of columns, down to 256. */
+size_t fgpu_contrastive_loss_backward_workspace_bytes(int nq, int nc, int dim, int dtype);
+fgpu_status fgpu_contrastive_loss_backward(const float* d_dloss, const void* d_q, const void* d_c, const int32_t* d_target,
+                                           const float* d_lse, const float* d_bias, const int32_t* d_ids, int nq, int nc,
+                                           int dim, int dtype, float scale, void* d_dq, void* d_dc, float* d_dbias,
+                                           void* d_workspace, size_t workspace_bytes, void* stream);
+
 /* ---- files (utils.h, build_global.cu:242-252) -------------------------- */
 
 fgpu_status fgpu_write_ivf_data(const char* path, int64_t total, int nlist, int pq_m, int dim,
