@@ -20,28 +20,91 @@ __device__ __forceinline__ void finish4(const Finish& f, f32x4 v, int64_t at, in
   store4_n((T*)f.out + at, v, cnt);
 }
 
-template <class T>
+template <class T, int ACT>
 struct ProductEpi {
   Finish f;
   float* part;  // [split][m][n4] in place of the result, or NULL
   int m, n;
 
   template <class G>
-  __device__ __forceinline__ void finish(f32x4 (&acc)[G::FN][G::FM], int m0, int n0, int, int, int sp, int wm, int wn,
-                                         int lane, char*) const {
-    const int n4 = (n + 3) & ~3;
+  __device__ __forceinline__ void finish(f32x4 (&acc)[G::FN][G::FM], const GemmWave<G>& w, char*) const {
+    if (w.first_col() + G::FN * 16 <= n)
+      whole(acc, w);
+    else
+      ragged(acc, w);
+  }
+  // Every column of the wave lies inside: straight from the accumulators, 16 bytes of bf16 a store.
+  template <class G>
+  __device__ __forceinline__ void whole(f32x4 (&acc)[G::FN][G::FM], const GemmWave<G>& w) const {
+    constexpr int P = G::FN / 2;
+    if (part) {
+      const int n4 = (n + 3) & ~3;
+#pragma unroll
+      for (int j = 0; j < G::FM; ++j) {
+        if (w.row(j) >= m) continue;
+        float* d = part + ((int64_t)w.sp * m + w.row(j)) * n4 + w.col(0);
+#pragma unroll
+        for (int p = 0; p < P; ++p) {
+          *reinterpret_cast<f32x4*>(d + 32 * p) = acc[2 * p][j];
+          *reinterpret_cast<f32x4*>(d + 32 * p + 4) = acc[2 * p + 1][j];
+        }
+      }
+      return;
+    }
+    f32x8 bias[P];
+#pragma unroll
+    for (int p = 0; p < P; ++p) bias[p] = f.bias ? load8((const T*)f.bias + w.col(p)) : f32x8{{0, 0, 0, 0}, {0, 0, 0, 0}};
 #pragma unroll
     for (int j = 0; j < G::FM; ++j) {
-      const int row = m0 + (wm * G::FM + j) * 16 + (lane & 15);
-      if (row >= m) continue;
+      if (w.row(j) >= m) continue;
+      const int64_t at = (int64_t)w.row(j) * n + w.col(0);
 #pragma unroll
-      for (int i = 0; i < G::FN; ++i) {
-        const int col = n0 + (wn * G::FN + i) * 16 + (lane >> 4) * 4;
-        if (col >= n) continue;
+      for (int p = 0; p < P; ++p) {
+        f32x8 v;
+#pragma unroll
+        for (int e = 0; e < 8; ++e) v.set(e, fmaf(acc[2 * p + e / 4][j][e % 4], f.alpha, bias[p][e]));
+        if (f.pre) store8((T*)f.pre + at + 32 * p, v);
+        if (ACT != FGPU_ACT_NONE) {
+#pragma unroll
+          for (int e = 0; e < 8; ++e) v.set(e, act_value(v[e], ACT));
+        }
+        if (f.residual) {
+          const f32x8 r = load8((const T*)f.residual + at + 32 * p);
+          v.lo += r.lo, v.hi += r.hi;
+        }
+        store8((T*)f.out + at + 32 * p, v);
+      }
+    }
+  }
+  // The wave holds the last columns: through LDS, four columns a lane, so the code that minds the edge stands once.
+  template <class G>
+  __device__ __forceinline__ void ragged(f32x4 (&acc)[G::FN][G::FM], const GemmWave<G>& w) const {
+    constexpr int kCols = G::FN * 16, kPass = GemmWave<G>::lds_bytes / (16 * kCols * 4) < G::FM
+                                                  ? GemmWave<G>::lds_bytes / (16 * kCols * 4) : G::FM;
+    static_assert(kPass > 0 && G::FM % kPass == 0, "whole passes");
+    float* lds = reinterpret_cast<float*>(w.lds);
+    const int n4 = (n + 3) & ~3;
+#pragma unroll
+    for (int j0 = 0; j0 < G::FM; j0 += kPass) {
+      wave_lds_sync();
+#pragma unroll
+      for (int j = 0; j < kPass; ++j)
+#pragma unroll
+        for (int i = 0; i < G::FN; ++i) {
+          const int row = j * 16 + (w.lane & 15), c4 = (w.col(i / 2) - w.first_col()) / 4 + (i & 1);
+          *reinterpret_cast<f32x4*>(lds + row * kCols + 4 * (c4 ^ (row & (kCols / 4 - 1)))) = acc[i][j0 + j];
+        }
+      wave_lds_sync();
+#pragma unroll 1
+      for (int t = w.lane; t < kPass * 16 * kCols / 4; t += kWave) {
+        const int row = t / (kCols / 4), c4 = t % (kCols / 4), col = w.first_col() + 4 * c4;
+        const int gm = w.m0 + (w.wm * G::FM + j0) * 16 + row;
+        if (gm >= m || col >= n) continue;
+        const f32x4 v = *reinterpret_cast<const f32x4*>(lds + row * kCols + 4 * (c4 ^ (row & (kCols / 4 - 1))));
         if (part)
-          *reinterpret_cast<f32x4*>(part + ((int64_t)sp * m + row) * n4 + col) = acc[i][j];
+          *reinterpret_cast<f32x4*>(part + ((int64_t)w.sp * m + gm) * n4 + col) = v;
         else
-          finish4<T>(f, acc[i][j], (int64_t)row * n + col, col, n - col);
+          finish4<T>(f, v, (int64_t)gm * n + col, col, n - col);
       }
     }
   }
@@ -94,11 +157,16 @@ fgpu_status run_tile(int tile, const GemmArgs& g, const E& e, hipStream_t s) {
   if (tile == 128) return run<Tile128, AKC, BKC, PAIRS>(g, e, s);
   return run<Tile64, AKC, BKC, PAIRS>(g, e, s);
 }
-template <int PAIRS, class E>
-fgpu_status run_form(bool a_kc, bool b_kc, int tile, const GemmArgs& g, const E& e, hipStream_t s) {
-  if (a_kc && b_kc) return run_tile<true, true, PAIRS>(tile, g, e, s);
-  if (a_kc) return run_tile<true, false, PAIRS>(tile, g, e, s);
-  return run_tile<false, false, PAIRS>(tile, g, e, s);
+// The activation is part of the kernel's type where the product finishes it (the forward product alone has one).
+template <int PAIRS, class T>
+fgpu_status run_form(bool a_kc, bool b_kc, int tile, const GemmArgs& g, const Finish& f, float* part, hipStream_t s) {
+  const ProductEpi<T, FGPU_ACT_NONE> plain{f, part, g.m, g.n};
+  if (a_kc && !b_kc) return run_tile<true, false, PAIRS>(tile, g, plain, s);
+  if (!a_kc) return run_tile<false, false, PAIRS>(tile, g, plain, s);
+  if (part || f.act == FGPU_ACT_NONE) return run_tile<true, true, PAIRS>(tile, g, plain, s);
+  if (f.act == FGPU_ACT_RELU) return run_tile<true, true, PAIRS>(tile, g, ProductEpi<T, FGPU_ACT_RELU>{f, part, g.m, g.n}, s);
+  if (f.act == FGPU_ACT_GELU) return run_tile<true, true, PAIRS>(tile, g, ProductEpi<T, FGPU_ACT_GELU>{f, part, g.m, g.n}, s);
+  return run_tile<true, true, PAIRS>(tile, g, ProductEpi<T, FGPU_ACT_SILU>{f, part, g.m, g.n}, s);
 }
 
 template <class T>
@@ -162,9 +230,9 @@ fgpu_status launch_product(const Product& p, const GemmOperand& a, bool a_kc, co
   const GemmArgs g{a, b, p.m, p.n, p.k, q.tiles_m, q.tiles_n, q.splits, q.k_per_split};
   float* part = q.splits > 1 || p.chunked ? static_cast<float*>(ws) : nullptr;
   if (p.f32)
-    FGPU_TRY((run_form<6>(a_kc, b_kc, q.tile, g, ProductEpi<float>{f, part, p.m, p.n}, s)));
+    FGPU_TRY((run_form<6, float>(a_kc, b_kc, q.tile, g, f, part, s)));
   else
-    FGPU_TRY((run_form<1>(a_kc, b_kc, q.tile, g, ProductEpi<bf16>{f, part, p.m, p.n}, s)));
+    FGPU_TRY((run_form<1, bf16>(a_kc, b_kc, q.tile, g, f, part, s)));
   if (part) {
     const int64_t total = (int64_t)p.m * ((p.n + 3) / 4);
     if (p.f32)

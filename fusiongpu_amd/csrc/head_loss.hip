@@ -23,14 +23,14 @@ struct LossArgs {
 
 __device__ __forceinline__ bool masked_bias(float b) { return b <= FGPU_MASK_BIAS; }
 
-// The scores of a lane's four columns n .. n + 3 at row m: s2 = scale2 acc + bias2, -inf where the column is masked, beyond the
-// candidates, or another copy of the row's document.
+// The scores of a lane's eight columns n .. n + 7 at row m: s2 = scale2 acc + bias2, -inf where the column is masked,
+// beyond the candidates, or another copy of the row's document.
 struct ColumnSide {
-  f32x4 bias2;
-  int id[4];
+  float bias2[8];
+  int id[8];
   __device__ __forceinline__ void load(const LossArgs& a, int n) {
 #pragma unroll
-    for (int r = 0; r < 4; ++r) {
+    for (int r = 0; r < 8; ++r) {
       const bool in = n + r < a.nc;
       float b = in ? (a.bias ? a.bias[n + r] : 0.0f) : -INFINITY;
       bias2[r] = masked_bias(b) ? -INFINITY : b * kLog2e;
@@ -62,29 +62,27 @@ struct StatsEpi {
   float* target2;  // [nq]
 
   template <class G>
-  __device__ __forceinline__ void finish(f32x4 (&acc)[G::FN][G::FM], int m0, int n0, int, int tn, int, int wm, int wn,
-                                         int lane, char* lds) const {
+  __device__ __forceinline__ void finish(f32x4 (&acc)[G::FN][G::FM], const GemmWave<G>& w, char* lds) const {
+    constexpr int P = G::FN / 2;
     f32x2* sh = reinterpret_cast<f32x2*>(lds);  // [WN][BM]
-    ColumnSide cs[G::FN];
+    ColumnSide cs[P];
 #pragma unroll
-    for (int i = 0; i < G::FN; ++i) cs[i].load(a, n0 + (wn * G::FN + i) * 16 + (lane >> 4) * 4);
+    for (int p = 0; p < P; ++p) cs[p].load(a, w.col(p));
 #pragma unroll
     for (int j = 0; j < G::FM; ++j) {
-      const int ml = (wm * G::FM + j) * 16 + (lane & 15), m = m0 + ml;
-      RowSide w;
-      w.load(a, m);
+      const int m = w.row(j);
+      RowSide rs;
+      rs.load(a, m);
       float top = -INFINITY;
 #pragma unroll
-      for (int i = 0; i < G::FN; ++i) {
-        const int n = n0 + (wn * G::FN + i) * 16 + (lane >> 4) * 4;
+      for (int p = 0; p < P; ++p)
 #pragma unroll
-        for (int r = 0; r < 4; ++r) {
-          const float s = score2(a, acc[i][j][r], cs[i], w, n, r);
-          acc[i][j][r] = s;
-          top = fmaxf(top, s);  // a NaN score makes the sum NaN
-          if (n + r == w.t) target2[m] = s;
+        for (int e = 0; e < 8; ++e) {
+          float& x = reinterpret_cast<float*>(&acc[2 * p + e / 4][j])[e % 4];
+          x = score2(a, x, cs[p], rs, w.col(p), e);
+          top = fmaxf(top, x);  // a NaN score makes the sum NaN
+          if (w.col(p) + e == rs.t) target2[m] = x;
         }
-      }
       top = fmaxf(top, shfl_xor_f(top, 16));
       top = fmaxf(top, shfl_xor_f(top, 32));
       const float base = top == -INFINITY ? 0.0f : top;
@@ -95,18 +93,18 @@ struct StatsEpi {
         for (int r = 0; r < 4; ++r) sum += fast_exp2(acc[i][j][r] - base);
       sum += shfl_xor_f(sum, 16);
       sum += shfl_xor_f(sum, 32);
-      if (lane < 16) sh[wn * G::BM + ml] = f32x2{top, sum};
+      if (w.lane < 16) sh[w.wn * G::BM + m - w.m0] = f32x2{top, sum};
     }
     __syncthreads();
     for (int ml = threadIdx.x; ml < G::BM; ml += G::threads) {
-      if (m0 + ml >= a.nq) continue;
+      if (w.m0 + ml >= a.nq) continue;
       float top = -INFINITY, sum = 0;
 #pragma unroll
-      for (int w = 0; w < G::WN; ++w) top = fmaxf(top, sh[w * G::BM + ml][0]);
+      for (int k = 0; k < G::WN; ++k) top = fmaxf(top, sh[k * G::BM + ml][0]);
       const float base = top == -INFINITY ? 0.0f : top;
 #pragma unroll
-      for (int w = 0; w < G::WN; ++w) sum += sh[w * G::BM + ml][1] * fast_exp2(sh[w * G::BM + ml][0] - base);
-      part[(int64_t)tn * a.nq + m0 + ml] = f32x2{top, sum};
+      for (int k = 0; k < G::WN; ++k) sum += sh[k * G::BM + ml][1] * fast_exp2(sh[k * G::BM + ml][0] - base);
+      part[(int64_t)w.tn * a.nq + w.m0 + ml] = f32x2{top, sum};
     }
   }
 };
@@ -163,74 +161,71 @@ struct GradEpi {
   int c0, n;          // the chunk's columns
 
   template <class G>
-  __device__ __forceinline__ void finish(f32x4 (&acc)[G::FN][G::FM], int m0, int n0, int tm, int, int, int wm, int wn,
-                                         int lane, char* lds) const {
-    ColumnSide cs[G::FN];
-    f32x4 col[G::FN];
+  __device__ __forceinline__ void finish(f32x4 (&acc)[G::FN][G::FM], const GemmWave<G>& w, char* lds) const {
+    constexpr int P = G::FN / 2;
+    ColumnSide cs[P];
+    f32x8 col[P];
 #pragma unroll
-    for (int i = 0; i < G::FN; ++i) {
-      cs[i].load(a, c0 + n0 + (wn * G::FN + i) * 16 + (lane >> 4) * 4);
-      col[i] = f32x4{0, 0, 0, 0};
+    for (int p = 0; p < P; ++p) {
+      cs[p].load(a, c0 + w.col(p));
+      col[p] = f32x8{{0, 0, 0, 0}, {0, 0, 0, 0}};
     }
 #pragma unroll
     for (int j = 0; j < G::FM; ++j) {
-      const int m = m0 + (wm * G::FM + j) * 16 + (lane & 15);
-      RowSide w;
-      w.load(a, m);
+      const int m = w.row(j);
+      RowSide rs;
+      rs.load(a, m);
       const f32x2 row = m < a.nq ? rows[m] : f32x2{INFINITY, 0.0f};
 #pragma unroll
-      for (int i = 0; i < G::FN; ++i) {
-        const int nl = n0 + (wn * G::FN + i) * 16 + (lane >> 4) * 4;
-        f32x4 v;
+      for (int p = 0; p < P; ++p) {
+        const int nl = w.col(p);
+        f32x8 v;
 #pragma unroll
-        for (int r = 0; r < 4; ++r) {
-          float p = fast_exp2(score2(a, acc[i][j][r], cs[i], w, c0 + nl, r) - row[0]);
-          if (c0 + nl + r == w.t) p -= 1.0f;
-          v[r] = p * row[1];
+        for (int e = 0; e < 8; ++e) {
+          float x = fast_exp2(score2(a, acc[2 * p + e / 4][j][e % 4], cs[p], rs, c0 + nl, e) - row[0]);
+          if (c0 + nl + e == rs.t) x -= 1.0f;
+          v.set(e, x * row[1]);
         }
-        col[i] += v;
+        col[p].lo += v.lo, col[p].hi += v.hi;
         if (m < a.nq && nl < ldg) {  // the padding's columns are zero
           uint16_t* d = g + (int64_t)m * ldg + nl;
           if constexpr (!F32) {
-            *reinterpret_cast<bf16x4*>(d) = __builtin_convertvector(v, bf16x4);
+            *reinterpret_cast<bf16x8*>(d) = to_bf16x8(v);
           } else {
-            bf16x4 h, mi, l;
+            bf16x8 h, mi, l;
 #pragma unroll
-            for (int r = 0; r < 4; ++r) {
+            for (int e = 0; e < 8; ++e) {
               bf16 x, y, z;
-              split_f32(v[r], x, y, z);
-              h[r] = x, mi[r] = y, l[r] = z;
+              split_f32(v[e], x, y, z);
+              h[e] = x, mi[e] = y, l[e] = z;
             }
-            *reinterpret_cast<bf16x4*>(d) = h;
-            *reinterpret_cast<bf16x4*>(d + plane) = mi;
-            *reinterpret_cast<bf16x4*>(d + 2 * plane) = l;
+            *reinterpret_cast<bf16x8*>(d) = h;
+            *reinterpret_cast<bf16x8*>(d + plane) = mi;
+            *reinterpret_cast<bf16x8*>(d + 2 * plane) = l;
           }
         }
       }
     }
     if (!dbias_part) return;
-    f32x4* sh = reinterpret_cast<f32x4*>(lds);  // [WM][BN / 4]
+    float* sh = reinterpret_cast<float*>(lds);  // [WM][BN]
 #pragma unroll
-    for (int i = 0; i < G::FN; ++i) {
+    for (int p = 0; p < P; ++p)
 #pragma unroll
-      for (int r = 0; r < 4; ++r) {
-        float v = col[i][r];
+      for (int e = 0; e < 8; ++e) {
+        float v = col[p][e];
         v += shfl_xor_f(v, 1);
         v += shfl_xor_f(v, 2);
         v += shfl_xor_f(v, 4);
         v += shfl_xor_f(v, 8);
-        col[i][r] = v;
+        if ((w.lane & 15) == 0) sh[w.wm * G::BN + w.col(p) - w.n0 + e] = v;
       }
-      if ((lane & 15) == 0) sh[wm * (G::BN / 4) + (wn * G::FN + i) * 4 + (lane >> 4)] = col[i];
-    }
     __syncthreads();
-    const float* flat = reinterpret_cast<const float*>(lds);
     for (int c = threadIdx.x; c < G::BN; c += G::threads) {
-      if (n0 + c >= n) continue;
+      if (w.n0 + c >= n) continue;
       float v = 0;
 #pragma unroll
-      for (int w = 0; w < G::WM; ++w) v += flat[w * G::BN + c];
-      dbias_part[(int64_t)tm * n + n0 + c] = v;
+      for (int k = 0; k < G::WM; ++k) v += sh[k * G::BN + c];
+      dbias_part[(int64_t)w.tm * n + w.n0 + c] = v;
     }
   }
 };

@@ -34,6 +34,30 @@ __device__ __forceinline__ void store4(float* p, f32x4 v) { *reinterpret_cast<f3
 __device__ __forceinline__ void store4(bf16* p, f32x4 v) {
   *reinterpret_cast<bf16x4u*>(p) = __builtin_convertvector(v, bf16x4);
 }
+struct f32x8 {
+  f32x4 lo, hi;
+  __device__ float operator[](int i) const { return i < 4 ? lo[i] : hi[i - 4]; }
+  __device__ void set(int i, float v) {
+    if (i < 4) lo[i] = v;
+    else hi[i - 4] = v;
+  }
+};
+typedef __bf16 bf16x8u __attribute__((ext_vector_type(8), aligned(2)));
+__device__ __forceinline__ f32x8 load8(const float* p) { return {load4(p), load4(p + 4)}; }
+__device__ __forceinline__ f32x8 load8(const bf16* p) {
+  const bf16x8 v = *reinterpret_cast<const bf16x8u*>(p);
+  const bf16x4 lo = {v[0], v[1], v[2], v[3]}, hi = {v[4], v[5], v[6], v[7]};
+  return {__builtin_convertvector(lo, f32x4), __builtin_convertvector(hi, f32x4)};
+}
+__device__ __forceinline__ void store8(float* p, const f32x8& v) {
+  store4(p, v.lo);
+  store4(p + 4, v.hi);
+}
+__device__ __forceinline__ bf16x8 to_bf16x8(const f32x8& v) {
+  const bf16x4 lo = __builtin_convertvector(v.lo, bf16x4), hi = __builtin_convertvector(v.hi, bf16x4);
+  return bf16x8{lo[0], lo[1], lo[2], lo[3], hi[0], hi[1], hi[2], hi[3]};
+}
+__device__ __forceinline__ void store8(bf16* p, const f32x8& v) { *reinterpret_cast<bf16x8u*>(p) = to_bf16x8(v); }
 // The first `n` (1 to 4) of them; the others read as zero and are not written.
 template <class T>
 __device__ __forceinline__ f32x4 load4_n(const T* p, int n) {
@@ -108,12 +132,18 @@ typedef __attribute__((address_space(3))) char lds_char;
 // rows of a fragment read spread over the banks.  k strided: 64 rows of R elements, read with the transposing LDS load,
 // in which 16 lanes read four rows of 32 bytes; chunk pairs are permuted by the row's low bits so that those rows, and
 // the ones eight further that the next 16 lanes read, lie in different banks.
-template <bool KC, int CHUNKS>
+// Rows of a B fragment are taken in the order b_row (below): their low bits differ elsewhere.
+template <bool KC, bool ISB, int CHUNKS>
 __device__ __forceinline__ int tile_swizzle(int row) {
+  if constexpr (KC && ISB) return (row & 3) | (((row >> 3) & 1) << 2);
   if constexpr (KC) return row & 7;
   return (2 * ((row & 3) | (((row >> 3) & 1) << 2))) & (CHUNKS - 1);
 }
-template <int R, int NT, bool KC>
+// Row i of fragment f of the B operand is n = 32 (f / 2) + 8 (i / 4) + 4 (f % 2) + i % 4: a lane's two accumulators of a
+// fragment pair (rows 4 (lane / 16) + r of each) are then eight consecutive columns, one 16-byte bf16 store.
+__device__ __forceinline__ int b_row(int f, int i) { return 32 * (f >> 1) + 8 * (i >> 2) + 4 * (f & 1) + (i & 3); }
+
+template <int R, int NT, bool KC, bool ISB>
 struct TileLoad {
   static constexpr int row_bytes = KC ? kGemmBK * 2 : R * 2;
   static constexpr int rows = KC ? R : kGemmBK;
@@ -129,7 +159,7 @@ struct TileLoad {
 
   __device__ void init(int64_t ld, int tid) {
     const int row = tid / chunks, slot = tid % chunks;
-    const int chunk = slot ^ tile_swizzle<KC, chunks>(row);
+    const int chunk = slot ^ tile_swizzle<KC, ISB, chunks>(row);
     voff = (uint32_t)((int64_t)row * ld * 2) + chunk * 16;
     vstep = (uint32_t)((int64_t)rows_a_load * ld * 2);
     kc = chunk * 8;
@@ -157,28 +187,33 @@ struct TileLoad {
 };
 
 // A lane's fragments of 16 rows x 32 k (k half kk of the 64) from the tile at `lds`.
-template <int R, bool KC>
+template <int R, bool KC, bool ISB>
 struct TileRead {
-  uint32_t base;  // k contiguous: address of (row l % 16, chunk l / 16); strided: in-row part and row part apart
-  uint32_t rowp;
+  uint32_t base;  // k contiguous: address of the lane's row and chunk in fragment 0; strided: the in-row part
+  uint32_t rowp;  // strided: the row's part
   __device__ void init(int lane, int first_row) {
+    const int i = lane & 15, g = lane >> 4;
     if constexpr (KC) {
-      base = (first_row + (lane & 15)) * 128 + (((lane >> 4) ^ (lane & 7)) * 16);
+      const int row = ISB ? b_row(0, i) : i;
+      base = (first_row + row) * 128 + ((g ^ tile_swizzle<KC, ISB, 8>(row)) * 16);
       rowp = 0;
     } else {
-      const int i = lane & 15, g = lane >> 4;
-      const int s = tile_swizzle<KC, R / 8>((i >> 2) | (g << 3));
+      const int s = tile_swizzle<KC, ISB, R / 8>((i >> 2) | (g << 3));
       rowp = (g * 8 + (i >> 2)) * R * 2;
-      base = (first_row * 2) ^ (s * 16 + ((i & 3) >> 1) * 16 + (i & 1) * 8);
+      const int in = ISB ? (i & 3) * 16 : ((i & 3) >> 1) * 16 + (i & 1) * 8;
+      base = (first_row * 2) ^ (s * 16) ^ in;
     }
   }
   __device__ __forceinline__ bf16x8 get(const lds_char* lds, int f, int kk) const {
     typedef __attribute__((address_space(3))) const bf16x8 lds_frag;
     typedef __attribute__((address_space(3))) s16x4 lds_half;
     if constexpr (KC) {
-      return *(lds_frag*)(lds + ((base ^ (kk * 64)) + f * 2048));
+      // In B, fragment 1 of a pair starts four rows on, which the permutation does not see.
+      const int rows = ISB ? 32 * (f >> 1) + 4 * (f & 1) : 16 * f;
+      return *(lds_frag*)(lds + ((base ^ (kk * 64)) + rows * 128));
     } else {
-      const uint32_t a = rowp + (base ^ (f * 32)) + kk * 32 * R * 2;
+      const uint32_t in = ISB ? (base ^ ((f >> 1) * 64)) + (f & 1) * 8 : base ^ (f * 32);
+      const uint32_t a = rowp + in + kk * 32 * R * 2;
       const s16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_half*)(lds + a));
       const s16x4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_half*)(lds + a + 4 * R * 2));
       s16x8 v = {lo[0], lo[1], lo[2], lo[3], hi[0], hi[1], hi[2], hi[3]};
@@ -201,7 +236,20 @@ __device__ __forceinline__ void gemm_tile_of(const GemmArgs& g, int wg, int tota
   tn = in / gm;
 }
 
-// acc[fn][fm] element r of a lane: n = 16 fn + 4 (lane / 16) + r, m = 16 fm + lane % 16 of the wave's part.
+// Where a wave's part of a tile lies, for its epilogue.
+template <class T>
+struct GemmWave {
+  int m0, n0;      // the tile's first row and column
+  int tm, tn, sp;  // the tile, and the split
+  int wm, wn, lane;
+  char* lds;       // the wave's own part of the tile buffers, lds_bytes long
+  static constexpr int lds_bytes = 2 * T::stage_bytes / T::waves;
+  __device__ int row(int j) const { return m0 + (wm * T::FM + j) * 16 + (lane & 15); }
+  __device__ int first_col() const { return n0 + wn * T::FN * 16; }
+  __device__ int col(int p) const { return first_col() + 32 * p + 8 * (lane >> 4); }
+};
+// acc[f][j]: a lane holds columns col(p) .. col(p) + 7 of row(j) in acc[2 p][j] and acc[2 p + 1][j].
+
 template <class T, bool AKC, bool BKC, int PAIRS, class Epi>
 __global__ __launch_bounds__(T::threads, T::threads == 512 ? 2 : 1) void gemm_kernel(GemmArgs g, Epi epi) {
   __shared__ __attribute__((aligned(1024))) char s0[T::stage_bytes];
@@ -213,12 +261,12 @@ __global__ __launch_bounds__(T::threads, T::threads == 512 ? 2 : 1) void gemm_ke
   const int m0 = tm * T::BM, n0 = tn * T::BN;
   const int kbeg = sp * g.k_per_split, kend = min(g.k, kbeg + g.k_per_split);
 
-  TileLoad<T::BM, T::threads, AKC> la;
-  TileLoad<T::BN, T::threads, BKC> lb;
+  TileLoad<T::BM, T::threads, AKC, false> la;
+  TileLoad<T::BN, T::threads, BKC, true> lb;
   la.init(g.a.ld, tid);
   lb.init(g.b.ld, tid);
-  TileRead<T::BM, AKC> ra;
-  TileRead<T::BN, BKC> rb;
+  TileRead<T::BM, AKC, false> ra;
+  TileRead<T::BN, BKC, true> rb;
   ra.init(lane, wm * (T::BM / T::WM));
   rb.init(lane, wn * (T::BN / T::WN));
 
@@ -258,18 +306,26 @@ __global__ __launch_bounds__(T::threads, T::threads == 512 ? 2 : 1) void gemm_ke
           acc[i][j] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(fb[i], fa[j], acc[i][j], 0, 0, 0);
     }
   };
+  // Two buffers, each a variable of its own: the compiler then knows that a buffer being read is not the one being
+  // filled and waits for loads only at the barriers.
   if (steps > 0) issue(s0);
-  for (int s = 0; s < steps; s += 2) {
-    __syncthreads();  // stage s has landed; nobody reads the other buffer any more
-    if (s + 1 < steps) issue(s1);
+  int left = steps;
+  for (; left >= 2; left -= 2) {
+    __syncthreads();  // s0 has landed; nobody reads s1 any more
+    issue(s1);
     compute(s0);
-    if (s + 1 >= steps) break;
     __syncthreads();
-    if (s + 2 < steps) issue(s0);
+    if (left > 2) issue(s0);
     compute(s1);
   }
+  if (left) {
+    __syncthreads();
+    compute(s0);
+  }
   __syncthreads();
-  epi.template finish<T>(acc, m0, n0, tm, tn, sp, wm, wn, lane, s0);
+  const int half = T::waves / 2;
+  const GemmWave<T> w{m0, n0, tm, tn, sp, wm, wn, lane, (wave < half ? s0 : s1) + wave % half * (T::stage_bytes / half)};
+  epi.template finish<T>(acc, w, s0);
 }
 
 }  // namespace fgpu
