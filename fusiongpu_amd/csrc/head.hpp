@@ -49,6 +49,20 @@ __device__ __forceinline__ float act_slope(float z, int act) {
   return 1.0f;
 }
 
+// ---- sums across lanes -----------------------------------------------------------
+// Sum over aligned groups of N lanes (16, 32 or 64), the same bits in all of them.  Four exchanges inside a row of 16
+// lanes (pairs, quads, then the mirrored half and the mirrored row, whose sums are already alike), two swaps beyond.
+template <int N>
+__device__ __forceinline__ float lanes_sum(float v) {
+  v += __int_as_float(dpp_mov<0xB1>(__float_as_int(v)));
+  v += __int_as_float(dpp_mov<0x4E>(__float_as_int(v)));
+  v += __int_as_float(dpp_mov<0x141>(__float_as_int(v)));
+  v += __int_as_float(dpp_mov<0x140>(__float_as_int(v)));
+  if constexpr (N >= 32) v += __int_as_float(xchg<16>(__float_as_int(v)));
+  if constexpr (N >= 64) v += __int_as_float(xchg<32>(__float_as_int(v)));
+  return v;
+}
+
 // ---- products (head_gemm.hip) -------------------------------------------------
 // What becomes of D: out = act(alpha D + bias) + residual, with the value before act in `pre`; out and residual [m][n].
 struct Finish {
@@ -96,6 +110,10 @@ fgpu_status launch_pack(const void* src, int64_t rows, int64_t cols, bool f32, c
 // fixed order.
 fgpu_status launch_column_finish(const float* part, int parts, int64_t stride, int64_t cols, bool f32_out, void* out,
                                  hipStream_t s);
+
+// Two such sums in one launch: the second one's parts lie `cols` after the first one's; either result may be NULL.
+fgpu_status launch_column_finish2(const float* part, int parts, int64_t stride, int64_t cols, bool f32_out, void* out0,
+                                  void* out1, hipStream_t s);
 
 inline int ceil_div(int64_t a, int64_t b) { return (int)((a + b - 1) / b); }
 

@@ -200,21 +200,26 @@ __global__ __launch_bounds__(256) void pack_kernel(const T* src, int64_t rows, i
   }
 }
 
-// 64 columns x 16 groups of parts a workgroup.
+// 16 columns x 64 groups of parts a workgroup; blockIdx.y: which of two sums.
+constexpr int kFinishCols = 16, kFinishGroups = 64;
 template <class T>
-__global__ __launch_bounds__(1024) void column_finish_kernel(const float* part, int parts, int64_t stride, int64_t cols, T* out) {
-  __shared__ float sum[16][64];
-  const int64_t c = (int64_t)blockIdx.x * 64 + (threadIdx.x & 63);
-  const int g = threadIdx.x >> 6;
+__global__ __launch_bounds__(1024) void column_finish_kernel(const float* part, int parts, int64_t stride, int64_t cols,
+                                                             T* out0, T* out1) {
+  __shared__ float sum[kFinishGroups][kFinishCols + 1];
+  T* out = blockIdx.y ? out1 : out0;
+  if (!out) return;
+  const int cl = threadIdx.x % kFinishCols, g = threadIdx.x / kFinishCols;
+  const int64_t c = (int64_t)blockIdx.x * kFinishCols + cl;
+  part += blockIdx.y * cols;
   float v = 0;
   if (c < cols)
-    for (int p = g; p < parts; p += 16) v += part[(int64_t)p * stride + c];
-  sum[g][threadIdx.x & 63] = v;
+    for (int p = g; p < parts; p += kFinishGroups) v += part[(int64_t)p * stride + c];
+  sum[g][cl] = v;
   __syncthreads();
-  if (g == 0 && c < cols) {
-    for (int k = 1; k < 16; ++k) v += sum[k][threadIdx.x];
-    out[c] = (T)v;
-  }
+  // one wave a column: its 64 groups across the lanes
+  const int w = threadIdx.x >> 6;
+  v = lanes_sum<64>(sum[threadIdx.x & 63][w]);
+  if ((threadIdx.x & 63) == 0 && (int64_t)blockIdx.x * kFinishCols + w < cols) out[(int64_t)blockIdx.x * kFinishCols + w] = (T)v;
 }
 
 }  // namespace
@@ -257,14 +262,20 @@ fgpu_status launch_pack(const void* src, int64_t rows, int64_t cols, bool f32, c
   return FGPU_OK;
 }
 
-fgpu_status launch_column_finish(const float* part, int parts, int64_t stride, int64_t cols, bool f32_out, void* out,
-                                 hipStream_t s) {
+fgpu_status launch_column_finish2(const float* part, int parts, int64_t stride, int64_t cols, bool f32_out, void* out0,
+                                  void* out1, hipStream_t s) {
+  const dim3 grid(ceil_div(cols, kFinishCols), out1 ? 2 : 1);
   if (f32_out)
-    column_finish_kernel<float><<<ceil_div(cols, 64), 1024, 0, s>>>(part, parts, stride, cols, (float*)out);
+    column_finish_kernel<float><<<grid, 1024, 0, s>>>(part, parts, stride, cols, (float*)out0, (float*)out1);
   else
-    column_finish_kernel<bf16><<<ceil_div(cols, 64), 1024, 0, s>>>(part, parts, stride, cols, (bf16*)out);
+    column_finish_kernel<bf16><<<grid, 1024, 0, s>>>(part, parts, stride, cols, (bf16*)out0, (bf16*)out1);
   FGPU_HIP(hipGetLastError());
   return FGPU_OK;
+}
+
+fgpu_status launch_column_finish(const float* part, int parts, int64_t stride, int64_t cols, bool f32_out, void* out,
+                                 hipStream_t s) {
+  return launch_column_finish2(part, parts, stride, cols, f32_out, out, nullptr, s);
 }
 
 }  // namespace fgpu
