@@ -26,6 +26,7 @@ from __future__ import annotations
 import contextlib
 import ctypes
 import os
+import sys
 
 import numpy as np
 
@@ -176,10 +177,14 @@ def _np_ptr(a: np.ndarray):
 
 
 # --------------------------------------------------------------------------- torch plumbing
-def _torch():
-    import torch  # noqa: PLC0415 -- only needed for device buffers
-    return torch
+_TORCH = sys.modules["torch"]  # _load imported it
 
+
+def _torch():
+    return _TORCH
+
+
+_raw_stream = getattr(_torch()._C, "_cuda_getCurrentRawStream", None)
 
 FAULT_ID = -2  # FGPU_FAULT_ID: every slot of a query a bounded-wait give-up may have touched
 
@@ -207,7 +212,10 @@ def _on(stream):
 
 def _stream():
     """hipStream_t of torch's current stream (the one _on made current)."""
-    return _vp(_torch().cuda.current_stream().cuda_stream)
+    cuda = _torch().cuda
+    if _raw_stream is not None:  # the handle without building a Stream object around it (3 us a call)
+        return _vp(_raw_stream(cuda.current_device()))
+    return _vp(cuda.current_stream().cuda_stream)
 
 
 def _workspace(nbytes: int):
@@ -984,7 +992,7 @@ def _act_code(act):
 def _head_first(a, name):
     """The array that decides a call's type, as a contiguous 16-byte-aligned device matrix."""
     torch = _torch()
-    if not (torch.is_tensor(a) and a.dtype == torch.bfloat16):
+    if not (torch.is_tensor(a) and (a.dtype is torch.bfloat16 or a.dtype is torch.float32)):
         a = _arg(a, torch.float32, name, (None, None))
     return _head(a, a.dtype, name, (None, None))
 
@@ -996,12 +1004,13 @@ def _head(a, dtype, name, shape):
         a = torch.from_numpy(np.ascontiguousarray(a))
     elif not torch.is_tensor(a):
         raise TypeError(f"{name}: expected a numpy array or a torch tensor, got {type(a).__name__}")
-    if a.dtype != dtype:
+    if a.dtype is not dtype:
         raise TypeError(f"{name}: dtype {str(a.dtype).replace('torch.', '')}, expected "
                         f"{str(dtype).replace('torch.', '')} as the call's other arrays have")
-    if a.dim() != len(shape) or any(w is not None and g != w for g, w in zip(a.shape, shape)):
+    have = a.shape
+    if have != shape and (len(have) != len(shape) or any(w is not None and g != w for g, w in zip(have, shape))):
         want = ["any" if w is None else w for w in shape]
-        raise ValueError(f"{name}: shape {tuple(a.shape)}, expected {want}")
+        raise ValueError(f"{name}: shape {tuple(have)}, expected {want}")
     if not a.is_cuda:
         a = a.to("cuda")
     if not a.is_contiguous():
@@ -1019,8 +1028,22 @@ def _ptr(t):
 
 def _head_out(out, like, shape, name="out"):
     if out is None:
-        return _torch().empty(shape, dtype=like.dtype, device=like.device)
+        return like.new_empty(shape)
     return _out(out, like.dtype, shape, name)
+
+
+def _head_ws(nbytes, like):
+    """(pointer, bytes, the tensor that holds them) of a call's workspace; nothing is allocated where none is needed."""
+    if not nbytes:
+        return None, 0, None
+    ws = _torch().empty(nbytes, dtype=_torch().uint8, device=like.device)
+    return ws.data_ptr(), nbytes, ws
+
+
+def _two_floats(rows, like):
+    torch = _torch()
+    return (torch.empty(rows, dtype=torch.float32, device=like.device),
+            torch.empty(rows, dtype=torch.float32, device=like.device))
 
 
 def _dtype_code(t):
@@ -1042,9 +1065,9 @@ def linear(x, weight, bias=None, residual=None, act: str = "none", save_pre: boo
         y = _head_out(out, x, (rows, n))
         pre = _head_out(None, x, (rows, n)) if save_pre else None
         dt = _dtype_code(x)
-        ws = _workspace(lib.fgpu_linear_workspace_bytes(rows, k, n, dt))
+        wp, wb, ws = _head_ws(lib.fgpu_linear_workspace_bytes(rows, k, n, dt), x)
         _check(lib.fgpu_linear(x.data_ptr(), w.data_ptr(), _ptr(b), _ptr(r), rows, k, n, dt, code, y.data_ptr(), _ptr(pre),
-                               ws.data_ptr(), ws.numel(), _stream()))
+                               wp, wb, _stream()))
     return (y, pre) if save_pre else y
 
 
@@ -1067,22 +1090,21 @@ def linear_backward(dy, x, weight, pre=None, act: str = "none", want=("x", "weig
         dw = _head_out(None, dy, (n, k)) if "weight" in want else None
         db = _head_out(None, dy, (n,)) if "bias" in want else None
         dt = _dtype_code(dy)
-        ws = _workspace(lib.fgpu_linear_backward_workspace_bytes(rows, k, n, dt))
+        wp, wb, ws = _head_ws(lib.fgpu_linear_backward_workspace_bytes(rows, k, n, dt), dy)
         _check(lib.fgpu_linear_backward(dy.data_ptr(), x.data_ptr(), w.data_ptr(), _ptr(z), rows, k, n, dt, code, _ptr(dx),
-                                        _ptr(dw), _ptr(db), ws.data_ptr(), ws.numel(), _stream()))
+                                        _ptr(dw), _ptr(db), wp, wb, _stream()))
     return dx, dw, db
 
 
 def layer_norm(x, gamma=None, beta=None, eps: float = 1e-5, out=None, stream=None):
     """Layer norm over the rows of x [rows][dim] (fgpu_layer_norm): (y, mean, rstd), the last two float32 [rows] for
     layer_norm_backward."""
-    torch = _torch()
     with _on(stream):
         x = _head_first(x, "x")
         (rows, dim), t = x.shape, x.dtype
         g, b = _head_opt(gamma, t, "gamma", (dim,)), _head_opt(beta, t, "beta", (dim,))
         y = _head_out(out, x, (rows, dim))
-        mean, rstd = torch.empty((2, rows), dtype=torch.float32, device=x.device).unbind()
+        mean, rstd = _two_floats(rows, x)
         _check(lib.fgpu_layer_norm(x.data_ptr(), _ptr(g), _ptr(b), rows, dim, _dtype_code(x), eps, y.data_ptr(),
                                    mean.data_ptr(), rstd.data_ptr(), _stream()))
     return y, mean, rstd
@@ -1098,15 +1120,22 @@ def layer_norm_backward(dy, x, gamma, mean, rstd, want=("x", "gamma", "beta"), s
         (rows, dim), t = dy.shape, dy.dtype
         x = _head(x, t, "x", (rows, dim))
         g = _head_opt(gamma, t, "gamma", (dim,))
-        mean, rstd = _dev(mean, torch.float32, "mean", (rows,)), _dev(rstd, torch.float32, "rstd", (rows,))
+        mean, rstd = _row(mean, torch.float32, "mean", rows), _row(rstd, torch.float32, "rstd", rows)
         dx = _head_out(None, dy, (rows, dim)) if "x" in want else None
         dg = _head_out(None, dy, (dim,)) if "gamma" in want else None
         db = _head_out(None, dy, (dim,)) if "beta" in want else None
         dt = _dtype_code(dy)
-        ws = _workspace(lib.fgpu_layer_norm_backward_workspace_bytes(rows, dim, dt))
+        wp, wb, ws = _head_ws(lib.fgpu_layer_norm_backward_workspace_bytes(rows, dim, dt), dy)
         _check(lib.fgpu_layer_norm_backward(dy.data_ptr(), x.data_ptr(), _ptr(g), mean.data_ptr(), rstd.data_ptr(), rows,
-                                            dim, dt, _ptr(dx), _ptr(dg), _ptr(db), ws.data_ptr(), ws.numel(), _stream()))
+                                            dim, dt, _ptr(dx), _ptr(dg), _ptr(db), wp, wb, _stream()))
     return dx, dg, db
+
+
+def _row(a, dtype, name, n):
+    """_dev of a vector of n, without its conversions where nothing is to convert."""
+    if getattr(a, "dtype", None) is dtype and a.shape == (n,) and a.is_cuda and a.is_contiguous():
+        return a
+    return _dev(a, dtype, name, (n,))
 
 
 def _loss_args(queries, candidates, targets, bias, ids):
@@ -1115,9 +1144,9 @@ def _loss_args(queries, candidates, targets, bias, ids):
     nq, dim = q.shape
     c = _head(candidates, q.dtype, "candidates", (None, dim))
     nc = c.shape[0]
-    t = _dev(targets, torch.int32, "targets", (nq,))
-    b = None if bias is None else _dev(bias, torch.float32, "bias", (nc,))
-    i = None if ids is None else _dev(ids, torch.int32, "ids", (nc,))
+    t = _row(targets, torch.int32, "targets", nq)
+    b = None if bias is None else _row(bias, torch.float32, "bias", nc)
+    i = None if ids is None else _row(ids, torch.int32, "ids", nc)
     return q, c, t, b, i, nq, nc, dim, _dtype_code(q)
 
 
@@ -1126,13 +1155,12 @@ def contrastive_loss(queries, candidates, targets, scale: float = 1.0, bias=None
     targets_i}.  queries [nq][dim], candidates [nc][dim], targets int32 [nq] (outside [0, nc): the row is ignored), bias
     float32 [nc] (-inf masks a candidate; -scale |c|^2 / 2 makes the scores the index's L2 metric), ids int32 [nc]
     (copies of the target's document are left out).  Returns (loss, lse), float32 [nq]."""
-    torch = _torch()
     with _on(stream):
         q, c, t, b, i, nq, nc, dim, dt = _loss_args(queries, candidates, targets, bias, ids)
-        loss, lse = torch.empty((2, nq), dtype=torch.float32, device=q.device).unbind()
-        ws = _workspace(lib.fgpu_contrastive_loss_workspace_bytes(nq, nc, dim, dt))
+        loss, lse = _two_floats(nq, q)
+        wp, wb, ws = _head_ws(lib.fgpu_contrastive_loss_workspace_bytes(nq, nc, dim, dt), q)
         _check(lib.fgpu_contrastive_loss(q.data_ptr(), c.data_ptr(), t.data_ptr(), _ptr(b), _ptr(i), nq, nc, dim, dt, scale,
-                                         loss.data_ptr(), lse.data_ptr(), ws.data_ptr(), ws.numel(), _stream()))
+                                         loss.data_ptr(), lse.data_ptr(), wp, wb, _stream()))
     return loss, lse
 
 
@@ -1144,7 +1172,7 @@ def contrastive_loss_backward(dloss, queries, candidates, targets, lse, scale: f
     torch = _torch()
     with _on(stream):
         q, c, t, b, i, nq, nc, dim, dt = _loss_args(queries, candidates, targets, bias, ids)
-        g, lse = _dev(dloss, torch.float32, "dloss", (nq,)), _dev(lse, torch.float32, "lse", (nq,))
+        g, lse = _row(dloss, torch.float32, "dloss", nq), _row(lse, torch.float32, "lse", nq)
         dq = _head_out(None, q, (nq, dim))
         dc = _head_out(None, q, (nc, dim)) if candidate_grads else None
         db = torch.empty(nc, dtype=torch.float32, device=q.device) if candidate_grads else None

@@ -5,6 +5,8 @@
 
 namespace fgpu {
 
+inline int ceil_div(int64_t a, int64_t b) { return (int)((a + b - 1) / b); }
+
 // ---- activations -------------------------------------------------------------
 // gelu(z) = z Phi(z).  Phi's tail T(|z|) = 1 - Phi(|z|) is the rational form 7.1.26 of Abramowitz and Stegun's handbook,
 // erfc(x) = t (a1 + t (a2 + ...)) exp(-x^2) with t = 1 / (1 + p x), whose error stays below 1.5e-7 (under a float32 ulp
@@ -72,11 +74,26 @@ struct Finish {
   void* pre = nullptr;
   float alpha = 1.0f;
   int act = FGPU_ACT_NONE;
+  bool stream = false;  // results past the caches (launch_products decides)
   // Products added up over several calls (Product::chunked): D += add before the rest, and `sum` takes D in place of the
   // result; both [m][n rounded up to 4] float32.
   const float* add = nullptr;
   float* sum = nullptr;
 };
+
+// out = act(alpha D + bias) + residual for four consecutive columns n .. n + 3 of row m (cnt of them inside).
+template <class T>
+__device__ __forceinline__ void finish4(const Finish& f, f32x4 v, int64_t at, int n, int cnt) {
+  v *= f.alpha;
+  if (f.bias) v += load4_n((const T*)f.bias + n, cnt);
+  if (f.pre) store4_n((T*)f.pre + at, v, cnt);
+  if (f.act != FGPU_ACT_NONE) {
+#pragma unroll
+    for (int r = 0; r < 4; ++r) v[r] = act_value(v[r], f.act);
+  }
+  if (f.residual) v += load4_n((const T*)f.residual + at, cnt);
+  store4_n((T*)f.out + at, v, cnt);
+}
 
 // A product of m x n over k, of bf16 operands and results, or (f32) of split planes and float32 results.
 struct Product {
@@ -84,10 +101,26 @@ struct Product {
   bool f32;
   bool chunked = false;
 };
-size_t product_workspace_bytes(const Product& p);
-// `ws`: product_workspace_bytes.
-fgpu_status launch_product(const Product& p, const GemmOperand& a, bool a_kc, const GemmOperand& b, bool b_kc,
-                           const Finish& f, void* ws, hipStream_t s);
+// One product and where its result goes.
+struct ProductJob {
+  Product p;
+  GemmOperand a, b;
+  bool a_kc, b_kc;
+  Finish f;
+};
+// out[c] = sum over the parts of part[p * stride + c], c < cols, added in a fixed order; f32 0: rounded to bf16.
+struct ColumnSum {
+  const float* part = nullptr;
+  int parts = 0;
+  int64_t stride = 0, cols = 0;
+  void* out = nullptr;
+  int f32 = 1;
+};
+// The products (one, or an input's gradient followed by a weight's), then what joins split products and the column sums
+// (NULL: none): one launch for the products where they are small, one to join where there is something to join.
+size_t products_workspace_bytes(const Product* p, int count);
+fgpu_status launch_products(const ProductJob* jobs, int count, const ColumnSum* sums, void* ws, hipStream_t s);
+double products_estimate_us(const Product* p, int count);  // the time that the rule between kernels goes by
 
 // An array as an operand: itself where its rows can be read as they are (bf16, cols % 8 == 0), otherwise a copy with
 // rows of packed_ld(cols) elements, float32 as three planes.
@@ -100,21 +133,74 @@ inline GemmOperand as_is(const void* p, int64_t cols) { return {static_cast<cons
 inline GemmOperand packed(void* p, int64_t rows, int64_t cols) {
   return {static_cast<uint16_t*>(p), packed_ld(cols), rows * packed_ld(cols)};
 }
-// Copies src [rows][cols] to `dst`.  zero_bias (NULL: no row): rows whose bias masks them become zero; zero_target: rows
-// whose target lies outside [0, nc) do.
-fgpu_status launch_pack(const void* src, int64_t rows, int64_t cols, bool f32, const GemmOperand& dst,
-                        const float* zero_bias, const int32_t* zero_target, int nc, hipStream_t s);
+// ---- what comes before the products, in one launch (head_prep.hip) ---------------------
+// What the contrastive loss's backward pass needs of a row: lse in units of log 2 and its weight; a row without a gradient
+// (no target, a masked one, nothing left) has weight 0 and an infinite lse, so its score gradient is zero.
+struct LossRows {
+  const float* bias;
+  const int32_t* target;
+  const float* lse;
+  const float* dloss;
+  int nq, nc;
+  f32x2* rows;
+  int32_t* live_target;
+};
+// A copy of src [rows][cols] as an operand; rows that a mask takes out become zero.
+struct CopyJob {
+  const void* src = nullptr;
+  int64_t rows = 0, cols = 0;
+  GemmOperand dst{};
+  const float* row_bias = nullptr;  // zero: rows whose bias masks them
+  bool loss_rows = false;           // zero: rows without a gradient
+};
+// dz = dy act'(pre) as an operand (dst.p NULL: not stored) and the column sums of dz, part [chunk][cols] (NULL: none).
+struct DzJob {
+  const void* dy = nullptr;
+  const void* pre = nullptr;
+  int act = 0, rows = 0, cols = 0, chunks = 0;
+  GemmOperand dst{};
+  float* part = nullptr;
+};
+int dz_chunks(int rows, int cols);
+struct Prep {
+  CopyJob copy[2];
+  DzJob dz;
+  LossRows loss{};
+};
+fgpu_status launch_prep(const Prep& p, bool f32, hipStream_t s);
+
+// ---- products of few tiles (head_direct.hip) ---------------------------------------
+// An operand as the caller's array holds it: rows of ld elements, `count` elements in all.  With `pre`, each element is
+// multiplied by the activation's slope at pre's (dz from dy).
+struct DirectOperand {
+  const void* p;
+  int64_t ld, count;
+  const void* pre;
+};
+struct DirectJob {
+  DirectOperand a, b;
+  int m, n, k;
+  int act;           // of `pre`
+  Finish f;
+  void* column_sum;  // both operands strided: gets the sums of a over k, [m] (NULL: not wanted)
+};
+// D = A B^T, both with k contiguous.
+fgpu_status launch_direct_forward(const DirectJob& j, bool f32, hipStream_t s);
+// In one launch: x (A with k contiguous, B strided), w (both strided); either may be NULL.
+fgpu_status launch_direct_backward(const DirectJob* x, const DirectJob* w, bool f32, hipStream_t s);
+// The times that the rule between these and the tiled products goes by.
+double direct_forward_estimate_us(const Product& p);
+double direct_backward_estimate_us(int rows, int in_dim, int out_dim, bool f32);
 
 // ---- column sums ---------------------------------------------------------------
-// out[c] = sum over the parts of part[p * stride + c], c < cols, rounded to the result's type; parts are added in a
-// fixed order.
-fgpu_status launch_column_finish(const float* part, int parts, int64_t stride, int64_t cols, bool f32_out, void* out,
-                                 hipStream_t s);
+// Two sums of the same length, the second one's parts `cols` after the first one's; either result may be NULL.
+fgpu_status launch_column_sums(const ColumnSum& c, void* out1, hipStream_t s);
+// Zeros, as the sums over no rows.
+inline fgpu_status launch_no_sums(int64_t cols, bool f32, void* out, hipStream_t s) {
+  ColumnSum c;
+  c.cols = cols, c.out = out, c.f32 = f32;
+  return launch_column_sums(c, nullptr, s);
+}
 
-// Two such sums in one launch: the second one's parts lie `cols` after the first one's; either result may be NULL.
-fgpu_status launch_column_finish2(const float* part, int parts, int64_t stride, int64_t cols, bool f32_out, void* out0,
-                                  void* out1, hipStream_t s);
-
-inline int ceil_div(int64_t a, int64_t b) { return (int)((a + b - 1) / b); }
 
 }  // namespace fgpu

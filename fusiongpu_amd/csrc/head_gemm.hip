@@ -1,24 +1,10 @@
-// head_gemm.hip -- products with a fused epilogue, the packing of their operands and the last step of column sums.
+// head_gemm.hip -- products with a fused epilogue, and what joins split ones and column sums.
 #include <algorithm>
 
 #include "head.hpp"
 
 namespace fgpu {
 namespace {
-
-// out = act(alpha D + bias) + residual for four consecutive columns n .. n + 3 of row m (cnt of them inside).
-template <class T>
-__device__ __forceinline__ void finish4(const Finish& f, f32x4 v, int64_t at, int n, int cnt) {
-  v *= f.alpha;
-  if (f.bias) v += load4_n((const T*)f.bias + n, cnt);
-  if (f.pre) store4_n((T*)f.pre + at, v, cnt);
-  if (f.act != FGPU_ACT_NONE) {
-#pragma unroll
-    for (int r = 0; r < 4; ++r) v[r] = act_value(v[r], f.act);
-  }
-  if (f.residual) v += load4_n((const T*)f.residual + at, cnt);
-  store4_n((T*)f.out + at, v, cnt);
-}
 
 template <class T, int ACT>
 struct ProductEpi {
@@ -51,6 +37,12 @@ struct ProductEpi {
       }
       return;
     }
+    f.stream ? rows<true>(acc, w) : rows<false>(acc, w);
+  }
+  // STREAM: results past the caches.  (A test at each store would be merged away, and the hint with it.)
+  template <bool STREAM, class G>
+  __device__ __forceinline__ void rows(f32x4 (&acc)[G::FN][G::FM], const GemmWave<G>& w) const {
+    constexpr int P = G::FN / 2;
     f32x8 bias[P];
 #pragma unroll
     for (int p = 0; p < P; ++p) bias[p] = f.bias ? load8((const T*)f.bias + w.col(p)) : f32x8{{0, 0, 0, 0}, {0, 0, 0, 0}};
@@ -63,7 +55,7 @@ struct ProductEpi {
         f32x8 v;
 #pragma unroll
         for (int e = 0; e < 8; ++e) v.set(e, fmaf(acc[2 * p + e / 4][j][e % 4], f.alpha, bias[p][e]));
-        if (f.pre) store8((T*)f.pre + at + 32 * p, v);
+        if (f.pre) put<STREAM>((T*)f.pre + at + 32 * p, v);
         if (ACT != FGPU_ACT_NONE) {
 #pragma unroll
           for (int e = 0; e < 8; ++e) v.set(e, act_value(v[e], ACT));
@@ -72,9 +64,14 @@ struct ProductEpi {
           const f32x8 r = load8((const T*)f.residual + at + 32 * p);
           v.lo += r.lo, v.hi += r.hi;
         }
-        store8((T*)f.out + at + 32 * p, v);
+        put<STREAM>((T*)f.out + at + 32 * p, v);
       }
     }
+  }
+  template <bool STREAM>
+  __device__ static __forceinline__ void put(T* p, const f32x8& v) {
+    if constexpr (STREAM) stream8(p, v);
+    else store8(p, v);
   }
   // The wave holds the last columns: through LDS, four columns a lane, so the code that minds the edge stands once.
   template <class G>
@@ -111,38 +108,105 @@ struct ProductEpi {
 };
 
 // Adds the parts of a split product in order and finishes it: one thread four columns.
+struct SplitJob {
+  const float* part = nullptr;
+  int m = 0, n = 0, splits = 0;
+  Finish f;
+};
 template <class T>
-__global__ __launch_bounds__(256) void split_finish_kernel(const float* part, int m, int n, int splits, Finish f) {
-  const int n4 = (n + 3) >> 2;
-  const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x, total = (int64_t)m * n4;
+__device__ __forceinline__ void split_finish(const SplitJob& j, int block) {
+  const int n4 = (j.n + 3) >> 2;
+  const int64_t i = (int64_t)block * 256 + threadIdx.x, total = (int64_t)j.m * n4;
   if (i >= total) return;
   const int64_t row = i / n4;
   const int col = (int)(i - row * n4) * 4;
   f32x4 v = {0, 0, 0, 0};
-  if (f.add) v = *reinterpret_cast<const f32x4*>(f.add + i * 4);
-  for (int s = 0; s < splits; ++s) v += *reinterpret_cast<const f32x4*>(part + ((int64_t)s * total + i) * 4);
-  if (f.sum)
-    *reinterpret_cast<f32x4*>(f.sum + i * 4) = v;
+  if (j.f.add) v = *reinterpret_cast<const f32x4*>(j.f.add + i * 4);
+#pragma unroll 4
+  for (int s = 0; s < j.splits; ++s) v += *reinterpret_cast<const f32x4*>(j.part + ((int64_t)s * total + i) * 4);
+  if (j.f.sum)
+    *reinterpret_cast<f32x4*>(j.f.sum + i * 4) = v;
   else
-    finish4<T>(f, v, row * n + col, col, n - col);
+    finish4<T>(j.f, v, row * j.n + col, col, j.n - col);
+}
+
+// 16 columns x 16 groups of parts a workgroup.
+constexpr int kSumCols = 16, kSumGroups = 16;
+__device__ __forceinline__ void column_sum(const ColumnSum& c, const float* part, void* out, int block) {
+  __shared__ float sum[kSumGroups][kSumCols + 1];
+  const int cl = threadIdx.x % kSumCols, g = threadIdx.x / kSumCols;
+  const int64_t col = (int64_t)block * kSumCols + cl;
+  float v = 0;
+  if (col < c.cols)
+#pragma unroll 4
+    for (int p = g; p < c.parts; p += kSumGroups) v += part[(int64_t)p * c.stride + col];
+  sum[g][cl] = v;
+  __syncthreads();
+  if (g == 0 && col < c.cols) {
+#pragma unroll
+    for (int k = 1; k < kSumGroups; ++k) v += sum[k][cl];
+    if (c.f32) ((float*)out)[col] = v;
+    else ((bf16*)out)[col] = (bf16)v;
+  }
+}
+__global__ __launch_bounds__(256) void column_sum_kernel(ColumnSum c, void* out1) {
+  void* out = blockIdx.y ? out1 : c.out;
+  if (out) column_sum(c, c.part + blockIdx.y * c.cols, out, blockIdx.x);
+}
+
+// What is left after the products, in one launch: the joining of up to two split ones, and column sums.
+template <class T>
+__global__ __launch_bounds__(256) void join_kernel(SplitJob a, int a_blocks, SplitJob b, int b_blocks, ColumnSum c) {
+  const int k = blockIdx.x;
+  if (k < a_blocks)
+    split_finish<T>(a, k);
+  else if (k < a_blocks + b_blocks)
+    split_finish<T>(b, k - a_blocks);
+  else
+    column_sum(c, c.part, c.out, k - a_blocks - b_blocks);
 }
 
 struct Plan {
   int tile, tiles_m, tiles_n, splits, k_per_split;
+  double us;
 };
-Plan plan_of(const Product& p) {
-  Plan q;
-  auto tiles = [&](int t) { return (int64_t)ceil_div(p.m, t) * ceil_div(p.n, t); };
-  q.tile = tiles(256) >= 192 ? 256 : tiles(128) >= 256 ? 128 : 64;
-  q.tiles_m = ceil_div(p.m, q.tile);
-  q.tiles_n = ceil_div(p.n, q.tile);
-  const int64_t t = (int64_t)q.tiles_m * q.tiles_n;
-  const int steps = ceil_div(p.k, kGemmBK);
-  int64_t want = q.tile == 256 ? 1 : std::max<int64_t>(1, 512 / t);
-  want = std::min<int64_t>(want, std::max(1, steps / 4));
-  q.k_per_split = ceil_div(steps, want) * kGemmBK;
+// Microseconds of a product on `tile` tiles with k in `splits` parts.  A workgroup's k step takes `alone` while few share
+// a CU and `shared` for each that does (measured: 256 x 256 1.6 / 1.6 at one a CU, 128 x 128 0.64 / 0.5 at two, 64 x 64
+// 0.35 / 0.21 at five), its start and epilogue `fixed`; the parts of a split product are written and read once more.
+Plan plan_at(const Product& p, int tile, int splits) {
+  Plan q{tile, ceil_div(p.m, tile), ceil_div(p.n, tile), splits, 0, 0};
+  const int steps = ceil_div(p.k, kGemmBK), per = ceil_div(steps, splits);
+  q.k_per_split = per * kGemmBK;
   q.splits = ceil_div(p.k, q.k_per_split);
+  const double alone = tile == 256 ? 1.6 : tile == 128 ? 0.64 : 0.35, shared = tile == 256 ? 1.6 : tile == 128 ? 0.5 : 0.21;
+  const double fixed = tile == 256 ? 8 : tile == 128 ? 4 : 3;
+  const int most = tile == 256 ? 1 : tile == 128 ? 2 : 5;
+  const int64_t wgs = (int64_t)q.tiles_m * q.tiles_n * q.splits, full = wgs / (256 * most), rest = wgs % (256 * most);
+  const double k = (double)per * (p.f32 ? 6 : 1);
+  q.us = full * (k * std::max(alone, most * shared) + fixed);
+  if (rest) q.us += k * std::max(alone, ceil_div(rest, 256) * shared) + fixed;
+  if (q.splits > 1) q.us += 3 + 8.0 * q.splits * p.m * ((p.n + 3) & ~3) / 6e6;
   return q;
+}
+Plan plan_of(const Product& p, int only = 0) {
+  Plan best{};
+  for (int tile : {256, 128, 64}) {
+    if (only && tile != only) continue;
+    for (int splits : {1, 2, 3, 4, 6, 8, 12, 16, 24, 32, 48, 64}) {
+      if (splits > 1 && splits > ceil_div(p.k, 2 * kGemmBK)) break;
+      const Plan q = plan_at(p, tile, splits);
+      if (!best.tile || q.us < best.us) best = q;
+    }
+  }
+  return best;
+}
+// Two products run in one launch where both take the smaller tiles; the tile is then one for both.
+int plans_of(const Product* p, int count, Plan* q) {
+  for (int i = 0; i < count; ++i) q[i] = plan_of(p[i]);
+  if (count == 1 || q[0].tile == 256 || q[1].tile == 256) return 0;
+  const int tile = std::min(q[0].tile, q[1].tile);
+  for (int i = 0; i < count; ++i) q[i] = plan_of(p[i], tile);
+  return tile;
 }
 
 template <class T, bool AKC, bool BKC, int PAIRS, class E>
@@ -169,113 +233,88 @@ fgpu_status run_form(bool a_kc, bool b_kc, int tile, const GemmArgs& g, const Fi
   return run_tile<true, true, PAIRS>(tile, g, ProductEpi<T, FGPU_ACT_SILU>{f, part, g.m, g.n}, s);
 }
 
-template <class T>
-__device__ __forceinline__ bool row_is_zero(int64_t r, const float* zb, const int32_t* zt, int nc) {
-  return (zb && zb[r] <= FGPU_MASK_BIAS) || (zt && (uint32_t)zt[r] >= (uint32_t)nc);
+size_t parts_bytes(const Product& p, const Plan& q) {
+  return q.splits > 1 || p.chunked ? carve_bytes<float>((size_t)q.splits * p.m * ((p.n + 3) & ~3)) : 0;
 }
 
-// One thread four columns of a row.
-template <class T>
-__global__ __launch_bounds__(256) void pack_kernel(const T* src, int64_t rows, int64_t cols, int64_t ldp, int64_t plane,
-                                                   uint16_t* dst, const float* zb, const int32_t* zt, int nc) {
-  const int64_t per = ldp / 4, total = rows * per;
-  for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < total; i += (int64_t)gridDim.x * 256) {
-    const int64_t r = i / per, c = (i - r * per) * 4;
-    f32x4 v = {0, 0, 0, 0};
-    if (c < cols && !row_is_zero<T>(r, zb, zt, nc)) v = load4_n(src + r * cols + c, (int)min(cols - c, (int64_t)4));
-    if constexpr (sizeof(T) == 2) {
-      *reinterpret_cast<bf16x4*>(dst + r * ldp + c) = __builtin_convertvector(v, bf16x4);
-    } else {
-      bf16x4 h, m, l;
-#pragma unroll
-      for (int k = 0; k < 4; ++k) {
-        bf16 a, b, d;
-        split_f32(v[k], a, b, d);
-        h[k] = a, m[k] = b, l[k] = d;
-      }
-      *reinterpret_cast<bf16x4*>(dst + r * ldp + c) = h;
-      *reinterpret_cast<bf16x4*>(dst + plane + r * ldp + c) = m;
-      *reinterpret_cast<bf16x4*>(dst + 2 * plane + r * ldp + c) = l;
-    }
+template <int PAIRS, class O>
+fgpu_status run_products(const ProductJob* jobs, int count, const Plan* q, int pair, float* const* part, const ColumnSum* sums,
+                         hipStream_t s) {
+  GemmArgs g[2];
+  Finish f[2];
+  for (int i = 0; i < count; ++i) {
+    const ProductJob& j = jobs[i];
+    g[i] = {j.a, j.b, j.p.m, j.p.n, j.p.k, q[i].tiles_m, q[i].tiles_n, q[i].splits, q[i].k_per_split};
+    f[i] = j.f;
+    // Results of more than the last-level cache's 256 MB go past it: what is written would only push the operands out
+    // (65536 x 4096 x 1024 with its pre-activation 731 -> 624 us; at 134 MB it would cost 102 -> 128 us).
+    f[i].stream = (int64_t)j.p.m * j.p.n * (int64_t)sizeof(O) * (j.f.pre ? 2 : 1) > (int64_t)256 << 20;
   }
-}
-
-// 16 columns x 64 groups of parts a workgroup; blockIdx.y: which of two sums.
-constexpr int kFinishCols = 16, kFinishGroups = 64;
-template <class T>
-__global__ __launch_bounds__(1024) void column_finish_kernel(const float* part, int parts, int64_t stride, int64_t cols,
-                                                             T* out0, T* out1) {
-  __shared__ float sum[kFinishGroups][kFinishCols + 1];
-  T* out = blockIdx.y ? out1 : out0;
-  if (!out) return;
-  const int cl = threadIdx.x % kFinishCols, g = threadIdx.x / kFinishCols;
-  const int64_t c = (int64_t)blockIdx.x * kFinishCols + cl;
-  part += blockIdx.y * cols;
-  float v = 0;
-  if (c < cols)
-    for (int p = g; p < parts; p += kFinishGroups) v += part[(int64_t)p * stride + c];
-  sum[g][cl] = v;
-  __syncthreads();
-  // one wave a column: its 64 groups across the lanes
-  const int w = threadIdx.x >> 6;
-  v = lanes_sum<64>(sum[threadIdx.x & 63][w]);
-  if ((threadIdx.x & 63) == 0 && (int64_t)blockIdx.x * kFinishCols + w < cols) out[(int64_t)blockIdx.x * kFinishCols + w] = (T)v;
+  if (pair) {
+    const ProductEpi<O, FGPU_ACT_NONE> ex{f[0], part[0], g[0].m, g[0].n}, ew{f[1], part[1], g[1].m, g[1].n};
+    const int nx = g[0].tiles_m * g[0].tiles_n * g[0].splits, nw = g[1].tiles_m * g[1].tiles_n * g[1].splits;
+    if (pair == 128)
+      gemm_pair_kernel<Tile128, PAIRS><<<nx + nw, Tile128::threads, 0, s>>>(g[0], ex, nx, g[1], ew);
+    else
+      gemm_pair_kernel<Tile64, PAIRS><<<nx + nw, Tile64::threads, 0, s>>>(g[0], ex, nx, g[1], ew);
+    FGPU_HIP(hipGetLastError());
+  } else {
+    for (int i = 0; i < count; ++i)
+      FGPU_TRY((run_form<PAIRS, O>(jobs[i].a_kc, jobs[i].b_kc, q[i].tile, g[i], f[i], part[i], s)));
+  }
+  SplitJob sj[2];
+  int blocks[2] = {0, 0};
+  for (int i = 0; i < count; ++i) {
+    if (!part[i]) continue;
+    sj[i].part = part[i], sj[i].m = g[i].m, sj[i].n = g[i].n, sj[i].splits = g[i].splits, sj[i].f = f[i];
+    blocks[i] = ceil_div((int64_t)g[i].m * ((g[i].n + 3) / 4), 256);
+  }
+  const int sum_blocks = sums ? ceil_div(sums->cols, kSumCols) : 0;
+  if (blocks[0] + blocks[1] + sum_blocks == 0) return FGPU_OK;
+  join_kernel<O><<<blocks[0] + blocks[1] + sum_blocks, 256, 0, s>>>(sj[0], blocks[0], sj[1], blocks[1],
+                                                                   sums ? *sums : ColumnSum{});
+  FGPU_HIP(hipGetLastError());
+  return FGPU_OK;
 }
 
 }  // namespace
 
-size_t product_workspace_bytes(const Product& p) {
-  const Plan q = plan_of(p);
-  return q.splits > 1 || p.chunked ? carve_bytes<float>((size_t)q.splits * p.m * ((p.n + 3) & ~3)) : 0;
+size_t products_workspace_bytes(const Product* p, int count) {
+  Plan q[2];
+  plans_of(p, count, q);
+  size_t b = 0;
+  for (int i = 0; i < count; ++i) b += parts_bytes(p[i], q[i]);
+  return b;
+}
+double products_estimate_us(const Product* p, int count) {
+  Plan q[2];
+  const int pair = plans_of(p, count, q);
+  double us = 0;
+  for (int i = 0; i < count; ++i) us += q[i].us;
+  return pair ? us - 3 : us;
 }
 
-fgpu_status launch_product(const Product& p, const GemmOperand& a, bool a_kc, const GemmOperand& b, bool b_kc,
-                           const Finish& f, void* ws, hipStream_t s) {
-  const Plan q = plan_of(p);
-  const GemmArgs g{a, b, p.m, p.n, p.k, q.tiles_m, q.tiles_n, q.splits, q.k_per_split};
-  float* part = q.splits > 1 || p.chunked ? static_cast<float*>(ws) : nullptr;
-  if (p.f32)
-    FGPU_TRY((run_form<6, float>(a_kc, b_kc, q.tile, g, f, part, s)));
-  else
-    FGPU_TRY((run_form<1, bf16>(a_kc, b_kc, q.tile, g, f, part, s)));
-  if (part) {
-    const int64_t total = (int64_t)p.m * ((p.n + 3) / 4);
-    if (p.f32)
-      split_finish_kernel<float><<<ceil_div(total, 256), 256, 0, s>>>(part, p.m, p.n, q.splits, f);
-    else
-      split_finish_kernel<bf16><<<ceil_div(total, 256), 256, 0, s>>>(part, p.m, p.n, q.splits, f);
-    FGPU_HIP(hipGetLastError());
+fgpu_status launch_products(const ProductJob* jobs, int count, const ColumnSum* sums, void* ws, hipStream_t s) {
+  Product p[2];
+  Plan q[2];
+  for (int i = 0; i < count; ++i) p[i] = jobs[i].p;
+  const int pair = plans_of(p, count, q);
+  float* part[2] = {nullptr, nullptr};
+  char* at = static_cast<char*>(ws);
+  for (int i = 0; i < count; ++i) {
+    const size_t b = parts_bytes(p[i], q[i]);
+    if (b) part[i] = reinterpret_cast<float*>(at);
+    at += b;
   }
-  return FGPU_OK;
+  if (p[0].f32) return run_products<6, float>(jobs, count, q, pair, part, sums, s);
+  return run_products<1, bf16>(jobs, count, q, pair, part, sums, s);
 }
 
-fgpu_status launch_pack(const void* src, int64_t rows, int64_t cols, bool f32, const GemmOperand& dst,
-                        const float* zero_bias, const int32_t* zero_target, int nc, hipStream_t s) {
-  const int64_t total = rows * (dst.ld / 4);
-  const int grid = (int)std::min<int64_t>(ceil_div(total, 256), 8192);
-  uint16_t* d = const_cast<uint16_t*>(dst.p);
-  if (f32)
-    pack_kernel<float><<<grid, 256, 0, s>>>((const float*)src, rows, cols, dst.ld, dst.plane, d, zero_bias, zero_target, nc);
-  else
-    pack_kernel<bf16><<<grid, 256, 0, s>>>((const bf16*)src, rows, cols, dst.ld, dst.plane, d, zero_bias, zero_target, nc);
+fgpu_status launch_column_sums(const ColumnSum& c, void* out1, hipStream_t s) {
+  const dim3 grid(ceil_div(c.cols, kSumCols), out1 ? 2 : 1);
+  column_sum_kernel<<<grid, 256, 0, s>>>(c, out1);
   FGPU_HIP(hipGetLastError());
   return FGPU_OK;
-}
-
-fgpu_status launch_column_finish2(const float* part, int parts, int64_t stride, int64_t cols, bool f32_out, void* out0,
-                                  void* out1, hipStream_t s) {
-  const dim3 grid(ceil_div(cols, kFinishCols), out1 ? 2 : 1);
-  if (f32_out)
-    column_finish_kernel<float><<<grid, 1024, 0, s>>>(part, parts, stride, cols, (float*)out0, (float*)out1);
-  else
-    column_finish_kernel<bf16><<<grid, 1024, 0, s>>>(part, parts, stride, cols, (bf16*)out0, (bf16*)out1);
-  FGPU_HIP(hipGetLastError());
-  return FGPU_OK;
-}
-
-fgpu_status launch_column_finish(const float* part, int parts, int64_t stride, int64_t cols, bool f32_out, void* out,
-                                 hipStream_t s) {
-  return launch_column_finish2(part, parts, stride, cols, f32_out, out, nullptr, s);
 }
 
 }  // namespace fgpu

@@ -7,6 +7,7 @@
 // in column chunks that bound the workspace.  Scores live in units of log 2 (s log2 e), so an exponential is one
 // instruction.
 #include <algorithm>
+#include <type_traits>
 
 #include "head.hpp"
 
@@ -138,20 +139,15 @@ __global__ __launch_bounds__(1024) void loss_join_kernel(LossArgs a, const f32x2
   loss[m] = live ? (l2 - target2[m]) * kLn2 : 0.0f;
 }
 
-// What the backward pass needs of each row: lse in units of log 2 and the row's weight; a row without a gradient has
-// weight 0 and an infinite lse, so its G is zero.
-__global__ __launch_bounds__(256) void loss_rows_kernel(LossArgs a, const float* dloss, const float* lse, f32x2* rows,
-                                                        int32_t* live_target) {
-  const int m = blockIdx.x * 256 + threadIdx.x;
-  if (m >= a.nq) return;
-  const int t = a.target[m];
-  const bool live = (uint32_t)t < (uint32_t)a.nc && lse[m] != -INFINITY && !(a.bias && masked_bias(a.bias[t]));
-  rows[m] = live ? f32x2{lse[m] * kLog2e, dloss[m]} : f32x2{INFINITY, 0.0f};
-  live_target[m] = live ? t : -1;
+template <bool STREAM>
+__device__ __forceinline__ void store_g(uint16_t* d, const bf16x8& v) {
+  if constexpr (STREAM) __builtin_nontemporal_store(v, reinterpret_cast<bf16x8*>(d));
+  else *reinterpret_cast<bf16x8*>(d) = v;
 }
 
 // Backward: G of the columns c0 .. c0 + n - 1, as an operand [nq][ldg], and its column sums a tile row.
-template <bool F32>
+// STREAM: past the caches (a G larger than the last-level cache comes back from memory anyway).
+template <bool F32, bool STREAM>
 struct GradEpi {
   LossArgs a;         // target: live_target
   const f32x2* rows;
@@ -190,7 +186,7 @@ struct GradEpi {
         if (m < a.nq && nl < ldg) {  // the padding's columns are zero
           uint16_t* d = g + (int64_t)m * ldg + nl;
           if constexpr (!F32) {
-            *reinterpret_cast<bf16x8*>(d) = to_bf16x8(v);
+            store_g<STREAM>(d, to_bf16x8(v));
           } else {
             bf16x8 h, mi, l;
 #pragma unroll
@@ -199,9 +195,9 @@ struct GradEpi {
               split_f32(v[e], x, y, z);
               h[e] = x, mi[e] = y, l[e] = z;
             }
-            *reinterpret_cast<bf16x8*>(d) = h;
-            *reinterpret_cast<bf16x8*>(d + plane) = mi;
-            *reinterpret_cast<bf16x8*>(d + 2 * plane) = l;
+            store_g<STREAM>(d, h);
+            store_g<STREAM>(d + plane, mi);
+            store_g<STREAM>(d + 2 * plane, l);
           }
         }
       }
@@ -269,13 +265,23 @@ int64_t most_columns(int nq, int nc) {
   const int64_t most = std::min<int64_t>((int64_t)1 << 20, ((int64_t)1 << 31) / std::max(1, nq));
   return std::min<int64_t>(nc, most / 256 * 256);
 }
+// Room for the products of a chunk of `step` columns and of the last, shorter one, for both gradients or one.
+size_t chunk_products_bytes(int nq, int nc, int dim, bool f32, int step) {
+  size_t most = 0;
+  for (int n : {step, nc % step}) {
+    if (n == 0) continue;
+    const Product p[2] = {{nq, dim, n, f32, step < nc}, {n, dim, nq, f32}};
+    most = std::max({most, products_workspace_bytes(p, 2), products_workspace_bytes(p, 1), products_workspace_bytes(p + 1, 1)});
+  }
+  return most;
+}
 // The backward pass's workspace when it holds `step` columns of G.
 size_t backward_bytes(int nq, int nc, int dim, bool f32, int step) {
   const bool chunked = step < nc;
   size_t b = carve_bytes<f32x2>(nq) + carve_bytes<int32_t>(nq) + packed_bytes(nq, dim, f32) + packed_bytes(nc, dim, f32) +
              packed_bytes(nq, step, f32) + carve_bytes<float>((size_t)ceil_div(nq, 64) * step);
   if (chunked) b += carve_bytes<float>((size_t)nq * ((dim + 3) & ~3));
-  return b + std::max(product_workspace_bytes({nq, dim, step, f32, chunked}), product_workspace_bytes({step, dim, nq, f32}));
+  return b + chunk_products_bytes(nq, nc, dim, f32, step);
 }
 
 }  // namespace
@@ -314,8 +320,10 @@ fgpu_status fgpu_contrastive_loss(const void* d_q, const void* d_c, const int32_
   if (pk) {
     q = packed(qp, nq, dim);
     c = packed(cp, nc, dim);
-    FGPU_TRY(launch_pack(d_q, nq, dim, f32, q, nullptr, nullptr, 0, s));
-    FGPU_TRY(launch_pack(d_c, nc, dim, f32, c, nullptr, nullptr, 0, s));
+    Prep prep;
+    prep.copy[0] = {d_q, nq, dim, q};
+    prep.copy[1] = {d_c, nc, dim, c};
+    FGPU_TRY(launch_prep(prep, f32, s));
   }
   const LossArgs a{d_bias, d_ids, d_target, scale * kLog2e, nq, nc};
   const StatsEpi e{a, part, target2};
@@ -339,8 +347,8 @@ fgpu_status fgpu_contrastive_loss_backward(const float* d_dloss, const void* d_q
   const bool f32 = dtype == FGPU_DTYPE_F32;
   hipStream_t s = as_stream(stream);
   if (nq == 0) {
-    if (d_dc) FGPU_TRY(launch_column_finish(nullptr, 0, 0, (int64_t)nc * dim, f32, d_dc, s));
-    if (d_dbias) FGPU_TRY(launch_column_finish(nullptr, 0, 0, nc, true, d_dbias, s));
+    if (d_dc) FGPU_TRY(launch_no_sums((int64_t)nc * dim, f32, d_dc, s));
+    if (d_dbias) FGPU_TRY(launch_no_sums(nc, true, d_dbias, s));
     return FGPU_OK;
   }
   FGPU_CHECK(d_dloss && d_q && d_c && d_target && d_lse, FGPU_ERR_ARG, "contrastive loss backward: null argument");
@@ -357,45 +365,55 @@ fgpu_status fgpu_contrastive_loss_backward(const float* d_dloss, const void* d_q
   char* gp = ws.take<char>(packed_bytes(nq, step, f32));
   float* dbias_part = d_dbias ? ws.take<float>((size_t)ceil_div(nq, 64) * step) : nullptr;
   float* dq_sum = step < nc && d_dq ? ws.take<float>((size_t)nq * ((dim + 3) & ~3)) : nullptr;
-  char* pw = ws.take<char>(std::max(d_dq ? product_workspace_bytes({nq, dim, step, f32, step < nc}) : 0,
-                                    d_dc ? product_workspace_bytes({step, dim, nq, f32}) : 0));
+  char* pw = ws.take<char>(chunk_products_bytes(nq, nc, dim, f32, step));
   FGPU_CHECK(ws.ok(), FGPU_ERR_WORKSPACE,
              "contrastive loss backward: workspace too small for 256 columns of the score gradient");
-  LossArgs a{d_bias, d_ids, d_target, scale * kLog2e, nq, nc};
-  loss_rows_kernel<<<ceil_div(nq, 256), 256, 0, s>>>(a, d_dloss, d_lse, rows, live_target);
-  FGPU_HIP(hipGetLastError());
-  a.target = live_target;
+  const LossArgs a{d_bias, d_ids, live_target, scale * kLog2e, nq, nc};
   // Rows without a gradient and masked candidates become zero vectors: their G is zero, and what they hold (infinities
   // and NaN included) must not reach the products.
+  Prep prep;
+  prep.loss = {d_bias, d_target, d_lse, d_dloss, nq, nc, rows, live_target};
   const GemmOperand q = packed(qp, nq, dim);
-  FGPU_TRY(launch_pack(d_q, nq, dim, f32, q, nullptr, live_target, nc, s));
+  prep.copy[0] = {d_q, nq, dim, q, nullptr, true};
   GemmOperand c = as_is(d_c, dim);
   if (copy_c) {
     c = packed(cp, nc, dim);
-    FGPU_TRY(launch_pack(d_c, nc, dim, f32, c, d_bias, nullptr, 0, s));
+    prep.copy[1] = {d_c, nc, dim, c, d_bias, false};
   }
+  FGPU_TRY(launch_prep(prep, f32, s));
   for (int c0 = 0; c0 < nc; c0 += step) {
     const int n = std::min(step, nc - c0);
     const GemmOperand g = packed(gp, nq, n), cc{c.p + (int64_t)c0 * c.ld, c.ld, c.plane};
     const ScorePlan sp = score_plan(nq, n);
-    uint16_t* gw = const_cast<uint16_t*>(g.p);
-    if (f32)
-      FGPU_TRY(launch_scores<6>(sp, q, cc, nq, n, dim, GradEpi<true>{a, rows, gw, g.ld, g.plane, dbias_part, c0, n}, s));
-    else
-      FGPU_TRY(launch_scores<1>(sp, q, cc, nq, n, dim, GradEpi<false>{a, rows, gw, g.ld, g.plane, dbias_part, c0, n}, s));
-    if (d_dbias) FGPU_TRY(launch_column_finish(dbias_part, sp.tiles_m, n, n, true, d_dbias + c0, s));
+    auto grad = [&](auto f, auto stream) -> fgpu_status {
+      constexpr bool F = decltype(f)::value;
+      const GradEpi<F, decltype(stream)::value> e{a, rows, const_cast<uint16_t*>(g.p), g.ld, g.plane, dbias_part, c0, n};
+      return launch_scores<F ? 6 : 1>(sp, q, cc, nq, n, dim, e, s);
+    };
+    const bool past = (int64_t)nq * n * (f32 ? 6 : 2) > (int64_t)256 << 20;
+    const std::true_type yes;
+    const std::false_type no;
+    FGPU_TRY(f32 ? (past ? grad(yes, yes) : grad(yes, no)) : (past ? grad(no, yes) : grad(no, no)));
+    ColumnSum sums;
+    sums.part = dbias_part, sums.parts = sp.tiles_m, sums.stride = sums.cols = n, sums.out = d_dbias ? d_dbias + c0 : nullptr;
+    ProductJob jobs[2];
+    int count = 0;
     if (d_dq) {
       Finish f;
       f.out = d_dq, f.alpha = scale;
       f.add = c0 > 0 ? dq_sum : nullptr;
       f.sum = c0 + n < nc ? dq_sum : nullptr;
-      FGPU_TRY(launch_product({nq, dim, n, f32, step < nc}, g, true, cc, false, f, pw, s));
+      jobs[count++] = {{nq, dim, n, f32, step < nc}, g, cc, true, false, f};
     }
     if (d_dc) {
       Finish f;
       f.out = static_cast<char*>(d_dc) + (int64_t)c0 * dim * (f32 ? 4 : 2), f.alpha = scale;
-      FGPU_TRY(launch_product({n, dim, nq, f32}, g, false, q, false, f, pw, s));
+      jobs[count++] = {{n, dim, nq, f32}, g, q, false, false, f};
     }
+    if (count)
+      FGPU_TRY(launch_products(jobs, count, d_dbias ? &sums : nullptr, pw, s));
+    else if (d_dbias)
+      FGPU_TRY(launch_column_sums(sums, nullptr, s));
   }
   return FGPU_OK;
 }

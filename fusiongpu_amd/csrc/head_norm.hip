@@ -353,8 +353,8 @@ fgpu_status fgpu_layer_norm_backward(const void* d_dy, const void* d_x, const vo
   const bool f32 = dtype == FGPU_DTYPE_F32;
   hipStream_t s = as_stream(stream);
   if (rows == 0) {
-    if (d_dgamma) FGPU_TRY(launch_column_finish(nullptr, 0, 0, dim, f32, d_dgamma, s));
-    if (d_dbeta) FGPU_TRY(launch_column_finish(nullptr, 0, 0, dim, f32, d_dbeta, s));
+    if (d_dgamma) FGPU_TRY(launch_no_sums(dim, f32, d_dgamma, s));
+    if (d_dbeta) FGPU_TRY(launch_no_sums(dim, f32, d_dbeta, s));
     return FGPU_OK;
   }
   FGPU_CHECK(d_dy && d_x && d_mean && d_rstd, FGPU_ERR_ARG, "layer norm backward: null dy, x, mean or rstd");
@@ -379,7 +379,11 @@ fgpu_status fgpu_layer_norm_backward(const void* d_dy, const void* d_x, const vo
     });
   };
   FGPU_TRY(f32 ? run(float{}) : run(bf16{}));
-  if (part) FGPU_TRY(launch_column_finish2(part, groups, 2 * dim, dim, f32, d_dgamma, d_dbeta, s));
+  if (part) {
+    ColumnSum c;
+    c.part = part, c.parts = groups, c.stride = 2 * dim, c.cols = dim, c.out = d_dgamma, c.f32 = f32;
+    FGPU_TRY(launch_column_sums(c, d_dbeta, s));
+  }
   return FGPU_OK;
 }
 

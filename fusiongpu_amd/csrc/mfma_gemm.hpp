@@ -58,6 +58,14 @@ __device__ __forceinline__ bf16x8 to_bf16x8(const f32x8& v) {
   return bf16x8{lo[0], lo[1], lo[2], lo[3], hi[0], hi[1], hi[2], hi[3]};
 }
 __device__ __forceinline__ void store8(bf16* p, const f32x8& v) { *reinterpret_cast<bf16x8u*>(p) = to_bf16x8(v); }
+// The same past the caches.
+__device__ __forceinline__ void stream8(float* p, const f32x8& v) {
+  __builtin_nontemporal_store(v.lo, reinterpret_cast<f32x4u*>(p));
+  __builtin_nontemporal_store(v.hi, reinterpret_cast<f32x4u*>(p + 4));
+}
+__device__ __forceinline__ void stream8(bf16* p, const f32x8& v) {
+  __builtin_nontemporal_store(to_bf16x8(v), reinterpret_cast<bf16x8u*>(p));
+}
 // The first `n` (1 to 4) of them; the others read as zero and are not written.
 template <class T>
 __device__ __forceinline__ f32x4 load4_n(const T* p, int n) {
@@ -121,7 +129,6 @@ struct GemmTile {
 using Tile256 = GemmTile<256, 256, 2, 4>;
 using Tile128 = GemmTile<128, 128, 2, 2>;
 using Tile64 = GemmTile<64, 64, 2, 2>;
-
 typedef __attribute__((address_space(3))) void lds_void;
 typedef __attribute__((address_space(3))) char lds_char;
 
@@ -137,7 +144,7 @@ template <bool KC, bool ISB, int CHUNKS>
 __device__ __forceinline__ int tile_swizzle(int row) {
   if constexpr (KC && ISB) return (row & 3) | (((row >> 3) & 1) << 2);
   if constexpr (KC) return row & 7;
-  return (2 * ((row & 3) | (((row >> 3) & 1) << 2))) & (CHUNKS - 1);
+  return (ISB ? 4 * (row & 3) : 2 * (row & 3)) & (CHUNKS - 1);
 }
 // Row i of fragment f of the B operand is n = 32 (f / 2) + 8 (i / 4) + 4 (f % 2) + i % 4: a lane's two accumulators of a
 // fragment pair (rows 4 (lane / 16) + r of each) are then eight consecutive columns, one 16-byte bf16 store.
@@ -198,7 +205,7 @@ struct TileRead {
       base = (first_row + row) * 128 + ((g ^ tile_swizzle<KC, ISB, 8>(row)) * 16);
       rowp = 0;
     } else {
-      const int s = tile_swizzle<KC, ISB, R / 8>((i >> 2) | (g << 3));
+      const int s = tile_swizzle<KC, ISB, R / 8>(i >> 2);
       rowp = (g * 8 + (i >> 2)) * R * 2;
       const int in = ISB ? (i & 3) * 16 : ((i & 3) >> 1) * 16 + (i & 1) * 8;
       base = (first_row * 2) ^ (s * 16) ^ in;
@@ -212,7 +219,9 @@ struct TileRead {
       const int rows = ISB ? 32 * (f >> 1) + 4 * (f & 1) : 16 * f;
       return *(lds_frag*)(lds + ((base ^ (kk * 64)) + rows * 128));
     } else {
-      const uint32_t in = ISB ? (base ^ ((f >> 1) * 64)) + (f & 1) * 8 : base ^ (f * 32);
+      // The permutation stays inside 128 bytes of A's rows and 256 of B's: what lies above is added as an immediate.
+      const uint32_t in = ISB ? (base ^ ((f >> 1) * 64 & 255)) + (f & 1) * 8 + ((f >> 1) * 64 & ~255)
+                              : (base ^ (f * 32 & 127)) + (f * 32 & ~127);
       const uint32_t a = rowp + in + kk * 32 * R * 2;
       const s16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_half*)(lds + a));
       const s16x4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_half*)(lds + a + 4 * R * 2));
@@ -242,24 +251,30 @@ struct GemmWave {
   int m0, n0;      // the tile's first row and column
   int tm, tn, sp;  // the tile, and the split
   int wm, wn, lane;
-  char* lds;       // the wave's own part of the tile buffers, lds_bytes long
-  static constexpr int lds_bytes = 2 * T::stage_bytes / T::waves;
+  char* lds;       // the wave's own part of a tile buffer, lds_bytes long
+  static constexpr int lds_bytes = T::stage_bytes / T::waves;
   __device__ int row(int j) const { return m0 + (wm * T::FM + j) * 16 + (lane & 15); }
   __device__ int first_col() const { return n0 + wn * T::FN * 16; }
   __device__ int col(int p) const { return first_col() + 32 * p + 8 * (lane >> 4); }
 };
 // acc[f][j]: a lane holds columns col(p) .. col(p) + 7 of row(j) in acc[2 p][j] and acc[2 p + 1][j].
 
+// One workgroup a tile.  Of a k step's 64, the fragments of one half are read while the other half's products run, so the
+// LDS's latency passes behind the matrix instructions; the step's only barrier lies between its halves, when every wave
+// holds the last fragments of this buffer and the next one's loads, issued a whole step before, have to have landed.
+//
+// s0 and s1 are two variables of the kernel: the compiler then knows that the buffer being read is not the one being
+// filled and waits for loads only at the barriers.
 template <class T, bool AKC, bool BKC, int PAIRS, class Epi>
-__global__ __launch_bounds__(T::threads, T::threads == 512 ? 2 : 1) void gemm_kernel(GemmArgs g, Epi epi) {
-  __shared__ __attribute__((aligned(1024))) char s0[T::stage_bytes];
-  __shared__ __attribute__((aligned(1024))) char s1[T::stage_bytes];
+__device__ __forceinline__ void gemm_tile(const GemmArgs& g, const Epi& epi, int wg, int wgs, char (&s0)[T::stage_bytes],
+                                          char (&s1)[T::stage_bytes]) {
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int wm = wave / T::WN, wn = wave % T::WN;
   int tm, tn, sp;
-  gemm_tile_of(g, blockIdx.x, gridDim.x, tm, tn, sp);
+  gemm_tile_of(g, wg, wgs, tm, tn, sp);
   const int m0 = tm * T::BM, n0 = tn * T::BN;
   const int kbeg = sp * g.k_per_split, kend = min(g.k, kbeg + g.k_per_split);
+  const int steps = max(0, (kend - kbeg + kGemmBK - 1) / kGemmBK) * PAIRS;
 
   TileLoad<T::BM, T::threads, AKC, false> la;
   TileLoad<T::BN, T::threads, BKC, true> lb;
@@ -269,63 +284,86 @@ __global__ __launch_bounds__(T::threads, T::threads == 512 ? 2 : 1) void gemm_ke
   TileRead<T::BN, BKC, true> rb;
   ra.init(lane, wm * (T::BM / T::WM));
   rb.init(lane, wn * (T::BN / T::WN));
+  constexpr int boff = T::BM * kGemmBK * 2;
 
+  int pk = kbeg, pp = 0;  // the next stage to load
+  // The pairs of one k step follow one another, so a plane's tile is read again while it is in the L2.
+  auto issue = [&](char* s) {
+    const int qa = PAIRS == 1 ? 0 : pair_a(pp), qb = PAIRS == 1 ? 0 : pair_b(pp);
+    la.issue(g.a, qa, m0, g.m, pk, g.k, (lds_char*)s, wave);
+    lb.issue(g.b, qb, n0, g.n, pk, g.k, (lds_char*)s + boff, wave);
+    if (PAIRS == 1 || ++pp == PAIRS) {
+      pp = 0;
+      pk += kGemmBK;
+    }
+  };
+  struct Half {
+    bf16x8 a[T::FM], b[T::FN];
+  };
+  auto read = [&](Half& h, char* s, int kk) {
+#pragma unroll
+    for (int i = 0; i < T::FN; ++i) h.b[i] = rb.get((const lds_char*)s + boff, i, kk);
+#pragma unroll
+    for (int j = 0; j < T::FM; ++j) h.a[j] = ra.get((const lds_char*)s, j, kk);
+  };
   f32x4 acc[T::FN][T::FM];
 #pragma unroll
   for (int i = 0; i < T::FN; ++i)
 #pragma unroll
     for (int j = 0; j < T::FM; ++j) acc[i][j] = f32x4{0, 0, 0, 0};
-
-  constexpr int boff = T::BM * kGemmBK * 2;
-  const int nk = max(0, (kend - kbeg + kGemmBK - 1) / kGemmBK), steps = nk * PAIRS;
-  int pk = kbeg, pp = 0;  // the next stage to load
-  auto issue = [&](char* s) {
-    const int qa = PAIRS == 1 ? 0 : pair_a(pp), qb = PAIRS == 1 ? 0 : pair_b(pp);
-    la.issue(g.a, qa, m0, g.m, pk, g.k, (lds_char*)s, wave);
-    lb.issue(g.b, qb, n0, g.n, pk, g.k, (lds_char*)s + boff, wave);
-    pk += kGemmBK;
-    if (PAIRS > 1 && pk >= kend) {
-      pk = kbeg;
-      ++pp;
-    }
+  auto multiply = [&](const Half& h) {
+#pragma unroll
+    for (int j = 0; j < T::FM; ++j)
+#pragma unroll
+      for (int i = 0; i < T::FN; ++i)
+        acc[i][j] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(h.b[i], h.a[j], acc[i][j], 0, 0, 0);
   };
-  auto compute = [&](char* s) {
-    const lds_char* sa = (const lds_char*)s;
-    const lds_char* sb = (const lds_char*)s + boff;
-#pragma unroll
-    for (int kk = 0; kk < 2; ++kk) {
-      bf16x8 fa[T::FM], fb[T::FN];
-#pragma unroll
-      for (int i = 0; i < T::FN; ++i) fb[i] = rb.get(sb, i, kk);
-#pragma unroll
-      for (int j = 0; j < T::FM; ++j) fa[j] = ra.get(sa, j, kk);
-#pragma unroll
-      for (int j = 0; j < T::FM; ++j)
-#pragma unroll
-        for (int i = 0; i < T::FN; ++i)
-          acc[i][j] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(fb[i], fa[j], acc[i][j], 0, 0, 0);
-    }
+  Half h0, h1;
+  // One step: the buffer `cur` holds it, `next` the following one; `more`: the one after that exists.
+  auto step = [&](char* cur, char* next, bool more) {
+    read(h1, cur, 1);
+    multiply(h0);
+    __syncthreads();
+    if (more) issue(cur);
+    read(h0, next, 0);
+    multiply(h1);
   };
-  // Two buffers, each a variable of its own: the compiler then knows that a buffer being read is not the one being
-  // filled and waits for loads only at the barriers.
-  if (steps > 0) issue(s0);
   int left = steps;
-  for (; left >= 2; left -= 2) {
-    __syncthreads();  // s0 has landed; nobody reads s1 any more
-    issue(s1);
-    compute(s0);
+  if (left > 0) {
+    issue(s0);
     __syncthreads();
-    if (left > 2) issue(s0);
-    compute(s1);
-  }
-  if (left) {
-    __syncthreads();
-    compute(s0);
+    if (left > 1) issue(s1);
+    read(h0, s0, 0);
+    for (; left >= 2; left -= 2) {
+      step(s0, s1, left > 2);
+      step(s1, s0, left > 3);
+    }
+    if (left) step(s0, s1, false);
   }
   __syncthreads();
-  const int half = T::waves / 2;
-  const GemmWave<T> w{m0, n0, tm, tn, sp, wm, wn, lane, (wave < half ? s0 : s1) + wave % half * (T::stage_bytes / half)};
-  epi.template finish<T>(acc, w, s0);
+  const GemmWave<T> w{m0, n0, tm, tn, sp, wm, wn, lane, s1 + wave * (T::stage_bytes / T::waves)};
+  epi.template finish<T>(acc, w, s1);
+}
+
+// Registers for two waves a SIMD: one workgroup of 256 x 256 a CU, two of 128 x 128.
+template <class T, bool AKC, bool BKC, int PAIRS, class Epi>
+__global__ __launch_bounds__(T::threads, 2) void gemm_kernel(GemmArgs g, Epi epi) {
+  __shared__ __attribute__((aligned(1024))) char s0[T::stage_bytes];
+  __shared__ __attribute__((aligned(1024))) char s1[T::stage_bytes];
+  gemm_tile<T, AKC, BKC, PAIRS>(g, epi, blockIdx.x, gridDim.x, s0, s1);
+}
+
+// Both gradients of a small layer in one launch: the first x_wgs workgroups form x (A with k contiguous, B strided), the
+// others w (both strided).
+template <class T, int PAIRS, class Epi>
+__global__ __launch_bounds__(T::threads, 2) void gemm_pair_kernel(GemmArgs x, Epi ex, int x_wgs, GemmArgs w, Epi ew) {
+  __shared__ __attribute__((aligned(1024))) char s0[T::stage_bytes];
+  __shared__ __attribute__((aligned(1024))) char s1[T::stage_bytes];
+  const int b = blockIdx.x;
+  if (b < x_wgs)
+    gemm_tile<T, true, false, PAIRS>(x, ex, b, x_wgs, s0, s1);
+  else
+    gemm_tile<T, false, false, PAIRS>(w, ew, b - x_wgs, gridDim.x - x_wgs, s0, s1);
 }
 
 }  // namespace fgpu
