@@ -13,7 +13,12 @@
 namespace fgpu {
 namespace {
 
-constexpr int kDirectWaves = 8, kDirectThreads = kDirectWaves * kWave;
+#ifdef W4
+constexpr int kDirectWaves = 4;
+#else
+constexpr int kDirectWaves = 8;
+#endif
+constexpr int kDirectThreads = kDirectWaves * kWave;
 typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
 typedef uint32_t u32x4u __attribute__((ext_vector_type(4), aligned(2)));
 

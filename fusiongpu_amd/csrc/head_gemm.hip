@@ -13,7 +13,11 @@ struct ProductEpi {
   int m, n;
 
   template <class G>
-  __device__ __forceinline__ void finish(f32x4 (&acc)[G::FN][G::FM], const GemmWave<G>& w, char*) const {
+  struct Side {
+    __device__ void fetch(const ProductEpi&, int, int, int) {}
+  };
+  template <class G>
+  __device__ __forceinline__ void finish(f32x4 (&acc)[G::FN][G::FM], const GemmWave<G>& w, char*, const Side<G>&) const {
     if (w.first_col() + G::FN * 16 <= n)
       whole(acc, w);
     else

@@ -22,38 +22,96 @@ struct LossArgs {
   int nq, nc;
 };
 
-__device__ __forceinline__ bool masked_bias(float b) { return b <= FGPU_MASK_BIAS; }
+// What the epilogues need of a tile's rows and columns: fetched a row or column a thread while the products run, laid out
+// in LDS after them.  grad: the rows' (lse, weight) too.
+template <class G, bool GRAD>
+struct LossSide {
+  static_assert(G::threads >= G::BM + G::BN, "a thread a row and column");
+  int t = -1, id = 0;  // a row's target (-1: none) and its document, or a column's bias in units of log 2 and document
+  float bias2 = -INFINITY;
+  f32x2 row = {INFINITY, 0.0f};
+  struct Lds {
+    int t[G::BM], row_id[G::BM];
+    f32x2 row[GRAD ? G::BM : 1];
+    float bias2[G::BN];
+    int col_id[G::BN];
+  };
+  static_assert(sizeof(Lds) <= G::stage_bytes / 2, "beside the epilogue's own buffers");
 
-// The scores of a lane's eight columns n .. n + 7 at row m: s2 = scale2 acc + bias2, -inf where the column is masked,
-// beyond the candidates, or another copy of the row's document.
-struct ColumnSide {
-  float bias2[8];
-  int id[8];
-  __device__ __forceinline__ void load(const LossArgs& a, int n) {
-#pragma unroll
-    for (int r = 0; r < 8; ++r) {
-      const bool in = n + r < a.nc;
-      float b = in ? (a.bias ? a.bias[n + r] : 0.0f) : -INFINITY;
-      bias2[r] = masked_bias(b) ? -INFINITY : b * kLog2e;
-      id[r] = in && a.ids ? a.ids[n + r] : 0;
+  __device__ __forceinline__ void fetch(const LossArgs& a, const f32x2* rows, int m0, int n, int tid) {
+    if (tid < G::BM) {
+      const int m = m0 + tid;
+      if (m >= a.nq) return;
+      t = a.target[m];
+      if (GRAD) row = rows[m];
+      if ((uint32_t)t >= (uint32_t)a.nc) t = -1;
+      if (a.ids && t >= 0) id = a.ids[t];
+    } else if (tid < G::BM + G::BN) {
+      n += tid - G::BM;
+      if (n >= a.nc) return;
+      const float b = a.bias ? a.bias[n] : 0.0f;
+      bias2 = b <= FGPU_MASK_BIAS ? -INFINITY : b * kLog2e;
+      if (a.ids) id = a.ids[n];
     }
+  }
+  __device__ __forceinline__ Lds& put(char* lds, int tid) const {
+    Lds& l = *reinterpret_cast<Lds*>(lds);
+    if (tid < G::BM) {
+      l.t[tid] = t, l.row_id[tid] = id;
+      if (GRAD) l.row[tid] = row;
+    } else if (tid < G::BM + G::BN) {
+      l.bias2[tid - G::BM] = bias2, l.col_id[tid - G::BM] = id;
+    }
+    __syncthreads();
+    return l;
+  }
+};
+// A lane's eight columns.
+struct ColumnSide {
+  float bias2[8];  // -inf: masked, or beyond the candidates
+  int id[8];
+  bool masked;  // some lane of the wave has such a column
+  template <class L>
+  __device__ __forceinline__ void load(const L& l, int c) {
+    bool some = false;
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+      bias2[e] = l.bias2[c + e], id[e] = l.col_id[c + e];
+      some |= bias2[e] == -INFINITY;
+    }
+    masked = __any(some);
   }
 };
 struct RowSide {
-  int t;       // target column, -1: none
-  int id;      // its document
-  bool dedup;  // copies of it are left out
-  __device__ __forceinline__ void load(const LossArgs& a, int m) {
-    t = m < a.nq ? a.target[m] : -1;
-    if ((uint32_t)t >= (uint32_t)a.nc) t = -1;
-    dedup = a.ids && t >= 0;
-    id = dedup ? a.ids[t] : 0;
-  }
+  int t, id;
 };
-__device__ __forceinline__ float score2(const LossArgs& a, float acc, const ColumnSide& c, const RowSide& w, int n, int r) {
-  float s = c.bias2[r] == -INFINITY ? -INFINITY : fmaf(a.scale2, acc, c.bias2[r]);
-  if (w.dedup && c.id[r] == w.id && n + r != w.t) s = -INFINITY;
-  return s;
+// The scores of those columns at one row, from the product's elements: s = scale2 x + bias2, -inf where the column is
+// masked or holds another copy of the row's document.  Masked columns, copies and the target itself are few: they stand
+// behind tests that a wave passes as one (comparing ids costs an instruction an element, selecting would cost four more).
+// Returns whether the row's target is among the columns (`at`: which one).
+__device__ __forceinline__ bool scores8(const LossArgs& a, f32x8& v, const ColumnSide& c, const RowSide& w, int n, uint32_t& at) {
+  float s[8];
+#pragma unroll
+  for (int e = 0; e < 8; ++e) s[e] = fmaf(a.scale2, v[e], c.bias2[e]);
+  if (c.masked) {
+#pragma unroll
+    for (int e = 0; e < 8; ++e) s[e] = c.bias2[e] == -INFINITY ? -INFINITY : s[e];  // whatever its vector holds
+  }
+  at = (uint32_t)(w.t - n);
+  const bool here = w.t >= 0 && at < 8;
+  if (a.ids) {
+    bool same = false;
+#pragma unroll
+    for (int e = 0; e < 8; ++e) same |= c.id[e] == w.id;
+    if (__any(same)) {
+#pragma unroll
+      for (int e = 0; e < 8; ++e)
+        if (w.t >= 0 && c.id[e] == w.id && !(here && at == e)) s[e] = -INFINITY;
+    }
+  }
+#pragma unroll
+  for (int e = 0; e < 8; ++e) v.set(e, s[e]);
+  return here;
 }
 
 // Forward: per row and column tile (maximum, sum of exp2(s - maximum)), and the target's score.
@@ -63,37 +121,49 @@ struct StatsEpi {
   float* target2;  // [nq]
 
   template <class G>
-  __device__ __forceinline__ void finish(f32x4 (&acc)[G::FN][G::FM], const GemmWave<G>& w, char* lds) const {
+  struct Side : LossSide<G, false> {
+    __device__ __forceinline__ void fetch(const StatsEpi& e, int m0, int n0, int tid) {
+      LossSide<G, false>::fetch(e.a, nullptr, m0, n0, tid);
+    }
+  };
+  template <class G>
+  __device__ __forceinline__ void finish(f32x4 (&acc)[G::FN][G::FM], const GemmWave<G>& w, char* lds, const Side<G>& side) const {
     constexpr int P = G::FN / 2;
-    f32x2* sh = reinterpret_cast<f32x2*>(lds);  // [WN][BM]
+    const auto& l = side.put(lds, threadIdx.x);
+    f32x2* sh = reinterpret_cast<f32x2*>(lds + G::stage_bytes / 2);  // [WN][BM]
     ColumnSide cs[P];
 #pragma unroll
-    for (int p = 0; p < P; ++p) cs[p].load(a, w.col(p));
+    for (int p = 0; p < P; ++p) cs[p].load(l, w.col(p) - w.n0);
 #pragma unroll
     for (int j = 0; j < G::FM; ++j) {
       const int m = w.row(j);
-      RowSide rs;
-      rs.load(a, m);
+      const RowSide rs{l.t[m - w.m0], l.row_id[m - w.m0]};
+      f32x8 v[P];
       float top = -INFINITY;
 #pragma unroll
-      for (int p = 0; p < P; ++p)
+      for (int p = 0; p < P; ++p) {
+        v[p] = f32x8{acc[2 * p][j], acc[2 * p + 1][j]};
+        uint32_t at;
+        const bool here = scores8(a, v[p], cs[p], rs, w.col(p), at);
 #pragma unroll
-        for (int e = 0; e < 8; ++e) {
-          float& x = reinterpret_cast<float*>(&acc[2 * p + e / 4][j])[e % 4];
-          x = score2(a, x, cs[p], rs, w.col(p), e);
-          top = fmaxf(top, x);  // a NaN score makes the sum NaN
-          if (w.col(p) + e == rs.t) target2[m] = x;
+        for (int e = 0; e < 8; ++e) top = fmaxf(top, v[p][e]);  // a NaN score makes the sum NaN
+        if (here) {
+          float x = 0;
+#pragma unroll
+          for (int e = 0; e < 8; ++e) x = at == e ? v[p][e] : x;
+          target2[m] = x;
         }
-      top = fmaxf(top, shfl_xor_f(top, 16));
-      top = fmaxf(top, shfl_xor_f(top, 32));
+      }
+      top = fmaxf(top, __int_as_float(xchg<16>(__float_as_int(top))));
+      top = fmaxf(top, __int_as_float(xchg<32>(__float_as_int(top))));
       const float base = top == -INFINITY ? 0.0f : top;
       float sum = 0;
 #pragma unroll
-      for (int i = 0; i < G::FN; ++i)
+      for (int p = 0; p < P; ++p)
 #pragma unroll
-        for (int r = 0; r < 4; ++r) sum += fast_exp2(acc[i][j][r] - base);
-      sum += shfl_xor_f(sum, 16);
-      sum += shfl_xor_f(sum, 32);
+        for (int e = 0; e < 8; ++e) sum += fast_exp2(v[p][e] - base);
+      sum += __int_as_float(xchg<16>(__float_as_int(sum)));
+      sum += __int_as_float(xchg<32>(__float_as_int(sum)));
       if (w.lane < 16) sh[w.wn * G::BM + m - w.m0] = f32x2{top, sum};
     }
     __syncthreads();
@@ -110,28 +180,34 @@ struct StatsEpi {
   }
 };
 
-// Joins a row's parts: 64 rows a workgroup, sixteen groups of parts.
+// Joins a row's parts: 16 rows a workgroup, 64 groups of parts.
+constexpr int kJoinRows = 16, kJoinGroups = 64;
+__device__ __forceinline__ void join_stats(float& top, float& sum, float t, float s) {
+  const float both = fmaxf(top, t);
+  sum = both == -INFINITY ? sum + s : sum * fast_exp2(top - both) + s * fast_exp2(t - both);  // nothing yet: zero, or NaN
+  top = both;
+}
 __global__ __launch_bounds__(1024) void loss_join_kernel(LossArgs a, const f32x2* part, int parts, const float* target2,
                                                          float* loss, float* lse) {
-  __shared__ f32x2 sh[16][64];
-  const int lane = threadIdx.x & 63, g = threadIdx.x >> 6, m = blockIdx.x * 64 + lane;
-  float top = -INFINITY, sum = 0;
-  if (m < a.nq)
-    for (int p = g; p < parts; p += 16) {
-      const f32x2 v = part[(int64_t)p * a.nq + m];
-      const float t = fmaxf(top, v[0]);
-      if (t != -INFINITY) sum = sum * fast_exp2(top - t) + v[1] * fast_exp2(v[0] - t);
-      else sum += v[1];  // zero, or NaN
-      top = t;
-    }
-  sh[g][lane] = f32x2{top, sum};
+  __shared__ f32x2 sh[kJoinRows][kJoinGroups + 1];
+  const int r = threadIdx.x % kJoinRows, g = threadIdx.x / kJoinRows;
+  {
+    const int m = blockIdx.x * kJoinRows + r;
+    float top = -INFINITY, sum = 0;
+    if (m < a.nq)
+      for (int p = g; p < parts; p += kJoinGroups) {
+        const f32x2 v = part[(int64_t)p * a.nq + m];
+        join_stats(top, sum, v[0], v[1]);
+      }
+    sh[r][g] = f32x2{top, sum};
+  }
   __syncthreads();
-  if (g || m >= a.nq) return;
-  float all = top;
-  for (int k = 1; k < 16; ++k) all = fmaxf(all, sh[k][lane][0]);
-  const float base = all == -INFINITY ? 0.0f : all;
-  sum = 0;
-  for (int k = 0; k < 16; ++k) sum += sh[k][lane][1] * fast_exp2(sh[k][lane][0] - base);
+  // a wave a row
+  const int w = threadIdx.x >> 6, m = blockIdx.x * kJoinRows + w;
+  const f32x2 v = sh[w][threadIdx.x & 63];
+  const float top = wave_max_f(v[0]), base = top == -INFINITY ? 0.0f : top;
+  const float sum = lanes_sum<64>(v[1] * fast_exp2(v[0] - base));
+  if (threadIdx.x % kWave || m >= a.nq) return;
   const float l2 = base + __builtin_amdgcn_logf(sum);  // log2; of 0: -inf
   lse[m] = l2 * kLn2;
   const int t = a.target[m];
@@ -157,31 +233,40 @@ struct GradEpi {
   int c0, n;          // the chunk's columns
 
   template <class G>
-  __device__ __forceinline__ void finish(f32x4 (&acc)[G::FN][G::FM], const GemmWave<G>& w, char* lds) const {
+  struct Side : LossSide<G, true> {
+    __device__ __forceinline__ void fetch(const GradEpi& e, int m0, int n0, int tid) {
+      LossSide<G, true>::fetch(e.a, e.rows, m0, e.c0 + n0, tid);
+    }
+  };
+  template <class G>
+  __device__ __forceinline__ void finish(f32x4 (&acc)[G::FN][G::FM], const GemmWave<G>& w, char* lds, const Side<G>& side) const {
     constexpr int P = G::FN / 2;
+    const auto& l = side.put(lds, threadIdx.x);
     ColumnSide cs[P];
     f32x8 col[P];
 #pragma unroll
     for (int p = 0; p < P; ++p) {
-      cs[p].load(a, c0 + w.col(p));
+      cs[p].load(l, w.col(p) - w.n0);
       col[p] = f32x8{{0, 0, 0, 0}, {0, 0, 0, 0}};
     }
 #pragma unroll
     for (int j = 0; j < G::FM; ++j) {
       const int m = w.row(j);
-      RowSide rs;
-      rs.load(a, m);
-      const f32x2 row = m < a.nq ? rows[m] : f32x2{INFINITY, 0.0f};
+      const RowSide rs{l.t[m - w.m0], l.row_id[m - w.m0]};
+      const f32x2 row = l.row[m - w.m0];
 #pragma unroll
       for (int p = 0; p < P; ++p) {
         const int nl = w.col(p);
-        f32x8 v;
+        f32x8 v{acc[2 * p][j], acc[2 * p + 1][j]};
+        uint32_t at;
+        const bool here = scores8(a, v, cs[p], rs, c0 + nl, at);
 #pragma unroll
-        for (int e = 0; e < 8; ++e) {
-          float x = fast_exp2(score2(a, acc[2 * p + e / 4][j][e % 4], cs[p], rs, c0 + nl, e) - row[0]);
-          if (c0 + nl + e == rs.t) x -= 1.0f;
-          v.set(e, x * row[1]);
+        for (int e = 0; e < 8; ++e) v.set(e, fast_exp2(v[e] - row[0]));
+        if (here) {
+#pragma unroll
+          for (int e = 0; e < 8; ++e) v.set(e, at == e ? v[e] - 1.0f : v[e]);
         }
+        v.lo *= row[1], v.hi *= row[1];
         col[p].lo += v.lo, col[p].hi += v.hi;
         if (m < a.nq && nl < ldg) {  // the padding's columns are zero
           uint16_t* d = g + (int64_t)m * ldg + nl;
@@ -203,16 +288,13 @@ struct GradEpi {
       }
     }
     if (!dbias_part) return;
-    float* sh = reinterpret_cast<float*>(lds);  // [WM][BN]
+    float* sh = reinterpret_cast<float*>(lds + G::stage_bytes / 2);  // [WM][BN]
 #pragma unroll
     for (int p = 0; p < P; ++p)
 #pragma unroll
       for (int e = 0; e < 8; ++e) {
         float v = col[p][e];
-        v += shfl_xor_f(v, 1);
-        v += shfl_xor_f(v, 2);
-        v += shfl_xor_f(v, 4);
-        v += shfl_xor_f(v, 8);
+        v = lanes_sum<16>(v);
         if ((w.lane & 15) == 0) sh[w.wm * G::BN + w.col(p) - w.n0 + e] = v;
       }
     __syncthreads();
@@ -328,7 +410,7 @@ fgpu_status fgpu_contrastive_loss(const void* d_q, const void* d_c, const int32_
   const LossArgs a{d_bias, d_ids, d_target, scale * kLog2e, nq, nc};
   const StatsEpi e{a, part, target2};
   FGPU_TRY(f32 ? launch_scores<6>(sp, q, c, nq, nc, dim, e, s) : launch_scores<1>(sp, q, c, nq, nc, dim, e, s));
-  loss_join_kernel<<<ceil_div(nq, 64), 1024, 0, s>>>(a, part, sp.tiles_n, target2, d_loss, d_lse);
+  loss_join_kernel<<<ceil_div(nq, kJoinRows), 1024, 0, s>>>(a, part, sp.tiles_n, target2, d_loss, d_lse);
   FGPU_HIP(hipGetLastError());
   return FGPU_OK;
 }

@@ -237,8 +237,9 @@ __device__ __forceinline__ void gemm_tile_of(const GemmArgs& g, int wg, int tota
   constexpr int kXcd = 8, kGroup = 8;
   const int per = total / kXcd, rest = total % kXcd, x = wg % kXcd;
   int t = x * per + min(x, rest) + wg / kXcd;
-  sp = t % g.splits;
-  t /= g.splits;
+  const int tiles = g.tiles_m * g.tiles_n;
+  sp = t / tiles;  // a split's tiles follow one another: they share its part of the operands
+  t -= sp * tiles;
   const int group = kGroup * g.tiles_n, first = t / group * kGroup;
   const int gm = min(g.tiles_m - first, kGroup), in = t % group;
   tm = first + in % gm;
@@ -319,6 +320,7 @@ __device__ __forceinline__ void gemm_tile(const GemmArgs& g, const Epi& epi, int
         acc[i][j] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(h.b[i], h.a[j], acc[i][j], 0, 0, 0);
   };
   Half h0, h1;
+  typename Epi::template Side<T> side;
   // One step: the buffer `cur` holds it, `next` the following one; `more`: the one after that exists.
   auto step = [&](char* cur, char* next, bool more) {
     read(h1, cur, 1);
@@ -331,6 +333,7 @@ __device__ __forceinline__ void gemm_tile(const GemmArgs& g, const Epi& epi, int
   int left = steps;
   if (left > 0) {
     issue(s0);
+    side.fetch(epi, m0, n0, tid);  // what the epilogue needs from memory comes in behind the products
     __syncthreads();
     if (left > 1) issue(s1);
     read(h0, s0, 0);
@@ -339,10 +342,12 @@ __device__ __forceinline__ void gemm_tile(const GemmArgs& g, const Epi& epi, int
       step(s1, s0, left > 3);
     }
     if (left) step(s0, s1, false);
+  } else {
+    side.fetch(epi, m0, n0, tid);
   }
   __syncthreads();
   const GemmWave<T> w{m0, n0, tm, tn, sp, wm, wn, lane, s1 + wave * (T::stage_bytes / T::waves)};
-  epi.template finish<T>(acc, w, s1);
+  epi.template finish<T>(acc, w, s1, side);
 }
 
 // Registers for two waves a SIMD: one workgroup of 256 x 256 a CU, two of 128 x 128.
