@@ -13,11 +13,7 @@
 namespace fgpu {
 namespace {
 
-#ifdef W4
-constexpr int kDirectWaves = 4;
-#else
 constexpr int kDirectWaves = 8;
-#endif
 constexpr int kDirectThreads = kDirectWaves * kWave;
 typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
 typedef uint32_t u32x4u __attribute__((ext_vector_type(4), aligned(2)));
@@ -323,20 +319,21 @@ fgpu_status launch_direct_backward(const DirectJob* x, const DirectJob* w, bool 
   return FGPU_OK;
 }
 
-// Microseconds, fitted to this kernel alone over 1 to 16384 rows and 96 to 2048 dims: a start, then tile steps (32 k of a
-// wave) at what 256 CUs take for one each; rows that are not whole 16-byte groups load at less than half the rate.
+// Microseconds, fitted over 1 to 16384 rows and 64 to 2048 dims: a start, the k steps (32) of a wave one after the other,
+// and all tiles' steps at what 256 CUs take for one each.
 namespace {
-double tile_steps(int64_t m, int64_t n, int64_t k) {
-  return (double)ceil_div(m, 32) * ceil_div(n, 32) * ceil_div(ceil_div(k, 32), kDirectWaves) / 256;
-}
+int wave_steps(int64_t k) { return ceil_div(ceil_div(k, 32), kDirectWaves); }
+double tile_steps(int64_t m, int64_t n, int64_t k) { return (double)ceil_div(m, 32) * ceil_div(n, 32) * wave_steps(k) / 256; }
 }  // namespace
 double direct_forward_estimate_us(const Product& p) {
   if (p.m <= 16) return p.f32 ? 7.5 : 4.5;
-  return 3 + std::max(1.0, tile_steps(p.m, p.n, p.k)) * (p.f32 ? 2.6 : 0.95) * (p.k % 8 ? (p.f32 ? 1.2 : 2.4) : 1);
+  // Rows that are not whole 16-byte groups load at half the rate or less.
+  return 3 + std::max<double>(wave_steps(p.k), tile_steps(p.m, p.n, p.k)) * (p.f32 ? 2.6 : 0.95) * (p.k % 8 ? (p.f32 ? 1.2 : 2.4) : 1);
 }
 double direct_backward_estimate_us(int rows, int in_dim, int out_dim, bool f32) {
-  const double t = tile_steps(rows, in_dim, out_dim) + tile_steps(out_dim, in_dim, rows);
-  return 5 + t * (f32 ? 5 : 1.75);
+  const int longest = std::max(wave_steps(out_dim), wave_steps(rows));
+  const double all = tile_steps(rows, in_dim, out_dim) + tile_steps(out_dim, in_dim, rows);
+  return f32 ? 4 + 3.6 * longest + 2.5 * all : 3 + 2.4 * longest + 1.2 * all;
 }
 
 }  // namespace fgpu

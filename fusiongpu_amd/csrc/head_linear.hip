@@ -17,9 +17,10 @@ fgpu_status check_common(int64_t rows, int in_dim, int out_dim, int dtype, int a
 DirectOperand direct(const void* p, int64_t rows, int64_t cols, const void* pre = nullptr) { return {p, cols, rows * cols, pre}; }
 
 // Whether the products of few tiles take the direct kernels (head_direct.hip): by the estimates of both, fitted to
-// measurements; a launch is priced at 2.7 us, what a caller pays for it in a row of small calls.  Measured (us, tiled /
-// direct): forward bf16 1 x 1024 x 1024 6.3 / 4.2, 128 x 768 x 2048 8.4 / 6.3, 1024^3 9.2 / 18; float32 128 x 768 x 2048
-// 26 / 12, 2048 x 1024 x 1024 65 / 82; backward bf16 64 x 768 x 768 16 / 11, 1024^3 38 / 61.
+// measurements; a launch is priced at 2.7 us, what a caller pays for it in a row of small calls.  Measured on the GPU alone
+// (us, tiled / direct): forward bf16 1 x 1024 x 1024 (rows, in, out) 5.8 / 4.2, 128 x 768 x 2048 6.5 / 6.3, 512 x 1024 x
+// 1024 7.6 / 10.9; float32 128 x 768 x 2048 22 / 12, 1024^3 36 / 44; backward bf16 128^3 10.6 / 5.7, 256 x 1024 x 1024
+// 17 / 21; float32 400 x 256 x 256 17 / 11, 128 x 768 x 2048 30 / 46.
 constexpr double kLaunch = 2.7;
 bool forward_direct(const Product& p) {
   double tiled = products_estimate_us(&p, 1);
