@@ -20,6 +20,8 @@ Reference interfaces mirrored (Hello-day/FusionGPU):
   * pq_train                        -> train_residual_pq_codebooks (pq_utils.h:77-138)
   * pq_encode                       -> encode_residuals_to_pq_gpu (kmeans_gpu.cuh:450-508)
   * build_ivfpq                     -> build_global main (build_global.cu:21-258), no rebalancing
+and, without a counterpart there, the layers and the loss of a query head (linear, layer_norm, contrastive_loss and
+their backward calls), which query_head.py puts together.
 """
 from __future__ import annotations
 
