@@ -116,6 +116,15 @@ struct ColumnSum {
   void* out = nullptr;
   int f32 = 1;
 };
+// A product in parts [split][m][n rounded up to 4], to be added up and finished.
+struct SplitJob {
+  const float* part = nullptr;
+  int m = 0, n = 0, splits = 0;
+  Finish f;
+};
+// Up to two such products (part NULL: none) and column sums (NULL: none), in one launch.
+fgpu_status launch_join(const SplitJob& a, const SplitJob& b, const ColumnSum* sums, bool f32, hipStream_t s);
+
 // The products (one, or an input's gradient followed by a weight's), then what joins split products and the column sums
 // (NULL: none): one launch for the products where they are small, one to join where there is something to join.
 size_t products_workspace_bytes(const Product* p, int count);
@@ -134,16 +143,21 @@ inline GemmOperand packed(void* p, int64_t rows, int64_t cols) {
   return {static_cast<uint16_t*>(p), packed_ld(cols), rows * packed_ld(cols)};
 }
 // ---- what comes before the products, in one launch (head_prep.hip) ---------------------
-// What the contrastive loss's backward pass needs of a row: lse in units of log 2 and its weight; a row without a gradient
-// (no target, a masked one, nothing left) has weight 0 and an infinite lse, so its score gradient is zero.
+// What the contrastive loss's backward pass needs of a row: lse in units of log 2, its weight, target and the target's
+// document; a row without a gradient (no target, a masked one, nothing left) has weight 0, an infinite lse, so that its
+// score gradient is zero, and target -1.
+struct LossRow {
+  float lse2, weight;
+  int target, id;
+};
 struct LossRows {
   const float* bias;
   const int32_t* target;
   const float* lse;
   const float* dloss;
+  const int32_t* ids;
   int nq, nc;
-  f32x2* rows;
-  int32_t* live_target;
+  LossRow* rows;
 };
 // A copy of src [rows][cols] as an operand; rows that a mask takes out become zero.
 struct CopyJob {
@@ -191,6 +205,34 @@ fgpu_status launch_direct_backward(const DirectJob* x, const DirectJob* w, bool 
 // The times that the rule between these and the tiled products goes by.
 double direct_forward_estimate_us(const Product& p);
 double direct_backward_estimate_us(int rows, int in_dim, int out_dim, bool f32);
+
+// ---- the contrastive loss of up to 128 dims (head_narrow.hip) ---------------------------
+struct LossArgs {
+  const float* bias;       // [nc] or NULL
+  const int32_t* ids;      // [nc] or NULL
+  const int32_t* target;   // [nq]
+  float scale2;            // scale * log2(e)
+  int nq, nc;
+};
+constexpr int kNarrowDim = 128;
+// Forward: parts [split][nq] of (maximum, sum of exp2(s - maximum)) in units of log 2, and the targets' scores.
+int narrow_stats_splits(int nq, int nc, bool f32);
+fgpu_status launch_narrow_stats(const LossArgs& a, const GemmOperand& q, const GemmOperand& c, int dim, bool f32, int splits,
+                                f32x2* part, float* target2, hipStream_t s);
+// Backward, without holding the score gradient: each gradient forms the scores again.  dc and dbias may be NULL.
+struct NarrowBackward {
+  LossArgs a;
+  const LossRow* rows;
+  GemmOperand q, c;
+  int dim;
+  bool f32;
+  float scale;
+  void* dq;
+  void* dc;
+  float* dbias;
+};
+size_t narrow_backward_bytes(int nq, int nc, int dim, bool f32, int most_splits);
+fgpu_status launch_narrow_backward(const NarrowBackward& b, int most_splits, void* ws, hipStream_t s);
 
 // ---- column sums ---------------------------------------------------------------
 // Two sums of the same length, the second one's parts `cols` after the first one's; either result may be NULL.

@@ -55,12 +55,6 @@ struct Run8 {
   }
 };
 
-// A lane's eight k of one row as MFMA operands: one bf16 vector, or the three planes of float32.
-template <class T>
-struct Frag {
-  static constexpr int planes = sizeof(T) == 4 ? 3 : 1;
-  bf16x8 p[planes];
-};
 template <class T>
 __device__ __forceinline__ Frag<T> to_frag(const Run8<T>& r) {
   Frag<T> f;
@@ -76,19 +70,6 @@ __device__ __forceinline__ Frag<T> to_frag(const Run8<T>& r) {
   }
   return f;
 }
-__device__ __forceinline__ f32x4 mma(const bf16x8& n, const bf16x8& m, f32x4 c) {
-  return __builtin_amdgcn_mfma_f32_16x16x32_bf16(n, m, c, 0, 0, 0);
-}
-__device__ __forceinline__ f32x4 mma(const Frag<bf16>& n, const Frag<bf16>& m, f32x4 c) { return mma(n.p[0], m.p[0], c); }
-__device__ __forceinline__ f32x4 mma(const Frag<float>& n, const Frag<float>& m, f32x4 c) {
-  c = mma(n.p[2], m.p[0], c);
-  c = mma(n.p[0], m.p[2], c);
-  c = mma(n.p[1], m.p[1], c);
-  c = mma(n.p[1], m.p[0], c);
-  c = mma(n.p[0], m.p[1], c);
-  return mma(n.p[0], m.p[0], c);
-}
-
 // How a wave reads one operand's F fragments (16 F rows x 32 k).
 template <class T, int F, bool KC, bool DZ>
 struct DirectRead {

@@ -111,23 +111,31 @@ struct ProductEpi {
   }
 };
 
-// Adds the parts of a split product in order and finishes it: one thread four columns.
-struct SplitJob {
-  const float* part = nullptr;
-  int m = 0, n = 0, splits = 0;
-  Finish f;
-};
+// Adds the parts of a split product in a fixed order and finishes it: a thread four columns, or, of many parts, sixteen
+// threads four columns (each a sixteenth of the parts), so that few outputs of many parts are not one long chain of loads.
+constexpr int kManyParts = 32;
 template <class T>
 __device__ __forceinline__ void split_finish(const SplitJob& j, int block) {
-  const int n4 = (j.n + 3) >> 2;
-  const int64_t i = (int64_t)block * 256 + threadIdx.x, total = (int64_t)j.m * n4;
+  __shared__ f32x4 sums[16][17];
+  const bool many = j.splits >= kManyParts;
+  const int n4 = (j.n + 3) >> 2, out = many ? threadIdx.x & 15 : threadIdx.x, group = many ? threadIdx.x >> 4 : 0;
+  const int64_t i = (int64_t)block * (many ? 16 : 256) + out, total = (int64_t)j.m * n4;
+  f32x4 v = {0, 0, 0, 0};
+  if (i < total) {
+    if (j.f.add && group == 0) v = *reinterpret_cast<const f32x4*>(j.f.add + i * 4);
+#pragma unroll 4
+    for (int s = group; s < j.splits; s += many ? 16 : 1) v += *reinterpret_cast<const f32x4*>(j.part + ((int64_t)s * total + i) * 4);
+  }
+  if (many) {
+    sums[group][out] = v;
+    __syncthreads();
+    if (group) return;
+#pragma unroll
+    for (int s = 1; s < 16; ++s) v += sums[s][out];
+  }
   if (i >= total) return;
   const int64_t row = i / n4;
   const int col = (int)(i - row * n4) * 4;
-  f32x4 v = {0, 0, 0, 0};
-  if (j.f.add) v = *reinterpret_cast<const f32x4*>(j.f.add + i * 4);
-#pragma unroll 4
-  for (int s = 0; s < j.splits; ++s) v += *reinterpret_cast<const f32x4*>(j.part + ((int64_t)s * total + i) * 4);
   if (j.f.sum)
     *reinterpret_cast<f32x4*>(j.f.sum + i * 4) = v;
   else
@@ -267,21 +275,24 @@ fgpu_status run_products(const ProductJob* jobs, int count, const Plan* q, int p
       FGPU_TRY((run_form<PAIRS, O>(jobs[i].a_kc, jobs[i].b_kc, q[i].tile, g[i], f[i], part[i], s)));
   }
   SplitJob sj[2];
-  int blocks[2] = {0, 0};
-  for (int i = 0; i < count; ++i) {
-    if (!part[i]) continue;
-    sj[i].part = part[i], sj[i].m = g[i].m, sj[i].n = g[i].n, sj[i].splits = g[i].splits, sj[i].f = f[i];
-    blocks[i] = ceil_div((int64_t)g[i].m * ((g[i].n + 3) / 4), 256);
-  }
-  const int sum_blocks = sums ? ceil_div(sums->cols, kSumCols) : 0;
-  if (blocks[0] + blocks[1] + sum_blocks == 0) return FGPU_OK;
-  join_kernel<O><<<blocks[0] + blocks[1] + sum_blocks, 256, 0, s>>>(sj[0], blocks[0], sj[1], blocks[1],
-                                                                   sums ? *sums : ColumnSum{});
-  FGPU_HIP(hipGetLastError());
-  return FGPU_OK;
+  for (int i = 0; i < count; ++i)
+    if (part[i]) sj[i].part = part[i], sj[i].m = g[i].m, sj[i].n = g[i].n, sj[i].splits = g[i].splits, sj[i].f = f[i];
+  return launch_join(sj[0], sj[1], sums, sizeof(O) == 4, s);
 }
 
 }  // namespace
+
+fgpu_status launch_join(const SplitJob& a, const SplitJob& b, const ColumnSum* sums, bool f32, hipStream_t s) {
+  auto blocks = [](const SplitJob& j) { return j.part ? ceil_div((int64_t)j.m * ((j.n + 3) / 4), j.splits >= kManyParts ? 16 : 256) : 0; };
+  const int na = blocks(a), nb = blocks(b), nc = sums ? ceil_div(sums->cols, kSumCols) : 0;
+  if (na + nb + nc == 0) return FGPU_OK;
+  if (f32)
+    join_kernel<float><<<na + nb + nc, 256, 0, s>>>(a, na, b, nb, sums ? *sums : ColumnSum{});
+  else
+    join_kernel<bf16><<<na + nb + nc, 256, 0, s>>>(a, na, b, nb, sums ? *sums : ColumnSum{});
+  FGPU_HIP(hipGetLastError());
+  return FGPU_OK;
+}
 
 size_t products_workspace_bytes(const Product* p, int count) {
   Plan q[2];

@@ -1,7 +1,8 @@
 // head_loss.hip -- the softmax contrastive loss of queries against candidate vectors, and its gradient.
 //
 // s_ij = scale q_i.c_j + bias_j over the candidates j that row i keeps; lse_i = log sum_j exp s_ij and
-// loss_i = lse_i - s_i,t(i).  Neither pass holds the score matrix: the forward pass keeps a running maximum and sum a
+// loss_i = lse_i - s_i,t(i).  Up to 128 dims the kernels of head_narrow.hip serve; here are the wider ones and the entry
+// points.  Neither pass holds the score matrix: the forward pass keeps a running maximum and sum a
 // (row, column tile) in the product's epilogue and joins them; the backward pass forms the product again, turns it
 // into G_ij = g_i (exp(s_ij - lse_i) - [j = t(i)]) in the epilogue and takes dq = scale G c and dc = scale G^T q from it
 // in column chunks that bound the workspace.  Scores live in units of log 2 (s log2 e), so an exponential is one
@@ -9,18 +10,10 @@
 #include <algorithm>
 #include <type_traits>
 
-#include "head.hpp"
+#include "loss_scores.hpp"
 
 namespace fgpu {
 namespace {
-
-struct LossArgs {
-  const float* bias;       // [nc] or NULL
-  const int32_t* ids;      // [nc] or NULL
-  const int32_t* target;   // [nq]
-  float scale2;            // scale * log2(e)
-  int nq, nc;
-};
 
 // What the epilogues need of a tile's rows and columns: fetched a row or column a thread while the products run, laid out
 // in LDS after them.  grad: the rows' (lse, weight) too.
@@ -38,14 +31,19 @@ struct LossSide {
   };
   static_assert(sizeof(Lds) <= G::stage_bytes / 2, "beside the epilogue's own buffers");
 
-  __device__ __forceinline__ void fetch(const LossArgs& a, const f32x2* rows, int m0, int n, int tid) {
+  __device__ __forceinline__ void fetch(const LossArgs& a, const LossRow* rows, int m0, int n, int tid) {
     if (tid < G::BM) {
       const int m = m0 + tid;
       if (m >= a.nq) return;
-      t = a.target[m];
-      if (GRAD) row = rows[m];
-      if ((uint32_t)t >= (uint32_t)a.nc) t = -1;
-      if (a.ids && t >= 0) id = a.ids[t];
+      if constexpr (GRAD) {
+        const LossRow r = rows[m];
+        row = f32x2{r.lse2, r.weight};
+        t = r.target, id = r.id;
+      } else {
+        t = a.target[m];
+        if ((uint32_t)t >= (uint32_t)a.nc) t = -1;
+        if (a.ids && t >= 0) id = a.ids[t];
+      }
     } else if (tid < G::BM + G::BN) {
       n += tid - G::BM;
       if (n >= a.nc) return;
@@ -66,54 +64,6 @@ struct LossSide {
     return l;
   }
 };
-// A lane's eight columns.
-struct ColumnSide {
-  float bias2[8];  // -inf: masked, or beyond the candidates
-  int id[8];
-  bool masked;  // some lane of the wave has such a column
-  template <class L>
-  __device__ __forceinline__ void load(const L& l, int c) {
-    bool some = false;
-#pragma unroll
-    for (int e = 0; e < 8; ++e) {
-      bias2[e] = l.bias2[c + e], id[e] = l.col_id[c + e];
-      some |= bias2[e] == -INFINITY;
-    }
-    masked = __any(some);
-  }
-};
-struct RowSide {
-  int t, id;
-};
-// The scores of those columns at one row, from the product's elements: s = scale2 x + bias2, -inf where the column is
-// masked or holds another copy of the row's document.  Masked columns, copies and the target itself are few: they stand
-// behind tests that a wave passes as one (comparing ids costs an instruction an element, selecting would cost four more).
-// Returns whether the row's target is among the columns (`at`: which one).
-__device__ __forceinline__ bool scores8(const LossArgs& a, f32x8& v, const ColumnSide& c, const RowSide& w, int n, uint32_t& at) {
-  float s[8];
-#pragma unroll
-  for (int e = 0; e < 8; ++e) s[e] = fmaf(a.scale2, v[e], c.bias2[e]);
-  if (c.masked) {
-#pragma unroll
-    for (int e = 0; e < 8; ++e) s[e] = c.bias2[e] == -INFINITY ? -INFINITY : s[e];  // whatever its vector holds
-  }
-  at = (uint32_t)(w.t - n);
-  const bool here = w.t >= 0 && at < 8;
-  if (a.ids) {
-    bool same = false;
-#pragma unroll
-    for (int e = 0; e < 8; ++e) same |= c.id[e] == w.id;
-    if (__any(same)) {
-#pragma unroll
-      for (int e = 0; e < 8; ++e)
-        if (w.t >= 0 && c.id[e] == w.id && !(here && at == e)) s[e] = -INFINITY;
-    }
-  }
-#pragma unroll
-  for (int e = 0; e < 8; ++e) v.set(e, s[e]);
-  return here;
-}
-
 // Forward: per row and column tile (maximum, sum of exp2(s - maximum)), and the target's score.
 struct StatsEpi {
   LossArgs a;
@@ -225,8 +175,8 @@ __device__ __forceinline__ void store_g(uint16_t* d, const bf16x8& v) {
 // STREAM: past the caches (a G larger than the last-level cache comes back from memory anyway).
 template <bool F32, bool STREAM>
 struct GradEpi {
-  LossArgs a;         // target: live_target
-  const f32x2* rows;
+  LossArgs a;
+  const LossRow* rows;
   uint16_t* g;
   int64_t ldg, plane;
   float* dbias_part;  // [tiles_m][n] or NULL
@@ -357,11 +307,15 @@ size_t chunk_products_bytes(int nq, int nc, int dim, bool f32, int step) {
   }
   return most;
 }
+// The rows' constants and the cleaned copies.
+size_t common_bytes(int nq, int nc, int dim, bool f32) {
+  return carve_bytes<LossRow>(nq) + packed_bytes(nq, dim, f32) + packed_bytes(nc, dim, f32);
+}
+constexpr int kMostSplits = 256;
 // The backward pass's workspace when it holds `step` columns of G.
 size_t backward_bytes(int nq, int nc, int dim, bool f32, int step) {
   const bool chunked = step < nc;
-  size_t b = carve_bytes<f32x2>(nq) + carve_bytes<int32_t>(nq) + packed_bytes(nq, dim, f32) + packed_bytes(nc, dim, f32) +
-             packed_bytes(nq, step, f32) + carve_bytes<float>((size_t)ceil_div(nq, 64) * step);
+  size_t b = common_bytes(nq, nc, dim, f32) + packed_bytes(nq, step, f32) + carve_bytes<float>((size_t)ceil_div(nq, 64) * step);
   if (chunked) b += carve_bytes<float>((size_t)nq * ((dim + 3) & ~3));
   return b + chunk_products_bytes(nq, nc, dim, f32, step);
 }
@@ -376,7 +330,8 @@ extern "C" {
 size_t fgpu_contrastive_loss_workspace_bytes(int nq, int nc, int dim, int dtype) {
   if (check_loss(nq, nc, dim, dtype) != FGPU_OK || nq == 0) return 0;
   const bool f32 = dtype == FGPU_DTYPE_F32;
-  size_t b = carve_bytes<f32x2>((size_t)score_plan(nq, nc).tiles_n * nq) + carve_bytes<float>(nq);
+  const int parts = dim <= kNarrowDim ? narrow_stats_splits(nq, nc, f32) : score_plan(nq, nc).tiles_n;
+  size_t b = carve_bytes<f32x2>((size_t)parts * nq) + carve_bytes<float>(nq);
   if (needs_pack(dim, f32)) b += packed_bytes(nq, dim, f32) + packed_bytes(nc, dim, f32);
   return b;
 }
@@ -390,9 +345,11 @@ fgpu_status fgpu_contrastive_loss(const void* d_q, const void* d_c, const int32_
   FGPU_CHECK(aligned16(d_q) && aligned16(d_c) && aligned16(d_workspace), FGPU_ERR_ARG,
              "contrastive loss: queries, candidates and workspace must be 16-byte aligned");
   const bool f32 = dtype == FGPU_DTYPE_F32, pk = needs_pack(dim, f32);
+  const bool narrow = dim <= kNarrowDim;
   const ScorePlan sp = score_plan(nq, nc);
+  const int parts = narrow ? narrow_stats_splits(nq, nc, f32) : sp.tiles_n;
   Carve ws(d_workspace, workspace_bytes);
-  f32x2* part = ws.take<f32x2>((size_t)sp.tiles_n * nq);
+  f32x2* part = ws.take<f32x2>((size_t)parts * nq);
   float* target2 = ws.take<float>(nq);
   char* qp = pk ? ws.take<char>(packed_bytes(nq, dim, f32)) : nullptr;
   char* cp = pk ? ws.take<char>(packed_bytes(nc, dim, f32)) : nullptr;
@@ -408,9 +365,13 @@ fgpu_status fgpu_contrastive_loss(const void* d_q, const void* d_c, const int32_
     FGPU_TRY(launch_prep(prep, f32, s));
   }
   const LossArgs a{d_bias, d_ids, d_target, scale * kLog2e, nq, nc};
-  const StatsEpi e{a, part, target2};
-  FGPU_TRY(f32 ? launch_scores<6>(sp, q, c, nq, nc, dim, e, s) : launch_scores<1>(sp, q, c, nq, nc, dim, e, s));
-  loss_join_kernel<<<ceil_div(nq, kJoinRows), 1024, 0, s>>>(a, part, sp.tiles_n, target2, d_loss, d_lse);
+  if (narrow) {
+    FGPU_TRY(launch_narrow_stats(a, q, c, dim, f32, parts, part, target2, s));
+  } else {
+    const StatsEpi e{a, part, target2};
+    FGPU_TRY(f32 ? launch_scores<6>(sp, q, c, nq, nc, dim, e, s) : launch_scores<1>(sp, q, c, nq, nc, dim, e, s));
+  }
+  loss_join_kernel<<<ceil_div(nq, kJoinRows), 1024, 0, s>>>(a, part, parts, target2, d_loss, d_lse);
   FGPU_HIP(hipGetLastError());
   return FGPU_OK;
 }
@@ -418,6 +379,7 @@ fgpu_status fgpu_contrastive_loss(const void* d_q, const void* d_c, const int32_
 size_t fgpu_contrastive_loss_backward_workspace_bytes(int nq, int nc, int dim, int dtype) {
   if (check_loss(nq, nc, dim, dtype) != FGPU_OK || nq == 0) return 0;
   const bool f32 = dtype == FGPU_DTYPE_F32;
+  if (dim <= kNarrowDim) return common_bytes(nq, nc, dim, f32) + narrow_backward_bytes(nq, nc, dim, f32, kMostSplits);
   return backward_bytes(nq, nc, dim, f32, (int)most_columns(nq, nc));
 }
 
@@ -436,25 +398,36 @@ fgpu_status fgpu_contrastive_loss_backward(const float* d_dloss, const void* d_q
   FGPU_CHECK(d_dloss && d_q && d_c && d_target && d_lse, FGPU_ERR_ARG, "contrastive loss backward: null argument");
   FGPU_CHECK(aligned16(d_q) && aligned16(d_c) && aligned16(d_workspace), FGPU_ERR_ARG,
              "contrastive loss backward: queries, candidates and workspace must be 16-byte aligned");
-  int step = (int)most_columns(nq, nc);
-  while (step > 256 && backward_bytes(nq, nc, dim, f32, step) > workspace_bytes) step = std::max(256, step / 2 / 256 * 256);
-  const bool copy_c = d_bias || needs_pack(dim, f32);
+  const bool narrow = dim <= kNarrowDim, copy_c = d_bias || needs_pack(dim, f32);
+  int step = (int)most_columns(nq, nc), splits = kMostSplits;
+  if (narrow) {
+    while (splits > 1 && common_bytes(nq, nc, dim, f32) + narrow_backward_bytes(nq, nc, dim, f32, splits) > workspace_bytes)
+      splits /= 2;
+  } else {
+    while (step > 256 && backward_bytes(nq, nc, dim, f32, step) > workspace_bytes) step = std::max(256, step / 2 / 256 * 256);
+  }
   Carve ws(d_workspace, workspace_bytes);
-  f32x2* rows = ws.take<f32x2>(nq);
-  int32_t* live_target = ws.take<int32_t>(nq);
+  LossRow* rows = ws.take<LossRow>(nq);
   char* qp = ws.take<char>(packed_bytes(nq, dim, f32));
   char* cp = copy_c ? ws.take<char>(packed_bytes(nc, dim, f32)) : nullptr;
-  char* gp = ws.take<char>(packed_bytes(nq, step, f32));
-  float* dbias_part = d_dbias ? ws.take<float>((size_t)ceil_div(nq, 64) * step) : nullptr;
-  float* dq_sum = step < nc && d_dq ? ws.take<float>((size_t)nq * ((dim + 3) & ~3)) : nullptr;
-  char* pw = ws.take<char>(chunk_products_bytes(nq, nc, dim, f32, step));
+  char *np = nullptr, *gp = nullptr, *pw = nullptr;
+  float *dbias_part = nullptr, *dq_sum = nullptr;
+  if (narrow) {
+    np = ws.take<char>(narrow_backward_bytes(nq, nc, dim, f32, splits));
+  } else {
+    gp = ws.take<char>(packed_bytes(nq, step, f32));
+    if (d_dbias) dbias_part = ws.take<float>((size_t)ceil_div(nq, 64) * step);
+    if (step < nc && d_dq) dq_sum = ws.take<float>((size_t)nq * ((dim + 3) & ~3));
+    pw = ws.take<char>(chunk_products_bytes(nq, nc, dim, f32, step));
+  }
   FGPU_CHECK(ws.ok(), FGPU_ERR_WORKSPACE,
-             "contrastive loss backward: workspace too small for 256 columns of the score gradient");
-  const LossArgs a{d_bias, d_ids, live_target, scale * kLog2e, nq, nc};
+             "contrastive loss backward: workspace too small for 256 columns of the score gradient (up to 128 dims: for the "
+             "copies of queries and candidates)");
+  const LossArgs a{d_bias, d_ids, d_target, scale * kLog2e, nq, nc};
   // Rows without a gradient and masked candidates become zero vectors: their G is zero, and what they hold (infinities
   // and NaN included) must not reach the products.
   Prep prep;
-  prep.loss = {d_bias, d_target, d_lse, d_dloss, nq, nc, rows, live_target};
+  prep.loss = {d_bias, d_target, d_lse, d_dloss, d_ids, nq, nc, rows};
   const GemmOperand q = packed(qp, nq, dim);
   prep.copy[0] = {d_q, nq, dim, q, nullptr, true};
   GemmOperand c = as_is(d_c, dim);
@@ -463,6 +436,7 @@ fgpu_status fgpu_contrastive_loss_backward(const float* d_dloss, const void* d_q
     prep.copy[1] = {d_c, nc, dim, c, d_bias, false};
   }
   FGPU_TRY(launch_prep(prep, f32, s));
+  if (narrow) return launch_narrow_backward({a, rows, q, c, dim, f32, scale, d_dq, d_dc, d_dbias}, splits, np, s);
   for (int c0 = 0; c0 < nc; c0 += step) {
     const int n = std::min(step, nc - c0);
     const GemmOperand g = packed(gp, nq, n), cc{c.p + (int64_t)c0 * c.ld, c.ld, c.plane};

@@ -85,9 +85,12 @@ __device__ __forceinline__ void make_dz(const DzJob& j, int block) {
 
 __device__ __forceinline__ void loss_row(const LossRows& r, int m) {
   if (m >= r.nq) return;
-  const bool live = loss_row_live(r, m);
-  r.rows[m] = live ? f32x2{r.lse[m] * kLog2e, r.dloss[m]} : f32x2{INFINITY, 0.0f};
-  r.live_target[m] = live ? r.target[m] : -1;
+  LossRow o{INFINITY, 0.0f, -1, 0};
+  if (loss_row_live(r, m)) {
+    const int t = r.target[m];
+    o = {r.lse[m] * kLog2e, r.dloss[m], t, r.ids ? r.ids[t] : 0};
+  }
+  r.rows[m] = o;
 }
 
 struct Blocks {

@@ -112,6 +112,40 @@ struct GemmArgs {
   int k_per_split;  // a multiple of kGemmBK
 };
 
+// A lane's eight k of one row as MFMA operands: one bf16 vector, or the three planes of float32.
+template <class T>
+struct Frag {
+  static constexpr int planes = sizeof(T) == 4 ? 3 : 1;
+  bf16x8 p[planes];
+};
+template <class T>
+__device__ __forceinline__ Frag<T> to_planes(const f32x8& v) {
+  Frag<T> f;
+  if constexpr (sizeof(T) == 2) {
+    f.p[0] = to_bf16x8(v);
+  } else {
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+      bf16 h, m, l;
+      split_f32(v[e], h, m, l);
+      f.p[0][e] = h, f.p[1][e] = m, f.p[2][e] = l;
+    }
+  }
+  return f;
+}
+__device__ __forceinline__ f32x4 mma(const bf16x8& n, const bf16x8& m, f32x4 c) {
+  return __builtin_amdgcn_mfma_f32_16x16x32_bf16(n, m, c, 0, 0, 0);
+}
+__device__ __forceinline__ f32x4 mma(const Frag<bf16>& n, const Frag<bf16>& m, f32x4 c) { return mma(n.p[0], m.p[0], c); }
+__device__ __forceinline__ f32x4 mma(const Frag<float>& n, const Frag<float>& m, f32x4 c) {
+  c = mma(n.p[2], m.p[0], c);
+  c = mma(n.p[0], m.p[2], c);
+  c = mma(n.p[1], m.p[1], c);
+  c = mma(n.p[1], m.p[0], c);
+  c = mma(n.p[0], m.p[1], c);
+  return mma(n.p[0], m.p[0], c);
+}
+
 constexpr int kGemmBK = 64;
 
 // Plane pairs (a, b) in the order they are accumulated: the smallest products first.

@@ -366,7 +366,8 @@ def test_layer_norm_offsets_past_32_bits():
 
 # ---- contrastive loss -------------------------------------------------------------------------------------------------
 LOSS = [(1, 1, 1), (1, 2, 3), (3, 64, 8), (5, 9, 17), (64, 64, 64), (65, 63, 96), (100, 333, 128), (130, 1000, 100),
-        (257, 513, 40), (1024, 1024, 128), (700, 20001, 72), (4100, 8190, 64), (40, 3000, 1030)]
+        (257, 513, 40), (1024, 1024, 128), (700, 20001, 72), (4100, 8190, 64), (40, 3000, 1030),
+        (129, 700, 129), (300, 1500, 200), (257, 66, 33)]
 
 
 def scores64(q, c, t, scale, bias, ids):
@@ -538,11 +539,13 @@ def test_contrastive_gradient_against_differences():
         assert abs(diff - (g.double() * v.double()).sum().item()) <= bound
 
 
+@pytest.mark.parametrize("dim", [72, 200])
 @pytest.mark.parametrize("dt", ["f32", "bf16"])
-def test_contrastive_backward_in_chunks(dt):
-    """A workspace too small for all columns: the same gradients from column chunks, down to 256 columns."""
-    q, c, t, scale, bias, ids = loss_inputs(300, 2900, 72, dt)
-    full = fg.lib.fgpu_contrastive_loss_backward_workspace_bytes(300, 2900, 72, int(dt == "bf16"))
+def test_contrastive_backward_in_chunks(dt, dim):
+    """A workspace too small for all columns (up to 128 dims: for all splits): the same gradients from column chunks, down
+    to 256 columns."""
+    q, c, t, scale, bias, ids = loss_inputs(300, 2900, dim, dt)
+    full = fg.lib.fgpu_contrastive_loss_backward_workspace_bytes(300, 2900, dim, int(dt == "bf16"))
     seen = []
     for part in (0.8, 0.65, 0.6):
         ws = torch.empty(int(full * part), dtype=torch.uint8, device="cuda")
