@@ -42,10 +42,10 @@ def loss_bwd(g=P, q=P, c=P, t=P, lse=P, nq=4, nc=8, dim=8, dt=F32, ws=P, wsb=1 <
     (linear, dict(dt=2), ARG), (linear, dict(act=4), ARG), (linear, dict(act=-1), ARG), (linear, dict(rows=-1), ARG),
     (linear, dict(k=0), ARG), (linear, dict(n=0), ARG), (linear, dict(x=None), ARG), (linear, dict(w=None), ARG),
     (linear, dict(y=None), ARG), (linear, dict(x=P + 4), ARG), (linear, dict(w=P + 8), ARG), (linear, dict(ws=P + 4), ARG),
-    (linear, dict(wsb=0), WORKSPACE), (linear, dict(k=(1 << 16) + 1), UNSUPPORTED), (linear, dict(rows=(1 << 30) + 1), UNSUPPORTED),
+    (linear, dict(rows=1 << 16, k=1023, n=1024, dt=BF16, wsb=0), WORKSPACE), (linear, dict(k=(1 << 16) + 1), UNSUPPORTED), (linear, dict(rows=(1 << 30) + 1), UNSUPPORTED),
     (linear_bwd, dict(dt=-1), ARG), (linear_bwd, dict(act=2), ARG), (linear_bwd, dict(dy=None), ARG),
     (linear_bwd, dict(w=None), ARG), (linear_bwd, dict(x=None), ARG), (linear_bwd, dict(dy=P + 2), ARG),
-    (linear_bwd, dict(wsb=0), WORKSPACE), (linear_bwd, dict(n=0), ARG), (linear_bwd, dict(n=1 << 17), UNSUPPORTED),
+    (linear_bwd, dict(rows=1 << 16, k=1024, n=1024, dt=BF16, wsb=0), WORKSPACE), (linear_bwd, dict(n=0), ARG), (linear_bwd, dict(n=1 << 17), UNSUPPORTED),
     (norm, dict(dt=7), ARG), (norm, dict(dim=0), ARG), (norm, dict(eps=-1.0), ARG), (norm, dict(eps=float("nan")), ARG),
     (norm, dict(x=None), ARG), (norm, dict(y=None), ARG), (norm, dict(rows=-2), ARG), (norm, dict(dim=16385), UNSUPPORTED),
     (norm_bwd, dict(mean=None), ARG), (norm_bwd, dict(rstd=None), ARG), (norm_bwd, dict(dy=None), ARG),
@@ -77,10 +77,11 @@ def test_workspace_sizes():
     assert L.fgpu_linear_workspace_bytes(1 << 16, 1023, 4096, BF16) >= (1 << 16) * 1024 * 2
     assert L.fgpu_linear_workspace_bytes(1 << 16, 1024, 4096, F32) >= (1 << 16) * 1024 * 6
     assert L.fgpu_linear_workspace_bytes(4, 8, 8, 9) == 0
-    # the score gradient is held whole up to 2^31 elements, in column chunks beyond
-    whole = L.fgpu_contrastive_loss_backward_workspace_bytes(4096, 65536, 128, BF16)
+    # above 128 dims the score gradient is held whole up to 2^31 elements, in column chunks beyond; up to 128, not at all
+    whole = L.fgpu_contrastive_loss_backward_workspace_bytes(4096, 65536, 256, BF16)
     assert whole >= 4096 * 65536 * 2
-    assert L.fgpu_contrastive_loss_backward_workspace_bytes(1 << 16, 1 << 20, 8, BF16) < (1 << 33)
+    assert L.fgpu_contrastive_loss_backward_workspace_bytes(1 << 16, 1 << 20, 136, BF16) < (1 << 33)
+    assert L.fgpu_contrastive_loss_backward_workspace_bytes(4096, 65536, 128, BF16) < whole // 4
 
 
 @pytest.fixture
