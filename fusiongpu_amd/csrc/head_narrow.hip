@@ -276,12 +276,12 @@ __device__ __forceinline__ void narrow_rows(const NarrowArgs& g, int wg, int wgs
   };
   const bool active = r0 < g.nr;  // a wave without rows keeps to the barriers
   for (int t = t0; t < t1; t += 2) {
-    __syncthreads();  // tile t is in s0 and d0; nobody reads s1 and d1 any more
+    landed_barrier();  // tile t is in s0 and d0; nobody reads s1 and d1 any more
     if (t + 1 < t1) issue(t + 1, s1), fetch(t + 1);
     if (active) work(t, s0, d0);
     if (t + 1 >= t1) break;
     put(d1);
-    __syncthreads();
+    landed_barrier();
     if (t + 2 < t1) issue(t + 2, s0), fetch(t + 2);
     if (active) work(t + 1, s1, d1);
     if (t + 2 < t1) put(d0);

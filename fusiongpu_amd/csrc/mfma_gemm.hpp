@@ -166,6 +166,13 @@ using Tile64 = GemmTile<64, 64, 2, 2>;
 typedef __attribute__((address_space(3))) void lds_void;
 typedef __attribute__((address_space(3))) char lds_char;
 
+// A barrier behind which every wave's loads to LDS have landed.  The wait is written out: before a barrier at the head of
+// a loop the compiler leaves it away for loads that the loop's end issued.
+__device__ __forceinline__ void landed_barrier() {
+  __builtin_amdgcn_s_waitcnt(0x0f70);  // vmcnt(0), the other counters at their limits
+  __syncthreads();
+}
+
 // The part of an operand's LDS tile that one lane fills (16 bytes a load straight to LDS), and the addresses its
 // fragments are read from.  R: rows of m or n in the tile, NT: threads.
 //
@@ -359,7 +366,7 @@ __device__ __forceinline__ void gemm_tile(const GemmArgs& g, const Epi& epi, int
   auto step = [&](char* cur, char* next, bool more) {
     read(h1, cur, 1);
     multiply(h0);
-    __syncthreads();
+    landed_barrier();
     if (more) issue(cur);
     read(h0, next, 0);
     multiply(h1);
@@ -368,7 +375,7 @@ __device__ __forceinline__ void gemm_tile(const GemmArgs& g, const Epi& epi, int
   if (left > 0) {
     issue(s0);
     side.fetch(epi, m0, n0, tid);  // what the epilogue needs from memory comes in behind the products
-    __syncthreads();
+    landed_barrier();
     if (left > 1) issue(s1);
     read(h0, s0, 0);
     for (; left >= 2; left -= 2) {
