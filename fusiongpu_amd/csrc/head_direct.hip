@@ -15,7 +15,6 @@ namespace {
 
 constexpr int kDirectWaves = 8;
 constexpr int kDirectThreads = kDirectWaves * kWave;
-typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
 typedef uint32_t u32x4u __attribute__((ext_vector_type(4), aligned(2)));
 
 // Eight consecutive elements as they lie in memory.
@@ -61,12 +60,10 @@ __device__ __forceinline__ Frag<T> to_frag(const Run8<T>& r) {
   if constexpr (sizeof(T) == 2) {
     f.p[0] = __builtin_bit_cast(bf16x8, r.w[0]);
   } else {
+    f32x8 v;
 #pragma unroll
-    for (int e = 0; e < 8; ++e) {
-      bf16 h, m, l;
-      split_f32(r.get(e), h, m, l);
-      f.p[0][e] = h, f.p[1][e] = m, f.p[2][e] = l;
-    }
+    for (int e = 0; e < 8; ++e) v.set(e, r.get(e));
+    split8(v, f.p[0], f.p[1], f.p[2]);
   }
   return f;
 }

@@ -212,13 +212,11 @@ Plan plan_of(const Product& p, int only = 0) {
   }
   return best;
 }
-// Two products run in one launch where both take the smaller tiles; the tile is then one for both.
+// Two products run in one launch where each by itself takes the same of the smaller tiles: a gradient's bits then do not
+// depend on whether the other is asked for.
 int plans_of(const Product* p, int count, Plan* q) {
   for (int i = 0; i < count; ++i) q[i] = plan_of(p[i]);
-  if (count == 1 || q[0].tile == 256 || q[1].tile == 256) return 0;
-  const int tile = std::min(q[0].tile, q[1].tile);
-  for (int i = 0; i < count; ++i) q[i] = plan_of(p[i], tile);
-  return tile;
+  return count == 2 && q[0].tile == q[1].tile && q[0].tile != 256 ? q[0].tile : 0;
 }
 
 template <class T, bool AKC, bool BKC, int PAIRS, class E>

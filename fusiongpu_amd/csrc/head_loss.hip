@@ -224,12 +224,7 @@ struct GradEpi {
             store_g<STREAM>(d, to_bf16x8(v));
           } else {
             bf16x8 h, mi, l;
-#pragma unroll
-            for (int e = 0; e < 8; ++e) {
-              bf16 x, y, z;
-              split_f32(v[e], x, y, z);
-              h[e] = x, mi[e] = y, l[e] = z;
-            }
+            split8(v, h, mi, l);
             store_g<STREAM>(d, h);
             store_g<STREAM>(d + plane, mi);
             store_g<STREAM>(d + 2 * plane, l);

@@ -11,7 +11,6 @@ constexpr int kNormMaxDim = 16384;
 
 // 16 bytes of a row as they lie in memory, eight bf16 or four floats, held as four words (as elements, the compiler would
 // unpack them where they are loaded and wait there).
-typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
 typedef uint32_t u32x4u __attribute__((ext_vector_type(4), aligned(2)));
 template <class T, bool RAGGED>
 struct Raw {

@@ -14,12 +14,7 @@ __device__ __forceinline__ void put4(uint16_t* d, int64_t plane, const f32x4& v)
     *reinterpret_cast<bf16x4*>(d) = __builtin_convertvector(v, bf16x4);
   } else {
     bf16x4 h, m, l;
-#pragma unroll
-    for (int k = 0; k < 4; ++k) {
-      bf16 a, b, e;
-      split_f32(v[k], a, b, e);
-      h[k] = a, m[k] = b, l[k] = e;
-    }
+    split4(v, h, m, l);
     *reinterpret_cast<bf16x4*>(d) = h;
     *reinterpret_cast<bf16x4*>(d + plane) = m;
     *reinterpret_cast<bf16x4*>(d + 2 * plane) = l;

@@ -2,7 +2,7 @@
 //
 // D[m][n] = sum_k A(m, k) B(n, k) on bf16 MFMA with float32 accumulators.  Each operand is read either with k contiguous
 // (rows of k) or with k strided (rows of m or n, one row a k), so the forward product x W^T and both gradients dz W and
-// dz^T x come from one kernel without a transposed copy.  float32 operands are held as three bf16 planes (split_f32
+// dz^T x come from one kernel without a transposed copy.  float32 operands are held as three bf16 planes (split2
 // below) and the k loop walks the six plane pairs whose product is above 2^-24 of the whole.
 #pragma once
 
@@ -84,16 +84,37 @@ __device__ __forceinline__ void store4_n(T* p, f32x4 v, int n) {
 }
 
 // x = h + m + l exactly (24 significant bits in three bf16 of 8): the first cut off rather than rounded, so that no
-// finite x becomes infinite, the others rounded.  Of a value that is not finite only h is kept.
-__device__ __forceinline__ void split_f32(float x, bf16& h, bf16& m, bf16& l) {
-  const uint32_t u = __float_as_uint(x);
-  const float hf = __uint_as_float(u & 0xFFFF0000u);
-  const bool fin = (u & 0x7F800000u) != 0x7F800000u;
-  // A NaN whose payload lies in the low half would become infinite when cut.
-  h = fin ? (bf16)hf : (bf16)x;
-  const float r = fin ? x - hf : 0.0f;
-  m = (bf16)r;
-  l = (bf16)(r - (float)m);
+// finite x becomes infinite, the others rounded.  Of a value that is not finite, m and l are NaN.  Two values at a time,
+// the first in the low halves.
+__device__ __forceinline__ void split2(float x, float y, uint32_t& h, uint32_t& m, uint32_t& l) {
+  const uint32_t xh = __float_as_uint(x) & 0xFFFF0000u, yh = __float_as_uint(y) & 0xFFFF0000u;
+  h = __builtin_amdgcn_perm(__float_as_uint(y), __float_as_uint(x), 0x07060302u);  // the high halves
+  const f32x2 r = {x - __uint_as_float(xh), y - __uint_as_float(yh)};
+  m = __builtin_bit_cast(uint32_t, __builtin_convertvector(r, bf16x2));
+  const f32x2 q = {r[0] - __uint_as_float(m << 16), r[1] - __uint_as_float(m & 0xFFFF0000u)};
+  l = __builtin_bit_cast(uint32_t, __builtin_convertvector(q, bf16x2));
+}
+typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
+typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
+__device__ __forceinline__ void split8(const f32x8& v, bf16x8& h, bf16x8& m, bf16x8& l) {
+  u32x4 a, b, c;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    uint32_t x, y, z;
+    split2(v[2 * i], v[2 * i + 1], x, y, z);
+    a[i] = x, b[i] = y, c[i] = z;
+  }
+  h = __builtin_bit_cast(bf16x8, a), m = __builtin_bit_cast(bf16x8, b), l = __builtin_bit_cast(bf16x8, c);
+}
+__device__ __forceinline__ void split4(const f32x4& v, bf16x4& h, bf16x4& m, bf16x4& l) {
+  u32x2 a, b, c;
+#pragma unroll
+  for (int i = 0; i < 2; ++i) {
+    uint32_t x, y, z;
+    split2(v[2 * i], v[2 * i + 1], x, y, z);
+    a[i] = x, b[i] = y, c[i] = z;
+  }
+  h = __builtin_bit_cast(bf16x4, a), m = __builtin_bit_cast(bf16x4, b), l = __builtin_bit_cast(bf16x4, c);
 }
 
 // One operand of a product.  k_contig: element (r, k) at p[r ld + k]; k strided: at p[k ld + r].  p is 16-byte aligned
@@ -124,12 +145,7 @@ __device__ __forceinline__ Frag<T> to_planes(const f32x8& v) {
   if constexpr (sizeof(T) == 2) {
     f.p[0] = to_bf16x8(v);
   } else {
-#pragma unroll
-    for (int e = 0; e < 8; ++e) {
-      bf16 h, m, l;
-      split_f32(v[e], h, m, l);
-      f.p[0][e] = h, f.p[1][e] = m, f.p[2][e] = l;
-    }
+    split8(v, f.p[0], f.p[1], f.p[2]);
   }
   return f;
 }
@@ -183,6 +199,7 @@ __device__ __forceinline__ void landed_barrier() {
 // Rows of a B fragment are taken in the order b_row (below): their low bits differ elsewhere.
 template <bool KC, bool ISB, int CHUNKS>
 __device__ __forceinline__ int tile_swizzle(int row) {
+  if constexpr (KC && CHUNKS == 4) return (row >> (ISB ? 3 : 2)) & 3;  // rows of 64 bytes: four of them span the banks
   if constexpr (KC && ISB) return (row & 3) | (((row >> 3) & 1) << 2);
   if constexpr (KC) return row & 7;
   return (ISB ? 4 * (row & 3) : 2 * (row & 3)) & (CHUNKS - 1);
@@ -191,10 +208,10 @@ __device__ __forceinline__ int tile_swizzle(int row) {
 // fragment pair (rows 4 (lane / 16) + r of each) are then eight consecutive columns, one 16-byte bf16 store.
 __device__ __forceinline__ int b_row(int f, int i) { return 32 * (f >> 1) + 8 * (i >> 2) + 4 * (f & 1) + (i & 3); }
 
-template <int R, int NT, bool KC, bool ISB>
+template <int R, int NT, bool KC, bool ISB, int BK = kGemmBK>
 struct TileLoad {
-  static constexpr int row_bytes = KC ? kGemmBK * 2 : R * 2;
-  static constexpr int rows = KC ? R : kGemmBK;
+  static constexpr int row_bytes = KC ? BK * 2 : R * 2;
+  static constexpr int rows = KC ? R : BK;
   static constexpr int rows_a_load = NT * 16 / row_bytes;
   static constexpr int loads = rows / rows_a_load;
   static constexpr int chunks = row_bytes / 16;
@@ -212,7 +229,7 @@ struct TileLoad {
     vstep = (uint32_t)((int64_t)rows_a_load * ld * 2);
     kc = chunk * 8;
   }
-  // Issues the loads of k0 .. k0 + 63 into the tile at `lds`.  r0: the tile's first row (m or n) of nr.  Reads beyond the
+  // Issues the loads of k0 .. k0 + BK - 1 into the tile at `lds`.  r0: the tile's first row (m or n) of nr.  Reads beyond the
   // operand give zeros: the buffer ends with its last group of eight, and a chunk past the end of k is sent beyond it.
   __device__ __forceinline__ void issue(const GemmOperand& o, int plane, int r0, int nr, int k0, int nk, lds_char* lds,
                                         int wave) const {
@@ -220,10 +237,10 @@ struct TileLoad {
     int64_t last;  // elements from base to the end of the last one wanted
     if constexpr (KC) {
       base += (int64_t)r0 * o.ld + k0;
-      last = (int64_t)(min(nr - r0, R) - 1) * o.ld + min(((nk + 7) & ~7) - k0, kGemmBK);
+      last = (int64_t)(min(nr - r0, R) - 1) * o.ld + min(((nk + 7) & ~7) - k0, BK);
     } else {
       base += (int64_t)k0 * o.ld + r0;
-      last = (int64_t)(min(nk - k0, kGemmBK) - 1) * o.ld + min(((nr + 7) & ~7) - r0, R);
+      last = (int64_t)(min(nk - k0, BK) - 1) * o.ld + min(((nr + 7) & ~7) - r0, R);
     }
     auto rsrc = __builtin_amdgcn_make_buffer_rsrc(const_cast<uint16_t*>(base), 0, (int)(last * 2), 0x00027000);
     const uint32_t off = (KC && kc >= nk - k0) ? 0x80000000u : voff;
@@ -235,7 +252,7 @@ struct TileLoad {
 };
 
 // A lane's fragments of 16 rows x 32 k (k half kk of the 64) from the tile at `lds`.
-template <int R, bool KC, bool ISB>
+template <int R, bool KC, bool ISB, int BK = kGemmBK>
 struct TileRead {
   uint32_t base;  // k contiguous: address of the lane's row and chunk in fragment 0; strided: the in-row part
   uint32_t rowp;  // strided: the row's part
@@ -243,7 +260,7 @@ struct TileRead {
     const int i = lane & 15, g = lane >> 4;
     if constexpr (KC) {
       const int row = ISB ? b_row(0, i) : i;
-      base = (first_row + row) * 128 + ((g ^ tile_swizzle<KC, ISB, 8>(row)) * 16);
+      base = (first_row + row) * BK * 2 + ((g ^ tile_swizzle<KC, ISB, BK / 8>(row)) * 16);
       rowp = 0;
     } else {
       const int s = tile_swizzle<KC, ISB, R / 8>(i >> 2);
@@ -258,7 +275,7 @@ struct TileRead {
     if constexpr (KC) {
       // In B, fragment 1 of a pair starts four rows on, which the permutation does not see.
       const int rows = ISB ? 32 * (f >> 1) + 4 * (f & 1) : 16 * f;
-      return *(lds_frag*)(lds + ((base ^ (kk * 64)) + rows * 128));
+      return *(lds_frag*)(lds + ((base ^ (kk * 64)) + rows * BK * 2));
     } else {
       // The permutation stays inside 128 bytes of A's rows and 256 of B's: what lies above is added as an immediate.
       const uint32_t in = ISB ? (base ^ ((f >> 1) * 64 & 255)) + (f & 1) * 8 + ((f >> 1) * 64 & ~255)
@@ -307,84 +324,149 @@ struct GemmWave {
 //
 // s0 and s1 are two variables of the kernel: the compiler then knows that the buffer being read is not the one being
 // filled and waits for loads only at the barriers.
+//
+// The smallest tiles hold all three planes of float32 operands for 32 k at a time and form the six products from them:
+// a barrier for 24 matrix instructions a wave instead of eight, and half the loads (4099 x 771 x 96 backward: see
+// head_gemm.hip).
+constexpr int kPlanesBK = 32;
+template <class T, int PAIRS>
+constexpr bool gemm_planes() { return PAIRS == 6 && T::BM == 64; }
+template <class T, int PAIRS>
+constexpr int gemm_stage() { return gemm_planes<T, PAIRS>() ? 3 * (T::BM + T::BN) * kPlanesBK * 2 : T::stage_bytes; }
+
+template <class T, bool AKC, bool BKC, class Acc>
+__device__ __forceinline__ void planes_products(const GemmArgs& g, Acc& acc, int m0, int n0, int kbeg, int kend, int wm, int wn,
+                                                char (&s0)[gemm_stage<T, 6>()], char (&s1)[gemm_stage<T, 6>()]) {
+  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  TileLoad<T::BM, T::threads, AKC, false, kPlanesBK> la;
+  TileLoad<T::BN, T::threads, BKC, true, kPlanesBK> lb;
+  la.init(g.a.ld, tid);
+  lb.init(g.b.ld, tid);
+  TileRead<T::BM, AKC, false, kPlanesBK> ra;
+  TileRead<T::BN, BKC, true, kPlanesBK> rb;
+  ra.init(lane, wm * (T::BM / T::WM));
+  rb.init(lane, wn * (T::BN / T::WN));
+  constexpr int pa = T::BM * kPlanesBK * 2, pb = T::BN * kPlanesBK * 2;  // bytes a plane
+  auto issue = [&](char* s, int k) {
+#pragma unroll
+    for (int p = 0; p < 3; ++p) {
+      la.issue(g.a, p, m0, g.m, k, g.k, (lds_char*)s + p * pa, wave);
+      lb.issue(g.b, p, n0, g.n, k, g.k, (lds_char*)s + 3 * pa + p * pb, wave);
+    }
+  };
+  auto work = [&](char* s) {
+    Frag<float> a[T::FM], b[T::FN];
+#pragma unroll
+    for (int p = 0; p < 3; ++p) {
+#pragma unroll
+      for (int i = 0; i < T::FN; ++i) b[i].p[p] = rb.get((const lds_char*)s + 3 * pa + p * pb, i, 0);
+#pragma unroll
+      for (int j = 0; j < T::FM; ++j) a[j].p[p] = ra.get((const lds_char*)s + p * pa, j, 0);
+    }
+#pragma unroll
+    for (int j = 0; j < T::FM; ++j)
+#pragma unroll
+      for (int i = 0; i < T::FN; ++i) acc[i][j] = mma(b[i], a[j], acc[i][j]);
+  };
+  if (kbeg < kend) issue(s0, kbeg);
+  int k = kbeg;
+  for (; k + kPlanesBK < kend; k += 2 * kPlanesBK) {
+    landed_barrier();
+    issue(s1, k + kPlanesBK);
+    work(s0);
+    landed_barrier();
+    if (k + 2 * kPlanesBK < kend) issue(s0, k + 2 * kPlanesBK);
+    work(s1);
+  }
+  if (k < kend) {
+    landed_barrier();
+    work(s0);
+  }
+}
+
 template <class T, bool AKC, bool BKC, int PAIRS, class Epi>
-__device__ __forceinline__ void gemm_tile(const GemmArgs& g, const Epi& epi, int wg, int wgs, char (&s0)[T::stage_bytes],
-                                          char (&s1)[T::stage_bytes]) {
+__device__ __forceinline__ void gemm_tile(const GemmArgs& g, const Epi& epi, int wg, int wgs, char (&s0)[gemm_stage<T, PAIRS>()],
+                                          char (&s1)[gemm_stage<T, PAIRS>()]) {
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int wm = wave / T::WN, wn = wave % T::WN;
   int tm, tn, sp;
   gemm_tile_of(g, wg, wgs, tm, tn, sp);
   const int m0 = tm * T::BM, n0 = tn * T::BN;
   const int kbeg = sp * g.k_per_split, kend = min(g.k, kbeg + g.k_per_split);
-  const int steps = max(0, (kend - kbeg + kGemmBK - 1) / kGemmBK) * PAIRS;
-
-  TileLoad<T::BM, T::threads, AKC, false> la;
-  TileLoad<T::BN, T::threads, BKC, true> lb;
-  la.init(g.a.ld, tid);
-  lb.init(g.b.ld, tid);
-  TileRead<T::BM, AKC, false> ra;
-  TileRead<T::BN, BKC, true> rb;
-  ra.init(lane, wm * (T::BM / T::WM));
-  rb.init(lane, wn * (T::BN / T::WN));
-  constexpr int boff = T::BM * kGemmBK * 2;
-
-  int pk = kbeg, pp = 0;  // the next stage to load
-  // The pairs of one k step follow one another, so a plane's tile is read again while it is in the L2.
-  auto issue = [&](char* s) {
-    const int qa = PAIRS == 1 ? 0 : pair_a(pp), qb = PAIRS == 1 ? 0 : pair_b(pp);
-    la.issue(g.a, qa, m0, g.m, pk, g.k, (lds_char*)s, wave);
-    lb.issue(g.b, qb, n0, g.n, pk, g.k, (lds_char*)s + boff, wave);
-    if (PAIRS == 1 || ++pp == PAIRS) {
-      pp = 0;
-      pk += kGemmBK;
-    }
-  };
-  struct Half {
-    bf16x8 a[T::FM], b[T::FN];
-  };
-  auto read = [&](Half& h, char* s, int kk) {
-#pragma unroll
-    for (int i = 0; i < T::FN; ++i) h.b[i] = rb.get((const lds_char*)s + boff, i, kk);
-#pragma unroll
-    for (int j = 0; j < T::FM; ++j) h.a[j] = ra.get((const lds_char*)s, j, kk);
-  };
   f32x4 acc[T::FN][T::FM];
 #pragma unroll
   for (int i = 0; i < T::FN; ++i)
 #pragma unroll
     for (int j = 0; j < T::FM; ++j) acc[i][j] = f32x4{0, 0, 0, 0};
-  auto multiply = [&](const Half& h) {
-#pragma unroll
-    for (int j = 0; j < T::FM; ++j)
-#pragma unroll
-      for (int i = 0; i < T::FN; ++i)
-        acc[i][j] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(h.b[i], h.a[j], acc[i][j], 0, 0, 0);
-  };
-  Half h0, h1;
   typename Epi::template Side<T> side;
-  // One step: the buffer `cur` holds it, `next` the following one; `more`: the one after that exists.
-  auto step = [&](char* cur, char* next, bool more) {
-    read(h1, cur, 1);
-    multiply(h0);
-    landed_barrier();
-    if (more) issue(cur);
-    read(h0, next, 0);
-    multiply(h1);
-  };
-  int left = steps;
-  if (left > 0) {
-    issue(s0);
-    side.fetch(epi, m0, n0, tid);  // what the epilogue needs from memory comes in behind the products
-    landed_barrier();
-    if (left > 1) issue(s1);
-    read(h0, s0, 0);
-    for (; left >= 2; left -= 2) {
-      step(s0, s1, left > 2);
-      step(s1, s0, left > 3);
-    }
-    if (left) step(s0, s1, false);
-  } else {
+  if constexpr (gemm_planes<T, PAIRS>()) {
     side.fetch(epi, m0, n0, tid);
+    planes_products<T, AKC, BKC>(g, acc, m0, n0, kbeg, kend, wm, wn, s0, s1);
+  } else {
+    const int steps = max(0, (kend - kbeg + kGemmBK - 1) / kGemmBK) * PAIRS;
+
+    TileLoad<T::BM, T::threads, AKC, false> la;
+    TileLoad<T::BN, T::threads, BKC, true> lb;
+    la.init(g.a.ld, tid);
+    lb.init(g.b.ld, tid);
+    TileRead<T::BM, AKC, false> ra;
+    TileRead<T::BN, BKC, true> rb;
+    ra.init(lane, wm * (T::BM / T::WM));
+    rb.init(lane, wn * (T::BN / T::WN));
+    constexpr int boff = T::BM * kGemmBK * 2;
+
+    int pk = kbeg, pp = 0;  // the next stage to load
+    // The pairs of one k step follow one another, so a plane's tile is read again while it is in the L2.
+    auto issue = [&](char* s) {
+      const int qa = PAIRS == 1 ? 0 : pair_a(pp), qb = PAIRS == 1 ? 0 : pair_b(pp);
+      la.issue(g.a, qa, m0, g.m, pk, g.k, (lds_char*)s, wave);
+      lb.issue(g.b, qb, n0, g.n, pk, g.k, (lds_char*)s + boff, wave);
+      if (PAIRS == 1 || ++pp == PAIRS) {
+        pp = 0;
+        pk += kGemmBK;
+      }
+    };
+    struct Half {
+      bf16x8 a[T::FM], b[T::FN];
+    };
+    auto read = [&](Half& h, char* s, int kk) {
+#pragma unroll
+      for (int i = 0; i < T::FN; ++i) h.b[i] = rb.get((const lds_char*)s + boff, i, kk);
+#pragma unroll
+      for (int j = 0; j < T::FM; ++j) h.a[j] = ra.get((const lds_char*)s, j, kk);
+    };
+    auto multiply = [&](const Half& h) {
+#pragma unroll
+      for (int j = 0; j < T::FM; ++j)
+#pragma unroll
+        for (int i = 0; i < T::FN; ++i)
+          acc[i][j] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(h.b[i], h.a[j], acc[i][j], 0, 0, 0);
+    };
+    Half h0, h1;
+    // One step: the buffer `cur` holds it, `next` the following one; `more`: the one after that exists.
+    auto step = [&](char* cur, char* next, bool more) {
+      read(h1, cur, 1);
+      multiply(h0);
+      landed_barrier();
+      if (more) issue(cur);
+      read(h0, next, 0);
+      multiply(h1);
+    };
+    int left = steps;
+    if (left > 0) {
+      issue(s0);
+      side.fetch(epi, m0, n0, tid);  // what the epilogue needs from memory comes in behind the products
+      landed_barrier();
+      if (left > 1) issue(s1);
+      read(h0, s0, 0);
+      for (; left >= 2; left -= 2) {
+        step(s0, s1, left > 2);
+        step(s1, s0, left > 3);
+      }
+      if (left) step(s0, s1, false);
+    } else {
+      side.fetch(epi, m0, n0, tid);
+    }
   }
   __syncthreads();
   const GemmWave<T> w{m0, n0, tm, tn, sp, wm, wn, lane, s1 + wave * (T::stage_bytes / T::waves)};
@@ -394,8 +476,8 @@ __device__ __forceinline__ void gemm_tile(const GemmArgs& g, const Epi& epi, int
 // Registers for two waves a SIMD: one workgroup of 256 x 256 a CU, two of 128 x 128.
 template <class T, bool AKC, bool BKC, int PAIRS, class Epi>
 __global__ __launch_bounds__(T::threads, 2) void gemm_kernel(GemmArgs g, Epi epi) {
-  __shared__ __attribute__((aligned(1024))) char s0[T::stage_bytes];
-  __shared__ __attribute__((aligned(1024))) char s1[T::stage_bytes];
+  __shared__ __attribute__((aligned(1024))) char s0[gemm_stage<T, PAIRS>()];
+  __shared__ __attribute__((aligned(1024))) char s1[gemm_stage<T, PAIRS>()];
   gemm_tile<T, AKC, BKC, PAIRS>(g, epi, blockIdx.x, gridDim.x, s0, s1);
 }
 
@@ -403,8 +485,8 @@ __global__ __launch_bounds__(T::threads, 2) void gemm_kernel(GemmArgs g, Epi epi
 // others w (both strided).
 template <class T, int PAIRS, class Epi>
 __global__ __launch_bounds__(T::threads, 2) void gemm_pair_kernel(GemmArgs x, Epi ex, int x_wgs, GemmArgs w, Epi ew) {
-  __shared__ __attribute__((aligned(1024))) char s0[T::stage_bytes];
-  __shared__ __attribute__((aligned(1024))) char s1[T::stage_bytes];
+  __shared__ __attribute__((aligned(1024))) char s0[gemm_stage<T, PAIRS>()];
+  __shared__ __attribute__((aligned(1024))) char s1[gemm_stage<T, PAIRS>()];
   const int b = blockIdx.x;
   if (b < x_wgs)
     gemm_tile<T, true, false, PAIRS>(x, ex, b, x_wgs, s0, s1);
