@@ -107,6 +107,7 @@ struct ProductJob {
   GemmOperand a, b;
   bool a_kc, b_kc;
   Finish f;
+  bool asked = true;  // false: only planned, so that the other's plan does not depend on what is asked for
 };
 // out[c] = sum over the parts of part[p * stride + c], c < cols, added in a fixed order; f32 0: rounded to bf16.
 struct ColumnSum {
@@ -125,8 +126,8 @@ struct SplitJob {
 // Up to two such products (part NULL: none) and column sums (NULL: none), in one launch.
 fgpu_status launch_join(const SplitJob& a, const SplitJob& b, const ColumnSum* sums, bool f32, hipStream_t s);
 
-// The products (one, or an input's gradient followed by a weight's), then what joins split products and the column sums
-// (NULL: none): one launch for the products where they are small, one to join where there is something to join.
+// The products (one, or an input's gradient followed by a weight's, either not asked for), then what joins split products
+// and the column sums (NULL: none): one launch for the products where they are small, one to join where there is something to join.
 size_t products_workspace_bytes(const Product* p, int count);
 fgpu_status launch_products(const ProductJob* jobs, int count, const ColumnSum* sums, void* ws, hipStream_t s);
 double products_estimate_us(const Product* p, int count);  // the time that the rule between kernels goes by

@@ -306,12 +306,13 @@ double tile_steps(int64_t m, int64_t n, int64_t k) { return (double)ceil_div(m, 
 double direct_forward_estimate_us(const Product& p) {
   if (p.m <= 16) return p.f32 ? 7.5 : 4.5;
   // Rows that are not whole 16-byte groups load at half the rate or less.
-  return 3 + std::max<double>(wave_steps(p.k), tile_steps(p.m, p.n, p.k)) * (p.f32 ? 2.6 : 0.95) * (p.k % 8 ? (p.f32 ? 1.2 : 2.4) : 1);
+  return 3 + std::max<double>(wave_steps(p.k), tile_steps(p.m, p.n, p.k)) * (p.f32 ? 2.2 : 0.95) * (p.k % 8 ? (p.f32 ? 1.2 : 2.4) : 1);
 }
 double direct_backward_estimate_us(int rows, int in_dim, int out_dim, bool f32) {
   const int longest = std::max(wave_steps(out_dim), wave_steps(rows));
   const double all = tile_steps(rows, in_dim, out_dim) + tile_steps(out_dim, in_dim, rows);
-  return f32 ? 4 + 3.6 * longest + 2.5 * all : 3 + 2.4 * longest + 1.2 * all;
+  const double ragged = in_dim % 8 || out_dim % 8 ? 1.3 : 1;
+  return f32 ? 2 + (1.8 * longest + 2.2 * all) * ragged : 2.5 + (1.0 * longest + 0.6 * all) * ragged;
 }
 
 }  // namespace fgpu

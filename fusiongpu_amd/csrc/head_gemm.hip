@@ -184,15 +184,17 @@ struct Plan {
 };
 // Microseconds of a product on `tile` tiles with k in `splits` parts.  A workgroup's k step takes `alone` while few share
 // a CU and `shared` for each that does (measured: 256 x 256 1.6 / 1.6 at one a CU, 128 x 128 0.64 / 0.5 at two, 64 x 64
-// 0.35 / 0.21 at five), its start and epilogue `fixed`; the parts of a split product are written and read once more.
+// 0.35 / 0.21 at five; float32's six plane products six times that, but 1.2 / 0.63 at three for 64 x 64, which holds all
+// planes), its start and epilogue `fixed`; the parts of a split product are written and read once more.
 Plan plan_at(const Product& p, int tile, int splits) {
   Plan q{tile, ceil_div(p.m, tile), ceil_div(p.n, tile), splits, 0, 0};
   const int steps = ceil_div(p.k, kGemmBK), per = ceil_div(steps, splits);
   q.k_per_split = per * kGemmBK;
   q.splits = ceil_div(p.k, q.k_per_split);
-  const double alone = tile == 256 ? 1.6 : tile == 128 ? 0.64 : 0.35, shared = tile == 256 ? 1.6 : tile == 128 ? 0.5 : 0.21;
+  const double alone = tile == 256 ? 1.6 : tile == 128 ? 0.64 : p.f32 ? 0.2 : 0.35;
+  const double shared = tile == 256 ? 1.6 : tile == 128 ? 0.5 : p.f32 ? 0.105 : 0.21;
   const double fixed = tile == 256 ? 8 : tile == 128 ? 4 : 3;
-  const int most = tile == 256 ? 1 : tile == 128 ? 2 : 5;
+  const int most = tile == 256 ? 1 : tile == 128 ? 2 : p.f32 ? 3 : 5;
   const int64_t wgs = (int64_t)q.tiles_m * q.tiles_n * q.splits, full = wgs / (256 * most), rest = wgs % (256 * most);
   const double k = (double)per * (p.f32 ? 6 : 1);
   q.us = full * (k * std::max(alone, most * shared) + fixed);
@@ -212,11 +214,18 @@ Plan plan_of(const Product& p, int only = 0) {
   }
   return best;
 }
-// Two products run in one launch where each by itself takes the same of the smaller tiles: a gradient's bits then do not
-// depend on whether the other is asked for.
+// Two products run in one launch, with one tile for both, where that costs less than their own tiles and a launch more.
+constexpr double kLaunchUs = 3;
 int plans_of(const Product* p, int count, Plan* q) {
   for (int i = 0; i < count; ++i) q[i] = plan_of(p[i]);
-  return count == 2 && q[0].tile == q[1].tile && q[0].tile != 256 ? q[0].tile : 0;
+  if (count == 1) return 0;
+  double us = q[0].us + q[1].us;
+  int pair = 0;
+  for (int tile : {128, 64}) {
+    const Plan a = plan_of(p[0], tile), b = plan_of(p[1], tile);
+    if (a.us + b.us - kLaunchUs < us) us = a.us + b.us - kLaunchUs, pair = tile, q[0] = a, q[1] = b;
+  }
+  return pair;
 }
 
 template <class T, bool AKC, bool BKC, int PAIRS, class E>
@@ -260,7 +269,7 @@ fgpu_status run_products(const ProductJob* jobs, int count, const Plan* q, int p
     // (65536 x 4096 x 1024 with its pre-activation 731 -> 624 us; at 134 MB it would cost 102 -> 128 us).
     f[i].stream = (int64_t)j.p.m * j.p.n * (int64_t)sizeof(O) * (j.f.pre ? 2 : 1) > (int64_t)256 << 20;
   }
-  if (pair) {
+  if (pair && jobs[0].asked && jobs[1].asked) {
     const ProductEpi<O, FGPU_ACT_NONE> ex{f[0], part[0], g[0].m, g[0].n}, ew{f[1], part[1], g[1].m, g[1].n};
     const int nx = g[0].tiles_m * g[0].tiles_n * g[0].splits, nw = g[1].tiles_m * g[1].tiles_n * g[1].splits;
     if (pair == 128)
@@ -270,7 +279,7 @@ fgpu_status run_products(const ProductJob* jobs, int count, const Plan* q, int p
     FGPU_HIP(hipGetLastError());
   } else {
     for (int i = 0; i < count; ++i)
-      FGPU_TRY((run_form<PAIRS, O>(jobs[i].a_kc, jobs[i].b_kc, q[i].tile, g[i], f[i], part[i], s)));
+      if (jobs[i].asked) FGPU_TRY((run_form<PAIRS, O>(jobs[i].a_kc, jobs[i].b_kc, q[i].tile, g[i], f[i], part[i], s)));
   }
   SplitJob sj[2];
   for (int i = 0; i < count; ++i)
@@ -304,7 +313,7 @@ double products_estimate_us(const Product* p, int count) {
   const int pair = plans_of(p, count, q);
   double us = 0;
   for (int i = 0; i < count; ++i) us += q[i].us;
-  return pair ? us - 3 : us;
+  return pair ? us - kLaunchUs : us;
 }
 
 fgpu_status launch_products(const ProductJob* jobs, int count, const ColumnSum* sums, void* ws, hipStream_t s) {
@@ -315,7 +324,7 @@ fgpu_status launch_products(const ProductJob* jobs, int count, const ColumnSum* 
   float* part[2] = {nullptr, nullptr};
   char* at = static_cast<char*>(ws);
   for (int i = 0; i < count; ++i) {
-    const size_t b = parts_bytes(p[i], q[i]);
+    const size_t b = jobs[i].asked ? parts_bytes(p[i], q[i]) : 0;
     if (b) part[i] = reinterpret_cast<float*>(at);
     at += b;
   }

@@ -18,9 +18,10 @@ DirectOperand direct(const void* p, int64_t rows, int64_t cols, const void* pre 
 
 // Whether the products of few tiles take the direct kernels (head_direct.hip): by the estimates of both, fitted to
 // measurements; a launch is priced at 2.7 us, what a caller pays for it in a row of small calls.  Measured on the GPU alone
-// (us, tiled / direct): forward bf16 1 x 1024 x 1024 (rows, in, out) 5.8 / 4.2, 128 x 768 x 2048 6.5 / 6.3, 512 x 1024 x
-// 1024 7.6 / 10.9; float32 128 x 768 x 2048 22 / 12, 1024^3 36 / 44; backward bf16 128^3 10.6 / 5.7, 256 x 1024 x 1024
-// 17 / 21; float32 400 x 256 x 256 17 / 11, 128 x 768 x 2048 30 / 46.
+// (us, tiled / direct): forward bf16 1 x 1024 x 1024 (rows, in, out) 7.4 / 5.3, 128 x 1024 x 1024 9.4 / 8.0, 512 x 1024 x
+// 1024 8.5 / 12; float32 128 x 768 x 2048 22 / 11, 512 x 1024 x 1024 27 / 21, 1024^3 33 / 38; backward bf16 400 x 256 x 256
+// 11.5 / 6.1, 256 x 1024 x 1024 15 / 11, 512 x 1024 x 1024 15.7 / 16.0, 1024^3 19 / 25; float32 400 x 256 x 256 18 / 8.8,
+// 777 x 333 x 555 26 / 21, 512 x 1024 x 1024 36 / 46.
 constexpr double kLaunch = 2.7;
 bool forward_direct(const Product& p) {
   double tiled = products_estimate_us(&p, 1);
@@ -91,8 +92,7 @@ size_t fgpu_linear_backward_workspace_bytes(int64_t rows, int in_dim, int out_di
   if (backward_direct(p[0], p[1])) return 0;
   size_t b = packed_bytes(rows, out_dim, f32) + carve_bytes<float>((size_t)dz_chunks((int)rows, out_dim) * out_dim);
   if (needs_pack(in_dim, f32)) b += packed_bytes(rows, in_dim, f32) + packed_bytes(out_dim, in_dim, f32);
-  // Either product alone may split k further than the two together.
-  return b + std::max({products_workspace_bytes(p, 2), products_workspace_bytes(p, 1), products_workspace_bytes(p + 1, 1)});
+  return b + products_workspace_bytes(p, 2);
 }
 
 fgpu_status fgpu_linear_backward(const void* d_dy, const void* d_x, const void* d_w, const void* d_pre, int64_t rows,
@@ -144,17 +144,13 @@ fgpu_status fgpu_linear_backward(const void* d_dy, const void* d_x, const void* 
     x = packed(ws.take<char>(packed_bytes(rows, in_dim, f32)), rows, in_dim);
     prep.copy[1] = {d_x, rows, in_dim, x};
   }
-  ProductJob jobs[2];
-  Product ps[2];
-  int count = 0;
-  if (d_dx) jobs[count++] = {px, z, w, true, false, fx};
-  if (d_dw) jobs[count++] = {pw, z, x, false, false, fw};
-  for (int i = 0; i < count; ++i) ps[i] = jobs[i].p;
-  void* parts = ws.take<char>(count ? products_workspace_bytes(ps, count) : 0);
+  const ProductJob jobs[2] = {{px, z, w, true, false, fx, d_dx != nullptr}, {pw, z, x, false, false, fw, d_dw != nullptr}};
+  const Product ps[2] = {px, pw};
+  void* parts = ws.take<char>(products_workspace_bytes(ps, 2));
   FGPU_CHECK(ws.ok(), FGPU_ERR_WORKSPACE, "linear backward: workspace smaller than fgpu_linear_backward_workspace_bytes");
   FGPU_TRY(launch_prep(prep, f32, s));
-  if (count == 0) return d_db ? launch_column_sums(sums, nullptr, s) : FGPU_OK;
-  return launch_products(jobs, count, d_db ? &sums : nullptr, parts, s);
+  if (!d_dx && !d_dw) return d_db ? launch_column_sums(sums, nullptr, s) : FGPU_OK;
+  return launch_products(jobs, 2, d_db ? &sums : nullptr, parts, s);
 }
 
 }  // extern "C"

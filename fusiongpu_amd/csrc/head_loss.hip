@@ -292,13 +292,13 @@ int64_t most_columns(int nq, int nc) {
   const int64_t most = std::min<int64_t>((int64_t)1 << 20, ((int64_t)1 << 31) / std::max(1, nq));
   return std::min<int64_t>(nc, most / 256 * 256);
 }
-// Room for the products of a chunk of `step` columns and of the last, shorter one, for both gradients or one.
+// Room for the products of a chunk of `step` columns and of the last, shorter one.
 size_t chunk_products_bytes(int nq, int nc, int dim, bool f32, int step) {
   size_t most = 0;
   for (int n : {step, nc % step}) {
     if (n == 0) continue;
     const Product p[2] = {{nq, dim, n, f32, step < nc}, {n, dim, nq, f32}};
-    most = std::max({most, products_workspace_bytes(p, 2), products_workspace_bytes(p, 1), products_workspace_bytes(p + 1, 1)});
+    most = std::max(most, products_workspace_bytes(p, 2));
   }
   return most;
 }
@@ -447,22 +447,16 @@ fgpu_status fgpu_contrastive_loss_backward(const float* d_dloss, const void* d_q
     FGPU_TRY(f32 ? (past ? grad(yes, yes) : grad(yes, no)) : (past ? grad(no, yes) : grad(no, no)));
     ColumnSum sums;
     sums.part = dbias_part, sums.parts = sp.tiles_m, sums.stride = sums.cols = n, sums.out = d_dbias ? d_dbias + c0 : nullptr;
-    ProductJob jobs[2];
-    int count = 0;
-    if (d_dq) {
-      Finish f;
-      f.out = d_dq, f.alpha = scale;
-      f.add = c0 > 0 ? dq_sum : nullptr;
-      f.sum = c0 + n < nc ? dq_sum : nullptr;
-      jobs[count++] = {{nq, dim, n, f32, step < nc}, g, cc, true, false, f};
-    }
-    if (d_dc) {
-      Finish f;
-      f.out = static_cast<char*>(d_dc) + (int64_t)c0 * dim * (f32 ? 4 : 2), f.alpha = scale;
-      jobs[count++] = {{n, dim, nq, f32}, g, q, false, false, f};
-    }
-    if (count)
-      FGPU_TRY(launch_products(jobs, count, d_dbias ? &sums : nullptr, pw, s));
+    Finish fq, fc;
+    fq.out = d_dq, fq.alpha = scale;
+    fq.add = c0 > 0 ? dq_sum : nullptr;
+    fq.sum = c0 + n < nc ? dq_sum : nullptr;
+    if (d_dc) fc.out = static_cast<char*>(d_dc) + (int64_t)c0 * dim * (f32 ? 4 : 2);
+    fc.alpha = scale;
+    const ProductJob jobs[2] = {{{nq, dim, n, f32, step < nc}, g, cc, true, false, fq, d_dq != nullptr},
+                                {{n, dim, nq, f32}, g, q, false, false, fc, d_dc != nullptr}};
+    if (d_dq || d_dc)
+      FGPU_TRY(launch_products(jobs, 2, d_dbias ? &sums : nullptr, pw, s));
     else if (d_dbias)
       FGPU_TRY(launch_column_sums(sums, nullptr, s));
   }
