@@ -14,15 +14,18 @@ namespace fgpu {
 namespace {
 
 constexpr int kNWaves = 8, kNThreads = kNWaves * kWave;
-// Streamed vectors a tile: more work between two barriers where the planes leave room.
-constexpr int narrow_tile(bool f32) { return f32 ? 64 : 128; }
+// Streamed vectors a tile: more work between two barriers where the planes leave room.  `small`: the shape for few rows and
+// columns, whose half tiles of half the rows reach four times the CUs (bf16, 128 dims, wide / small: forward 1024 x 1024
+// 15 / 9.7 us, 4096 x 4096 20.0 / 19.6, 1024 x 65536 44 / 48; backward 1024 x 1024 23 / 20, 4096 x 4096 51 / 56, 1024 x
+// 65536 125 / 151).  bf16 alone: float32's wide shape has the smaller tiles already.
+constexpr int narrow_tile(bool f32, bool small) { return f32 || small ? 64 : 128; }
 constexpr int kNRowBytes = 256;       // of a tile's row in LDS: 128 dims
 enum { kStats = 0, kDq = 1, kDc = 2 };
 
 // Fragments of 16 rows a wave holds: two, but one where the gradient and the three planes of float32 rows of more than 64
 // dims would not fit the registers of two waves a SIMD.
-constexpr int narrow_frags(bool f32, int mode, int kb) { return f32 && mode != kStats && kb > 2 ? 1 : 2; }
-constexpr int narrow_block_rows(bool f32, int mode, int kb) { return 16 * kNWaves * narrow_frags(f32, mode, kb); }
+constexpr int narrow_frags(bool f32, bool small, int mode, int kb) { return small || (f32 && mode != kStats && kb > 2) ? 1 : 2; }
+constexpr int narrow_block_rows(bool f32, bool small, int mode, int kb) { return 16 * kNWaves * narrow_frags(f32, small, mode, kb); }
 int dim_blocks(int dim) { return dim <= 64 ? 2 : dim <= 96 ? 3 : 4; }
 
 struct NarrowArgs {
@@ -55,16 +58,18 @@ struct CandidateSide {  // as ColumnSide reads it
   const int* col_id;
 };
 
-template <class T>
-constexpr int narrow_stage() { return Frag<T>::planes * narrow_tile(sizeof(T) == 4) * kNRowBytes; }
+template <class T, bool SMALL>
+constexpr int narrow_stage() { return Frag<T>::planes * narrow_tile(sizeof(T) == 4, SMALL) * kNRowBytes; }
+template <class T, bool SMALL>
+using Streamed = StreamSide<narrow_tile(sizeof(T) == 4, SMALL)>;
 
-template <class T, int KB, int MODE>
-__device__ __forceinline__ void narrow_rows(const NarrowArgs& g, int wg, int wgs, char (&s0)[narrow_stage<T>()],
-                                            char (&s1)[narrow_stage<T>()], StreamSide<narrow_tile(sizeof(T) == 4)>& d0,
-                                            StreamSide<narrow_tile(sizeof(T) == 4)>& d1) {
-  constexpr int kNTile = narrow_tile(sizeof(T) == 4);
+template <class T, int KB, int MODE, bool SMALL>
+__device__ __forceinline__ void narrow_rows(const NarrowArgs& g, int wg, int wgs, char (&s0)[narrow_stage<T, SMALL>()],
+                                            char (&s1)[narrow_stage<T, SMALL>()], Streamed<T, SMALL>& d0,
+                                            Streamed<T, SMALL>& d1) {
+  constexpr int kNTile = narrow_tile(sizeof(T) == 4, SMALL);
   constexpr int P = Frag<T>::planes, D = 2 * KB;  // D: 16-wide fragments of the gradient
-  constexpr int F = narrow_frags(P == 3, MODE, KB);
+  constexpr int F = narrow_frags(P == 3, SMALL, MODE, KB);
   typedef __attribute__((address_space(3))) const bf16x8 lds_frag;
   typedef __attribute__((address_space(3))) s16x4 lds_half;
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
@@ -317,49 +322,71 @@ __device__ __forceinline__ void narrow_rows(const NarrowArgs& g, int wg, int wgs
   }
 }
 
-#define FGPU_NARROW_LDS                                                                     \
-  __shared__ __attribute__((aligned(1024))) char s0[narrow_stage<T>()]; \
-  __shared__ __attribute__((aligned(1024))) char s1[narrow_stage<T>()]; \
-  __shared__ StreamSide<narrow_tile(sizeof(T) == 4)> d0, d1
+#define FGPU_NARROW_LDS                                                        \
+  __shared__ __attribute__((aligned(1024))) char s0[narrow_stage<T, SMALL>()]; \
+  __shared__ __attribute__((aligned(1024))) char s1[narrow_stage<T, SMALL>()]; \
+  __shared__ Streamed<T, SMALL> d0, d1
 
 // bf16: registers for two workgroups a CU.
-template <class T, int KB>
+template <class T, int KB, bool SMALL>
 __global__ __launch_bounds__(kNThreads, sizeof(T) == 2 ? 4 : 2) void narrow_stats_kernel(NarrowArgs g) {
   FGPU_NARROW_LDS;
-  narrow_rows<T, KB, kStats>(g, blockIdx.x, gridDim.x, s0, s1, d0, d1);
+  narrow_rows<T, KB, kStats, SMALL>(g, blockIdx.x, gridDim.x, s0, s1, d0, d1);
 }
 // The first q_wgs workgroups form dq, the others dc and dbias.
-template <class T, int KB>
+template <class T, int KB, bool SMALL>
 __global__ __launch_bounds__(kNThreads, 2) void narrow_backward_kernel(NarrowArgs q, int q_wgs, NarrowArgs c) {
   FGPU_NARROW_LDS;
   const int b = blockIdx.x;
   if (b < q_wgs)
-    narrow_rows<T, KB, kDq>(q, b, q_wgs, s0, s1, d0, d1);
+    narrow_rows<T, KB, kDq, SMALL>(q, b, q_wgs, s0, s1, d0, d1);
   else
-    narrow_rows<T, KB, kDc>(c, b - q_wgs, gridDim.x - q_wgs, s0, s1, d0, d1);
+    narrow_rows<T, KB, kDc, SMALL>(c, b - q_wgs, gridDim.x - q_wgs, s0, s1, d0, d1);
 }
 #undef FGPU_NARROW_LDS
 
+struct NarrowPlan {
+  bool small;
+  int tile, block_rows, splits;
+  double us;
+};
 // Splits of the streamed side: enough workgroups for `cus` CUs in even rounds, each tile at `tile_us`, the parts of a split
-// gradient written and read once more.
-int splits_of(int nr, int ns, int tile, int block_rows, int cus, double tile_us, double part_bytes, int most) {
-  const int blocks = ceil_div(nr, block_rows), tiles = ceil_div(ns, tile);
-  int best = 1;
-  double least = 0;
+// gradient written and read once more (1.5 TB/s at the sizes where it counts).  The small shape's two gradients share one
+// round between them.
+NarrowPlan plan_at(int nr, int ns, bool f32, bool small, int mode, int kb, int cus, double tile_us, double part_bytes, int most) {
+  NarrowPlan best{small, narrow_tile(f32, small), narrow_block_rows(f32, small, mode, kb), 0, 0};
+  const int blocks = ceil_div(nr, best.block_rows), tiles = ceil_div(ns, best.tile);
   for (int s = 1; s <= std::min(tiles, most); ++s) {
-    const double us = ceil_div((int64_t)blocks * s, cus) * (ceil_div(tiles, s) * tile_us + 4) + (s > 1 ? s * part_bytes / 3e6 : 0);
-    if (s == 1 || us < least) best = s, least = us;
+    const int64_t wgs = (int64_t)blocks * s;
+    int rounds = ceil_div(wgs, cus);
+    if (small && mode != kStats && wgs > cus / 2) rounds = std::max(2, rounds);
+    const double us = rounds * (ceil_div(tiles, s) * tile_us + (small ? 2.5 : 4)) + (s > 1 ? s * part_bytes / 1.5e6 : 0);
+    if (s == 1 || us < best.us) best.splits = s, best.us = us;
   }
   return best;
 }
-void set_splits(NarrowArgs& g, int tile, int block_rows, int splits) {
-  g.row_blocks = ceil_div(g.nr, block_rows);
-  g.tiles_per_split = ceil_div(ceil_div(g.ns, tile), splits);
-  g.splits = ceil_div(ceil_div(g.ns, tile), g.tiles_per_split);
+void set_splits(NarrowArgs& g, const NarrowPlan& p) {
+  g.row_blocks = ceil_div(g.nr, p.block_rows);
+  g.tiles_per_split = ceil_div(ceil_div(g.ns, p.tile), p.splits);
+  g.splits = ceil_div(ceil_div(g.ns, p.tile), g.tiles_per_split);
 }
-int gradient_splits(int nr, int ns, int dim, bool f32, int most) {
-  return splits_of(nr, ns, narrow_tile(f32), narrow_block_rows(f32, kDq, dim_blocks(dim)), 256, f32 ? 5.0 : 4.0,
-                   4.0 * nr * ((dim + 3) & ~3), most);
+NarrowPlan stats_plan(int nq, int nc, bool f32) {
+  if (f32) return plan_at(nq, nc, true, false, kStats, 0, 256, 2.5, 8.0 * nq, 512);
+  const NarrowPlan a = plan_at(nq, nc, false, false, kStats, 0, 512, 3.0, 8.0 * nq, 512);
+  const NarrowPlan b = plan_at(nq, nc, false, true, kStats, 0, 512, 1.2, 8.0 * nq, 512);
+  return b.us < a.us ? b : a;
+}
+// Of both gradients, whichever is asked for: their shape is one, and what is not asked for does not change the other's bits.
+void gradient_plans(int nq, int nc, int dim, bool f32, int most, NarrowPlan& q, NarrowPlan& c) {
+  const int kb = dim_blocks(dim);
+  const double row_bytes = 4.0 * ((dim + 3) & ~3);
+  for (bool small : {false, true}) {
+    if (small && f32) break;
+    const double tile_us = f32 ? 5.0 : small ? 1.65 : 5.1;
+    const NarrowPlan a = plan_at(nq, nc, f32, small, kDq, kb, 256, tile_us, nq * row_bytes, most);
+    const NarrowPlan b = plan_at(nc, nq, f32, small, kDc, kb, 256, tile_us, nc * row_bytes, most);
+    if (!small || a.us + b.us < q.us + c.us) q = a, c = b;
+  }
 }
 
 template <class F>
@@ -375,22 +402,23 @@ fgpu_status by_blocks(int dim, F&& f) {
 int narrow_stats_splits(int nq, int nc, bool f32) {
   NarrowArgs g{};
   g.nr = nq, g.ns = nc;
-  const int rows = narrow_block_rows(f32, kStats, 0);
-  set_splits(g, narrow_tile(f32), rows,
-             splits_of(nq, nc, narrow_tile(f32), rows, f32 ? 256 : 512, f32 ? 2.5 : 3.0, 8.0 * nq, 512));
+  set_splits(g, stats_plan(nq, nc, f32));
   return g.splits;
 }
 
 fgpu_status launch_narrow_stats(const LossArgs& a, const GemmOperand& q, const GemmOperand& c, int dim, bool f32, int splits,
                                 f32x2* part, float* target2, hipStream_t s) {
+  NarrowPlan plan = stats_plan(a.nq, a.nc, f32);
+  plan.splits = splits;
   NarrowArgs g{};
   g.r = q, g.s = c, g.nr = a.nq, g.ns = a.nc, g.dim = dim, g.a = a, g.stats = part, g.target2 = target2;
-  set_splits(g, narrow_tile(f32), narrow_block_rows(f32, kStats, 0), splits);
+  set_splits(g, plan);
   return by_blocks(dim, [&](auto kb) -> fgpu_status {
     constexpr int KB = decltype(kb)::value;
     const int grid = g.row_blocks * g.splits;
-    if (f32) narrow_stats_kernel<float, KB><<<grid, kNThreads, 0, s>>>(g);
-    else narrow_stats_kernel<bf16, KB><<<grid, kNThreads, 0, s>>>(g);
+    if (f32) narrow_stats_kernel<float, KB, false><<<grid, kNThreads, 0, s>>>(g);
+    else if (plan.small) narrow_stats_kernel<bf16, KB, true><<<grid, kNThreads, 0, s>>>(g);
+    else narrow_stats_kernel<bf16, KB, false><<<grid, kNThreads, 0, s>>>(g);
     FGPU_HIP(hipGetLastError());
     return FGPU_OK;
   });
@@ -398,7 +426,9 @@ fgpu_status launch_narrow_stats(const LossArgs& a, const GemmOperand& q, const G
 
 size_t narrow_backward_bytes(int nq, int nc, int dim, bool f32, int most_splits) {
   const size_t d4 = (dim + 3) & ~3;
-  const int sq = gradient_splits(nq, nc, dim, f32, most_splits), sc = gradient_splits(nc, nq, dim, f32, most_splits);
+  NarrowPlan pq, pc;
+  gradient_plans(nq, nc, dim, f32, most_splits, pq, pc);
+  const int sq = pq.splits, sc = pc.splits;
   return (sq > 1 ? carve_bytes<float>((size_t)sq * nq * d4) : 0) +
          (sc > 1 ? carve_bytes<float>((size_t)sc * nc * d4) + carve_bytes<float>((size_t)sc * nc) : 0);
 }
@@ -406,7 +436,8 @@ size_t narrow_backward_bytes(int nq, int nc, int dim, bool f32, int most_splits)
 fgpu_status launch_narrow_backward(const NarrowBackward& b, int most_splits, void* ws, hipStream_t s) {
   const int nq = b.a.nq, nc = b.a.nc;
   const size_t d4 = (b.dim + 3) & ~3;
-  const int block_rows = narrow_block_rows(b.f32, kDq, dim_blocks(b.dim));
+  NarrowPlan pq, pc;
+  gradient_plans(nq, nc, b.dim, b.f32, most_splits, pq, pc);
   char* at = static_cast<char*>(ws);
   auto take = [&](size_t floats) {
     float* p = reinterpret_cast<float*>(at);
@@ -421,22 +452,20 @@ fgpu_status launch_narrow_backward(const NarrowBackward& b, int most_splits, voi
   c.r = b.c, c.s = b.q, c.nr = nc, c.ns = nq;
   q.f.out = b.dq, c.f.out = b.dc, q.f.alpha = c.f.alpha = b.scale;
   if (b.dq) {
-    const int splits = gradient_splits(nq, nc, b.dim, b.f32, most_splits);
-    set_splits(q, narrow_tile(b.f32), block_rows, splits);
-    if (splits > 1) {
-      q.part = take((size_t)splits * nq * d4);
+    set_splits(q, pq);
+    if (pq.splits > 1) {
+      q.part = take((size_t)pq.splits * nq * d4);
       jq.part = q.part, jq.m = nq, jq.n = b.dim, jq.splits = q.splits, jq.f = q.f;
     }
   }
   if (b.dc || b.dbias) {
-    const int splits = gradient_splits(nc, nq, b.dim, b.f32, most_splits);
-    set_splits(c, narrow_tile(b.f32), block_rows, splits);
+    set_splits(c, pc);
     c.dbias = b.dbias;
-    if (splits > 1) {
-      c.part = take((size_t)splits * nc * d4);
+    if (pc.splits > 1) {
+      c.part = take((size_t)pc.splits * nc * d4);
       if (b.dc) jc.part = c.part, jc.m = nc, jc.n = b.dim, jc.splits = c.splits, jc.f = c.f;
       if (b.dbias) {
-        c.dbias = take((size_t)splits * nc);
+        c.dbias = take((size_t)pc.splits * nc);
         sums.part = c.dbias, sums.parts = c.splits, sums.stride = sums.cols = nc, sums.out = b.dbias;
         sum_up = true;
       }
@@ -446,8 +475,9 @@ fgpu_status launch_narrow_backward(const NarrowBackward& b, int most_splits, voi
   if (nwq + nwc == 0) return FGPU_OK;
   FGPU_TRY(by_blocks(b.dim, [&](auto kb) -> fgpu_status {
     constexpr int KB = decltype(kb)::value;
-    if (b.f32) narrow_backward_kernel<float, KB><<<nwq + nwc, kNThreads, 0, s>>>(q, nwq, c);
-    else narrow_backward_kernel<bf16, KB><<<nwq + nwc, kNThreads, 0, s>>>(q, nwq, c);
+    if (b.f32) narrow_backward_kernel<float, KB, false><<<nwq + nwc, kNThreads, 0, s>>>(q, nwq, c);
+    else if (pq.small) narrow_backward_kernel<bf16, KB, true><<<nwq + nwc, kNThreads, 0, s>>>(q, nwq, c);
+    else narrow_backward_kernel<bf16, KB, false><<<nwq + nwc, kNThreads, 0, s>>>(q, nwq, c);
     FGPU_HIP(hipGetLastError());
     return FGPU_OK;
   }));
