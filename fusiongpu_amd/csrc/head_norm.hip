@@ -1,4 +1,12 @@
 // head_norm.hip -- layer norm over the rows of [rows][dim], forward and backward.
+//
+// Forward: mean and variance of a row held in registers (two passes over the registers, one over memory: the variance is
+// that of the centred values), y = (x - mean) rstd gamma + beta.  Backward, with h = (x - mean) rstd and u = dy gamma:
+// dx = rstd (u - mean(u) - h mean(u h)), dgamma = sum of dy h, dbeta = sum of dy over the rows.
+//
+// Bound by HBM: every array passes once.  Measured: forward float32 100003 x 771 130 us (4.75 TB/s; a large copy reaches
+// 4.94), bf16 65536 x 1024 43 us (its output stays in the last-level cache); backward bf16 65536 x 1024 72 us + 4 us for
+// the column sums (5.3 TB/s), float32 153 us.  One row of 1024 takes 2.1 us, a launch's own time.
 #include <algorithm>
 #include <type_traits>
 

@@ -1,5 +1,8 @@
 // head_prep.hip -- what the products of the query head's operators need first, in one launch: operands copied where their
 // rows cannot be read as they are, dz with its column sums, the rows of the contrastive loss's backward pass.
+//
+// Bound by HBM: dz of 16384 x 4096 in bf16 (two arrays read, one written) takes 82 us, 4.9 TB/s.  It is formed once rather
+// than in both gradients' products, which read it in two orders and as many times as they have tiles beside it.
 #include <algorithm>
 
 #include "head.hpp"

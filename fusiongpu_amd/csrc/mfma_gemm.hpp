@@ -326,8 +326,8 @@ struct GemmWave {
 // filled and waits for loads only at the barriers.
 //
 // The smallest tiles hold all three planes of float32 operands for 32 k at a time and form the six products from them:
-// a barrier for 24 matrix instructions a wave instead of eight, and half the loads (4099 x 771 x 96 backward: see
-// head_gemm.hip).
+// a barrier for 24 matrix instructions a wave instead of eight, and half the loads (a 64-wide step of k 1.2 us instead of
+// 2.1 while a workgroup has its CU to itself; 1000 x 385 x 771 forward on them 23 us).
 constexpr int kPlanesBK = 32;
 template <class T, int PAIRS>
 constexpr bool gemm_planes() { return PAIRS == 6 && T::BM == 64; }

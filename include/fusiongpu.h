@@ -681,9 +681,11 @@ fgpu_status fgpu_contrastive_loss(const void* d_q, const void* d_c, const int32_
  * G_ij = dloss_i (exp(s_ij - lse_i) - [j = target_i]); dq = scale G c, dc = scale
  * G^T q, dbias_j = sum_i G_ij (float32).  Each of d_dq, d_dc, d_dbias may be
  * NULL (fixed candidates need no dc).  In bfloat16, G is rounded to bfloat16
- * before the two products (not before dbias).  G is held in the workspace, all
- * columns at once in the returned size (up to 2^31 elements); a smaller
- * workspace is used in chunks of columns, down to 256. */
+ * before the two products (not before dbias).  Above 128 dims G is held in the
+ * workspace, all columns at once in the returned size (up to 2^31 elements); a
+ * smaller workspace is used in chunks of columns, down to 256.  Up to 128 dims
+ * G never leaves the registers, and a smaller workspace (down to the copies of
+ * queries and candidates) splits the sums into fewer parts. */
 size_t fgpu_contrastive_loss_backward_workspace_bytes(int nq, int nc, int dim, int dtype);
 fgpu_status fgpu_contrastive_loss_backward(const float* d_dloss, const void* d_q, const void* d_c, const int32_t* d_target,
                                            const float* d_lse, const float* d_bias, const int32_t* d_ids, int nq, int nc,
