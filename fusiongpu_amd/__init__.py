@@ -208,8 +208,11 @@ def _on(stream):
     so memory freed when the call returns is only handed to later work on that
     same stream, never to other work while the kernels still read it."""
     if stream is None:
-        return contextlib.nullcontext()
+        return _NO_STREAM
     return _torch().cuda.stream(stream)
+
+
+_NO_STREAM = contextlib.nullcontext()
 
 
 def _stream():
@@ -993,7 +996,10 @@ def _act_code(act):
 
 def _head_first(a, name):
     """The array that decides a call's type, as a contiguous 16-byte-aligned device matrix."""
-    torch = _torch()
+    torch = _TORCH
+    if torch.is_tensor(a) and a.is_cuda and (a.dtype is torch.bfloat16 or a.dtype is torch.float32) and a.dim() == 2 \
+            and a.is_contiguous() and a.data_ptr() % 16 == 0:
+        return a
     if not (torch.is_tensor(a) and (a.dtype is torch.bfloat16 or a.dtype is torch.float32)):
         a = _arg(a, torch.float32, name, (None, None))
     return _head(a, a.dtype, name, (None, None))
@@ -1001,10 +1007,15 @@ def _head_first(a, name):
 
 def _head(a, dtype, name, shape):
     """`a` as a contiguous, 16-byte-aligned device tensor; its dtype must be `dtype`."""
-    torch = _torch()
-    if isinstance(a, np.ndarray):
+    torch = _TORCH
+    if isinstance(a, torch.Tensor):
+        if a.dtype is dtype and a.is_cuda and a.is_contiguous() and a.data_ptr() % 16 == 0:
+            have = a.shape  # nothing to convert: the shape is all that is left to check
+            if have == shape or (len(have) == 2 == len(shape) and shape[0] is None and have[1] == shape[1]):
+                return a
+    elif isinstance(a, np.ndarray):
         a = torch.from_numpy(np.ascontiguousarray(a))
-    elif not torch.is_tensor(a):
+    else:
         raise TypeError(f"{name}: expected a numpy array or a torch tensor, got {type(a).__name__}")
     if a.dtype is not dtype:
         raise TypeError(f"{name}: dtype {str(a.dtype).replace('torch.', '')}, expected "
@@ -1030,7 +1041,7 @@ def _ptr(t):
 
 def _head_out(out, like, shape, name="out"):
     if out is None:
-        return like.new_empty(shape)
+        return _TORCH.empty_like(like) if like.shape == shape else like.new_empty(shape)
     return _out(out, like.dtype, shape, name)
 
 
@@ -1043,9 +1054,8 @@ def _head_ws(nbytes, like):
 
 
 def _two_floats(rows, like):
-    torch = _torch()
-    return (torch.empty(rows, dtype=torch.float32, device=like.device),
-            torch.empty(rows, dtype=torch.float32, device=like.device))
+    a = _TORCH.empty(rows, dtype=_TORCH.float32, device=like.device)
+    return a, _TORCH.empty_like(a)
 
 
 def _dtype_code(t):
@@ -1178,9 +1188,12 @@ def contrastive_loss_backward(dloss, queries, candidates, targets, lse, scale: f
         dq = _head_out(None, q, (nq, dim))
         dc = _head_out(None, q, (nc, dim)) if candidate_grads else None
         db = torch.empty(nc, dtype=torch.float32, device=q.device) if candidate_grads else None
-        ws = workspace if workspace is not None else _workspace(
-            lib.fgpu_contrastive_loss_backward_workspace_bytes(nq, nc, dim, dt))
+        if workspace is not None:
+            wb = _ws_check(workspace)
+            wp = workspace.data_ptr()
+        else:
+            wp, wb, ws = _head_ws(lib.fgpu_contrastive_loss_backward_workspace_bytes(nq, nc, dim, dt), q)
         _check(lib.fgpu_contrastive_loss_backward(g.data_ptr(), q.data_ptr(), c.data_ptr(), t.data_ptr(), lse.data_ptr(),
                                                   _ptr(b), _ptr(i), nq, nc, dim, dt, scale, dq.data_ptr(), _ptr(dc), _ptr(db),
-                                                  ws.data_ptr(), _ws_check(ws), _stream()))
+                                                  wp, wb, _stream()))
     return dq, dc, db
