@@ -1,11 +1,15 @@
 // head_narrow.hip -- the contrastive loss of up to 128 dims, where a row's vector and its gradient fit the registers.
 //
-// A wave holds 32 rows, or 16 (their vectors as MFMA operands, and in the backward pass their gradients as accumulators); tiles
-// of 64 vectors of the other side pass through LDS.  The scores of a tile come out of the first product with eight
+// A wave holds 32 rows, or 16 (their vectors as MFMA operands, and in the backward pass their gradients as accumulators);
+// tiles of 64 or 128 vectors of the other side pass through LDS.  The scores of a tile come out of the first product with eight
 // consecutive columns a lane, which is just how the second product wants its k: the score gradient goes from the
 // accumulators through the exponential back into the matrix unit without leaving the registers, and the 2 (float32: 6)
 // bytes an element that a stored gradient would be written and read with, more than the product's own time at these
 // widths, are saved.  Rows are the queries for the statistics and dq, the candidates for dc and dbias.
+//
+// Bound by the matrix units and, beside them, by the LDS (every wave reads the whole tile, once a product) and the
+// exponentials.  1000 x 100000 x 128 in float32: statistics 139 us (1.1 PFLOP/s in bf16 products), dq 265 us (1.16, the
+// score product formed again); 8192 x 65536 x 128 in bf16: forward 224 us, both gradients 650 us (0.85 PFLOP/s).
 #include <algorithm>
 
 #include "loss_scores.hpp"
@@ -23,7 +27,8 @@ constexpr int kNRowBytes = 256;       // of a tile's row in LDS: 128 dims
 enum { kStats = 0, kDq = 1, kDc = 2 };
 
 // Fragments of 16 rows a wave holds: two, but one where the gradient and the three planes of float32 rows of more than 64
-// dims would not fit the registers of two waves a SIMD.
+// dims would not fit the registers of two waves a SIMD (four waves of two fragments, one a SIMD, take 315 us instead of
+// 290 at 1000 x 100000 x 128).
 constexpr int narrow_frags(bool f32, bool small, int mode, int kb) { return small || (f32 && mode != kStats && kb > 2) ? 1 : 2; }
 constexpr int narrow_block_rows(bool f32, bool small, int mode, int kb) { return 16 * kNWaves * narrow_frags(f32, small, mode, kb); }
 int dim_blocks(int dim) { return dim <= 64 ? 2 : dim <= 96 ? 3 : 4; }
@@ -351,7 +356,7 @@ struct NarrowPlan {
   double us;
 };
 // Splits of the streamed side: enough workgroups for `cus` CUs in even rounds, each tile at `tile_us`, the parts of a split
-// gradient written and read once more (1.5 TB/s at the sizes where it counts).  The small shape's two gradients share one
+// gradient written and read once more (3 TB/s; 1.5 where little is to be joined).  The small shape's two gradients share one
 // round between them.
 NarrowPlan plan_at(int nr, int ns, bool f32, bool small, int mode, int kb, int cus, double tile_us, double part_bytes, int most) {
   NarrowPlan best{small, narrow_tile(f32, small), narrow_block_rows(f32, small, mode, kb), 0, 0};
@@ -360,7 +365,7 @@ NarrowPlan plan_at(int nr, int ns, bool f32, bool small, int mode, int kb, int c
     const int64_t wgs = (int64_t)blocks * s;
     int rounds = ceil_div(wgs, cus);
     if (small && mode != kStats && wgs > cus / 2) rounds = std::max(2, rounds);
-    const double us = rounds * (ceil_div(tiles, s) * tile_us + (small ? 2.5 : 4)) + (s > 1 ? s * part_bytes / 1.5e6 : 0);
+    const double us = rounds * (ceil_div(tiles, s) * tile_us + (small ? 2.5 : 4)) + (s > 1 ? s * part_bytes / (small ? 1.5e6 : 3e6) : 0);
     if (s == 1 || us < best.us) best.splits = s, best.us = us;
   }
   return best;
