@@ -34,7 +34,7 @@ __device__ __forceinline__ bool loss_row_live(const LossRows& r, int m) {
 template <class T>
 __device__ __forceinline__ void copy_rows(const CopyJob& j, const LossRows& loss, int block, int blocks) {
   uint16_t* dst = const_cast<uint16_t*>(j.dst.p);
-  const int64_t per = j.dst.ld / 4, total = j.rows * per;
+  const int64_t per = whole8(j.cols) / 4, total = j.rows * per;
   for (int64_t i = (int64_t)block * 256 + threadIdx.x; i < total; i += (int64_t)blocks * 256) {
     const int64_t r = i / per, c = (i - r * per) * 4;
     f32x4 v = {0, 0, 0, 0};
@@ -49,7 +49,7 @@ constexpr int kDzCols = 256;  // columns of a workgroup: 64 lanes x 4; its four 
 template <class T>
 __device__ __forceinline__ void make_dz(const DzJob& j, int block) {
   __shared__ f32x4 sum[4][64];
-  const int64_t width = j.dst.p ? j.dst.ld : j.cols;
+  const int64_t width = j.dst.p ? whole8(j.cols) : j.cols;
   const int across = (int)((width + kDzCols - 1) / kDzCols), chunk = block / across;
   const int lane = threadIdx.x & 63, w = threadIdx.x >> 6;
   const int c = block % across * kDzCols + lane * 4, cnt = min(j.cols - c, 4);
@@ -116,10 +116,10 @@ int dz_chunks(int rows, int cols) {
 
 fgpu_status launch_prep(const Prep& p, bool f32, hipStream_t s) {
   auto copy_blocks = [](const CopyJob& j) {
-    return j.src ? (int)std::min<int64_t>(ceil_div(j.rows * (j.dst.ld / 4), 256), 8192) : 0;
+    return j.src ? (int)std::min<int64_t>(ceil_div(j.rows * (whole8(j.cols) / 4), 256), 8192) : 0;
   };
   Blocks n{0, copy_blocks(p.copy[0]), copy_blocks(p.copy[1])};
-  if (p.dz.dy) n.dz = ceil_div(p.dz.dst.p ? p.dz.dst.ld : p.dz.cols, kDzCols) * p.dz.chunks;
+  if (p.dz.dy) n.dz = ceil_div(p.dz.cols, kDzCols) * p.dz.chunks;
   const int total = n.dz + n.copy0 + n.copy1 + (p.loss.rows ? ceil_div(p.loss.nq, 256) : 0);
   if (total == 0) return FGPU_OK;
   if (f32)
