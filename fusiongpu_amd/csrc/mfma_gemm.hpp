@@ -188,6 +188,16 @@ __device__ __forceinline__ void landed_barrier() {
   __builtin_amdgcn_s_waitcnt(0x0f70);  // vmcnt(0), the other counters at their limits
   __syncthreads();
 }
+// The same for all loads but a wave's last N, which stay in flight (loads are counted in the order they were issued), and
+// behind which its own LDS reads have ended.
+template <int N>
+__device__ __forceinline__ void landed_barrier_but() {
+  static_assert(N < 16, "the counter's low bits");
+  asm volatile("" ::: "memory");  // no access passes
+  __builtin_amdgcn_s_waitcnt(0x0070 | N);  // vmcnt(N) lgkmcnt(0)
+  __builtin_amdgcn_s_barrier();
+  asm volatile("" ::: "memory");
+}
 
 // The part of an operand's LDS tile that one lane fills (16 bytes a load straight to LDS), and the addresses its
 // fragments are read from.  R: rows of m or n in the tile, NT: threads.
@@ -231,8 +241,9 @@ struct TileLoad {
   }
   // Issues the loads of k0 .. k0 + BK - 1 into the tile at `lds`.  r0: the tile's first row (m or n) of nr.  Reads beyond the
   // operand give zeros: the buffer ends with its last group of eight, and a chunk past the end of k is sent beyond it.
+  // Not `live`: all zeros, nothing read.
   __device__ __forceinline__ void issue(const GemmOperand& o, int plane, int r0, int nr, int k0, int nk, lds_char* lds,
-                                        int wave) const {
+                                        int wave, bool live = true) const {
     const uint16_t* base = o.p + plane * o.plane;
     int64_t last;  // elements from base to the end of the last one wanted
     if constexpr (KC) {
@@ -242,7 +253,7 @@ struct TileLoad {
       base += (int64_t)k0 * o.ld + r0;
       last = (int64_t)(min(nk - k0, BK) - 1) * o.ld + min(((nr + 7) & ~7) - r0, R);
     }
-    auto rsrc = __builtin_amdgcn_make_buffer_rsrc(const_cast<uint16_t*>(base), 0, (int)(last * 2), 0x00027000);
+    auto rsrc = __builtin_amdgcn_make_buffer_rsrc(const_cast<uint16_t*>(base), 0, live ? (int)(last * 2) : 0, 0x00027000);
     const uint32_t off = (KC && kc >= nk - k0) ? 0x80000000u : voff;
 #pragma unroll
     for (int i = 0; i < loads; ++i)
@@ -327,16 +338,23 @@ struct GemmWave {
 //
 // The smallest tiles hold all three planes of float32 operands for 32 k at a time and form the six products from them:
 // a barrier for 24 matrix instructions a wave instead of eight, and half the loads (a 64-wide step of k 1.2 us instead of
-// 2.1 while a workgroup has its CU to itself; 1000 x 385 x 771 forward on them 23 us).
+// 2.1 while a workgroup has its CU to itself).
 constexpr int kPlanesBK = 32;
 template <class T, int PAIRS>
 constexpr bool gemm_planes() { return PAIRS == 6 && T::BM == 64; }
 template <class T, int PAIRS>
 constexpr int gemm_stage() { return gemm_planes<T, PAIRS>() ? 3 * (T::BM + T::BN) * kPlanesBK * 2 : T::stage_bytes; }
 
+// k contiguous in both operands: a third buffer, so that two stages' loads are in flight (1000 x 385 x 771 forward 22.8 ->
+// 19.4 us, 4096 x 1024 x 1024 79 -> 76; with strided operands, whose fragments take twice the LDS loads, a third of the CU's
+// workgroups less costs as much as it gives: 16384 x 768 x 128 backward 86 -> 91).
+template <class T, int PAIRS, bool KC>
+constexpr int gemm_third() { return gemm_planes<T, PAIRS>() && KC ? gemm_stage<T, PAIRS>() : 16; }
+
 template <class T, bool AKC, bool BKC, class Acc>
 __device__ __forceinline__ void planes_products(const GemmArgs& g, Acc& acc, int m0, int n0, int kbeg, int kend, int wm, int wn,
-                                                char (&s0)[gemm_stage<T, 6>()], char (&s1)[gemm_stage<T, 6>()]) {
+                                                char (&s0)[gemm_stage<T, 6>()], char (&s1)[gemm_stage<T, 6>()],
+                                                char (&s2)[gemm_third<T, 6, AKC && BKC>()]) {
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   TileLoad<T::BM, T::threads, AKC, false, kPlanesBK> la;
   TileLoad<T::BN, T::threads, BKC, true, kPlanesBK> lb;
@@ -347,11 +365,17 @@ __device__ __forceinline__ void planes_products(const GemmArgs& g, Acc& acc, int
   ra.init(lane, wm * (T::BM / T::WM));
   rb.init(lane, wn * (T::BN / T::WN));
   constexpr int pa = T::BM * kPlanesBK * 2, pb = T::BN * kPlanesBK * 2;  // bytes a plane
+  if (kbeg >= kend) return;
+  const int klast = kbeg + (kend - kbeg - 1) / kPlanesBK * kPlanesBK;
+  // Past the end the loads read nothing: a step is the same everywhere, and the compiler sees which loads are older than
+  // the wait (a step that loads only sometimes would make it wait for all of them).
   auto issue = [&](char* s, int k) {
+    const bool live = k < kend;
+    k = min(k, klast);
 #pragma unroll
     for (int p = 0; p < 3; ++p) {
-      la.issue(g.a, p, m0, g.m, k, g.k, (lds_char*)s + p * pa, wave);
-      lb.issue(g.b, p, n0, g.n, k, g.k, (lds_char*)s + 3 * pa + p * pb, wave);
+      la.issue(g.a, p, m0, g.m, k, g.k, (lds_char*)s + p * pa, wave, live);
+      lb.issue(g.b, p, n0, g.n, k, g.k, (lds_char*)s + 3 * pa + p * pb, wave, live);
     }
   };
   auto work = [&](char* s) {
@@ -368,25 +392,48 @@ __device__ __forceinline__ void planes_products(const GemmArgs& g, Acc& acc, int
 #pragma unroll
       for (int i = 0; i < T::FN; ++i) acc[i][j] = mma(b[i], a[j], acc[i][j]);
   };
-  if (kbeg < kend) issue(s0, kbeg);
-  int k = kbeg;
-  for (; k + kPlanesBK < kend; k += 2 * kPlanesBK) {
-    landed_barrier();
-    issue(s1, k + kPlanesBK);
-    work(s0);
-    landed_barrier();
-    if (k + 2 * kPlanesBK < kend) issue(s0, k + 2 * kPlanesBK);
-    work(s1);
-  }
-  if (k < kend) {
-    landed_barrier();
-    work(s0);
+  constexpr int B = kPlanesBK, in_flight = 3 * (decltype(la)::loads + decltype(lb)::loads);  // of one stage
+  if constexpr (!(AKC && BKC)) {
+    issue(s0, kbeg);
+    int k = kbeg;
+    for (; k + B < kend; k += 2 * B) {
+      landed_barrier();
+      issue(s1, k + B);
+      work(s0);
+      landed_barrier();
+      if (k + 2 * B < kend) issue(s0, k + 2 * B);
+      work(s1);
+    }
+    if (k < kend) {
+      landed_barrier();
+      work(s0);
+    }
+  } else {
+    // The stage at k lies in `cur`, the next one's loads are in flight, and nobody reads `free` any more behind the barrier.
+    auto step = [&](char* cur, char* free, int k) {
+      landed_barrier_but<in_flight>();
+      issue(free, k + 2 * B);
+      work(cur);
+    };
+    issue(s0, kbeg);
+    issue(s1, kbeg + B);
+    int k = kbeg;
+    for (; k + 2 * B < kend; k += 3 * B) {
+      step(s0, s2, k);
+      step(s1, s0, k + B);
+      step(s2, s1, k + 2 * B);
+    }
+    if (k < kend) {
+      step(s0, s2, k);
+      if (k + B < kend) step(s1, s0, k + B);
+    }
+    __builtin_amdgcn_s_waitcnt(0x0f70);  // the epilogue writes where loads may still be under way
   }
 }
 
 template <class T, bool AKC, bool BKC, int PAIRS, class Epi>
 __device__ __forceinline__ void gemm_tile(const GemmArgs& g, const Epi& epi, int wg, int wgs, char (&s0)[gemm_stage<T, PAIRS>()],
-                                          char (&s1)[gemm_stage<T, PAIRS>()]) {
+                                          char (&s1)[gemm_stage<T, PAIRS>()], char (&s2)[gemm_third<T, PAIRS, AKC && BKC>()]) {
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int wm = wave / T::WN, wn = wave % T::WN;
   int tm, tn, sp;
@@ -401,7 +448,7 @@ __device__ __forceinline__ void gemm_tile(const GemmArgs& g, const Epi& epi, int
   typename Epi::template Side<T> side;
   if constexpr (gemm_planes<T, PAIRS>()) {
     side.fetch(epi, m0, n0, tid);
-    planes_products<T, AKC, BKC>(g, acc, m0, n0, kbeg, kend, wm, wn, s0, s1);
+    planes_products<T, AKC, BKC>(g, acc, m0, n0, kbeg, kend, wm, wn, s0, s1, s2);
   } else {
     const int steps = max(0, (kend - kbeg + kGemmBK - 1) / kGemmBK) * PAIRS;
 
@@ -478,7 +525,8 @@ template <class T, bool AKC, bool BKC, int PAIRS, class Epi>
 __global__ __launch_bounds__(T::threads, 2) void gemm_kernel(GemmArgs g, Epi epi) {
   __shared__ __attribute__((aligned(1024))) char s0[gemm_stage<T, PAIRS>()];
   __shared__ __attribute__((aligned(1024))) char s1[gemm_stage<T, PAIRS>()];
-  gemm_tile<T, AKC, BKC, PAIRS>(g, epi, blockIdx.x, gridDim.x, s0, s1);
+  __shared__ __attribute__((aligned(1024))) char s2[gemm_third<T, PAIRS, AKC && BKC>()];
+  gemm_tile<T, AKC, BKC, PAIRS>(g, epi, blockIdx.x, gridDim.x, s0, s1, s2);
 }
 
 // Both gradients of a small layer in one launch: the first x_wgs workgroups form x (A with k contiguous, B strided), the
@@ -487,11 +535,12 @@ template <class T, int PAIRS, class Epi>
 __global__ __launch_bounds__(T::threads, 2) void gemm_pair_kernel(GemmArgs x, Epi ex, int x_wgs, GemmArgs w, Epi ew) {
   __shared__ __attribute__((aligned(1024))) char s0[gemm_stage<T, PAIRS>()];
   __shared__ __attribute__((aligned(1024))) char s1[gemm_stage<T, PAIRS>()];
+  __shared__ __attribute__((aligned(1024))) char s2[gemm_third<T, PAIRS, false>()];
   const int b = blockIdx.x;
   if (b < x_wgs)
-    gemm_tile<T, true, false, PAIRS>(x, ex, b, x_wgs, s0, s1);
+    gemm_tile<T, true, false, PAIRS>(x, ex, b, x_wgs, s0, s1, s2);
   else
-    gemm_tile<T, false, false, PAIRS>(w, ew, b - x_wgs, gridDim.x - x_wgs, s0, s1);
+    gemm_tile<T, false, false, PAIRS>(w, ew, b - x_wgs, gridDim.x - x_wgs, s0, s1, s2);
 }
 
 }  // namespace fgpu
