@@ -127,7 +127,8 @@ struct SplitJob {
 fgpu_status launch_join(const SplitJob& a, const SplitJob& b, const ColumnSum* sums, bool f32, hipStream_t s);
 
 // The products (one, or an input's gradient followed by a weight's, either not asked for), then what joins split products
-// and the column sums (NULL: none): one launch for the products where they are small, one to join where there is something to join.
+// and the column sums (NULL: none): one launch for the products where they are small, one to join where there is something
+// to join.
 size_t products_workspace_bytes(const Product* p, int count);
 fgpu_status launch_products(const ProductJob* jobs, int count, const ColumnSum* sums, void* ws, hipStream_t s);
 double products_estimate_us(const Product* p, int count);  // the time that the rule between kernels goes by

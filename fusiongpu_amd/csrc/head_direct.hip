@@ -76,7 +76,7 @@ __device__ __forceinline__ Frag<T> to_frag(const Run8<T>& r) {
 template <class T, int F, bool KC, bool DZ>
 struct DirectRead {
   static constexpr int kLds = KC ? 0 : Frag<T>::planes * 32 * F * 16 * 2;  // bytes a wave
-  static constexpr int runs = KC ? F : F;  // runs of eight a lane (strided: 32 rows x 16 F columns over 64 lanes)
+  static constexpr int runs = F;  // of eight a lane (strided: 32 rows x 16 F columns over 64 lanes)
   Run8<T> r[runs], z[DZ ? runs : 1];
 
   __device__ __forceinline__ void load(const DirectOperand& o, int r0, int nr, int k0, int nk, int lane) {
@@ -309,7 +309,8 @@ double tile_steps(int64_t m, int64_t n, int64_t k) { return (double)ceil_div(m, 
 double direct_forward_estimate_us(const Product& p) {
   if (p.m <= 16) return p.f32 ? 7.5 : 4.5;
   // Rows that are not whole 16-byte groups load at half the rate or less.
-  return 3 + std::max<double>(wave_steps(p.k), tile_steps(p.m, p.n, p.k)) * (p.f32 ? 2.2 : 0.95) * (p.k % 8 ? (p.f32 ? 1.2 : 2.4) : 1);
+  const double ragged = p.k % 8 == 0 ? 1 : p.f32 ? 1.2 : 2.4;
+  return 3 + std::max<double>(wave_steps(p.k), tile_steps(p.m, p.n, p.k)) * (p.f32 ? 2.2 : 0.95) * ragged;
 }
 double direct_backward_estimate_us(int rows, int in_dim, int out_dim, bool f32) {
   const int longest = std::max(wave_steps(out_dim), wave_steps(rows));

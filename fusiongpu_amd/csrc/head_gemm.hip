@@ -128,7 +128,8 @@ __device__ __forceinline__ void split_finish(const SplitJob& j, int block) {
   if (i < total) {
     if (j.f.add && group == 0) v = *reinterpret_cast<const f32x4*>(j.f.add + i * 4);
 #pragma unroll 4
-    for (int s = group; s < j.splits; s += many ? 16 : 1) v += *reinterpret_cast<const f32x4*>(j.part + ((int64_t)s * total + i) * 4);
+    for (int s = group; s < j.splits; s += many ? 16 : 1)
+      v += *reinterpret_cast<const f32x4*>(j.part + ((int64_t)s * total + i) * 4);
   }
   if (many) {
     sums[group][out] = v;
@@ -294,7 +295,9 @@ fgpu_status run_products(const ProductJob* jobs, int count, const Plan* q, int p
 }  // namespace
 
 fgpu_status launch_join(const SplitJob& a, const SplitJob& b, const ColumnSum* sums, bool f32, hipStream_t s) {
-  auto blocks = [](const SplitJob& j) { return j.part ? ceil_div((int64_t)j.m * ((j.n + 3) / 4), j.splits >= kManyParts ? 16 : 256) : 0; };
+  auto blocks = [](const SplitJob& j) {
+    return j.part ? ceil_div((int64_t)j.m * ((j.n + 3) / 4), j.splits >= kManyParts ? 16 : 256) : 0;
+  };
   const int na = blocks(a), nb = blocks(b), nc = sums ? ceil_div(sums->cols, kSumCols) : 0;
   if (na + nb + nc == 0) return FGPU_OK;
   if (f32)

@@ -30,7 +30,9 @@ enum { kStats = 0, kDq = 1, kDc = 2 };
 // dims would not fit the registers of two waves a SIMD (four waves of two fragments, one a SIMD, take 315 us instead of
 // 290 at 1000 x 100000 x 128).
 constexpr int narrow_frags(bool f32, bool small, int mode, int kb) { return small || (f32 && mode != kStats && kb > 2) ? 1 : 2; }
-constexpr int narrow_block_rows(bool f32, bool small, int mode, int kb) { return 16 * kNWaves * narrow_frags(f32, small, mode, kb); }
+constexpr int narrow_block_rows(bool f32, bool small, int mode, int kb) {
+  return 16 * kNWaves * narrow_frags(f32, small, mode, kb);
+}
 int dim_blocks(int dim) { return dim <= 64 ? 2 : dim <= 96 ? 3 : 4; }
 
 struct NarrowArgs {
@@ -365,7 +367,8 @@ NarrowPlan plan_at(int nr, int ns, bool f32, bool small, int mode, int kb, int c
     const int64_t wgs = (int64_t)blocks * s;
     int rounds = ceil_div(wgs, cus);
     if (small && mode != kStats && wgs > cus / 2) rounds = std::max(2, rounds);
-    const double us = rounds * (ceil_div(tiles, s) * tile_us + (small ? 2.5 : 4)) + (s > 1 ? s * part_bytes / (small ? 1.5e6 : 3e6) : 0);
+    const double join = s > 1 ? s * part_bytes / (small ? 1.5e6 : 3e6) : 0;
+    const double us = rounds * (ceil_div(tiles, s) * tile_us + (small ? 2.5 : 4)) + join;
     if (s == 1 || us < best.us) best.splits = s, best.us = us;
   }
   return best;
