@@ -6,6 +6,9 @@
 namespace fgpu {
 
 inline int ceil_div(int64_t a, int64_t b) { return (int)((a + b - 1) / b); }
+// HIP counts a launch's threads in 32 bits: of 2^32 and more, what passes a multiple of 2^32 runs and no error comes back
+// (exact multiples are refused).  What may need that many goes out in launches of up to half of it.
+constexpr int64_t kLaunchThreads = (int64_t)1 << 31;
 
 // ---- activations -------------------------------------------------------------
 // gelu(z) = z Phi(z).  Phi's tail T(|z|) = 1 - Phi(|z|) is the rational form 7.1.26 of Abramowitz and Stegun's handbook,

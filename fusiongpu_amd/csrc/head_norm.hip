@@ -339,9 +339,15 @@ fgpu_status fgpu_layer_norm(const void* d_x, const void* d_gamma, const void* d_
     return by_dim<T>(dim, [&](auto shape) -> fgpu_status {
       using S = decltype(shape);
       const auto k = dim % Vec<T>::N ? norm_kernel<T, S, true> : norm_kernel<T, S, false>;
-      k<<<ceil_div(rows, S::rows), S::threads, 0, as_stream(stream)>>>((const T*)d_x, (const T*)d_gamma, (const T*)d_beta, rows,
-                                                                      dim, eps, (T*)d_y, d_mean, d_rstd);
-      FGPU_HIP(hipGetLastError());
+      constexpr int64_t kMost = kLaunchThreads / S::threads * S::rows;
+      for (int64_t r0 = 0; r0 < rows; r0 += kMost) {
+        const int64_t n = std::min(rows - r0, kMost);
+        k<<<ceil_div(n, S::rows), S::threads, 0, as_stream(stream)>>>((const T*)d_x + r0 * dim, (const T*)d_gamma,
+                                                                     (const T*)d_beta, n, dim, eps, (T*)d_y + r0 * dim,
+                                                                     d_mean ? d_mean + r0 : nullptr,
+                                                                     d_rstd ? d_rstd + r0 : nullptr);
+        FGPU_HIP(hipGetLastError());
+      }
       return FGPU_OK;
     });
   };
