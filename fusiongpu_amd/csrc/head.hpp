@@ -249,12 +249,7 @@ fgpu_status launch_narrow_backward(const NarrowBackward& b, int most_splits, voi
 // ---- column sums ---------------------------------------------------------------
 // Two sums of the same length, the second one's parts `cols` after the first one's; either result may be NULL.
 fgpu_status launch_column_sums(const ColumnSum& c, void* out1, hipStream_t s);
-// Zeros, as the sums over no rows.
-inline fgpu_status launch_no_sums(int64_t cols, bool f32, void* out, hipStream_t s) {
-  ColumnSum c;
-  c.cols = cols, c.out = out, c.f32 = f32;
-  return launch_column_sums(c, nullptr, s);
-}
-
+// Zeros: the sums over no rows, gradients without rows.
+fgpu_status launch_zeros(int64_t count, bool f32, void* out, hipStream_t s);
 
 }  // namespace fgpu

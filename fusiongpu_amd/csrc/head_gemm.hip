@@ -171,6 +171,14 @@ __global__ __launch_bounds__(256) void column_sum_kernel(ColumnSum c, void* out1
   if (out) column_sum(c, c.part + blockIdx.y * c.cols, out, blockIdx.x);
 }
 
+// Zeros: 16 bytes a thread and step, the `rest` (fewer than 16, a whole number of elements) by the first workgroup.
+__global__ __launch_bounds__(256) void zeros_kernel(char* out, int64_t vecs, int64_t rest) {
+  typedef uint32_t u32x4u __attribute__((ext_vector_type(4), aligned(2)));
+  for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < vecs; i += (int64_t)gridDim.x * 256)
+    reinterpret_cast<u32x4u*>(out)[i] = u32x4u{0, 0, 0, 0};
+  if (blockIdx.x == 0 && threadIdx.x < rest / 2) reinterpret_cast<uint16_t*>(out + vecs * 16)[threadIdx.x] = 0;
+}
+
 // What is left after the products, in one launch: the joining of up to two split ones, and column sums.
 template <class T>
 __global__ __launch_bounds__(256) void join_kernel(SplitJob a, int a_blocks, SplitJob b, int b_blocks, ColumnSum c) {
@@ -337,6 +345,13 @@ fgpu_status launch_products(const ProductJob* jobs, int count, const ColumnSum* 
   }
   if (p[0].f32) return run_products<6, float>(jobs, count, q, pair, part, sums, s);
   return run_products<1, bf16>(jobs, count, q, pair, part, sums, s);
+}
+
+fgpu_status launch_zeros(int64_t count, bool f32, void* out, hipStream_t s) {
+  const int64_t vecs = count / (f32 ? 4 : 8);
+  zeros_kernel<<<(int)std::min<int64_t>(vecs / 256 + 1, 4096), 256, 0, s>>>((char*)out, vecs, count * (f32 ? 4 : 2) - vecs * 16);
+  FGPU_HIP(hipGetLastError());
+  return FGPU_OK;
 }
 
 fgpu_status launch_column_sums(const ColumnSum& c, void* out1, hipStream_t s) {

@@ -107,8 +107,8 @@ fgpu_status fgpu_linear_backward(const void* d_dy, const void* d_x, const void* 
   FGPU_CHECK(aligned16(d_dy) && aligned16(d_x) && aligned16(d_w) && aligned16(d_workspace), FGPU_ERR_ARG,
              "linear backward: dy, x, weight and workspace must be 16-byte aligned");
   if (rows == 0) {
-    if (d_dw) FGPU_TRY(launch_no_sums((int64_t)out_dim * in_dim, f32, d_dw, s));
-    if (d_db) FGPU_TRY(launch_no_sums(out_dim, f32, d_db, s));
+    if (d_dw) FGPU_TRY(launch_zeros((int64_t)out_dim * in_dim, f32, d_dw, s));
+    if (d_db) FGPU_TRY(launch_zeros(out_dim, f32, d_db, s));
     return FGPU_OK;
   }
   const int m = (int)rows;

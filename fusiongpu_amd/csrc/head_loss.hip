@@ -391,8 +391,8 @@ fgpu_status fgpu_contrastive_loss_backward(const float* d_dloss, const void* d_q
   const bool f32 = dtype == FGPU_DTYPE_F32;
   hipStream_t s = as_stream(stream);
   if (nq == 0) {
-    if (d_dc) FGPU_TRY(launch_no_sums((int64_t)nc * dim, f32, d_dc, s));
-    if (d_dbias) FGPU_TRY(launch_no_sums(nc, true, d_dbias, s));
+    if (d_dc) FGPU_TRY(launch_zeros((int64_t)nc * dim, f32, d_dc, s));
+    if (d_dbias) FGPU_TRY(launch_zeros(nc, true, d_dbias, s));
     return FGPU_OK;
   }
   FGPU_CHECK(d_dloss && d_q && d_c && d_target && d_lse, FGPU_ERR_ARG, "contrastive loss backward: null argument");

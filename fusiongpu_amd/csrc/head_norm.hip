@@ -366,8 +366,8 @@ fgpu_status fgpu_layer_norm_backward(const void* d_dy, const void* d_x, const vo
   const bool f32 = dtype == FGPU_DTYPE_F32;
   hipStream_t s = as_stream(stream);
   if (rows == 0) {
-    if (d_dgamma) FGPU_TRY(launch_no_sums(dim, f32, d_dgamma, s));
-    if (d_dbeta) FGPU_TRY(launch_no_sums(dim, f32, d_dbeta, s));
+    if (d_dgamma) FGPU_TRY(launch_zeros(dim, f32, d_dgamma, s));
+    if (d_dbeta) FGPU_TRY(launch_zeros(dim, f32, d_dbeta, s));
     return FGPU_OK;
   }
   FGPU_CHECK(d_dy && d_x && d_mean && d_rstd, FGPU_ERR_ARG, "layer norm backward: null dy, x, mean or rstd");
