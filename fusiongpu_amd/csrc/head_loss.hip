@@ -69,16 +69,17 @@ struct LossSide {
     return l;
   }
 };
-// Forward: per row and column tile (maximum, sum of exp2(s - maximum)), and the target's score.
+// Forward, of the columns from c0 on: per row and column tile (maximum, sum of exp2(s - maximum)), and the target's score.
 struct StatsEpi {
   LossArgs a;
   f32x2* part;     // [tiles_n][nq]
   float* target2;  // [nq]
+  int c0;
 
   template <class G>
   struct Side : LossSide<G, false> {
     __device__ __forceinline__ void fetch(const StatsEpi& e, int m0, int n0, int tid) {
-      LossSide<G, false>::fetch(e.a, nullptr, m0, n0, tid);
+      LossSide<G, false>::fetch(e.a, nullptr, m0, e.c0 + n0, tid);
     }
   };
   template <class G>
@@ -99,7 +100,7 @@ struct StatsEpi {
       for (int p = 0; p < P; ++p) {
         v[p] = f32x8{acc[2 * p][j], acc[2 * p + 1][j]};
         uint32_t at;
-        const bool here = scores8(a, v[p], cs[p], rs, w.col(p), at);
+        const bool here = scores8(a, v[p], cs[p], rs, c0 + w.col(p), at);
 #pragma unroll
         for (int e = 0; e < 8; ++e) top = fmaxf(top, v[p][e]);  // a NaN score makes the sum NaN
         if (here) {
@@ -135,7 +136,8 @@ struct StatsEpi {
   }
 };
 
-// Joins a row's parts: 16 rows a workgroup, 64 groups of parts.
+// Joins a row's parts: 16 rows a workgroup, 64 groups of parts.  `carry` ([nq], may be the first of the parts; NULL: these
+// are the last columns): gets the joined part in place of the loss.
 constexpr int kJoinRows = 16, kJoinGroups = 64;
 __device__ __forceinline__ void join_stats(float& top, float& sum, float t, float s) {
   const float both = fmaxf(top, t);
@@ -143,7 +145,7 @@ __device__ __forceinline__ void join_stats(float& top, float& sum, float t, floa
   top = both;
 }
 __global__ __launch_bounds__(1024) void loss_join_kernel(LossArgs a, const f32x2* part, int parts, const float* target2,
-                                                         float* loss, float* lse) {
+                                                         float* loss, float* lse, f32x2* carry) {
   __shared__ f32x2 sh[kJoinRows][kJoinGroups + 1];
   const int r = threadIdx.x % kJoinRows, g = threadIdx.x / kJoinRows;
   {
@@ -163,6 +165,10 @@ __global__ __launch_bounds__(1024) void loss_join_kernel(LossArgs a, const f32x2
   const float top = wave_max_f(v[0]), base = top == -INFINITY ? 0.0f : top;
   const float sum = lanes_sum<64>(v[1] * fast_exp2(v[0] - base));
   if (threadIdx.x % kWave || m >= a.nq) return;
+  if (carry) {
+    carry[m] = f32x2{top, sum};
+    return;
+  }
   const float l2 = base + __builtin_amdgcn_logf(sum);  // log2; of 0: -inf
   lse[m] = l2 * kLn2;
   const int t = a.target[m];
@@ -282,6 +288,13 @@ fgpu_status launch_scores(const ScorePlan& p, const GemmOperand& q, const GemmOp
   return FGPU_OK;
 }
 
+fgpu_status launch_loss_join(const LossArgs& a, const f32x2* part, int parts, const float* target2, float* loss, float* lse,
+                             f32x2* carry, hipStream_t s) {
+  loss_join_kernel<<<ceil_div(a.nq, kJoinRows), 1024, 0, s>>>(a, part, parts, target2, loss, lse, carry);
+  FGPU_HIP(hipGetLastError());
+  return FGPU_OK;
+}
+
 fgpu_status check_loss(int nq, int nc, int dim, int dtype) {
   FGPU_CHECK(dtype == FGPU_DTYPE_F32 || dtype == FGPU_DTYPE_BF16, FGPU_ERR_ARG, "contrastive loss: unknown dtype");
   FGPU_CHECK(nq >= 0 && nc >= 1 && dim >= 1, FGPU_ERR_ARG, "contrastive loss: nq >= 0, nc and dim >= 1");
@@ -311,6 +324,17 @@ size_t chunk_products_bytes(int nq, int nc, int dim, bool f32, int step) {
 size_t common_bytes(int nq, int nc, int dim, bool f32) {
   return carve_bytes<LossRow>(nq) + packed_bytes(nq, dim, f32) + packed_bytes(nc, dim, f32);
 }
+// The forward pass above 128 dims: columns a launch, so that its parts (8 bytes a row and column tile) take at most 512 MB
+// however many candidates there are, and its grid stays far below 2^32 threads.  65536 x 262144 are still one launch.
+int stats_columns(int nq, int nc) {
+  const int64_t most = ((int64_t)1 << 34) / nq;
+  return (int)std::min<int64_t>(nc, most / 256 * 256);
+}
+// Its parts a row: a launch's tiles and, where there are several launches, what the ones before came to.
+int stats_parts(int nq, int nc) {
+  const int step = stats_columns(nq, nc);
+  return score_plan(nq, step).tiles_n + (step < nc);
+}
 constexpr int kMostSplits = 256;
 // The backward pass's workspace when it holds `step` columns of G.
 size_t backward_bytes(int nq, int nc, int dim, bool f32, int step) {
@@ -330,7 +354,7 @@ extern "C" {
 size_t fgpu_contrastive_loss_workspace_bytes(int nq, int nc, int dim, int dtype) {
   if (check_loss(nq, nc, dim, dtype) != FGPU_OK || nq == 0) return 0;
   const bool f32 = dtype == FGPU_DTYPE_F32;
-  const int parts = dim <= kNarrowDim ? narrow_stats_splits(nq, nc, f32) : score_plan(nq, nc).tiles_n;
+  const int parts = dim <= kNarrowDim ? narrow_stats_splits(nq, nc, f32) : stats_parts(nq, nc);
   size_t b = carve_bytes<f32x2>((size_t)parts * nq) + carve_bytes<float>(nq);
   if (needs_pack(dim, f32)) b += packed_bytes(nq, dim, f32) + packed_bytes(nc, dim, f32);
   return b;
@@ -346,8 +370,7 @@ fgpu_status fgpu_contrastive_loss(const void* d_q, const void* d_c, const int32_
              "contrastive loss: queries, candidates and workspace must be 16-byte aligned");
   const bool f32 = dtype == FGPU_DTYPE_F32, pk = needs_pack(dim, f32);
   const bool narrow = dim <= kNarrowDim;
-  const ScorePlan sp = score_plan(nq, nc);
-  const int parts = narrow ? narrow_stats_splits(nq, nc, f32) : sp.tiles_n;
+  const int parts = narrow ? narrow_stats_splits(nq, nc, f32) : stats_parts(nq, nc);
   Carve ws(d_workspace, workspace_bytes);
   f32x2* part = ws.take<f32x2>((size_t)parts * nq);
   float* target2 = ws.take<float>(nq);
@@ -367,12 +390,19 @@ fgpu_status fgpu_contrastive_loss(const void* d_q, const void* d_c, const int32_
   const LossArgs a{d_bias, d_ids, d_target, scale * kLog2e, nq, nc};
   if (narrow) {
     FGPU_TRY(launch_narrow_stats(a, q, c, dim, f32, parts, part, target2, s));
-  } else {
-    const StatsEpi e{a, part, target2};
-    FGPU_TRY(f32 ? launch_scores<6>(sp, q, c, nq, nc, dim, e, s) : launch_scores<1>(sp, q, c, nq, nc, dim, e, s));
+    return launch_loss_join(a, part, parts, target2, d_loss, d_lse, nullptr, s);
   }
-  loss_join_kernel<<<ceil_div(nq, kJoinRows), 1024, 0, s>>>(a, part, parts, target2, d_loss, d_lse);
-  FGPU_HIP(hipGetLastError());
+  const int step = stats_columns(nq, nc), later = step < nc;  // later: the parts begin with the columns before
+  ScorePlan sp = score_plan(nq, step);
+  for (int c0 = 0; c0 < nc; c0 += step) {
+    const int n = std::min(step, nc - c0);
+    sp.tiles_n = ceil_div(n, sp.tile);
+    const StatsEpi e{a, part + (int64_t)later * nq, target2, c0};
+    const GemmOperand cc{c.p + (int64_t)c0 * c.ld, c.ld, c.plane};
+    FGPU_TRY(f32 ? launch_scores<6>(sp, q, cc, nq, n, dim, e, s) : launch_scores<1>(sp, q, cc, nq, n, dim, e, s));
+    FGPU_TRY(launch_loss_join(a, c0 ? part : e.part, sp.tiles_n + (c0 > 0), target2, d_loss, d_lse,
+                              c0 + n < nc ? part : nullptr, s));
+  }
   return FGPU_OK;
 }
 

@@ -670,7 +670,9 @@ fgpu_status fgpu_layer_norm_backward(const void* d_dy, const void* d_x, const vo
  * and no gradient (its lse is over all unmasked candidates); a row with no
  * candidate left has lse -infinity, loss 0 and no gradient; a row whose target
  * is masked has an infinite loss and no gradient.  d_loss, d_lse [nq] float32.
- * nq <= FGPU_LOSS_MAX_QUERIES. */
+ * nq <= FGPU_LOSS_MAX_QUERIES.  Beside copies of operands that cannot be read
+ * as they are, the workspace holds partial sums: at most 512 MB of them however
+ * many candidates there are (above 128 dims; a few rows' worth up to 128). */
 #define FGPU_MASK_BIAS (-8.507059173023462e37f) /* -2^126 */
 #define FGPU_LOSS_MAX_QUERIES (1 << 20)
 size_t fgpu_contrastive_loss_workspace_bytes(int nq, int nc, int dim, int dtype);

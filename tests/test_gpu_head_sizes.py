@@ -65,3 +65,44 @@ def test_zeros_stop_where_the_array_does():
                                                          None, at, None, None, 0, None) == 0
             torch.cuda.synchronize()
             assert buf[:first].all() and buf[first + count:].all() and not buf[first:first + count].any()
+
+
+@pytest.mark.parametrize("nq,nc,dim,dtype", [(1 << 17, (1 << 22) + 77, 136, torch.bfloat16),
+                                             ((1 << 15) + 77, (1 << 19) + 300, 136, torch.float32)])
+def test_contrastive_loss_many_scores(nq, nc, dim, dtype):
+    """More scores than one launch takes (2^39 and 2^34), against 64 bits in a sample of the rows.  Targets, masks and copies
+    lie in the first launch's columns, the last one's and between.  Bound: a score's error is (dim + 14) 2^-24 of the
+    magnitudes in it; the sum's, of at most nc / 16 terms in a row of additions whose errors are of random sign, below
+    sqrt(nc) 2^-24 (times 8); and a few last places of the result."""
+    u = 2.0**-24
+    g = torch.Generator(device="cuda")
+    g.manual_seed(1)
+    c = torch.empty((nc, dim), dtype=dtype, device="cuda")
+    for i in range(0, nc, 1 << 20):
+        c[i:i + (1 << 20)] = torch.randn((min(1 << 20, nc - i), dim), generator=g, device="cuda").to(dtype)
+    q = torch.randn((nq, dim), generator=g, device="cuda").to(dtype)
+    t = torch.randint(nc, (nq,), generator=g, device="cuda", dtype=torch.int32)
+    rows = torch.tensor([0, 1, 2, 255, 256, 4097, nq // 2, nq - 2, nq - 1], device="cuda")
+    t[rows] = torch.tensor([0, nc - 1, nc // 2, 255, 256, 1 << 17, (1 << 17) - 1, -1, nc - 300], dtype=torch.int32, device="cuda")
+    ids = torch.arange(nc, device="cuda", dtype=torch.int32) % (nc - 1000)  # the first thousand's copies are the last ones
+    bias = torch.randn(nc, generator=g, device="cuda")
+    bias[7::1000] = -torch.inf
+    scale = 1 / dim**0.5
+    loss, lse = fg.contrastive_loss(q, c, t, scale, bias=bias, ids=ids)
+    for r in rows.tolist():
+        qd = q[r].double()
+        s, mag = torch.empty(nc, dtype=torch.float64, device="cuda"), 0.0
+        for i in range(0, nc, 1 << 20):
+            cd = c[i:i + (1 << 20)].double()
+            s[i:i + (1 << 20)] = scale * torch.mv(cd, qd)
+            mag = max(mag, (scale * torch.mv(cd.abs(), qd.abs())).max().item())
+        s += bias.double()
+        at = t[r].item()
+        if at >= 0:
+            same = ids == ids[at]
+            same[at] = False
+            s[same] = -torch.inf
+        want = torch.logsumexp(s, 0).item()
+        bound = (dim + 14) * u * mag + 8 * nc**0.5 * u + 16 * u * (mag + 8)
+        assert abs(lse[r].item() - want) <= bound, r
+        assert abs(loss[r].item() - (want - s[at].item() if at >= 0 else 0.0)) <= (2 * bound if at >= 0 else 0.0), r
