@@ -215,6 +215,10 @@ Plan plan_at(const Product& p, int tile, int splits) {
   if (q.splits > 1) q.us += 3 + 8.0 * q.splits * p.m * ((p.n + 3) & ~3) / 6e6;
   return q;
 }
+int64_t plan_threads(const Plan& q) {
+  return (int64_t)q.tiles_m * q.tiles_n * q.splits * (q.tile == 256 ? Tile256::threads : q.tile == 128 ? Tile128::threads : Tile64::threads);
+}
+// Of the plans that are one launch (2^30 rows of up to 64 columns on 64 x 64 tiles are not).
 Plan plan_of(const Product& p, int only = 0) {
   Plan best{};
   for (int tile : {256, 128, 64}) {
@@ -222,6 +226,7 @@ Plan plan_of(const Product& p, int only = 0) {
     for (int splits : {1, 2, 3, 4, 6, 8, 12, 16, 24, 32, 48, 64}) {
       if (splits > 1 && splits > ceil_div(p.k, 2 * kGemmBK)) break;
       const Plan q = plan_at(p, tile, splits);
+      if (plan_threads(q) >= 2 * kLaunchThreads) continue;
       if (!best.tile || q.us < best.us) best = q;
     }
   }
@@ -236,6 +241,7 @@ int plans_of(const Product* p, int count, Plan* q) {
   int pair = 0;
   for (int tile : {128, 64}) {
     const Plan a = plan_of(p[0], tile), b = plan_of(p[1], tile);
+    if (!a.tile || !b.tile || plan_threads(a) + plan_threads(b) >= 2 * kLaunchThreads) continue;
     if (a.us + b.us - kLaunchUs < us) us = a.us + b.us - kLaunchUs, pair = tile, q[0] = a, q[1] = b;
   }
   return pair;
@@ -336,6 +342,8 @@ fgpu_status launch_products(const ProductJob* jobs, int count, const ColumnSum* 
   Plan q[2];
   for (int i = 0; i < count; ++i) p[i] = jobs[i].p;
   const int pair = plans_of(p, count, q);
+  for (int i = 0; i < count; ++i)
+    FGPU_CHECK(q[i].tile, FGPU_ERR_UNSUPPORTED, "product: more tiles than one launch takes (2^39 results)");
   float* part[2] = {nullptr, nullptr};
   char* at = static_cast<char*>(ws);
   for (int i = 0; i < count; ++i) {

@@ -106,3 +106,17 @@ def test_contrastive_loss_many_scores(nq, nc, dim, dtype):
         bound = (dim + 14) * u * mag + 8 * nc**0.5 * u + 16 * u * (mag + 8)
         assert abs(lse[r].item() - want) <= bound, r
         assert abs(loss[r].item() - (want - s[at].item() if at >= 0 else 0.0)) <= (2 * bound if at >= 0 else 0.0), r
+
+
+def test_linear_most_rows():
+    """2^30 rows, where the smallest tiles would be 2^32 threads."""
+    x = torch.zeros((1 << 30, 8), dtype=torch.bfloat16, device="cuda")
+    at = torch.tensor([0, 1, 63, 64, (1 << 24) + 1, (1 << 29) - 1, 1 << 29, (1 << 30) - 1], device="cuda")
+    g = torch.Generator(device="cuda")
+    g.manual_seed(3)
+    x[at] = torch.randn((8, 8), generator=g, device="cuda").to(torch.bfloat16)
+    flip = torch.eye(8, device="cuda").flip(0).to(torch.bfloat16)
+    y = fg.linear(x, flip)
+    assert torch.equal(y[at], x[at].flip(1))
+    y[at] = 0
+    assert not any(part.any() for part in y.split(1 << 26))
