@@ -181,15 +181,18 @@ __global__ __launch_bounds__(256) void zeros_kernel(char* out, int64_t vecs, int
 
 // What is left after the products, in one launch: the joining of up to two split ones, and column sums.
 template <class T>
-__global__ __launch_bounds__(256) void join_kernel(SplitJob a, int a_blocks, SplitJob b, int b_blocks, ColumnSum c) {
-  const int k = blockIdx.x;
-  if (k < a_blocks)
-    split_finish<T>(a, k);
-  else if (k < a_blocks + b_blocks)
-    split_finish<T>(b, k - a_blocks);
-  else
-    column_sum(c, c.part, c.out, k - a_blocks - b_blocks);
+__global__ __launch_bounds__(256) void join_kernel(SplitJob a, int a_blocks, SplitJob b, int b_blocks, ColumnSum c, int blocks) {
+  for (int k = blockIdx.x; k < blocks; k += gridDim.x) {
+    if (k < a_blocks)
+      split_finish<T>(a, k);
+    else if (k < a_blocks + b_blocks)
+      split_finish<T>(b, k - a_blocks);
+    else
+      column_sum(c, c.part, c.out, k - a_blocks - b_blocks);
+    if (k + (int)gridDim.x < blocks) __syncthreads();  // the LDS sums are read
+  }
 }
+constexpr int kJoinGrid = 1 << 16;  // workgroups at most: what a workgroup does is the same whichever does it
 
 struct Plan {
   int tile, tiles_m, tiles_n, splits, k_per_split;
@@ -313,11 +316,12 @@ fgpu_status launch_join(const SplitJob& a, const SplitJob& b, const ColumnSum* s
     return j.part ? ceil_div((int64_t)j.m * ((j.n + 3) / 4), j.splits >= kManyParts ? 16 : 256) : 0;
   };
   const int na = blocks(a), nb = blocks(b), nc = sums ? ceil_div(sums->cols, kSumCols) : 0;
-  if (na + nb + nc == 0) return FGPU_OK;
+  const int all = na + nb + nc, grid = std::min(all, kJoinGrid);
+  if (all == 0) return FGPU_OK;
   if (f32)
-    join_kernel<float><<<na + nb + nc, 256, 0, s>>>(a, na, b, nb, sums ? *sums : ColumnSum{});
+    join_kernel<float><<<grid, 256, 0, s>>>(a, na, b, nb, sums ? *sums : ColumnSum{}, all);
   else
-    join_kernel<bf16><<<na + nb + nc, 256, 0, s>>>(a, na, b, nb, sums ? *sums : ColumnSum{});
+    join_kernel<bf16><<<grid, 256, 0, s>>>(a, na, b, nb, sums ? *sums : ColumnSum{}, all);
   FGPU_HIP(hipGetLastError());
   return FGPU_OK;
 }

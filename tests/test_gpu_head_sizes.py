@@ -4,6 +4,7 @@ import pytest
 torch = pytest.importorskip("torch")
 
 import fusiongpu_amd as fg  # noqa: E402
+from tests.test_gpu_head import check_loss, loss_inputs  # noqa: E402
 
 pytestmark = pytest.mark.gpu
 
@@ -120,3 +121,10 @@ def test_linear_most_rows():
     assert torch.equal(y[at], x[at].flip(1))
     y[at] = 0
     assert not any(part.any() for part in y.split(1 << 26))
+
+
+def test_contrastive_backward_chunks_many_results():
+    """A query gradient of 2^26 elements and more, added up over column chunks: more joining than one grid's workgroups hold."""
+    q, c, t, scale, bias, ids = loss_inputs((1 << 16) + 5, 5000, 1032, "bf16")
+    full = fg.lib.fgpu_contrastive_loss_backward_workspace_bytes((1 << 16) + 5, 5000, 1032, 1)
+    check_loss(q, c, t, scale, bias, ids, "bf16", workspace=torch.empty(int(full * 0.95), dtype=torch.uint8, device="cuda"))
