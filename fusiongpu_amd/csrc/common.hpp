@@ -56,6 +56,7 @@ struct Carve {
     return used <= cap ? reinterpret_cast<T*>(base + off) : nullptr;
   }
   bool ok() const { return used <= cap; }
+  bool held() const { return ok() && (base || used == 0); }  // for a caller's workspace: NULL holds nothing
 };
 template <class T>
 inline size_t carve_bytes(size_t count) { return align_up(count * sizeof(T), 256); }

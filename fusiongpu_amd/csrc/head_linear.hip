@@ -79,7 +79,7 @@ fgpu_status fgpu_linear(const void* d_x, const void* d_w, const void* d_bias, co
     prep.copy[1] = {d_w, out_dim, in_dim, b};
   }
   void* parts = ws.take<char>(products_workspace_bytes(&p, 1));
-  FGPU_CHECK(ws.ok(), FGPU_ERR_WORKSPACE, "linear: workspace smaller than fgpu_linear_workspace_bytes");
+  FGPU_CHECK(ws.held(), FGPU_ERR_WORKSPACE, "linear: workspace smaller than fgpu_linear_workspace_bytes");
   FGPU_TRY(launch_prep(prep, f32, s));
   const ProductJob j{p, a, b, true, true, f};
   return launch_products(&j, 1, nullptr, parts, s);
@@ -147,7 +147,7 @@ fgpu_status fgpu_linear_backward(const void* d_dy, const void* d_x, const void* 
   const ProductJob jobs[2] = {{px, z, w, true, false, fx, d_dx != nullptr}, {pw, z, x, false, false, fw, d_dw != nullptr}};
   const Product ps[2] = {px, pw};
   void* parts = ws.take<char>(products_workspace_bytes(ps, 2));
-  FGPU_CHECK(ws.ok(), FGPU_ERR_WORKSPACE, "linear backward: workspace smaller than fgpu_linear_backward_workspace_bytes");
+  FGPU_CHECK(ws.held(), FGPU_ERR_WORKSPACE, "linear backward: workspace smaller than fgpu_linear_backward_workspace_bytes");
   FGPU_TRY(launch_prep(prep, f32, s));
   if (!d_dx && !d_dw) return d_db ? launch_column_sums(sums, nullptr, s) : FGPU_OK;
   return launch_products(jobs, 2, d_db ? &sums : nullptr, parts, s);

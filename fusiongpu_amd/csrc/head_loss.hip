@@ -376,7 +376,7 @@ fgpu_status fgpu_contrastive_loss(const void* d_q, const void* d_c, const int32_
   float* target2 = ws.take<float>(nq);
   char* qp = pk ? ws.take<char>(packed_bytes(nq, dim, f32)) : nullptr;
   char* cp = pk ? ws.take<char>(packed_bytes(nc, dim, f32)) : nullptr;
-  FGPU_CHECK(ws.ok(), FGPU_ERR_WORKSPACE, "contrastive loss: workspace smaller than fgpu_contrastive_loss_workspace_bytes");
+  FGPU_CHECK(ws.held(), FGPU_ERR_WORKSPACE, "contrastive loss: workspace smaller than fgpu_contrastive_loss_workspace_bytes");
   hipStream_t s = as_stream(stream);
   GemmOperand q = as_is(d_q, dim), c = as_is(d_c, dim);
   if (pk) {
@@ -450,7 +450,7 @@ fgpu_status fgpu_contrastive_loss_backward(const float* d_dloss, const void* d_q
     if (step < nc && d_dq) dq_sum = ws.take<float>((size_t)nq * ((dim + 3) & ~3));
     pw = ws.take<char>(chunk_products_bytes(nq, nc, dim, f32, step));
   }
-  FGPU_CHECK(ws.ok(), FGPU_ERR_WORKSPACE,
+  FGPU_CHECK(ws.held(), FGPU_ERR_WORKSPACE,
              "contrastive loss backward: workspace too small for 256 columns of the score gradient (up to 128 dims: for the "
              "copies of queries and candidates)");
   const LossArgs a{d_bias, d_ids, d_target, scale * kLog2e, nq, nc};

@@ -375,7 +375,7 @@ fgpu_status fgpu_layer_norm_backward(const void* d_dy, const void* d_x, const vo
   if (d_dgamma || d_dbeta) {
     Carve ws(d_workspace, workspace_bytes);
     part = ws.take<float>((size_t)std::min<int64_t>(rows, kNormParts) * 2 * dim);
-    FGPU_CHECK(ws.ok(), FGPU_ERR_WORKSPACE,
+    FGPU_CHECK(ws.held(), FGPU_ERR_WORKSPACE,
                "layer norm backward: workspace smaller than fgpu_layer_norm_backward_workspace_bytes");
   }
   int groups = 0;

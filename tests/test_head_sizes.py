@@ -19,3 +19,17 @@ def test_loss_workspace_does_not_grow_with_the_scores(nq, nc, dim):
 def test_more_results_than_one_launch_are_refused():
     """No tile's grid fits (arrays of a terabyte): refused before anything is launched."""
     assert L.fgpu_linear(1 << 20, 1 << 20, None, None, 1 << 30, 8, 1 << 16, BF16, 0, 1 << 20, None, None, 0, None) == 2
+
+
+P = 1 << 20  # stands for a 16-byte-aligned device pointer: refused calls never read it
+
+
+@pytest.mark.parametrize("call", [
+    lambda: L.fgpu_linear(P, P, None, None, 1 << 16, 1023, 1024, BF16, 0, P, None, None, 1 << 40, None),
+    lambda: L.fgpu_linear_backward(P, P, P, None, 1 << 16, 1024, 1024, F32, 0, P, P, P, None, 1 << 40, None),
+    lambda: L.fgpu_layer_norm_backward(P, P, None, P, P, 4, 8, F32, P, P, None, None, 1 << 40, None),
+    lambda: L.fgpu_contrastive_loss(P, P, P, None, None, 4, 8, 8, F32, 1.0, P, P, None, 1 << 40, None),
+    lambda: L.fgpu_contrastive_loss_backward(P, P, P, P, P, None, None, 4, 8, 200, F32, 1.0, P, P, P, None, 1 << 40, None),
+])
+def test_no_workspace_whatever_its_stated_size(call):
+    assert call() == 6
