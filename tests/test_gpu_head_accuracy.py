@@ -1,0 +1,42 @@
+"""What the query head's arithmetic holds beyond the bounds of a whole operator's sums: each piece alone, against 64 bits.
+
+u = 2^-24, half a last place of float32 at most."""
+import math
+
+import pytest
+
+torch = pytest.importorskip("torch")
+
+import fusiongpu_amd as fg  # noqa: E402
+
+pytestmark = pytest.mark.gpu
+
+U = 2.0**-24
+TYPES = {"f32": torch.float32, "bf16": torch.bfloat16}
+HALF = {"f32": U, "bf16": 2.0**-8}
+
+
+@pytest.mark.parametrize("dt", ["f32", "bf16"])
+@pytest.mark.parametrize("rows", [70_000, 16])
+def test_gelu_and_its_slope_keep_their_digits(dt, rows):
+    """z Phi(z) relative to itself on the negative side as well, out to where it leaves float32's range.  The tail 1 -
+    Phi(|z|): one u for its polynomial, 1.5 z^2 u for the exponential's argument (two roundings of z^2 / 2 log2 e and the
+    constant's), 2 for the exponential, 4 for the reciprocal's part, 6 for the polynomial's and products' roundings: 13, and
+    3 more to be safe against none; 3 u of the value for 1 - tail and the product with z."""
+    t = TYPES[dt]
+    z = torch.linspace(-13, 13, rows, device="cuda").to(t)[:, None].contiguous()
+    one = torch.ones((1, 1), dtype=t, device="cuda")
+    y, pre = fg.linear(z, one, act="gelu", save_pre=True)
+    assert torch.equal(pre, z)
+    zd = z.double()
+    phi, tail = torch.special.erfc(-zd / math.sqrt(2)) / 2, torch.special.erfc(zd.abs() / math.sqrt(2)) / 2
+    te = (16 + 1.5 * zd**2) * U * tail  # the tail's error
+    want = zd * phi
+    bound = zd.abs() * te + 3 * U * want.abs()
+    assert ((y.double() - want).abs() <= bound + HALF[dt] * (want.abs() + bound) + 2.0**-126).all()
+    # its slope Phi(z) + z exp(-z^2 / 2) / sqrt(2 pi): the density's error is the exponential's and four roundings
+    dx, _, _ = fg.linear_backward(torch.ones_like(z), z, one, pre, act="gelu", want=("x",))
+    dens = zd * torch.exp(-zd * zd / 2) / math.sqrt(2 * math.pi)
+    want = phi + dens
+    bound = te + (8 + 1.5 * zd**2) * U * dens.abs() + 3 * U * (phi + dens.abs())
+    assert ((dx.double() - want).abs() <= bound + HALF[dt] * (want.abs() + bound) + 2.0**-126).all()
