@@ -179,8 +179,9 @@ __global__ __launch_bounds__(256) void zeros_kernel(char* out, int64_t vecs, int
   if (blockIdx.x == 0 && threadIdx.x < rest / 2) reinterpret_cast<uint16_t*>(out + vecs * 16)[threadIdx.x] = 0;
 }
 
-// What is left after the products, in one launch: the joining of up to two split ones, and column sums.
-template <class T>
+// What is left after the products, in one launch: the joining of up to two split ones, and column sums.  WALK: the grid does
+// not hold all blocks (for the others the loop would cost 0.6 us a launch).
+template <class T, bool WALK>
 __global__ __launch_bounds__(256) void join_kernel(SplitJob a, int a_blocks, SplitJob b, int b_blocks, ColumnSum c, int blocks) {
   for (int k = blockIdx.x; k < blocks; k += gridDim.x) {
     if (k < a_blocks)
@@ -189,10 +190,11 @@ __global__ __launch_bounds__(256) void join_kernel(SplitJob a, int a_blocks, Spl
       split_finish<T>(b, k - a_blocks);
     else
       column_sum(c, c.part, c.out, k - a_blocks - b_blocks);
-    if (k + (int)gridDim.x < blocks) __syncthreads();  // the LDS sums are read
+    if (!WALK) return;
+    __syncthreads();  // the LDS sums are read
   }
 }
-constexpr int kJoinGrid = 1 << 16;  // workgroups at most: what a workgroup does is the same whichever does it
+constexpr int kJoinGrid = 1 << 16;  // workgroups at most: a block's result is the same whichever takes it
 
 struct Plan {
   int tile, tiles_m, tiles_n, splits, k_per_split;
@@ -318,10 +320,9 @@ fgpu_status launch_join(const SplitJob& a, const SplitJob& b, const ColumnSum* s
   const int na = blocks(a), nb = blocks(b), nc = sums ? ceil_div(sums->cols, kSumCols) : 0;
   const int all = na + nb + nc, grid = std::min(all, kJoinGrid);
   if (all == 0) return FGPU_OK;
-  if (f32)
-    join_kernel<float><<<grid, 256, 0, s>>>(a, na, b, nb, sums ? *sums : ColumnSum{}, all);
-  else
-    join_kernel<bf16><<<grid, 256, 0, s>>>(a, na, b, nb, sums ? *sums : ColumnSum{}, all);
+  const auto k = f32 ? (all > grid ? join_kernel<float, true> : join_kernel<float, false>)
+                     : (all > grid ? join_kernel<bf16, true> : join_kernel<bf16, false>);
+  k<<<grid, 256, 0, s>>>(a, na, b, nb, sums ? *sums : ColumnSum{}, all);
   FGPU_HIP(hipGetLastError());
   return FGPU_OK;
 }
