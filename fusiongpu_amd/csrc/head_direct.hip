@@ -98,10 +98,11 @@ struct DirectRead {
       if (DZ) z[i].load((const T*)o.pre + at, n, o.count - at);
     }
   }
-  // The fragments, dz formed where DZ.  extra (bf16 dz): what its rounding to bf16 left, again in bf16.
-  __device__ __forceinline__ void frags(Frag<T> (&f)[F], bf16x8 (&extra)[F], int act, char* lds, int lane) {
+  // The fragments, dz formed where DZ.  extra (bf16 dz, if `sums`): what its rounding to bf16 left, again in bf16, and what
+  // was left of that: the three hold the float32 value, which the column sums take.
+  __device__ __forceinline__ void frags(Frag<T> (&f)[F], bf16x8 (&extra)[2][F], int act, bool sums, char* lds, int lane) {
     Frag<T> g[runs];
-    bf16x8 rest[runs];
+    f32x8 left[runs];  // of dz
 #pragma unroll
     for (int i = 0; i < runs; ++i) {
       if constexpr (DZ) {
@@ -114,7 +115,7 @@ struct DirectRead {
           for (int e = 0; e < 8; ++e) {
             const float v = r[i].get(e) * act_slope(z[i].get(e), act);
             g[i].p[0][e] = (bf16)v;
-            rest[i][e] = (bf16)(v - (float)(bf16)v);
+            left[i].set(e, v - (float)(bf16)v);
           }
         }
       } else {
@@ -127,8 +128,20 @@ struct DirectRead {
     } else {
       put_and_turn<Frag<T>::planes>(lds, lane, [&](int i, int p) { return g[i].p[p]; },
                                     [&](int i, int p, const bf16x8& v) { f[i].p[p] = v; });
-      if constexpr (DZ && sizeof(T) == 2)
-        put_and_turn<1>(lds, lane, [&](int i, int) { return rest[i]; }, [&](int i, int, const bf16x8& v) { extra[i] = v; });
+      if constexpr (DZ && sizeof(T) == 2) {
+        if (sums) {
+#pragma unroll
+          for (int q = 0; q < 2; ++q) {
+            put_and_turn<1>(lds, lane, [&](int i, int) { return to_bf16x8(left[i]); },
+                            [&](int i, int, const bf16x8& v) { extra[q][i] = v; });
+            if (q) break;
+#pragma unroll
+            for (int i = 0; i < runs; ++i)
+#pragma unroll
+              for (int e = 0; e < 8; ++e) left[i].set(e, left[i][e] - (float)(bf16)left[i][e]);
+          }
+        }
+      }
     }
   }
   // Rows of k in, fragments out, through the wave's own LDS and its transposing load.
@@ -190,9 +203,9 @@ __device__ __forceinline__ void direct_tile(const DirectJob& j, int tile, char* 
   const bf16x8 one = {one1, one1, one1, one1, one1, one1, one1, one1};
   auto work = [&](RA& a, RB& b) {
     Frag<T> fa[FM], fb[FN];
-    bf16x8 ea[FM], eb[FN];
-    a.frags(fa, ea, j.act, la, lane);
-    b.frags(fb, eb, 0, la + RA::kLds, lane);
+    bf16x8 ea[2][FM], eb[2][FN];
+    a.frags(fa, ea, j.act, sums, la, lane);
+    b.frags(fb, eb, 0, false, la + RA::kLds, lane);
 #pragma unroll
     for (int x = 0; x < FM; ++x)
 #pragma unroll
@@ -204,7 +217,8 @@ __device__ __forceinline__ void direct_tile(const DirectJob& j, int tile, char* 
           col[x] = mma(one, fa[x].p[2], col[x]);
           col[x] = mma(one, fa[x].p[1], col[x]);
         } else if constexpr (DZ) {
-          col[x] = mma(one, ea[x], col[x]);
+          col[x] = mma(one, ea[1][x], col[x]);
+          col[x] = mma(one, ea[0][x], col[x]);
         }
         col[x] = mma(one, fa[x].p[0], col[x]);
       }

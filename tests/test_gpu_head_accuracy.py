@@ -40,3 +40,22 @@ def test_gelu_and_its_slope_keep_their_digits(dt, rows):
     want = phi + dens
     bound = te + (8 + 1.5 * zd**2) * U * dens.abs() + 3 * U * (phi + dens.abs())
     assert ((dx.double() - want).abs() <= bound + HALF[dt] * (want.abs() + bound) + 2.0**-126).all()
+
+
+@pytest.mark.parametrize("m,n,k", [(2, 1024, 64), (2, 100, 8), (2, 1 << 15, 2048)])
+def test_bias_gradient_takes_dz_unrounded(m, n, k):
+    """bfloat16: two rows whose dz nearly cancel, where dz rounded on its way to the sum would be most of the result.  dz:
+    the reciprocal, exponential and products of the slope, 10 u, its sum 4 u more."""
+    g = torch.Generator(device="cuda")
+    g.manual_seed(1)
+    a = (1 + torch.rand(n, generator=g, device="cuda")).bfloat16()
+    z = (0.02 + 0.04 * torch.rand(n, generator=g, device="cuda")).bfloat16()
+    dy, pre = torch.stack([a, -a]), torch.stack([z, (z.view(torch.int16) + 1).view(torch.bfloat16)])
+    x, w = torch.randn((m, k), generator=g, device="cuda").bfloat16(), torch.randn((n, k), generator=g, device="cuda").bfloat16()
+    p = pre.double()
+    s = torch.sigmoid(p)
+    dz = dy.double() * s * (1 + p * (1 - s))
+    want, bound = dz.sum(0), 16 * U * dz.abs().sum(0)
+    for names in (("x", "weight", "bias"), ("bias",)):
+        db = fg.linear_backward(dy, x, w, pre, act="silu", want=names)[2].double()
+        assert ((db - want).abs() <= bound + 2.0**-8 * (want.abs() + bound)).all()
