@@ -607,9 +607,9 @@ int fgpu_tune_elbow(const int32_t* hits_per_rank, int n, int64_t total_hits, flo
  * one call's of one dtype unless said otherwise: FGPU_DTYPE_F32 or
  * FGPU_DTYPE_BF16 (results are rounded once, to nearest even; every sum,
  * softmax and statistic is held in float32).  float32 products are formed from
- * bfloat16 triples that hold the operands exactly (six products, the dropped
- * ones below 2^-24 of the result's terms); an operand that is not finite makes
- * the float32 results it touches NaN.  Calls only enqueue kernels on `stream`
+ * bfloat16 triples that hold operands from 2^-110 on exactly (six products; the
+ * ones left out are together at most 2^-22 of each term, 2^-26 on average); an
+ * operand that is not finite makes the float32 results it touches NaN.  Calls only enqueue kernels on `stream`
  * (no allocation, no synchronisation; they can be captured), results do not
  * depend on timing (no floating-point atomics), and rows = 0 is allowed.
  * Workspaces, and the matrices that enter a product (x, w, dy, queries,

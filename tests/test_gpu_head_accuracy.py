@@ -59,3 +59,24 @@ def test_bias_gradient_takes_dz_unrounded(m, n, k):
     for names in (("x", "weight", "bias"), ("bias",)):
         db = fg.linear_backward(dy, x, w, pre, act="silu", want=names)[2].double()
         assert ((db - want).abs() <= bound + 2.0**-8 * (want.abs() + bound)).all()
+
+
+@pytest.mark.parametrize("m", [1, 100, 4096])
+def test_float32_products_of_one_term(m):
+    """x w alone: the plane products left out are at most 4 u of it, the last addition rounds by two at most, the ones before
+    by 2^-7 of that.  Among the values, those whose first eight bits leave most over, and the type's ends, where no finite
+    product may become infinite."""
+    g = torch.Generator(device="cuda")
+    g.manual_seed(1)
+    w = torch.randn((2048, 1), generator=g, device="cuda")
+    w[:512, 0] = 1 + (65024 + torch.arange(512, device="cuda")) * 2.0**-23  # just below 1 + 2^-7
+    w[512:1024, 0] = 1 + (32512 + torch.arange(512, device="cuda")) * 2.0**-23  # about half of it
+    w[1024:1029, 0] = torch.tensor([3.4028235e38, -3.4028235e38, 3.3895314e38, 3.3961775e38, 2.0**-100], device="cuda")
+    x = torch.cat([w[700:701], w[:1024], torch.randn((3071, 1), generator=g, device="cuda").clamp(-0.99, 0.99)])[:m].contiguous()
+    want = x.double() @ w.double().t()
+    keep = want.abs() <= 3.4028235e38  # the others' float32 is infinite
+    y = fg.linear(x, w).double()
+    assert ((y - want).abs() <= 6.1 * U * want.abs())[keep].all()
+    dx, dw, _ = fg.linear_backward(x, torch.ones_like(x), w[:1], want=("x",))
+    want = x.double() * w[0].double()
+    assert ((dx.double() - want).abs() <= 6.1 * U * want.abs()).all() and dw is None
