@@ -69,11 +69,12 @@ class QueryHead:
 
     def loss(self, x, candidates, targets, scale: float = 1.0, ids=None, grads: bool = True):
         """(mean loss over the rows with a target, gradients by parameter name): targets [rows] index the candidates
-        [n][dim] (-1: no target), whose softmax is that of -scale |q - c|^2 / 2; ids [n] name their documents."""
+        [n][dim] (outside [0, n): no target), whose softmax is that of -scale |q - c|^2 / 2; ids [n] name their documents."""
         cand = candidates.to(self.dtype)
         bias = cand.float().square().sum(1) * (-0.5 * scale)
-        targets = targets.to(torch.int32)
-        live = ((targets >= 0) & (targets < cand.shape[0])).float()
+        live = (targets >= 0) & (targets < cand.shape[0])
+        targets = torch.where(live, targets, -1).to(torch.int32)  # before the type's range could wrap one into the candidates
+        live = live.float()
         weight = live / live.sum().clamp(min=1)
         e, kept = self._forward(x, grads)
         loss, lse = fg.contrastive_loss(e, cand, targets, scale, bias=bias, ids=ids)
