@@ -125,6 +125,8 @@ _SIGS = {
     "fgpu_write_fvecs": (_i32, [_c.c_char_p, _vp, _i64, _i32]),
     "fgpu_read_fvecs": (_i32, [_c.c_char_p, _i32, _c.POINTER(_i64), _vp]),
     "fgpu_read_ivecs": (_i32, [_c.c_char_p, _c.POINTER(_i32), _c.POINTER(_i64), _vp]),
+    "fgpu_linear_tile": (_i32, [_i64, _i32, _i32, _i32, _i32]),
+    "fgpu_contrastive_loss_tile": (_i32, [_i32, _i32, _i32, _i32]),
     "fgpu_linear_workspace_bytes": (_sz, [_i64, _i32, _i32, _i32]),
     "fgpu_linear": (_i32, [_vp, _vp, _vp, _vp, _i64, _i32, _i32, _i32, _i32, _vp, _vp, _vp, _sz, _vp]),
     "fgpu_linear_backward_workspace_bytes": (_sz, [_i64, _i32, _i32, _i32]),

@@ -141,6 +141,7 @@ fgpu_status launch_join(const SplitJob& a, const SplitJob& b, const ColumnSum* s
 size_t products_workspace_bytes(const Product* p, int count);
 fgpu_status launch_products(const ProductJob* jobs, int count, const ColumnSum* sums, void* ws, hipStream_t s);
 double products_estimate_us(const Product* p, int count);  // the time that the rule between kernels goes by
+int products_tile(const Product* p, int count, int which);  // the width of its tiles, + FGPU_TILE_PAIR if both are one launch
 
 // An array as an operand: itself where its rows can be read as they are (bf16, cols % 8 == 0), otherwise a copy with
 // rows of packed_ld(cols) elements, float32 as three planes.

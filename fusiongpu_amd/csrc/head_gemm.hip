@@ -342,6 +342,11 @@ double products_estimate_us(const Product* p, int count) {
   return pair ? us - kLaunchUs : us;
 }
 
+int products_tile(const Product* p, int count, int which) {
+  Plan q[2];
+  return plans_of(p, count, q) ? q[which].tile + FGPU_TILE_PAIR : q[which].tile;
+}
+
 fgpu_status launch_products(const ProductJob* jobs, int count, const ColumnSum* sums, void* ws, hipStream_t s) {
   Product p[2];
   Plan q[2];

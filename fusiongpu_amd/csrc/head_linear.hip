@@ -44,6 +44,14 @@ using namespace fgpu;
 
 extern "C" {
 
+int fgpu_linear_tile(int64_t rows, int in_dim, int out_dim, int dtype, int product) {
+  if (check_common(rows, in_dim, out_dim, dtype, 0) != FGPU_OK || rows == 0 || product < 0 || product > 2) return -1;
+  const bool f32 = dtype == FGPU_DTYPE_F32;
+  const Product p[3] = {{(int)rows, out_dim, in_dim, f32}, {(int)rows, in_dim, out_dim, f32}, {out_dim, in_dim, (int)rows, f32}};
+  if (product == 0) return forward_direct(p[0]) ? 0 : products_tile(p, 1, 0);
+  return backward_direct(p[1], p[2]) ? 0 : products_tile(p + 1, 2, product - 1);
+}
+
 size_t fgpu_linear_workspace_bytes(int64_t rows, int in_dim, int out_dim, int dtype) {
   if (check_common(rows, in_dim, out_dim, dtype, 0) != FGPU_OK || rows == 0) return 0;
   const bool f32 = dtype == FGPU_DTYPE_F32;

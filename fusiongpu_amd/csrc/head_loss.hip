@@ -351,6 +351,11 @@ using namespace fgpu;
 
 extern "C" {
 
+int fgpu_contrastive_loss_tile(int nq, int nc, int dim, int dtype) {
+  if (check_loss(nq, nc, dim, dtype) != FGPU_OK || nq == 0) return -1;
+  return dim <= kNarrowDim ? 0 : score_plan(nq, stats_columns(nq, nc)).tile;
+}
+
 size_t fgpu_contrastive_loss_workspace_bytes(int nq, int nc, int dim, int dtype) {
   if (check_loss(nq, nc, dim, dtype) != FGPU_OK || nq == 0) return 0;
   const bool f32 = dtype == FGPU_DTYPE_F32;

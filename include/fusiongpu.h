@@ -642,6 +642,13 @@ fgpu_status fgpu_linear_backward(const void* d_dy, const void* d_x, const void* 
                                  int in_dim, int out_dim, int dtype, int act, void* d_dx, void* d_dw, void* d_db,
                                  void* d_workspace, size_t workspace_bytes, void* stream);
 
+/* Which of its kernels a size takes, for tests and measurements: the width of
+ * the product's tiles (256, 128 or 64), plus FGPU_TILE_PAIR where both gradients
+ * are one launch; 0 for the kernels of few tiles; -1 for sizes that have none.
+ * product: 0 forward, 1 dx, 2 dw. */
+#define FGPU_TILE_PAIR 1024
+int fgpu_linear_tile(int64_t rows, int in_dim, int out_dim, int dtype, int product);
+
 /* y = (x - mean) rstd gamma + beta for each row of x [rows][dim], mean and
  * rstd = 1 / sqrt(variance + eps) its own (biased variance, about the mean).
  * d_gamma, d_beta [dim] may be NULL (one, zero); d_mean, d_rstd [rows] float32
@@ -679,6 +686,9 @@ size_t fgpu_contrastive_loss_workspace_bytes(int nq, int nc, int dim, int dtype)
 fgpu_status fgpu_contrastive_loss(const void* d_q, const void* d_c, const int32_t* d_target, const float* d_bias,
                                   const int32_t* d_ids, int nq, int nc, int dim, int dtype, float scale, float* d_loss,
                                   float* d_lse, void* d_workspace, size_t workspace_bytes, void* stream);
+/* The width of the tiles that the scores above 128 dims are formed in; 0 up to
+ * 128 dims, -1 for sizes that have none. */
+int fgpu_contrastive_loss_tile(int nq, int nc, int dim, int dtype);
 /* Its gradients for dloss [nq] float32, from the lse of the forward call:
  * G_ij = dloss_i (exp(s_ij - lse_i) - [j = target_i]); dq = scale G c, dc = scale
  * G^T q, dbias_j = sum_i G_ij (float32).  Each of d_dq, d_dc, d_dbias may be
