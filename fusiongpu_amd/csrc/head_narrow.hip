@@ -7,6 +7,12 @@
 // bytes an element that a stored gradient would be written and read with, more than the product's own time at these
 // widths, are saved.  Rows are the queries for the statistics and dq, the candidates for dc and dbias.
 //
+// In bfloat16 the score gradients enter the second product rounded, but where a target is among a wave's 32 x 16, its own,
+// about as large as its row's others together, would put its rounding on the whole result: there what the rounding left
+// enters too, as a second operand (few products: a row has one target).  In norm the gradients are then as far from the
+// exact ones as their own rounding puts them, 0.0017, instead of 0.0020 to 0.0026, for 2 % of the time (8192 x 65536 x 128,
+// both gradients, 713 -> 725 us).
+//
 // Bound by the matrix units and, beside them, by the LDS (every wave reads the whole tile, once a product) and the
 // exponentials.  1000 x 100000 x 128 in float32: statistics 139 us (1.1 PFLOP/s in bf16 products), dq 265 us (1.16, the
 // score product formed again); 8192 x 65536 x 128 in bf16: forward 224 us, both gradients 650 us (0.85 PFLOP/s).
@@ -204,6 +210,25 @@ __device__ __forceinline__ void narrow_rows(const NarrowArgs& g, int wg, int wgs
         }
       const int c8 = 32 * p + 8 * g4, n = t * kNTile + c8;
       Frag<T> gf[F];
+      // The tile's vectors with their dims 16 f .. 16 f + 15 as rows.
+      auto turned = [&](int f, int q) {
+        const lds_char* at = l + tr_row + (tr_in ^ (f * 32)) + 32 * p * kNRowBytes + q * (kNTile * kNRowBytes);
+        const s16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_half*)at);
+        const s16x4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_half*)(at + 4 * kNRowBytes));
+        const s16x8 v = {lo[0], lo[1], lo[2], lo[3], hi[0], hi[1], hi[2], hi[3]};
+        return __builtin_bit_cast(bf16x8, v);
+      };
+      // Score gradients as the second product's operand; bf16, `some` (the same in all lanes): also what rounding leaves.
+      auto operand = [&](int j, const f32x8& v, bool some) {
+        gf[j] = to_planes<T>(v);
+        if constexpr (P == 1) {
+          if (some) {
+            const bf16x8 left = to_bf16x8(v - to_f32x8(gf[j].p[0]));
+#pragma unroll
+            for (int f = 0; f < D; ++f) grad[f][j] = mma(turned(f, 0), left, grad[f][j]);
+          }
+        }
+      };
       if constexpr (MODE != kDc) {
         ColumnSide cs;
         cs.load(CandidateSide{d.v0, d.id}, c8);
@@ -234,7 +259,7 @@ __device__ __forceinline__ void narrow_rows(const NarrowArgs& g, int wg, int wgs
 #pragma unroll
               for (int e = 0; e < 8; ++e) v.set(e, at == e ? v[e] - 1.0f : v[e]);
             }
-            gf[j] = to_planes<T>(v);  // the row's weight waits for the sum
+            operand(j, v, P == 1 && __any(here));  // the row's weight waits for the sum
           }
         }
       } else {
@@ -253,7 +278,8 @@ __device__ __forceinline__ void narrow_rows(const NarrowArgs& g, int wg, int wgs
             rare |= qt[e] == cand;
             if (g.a.ids) rare |= qid[e] == row_id[j];
           }
-          if (__any(rare)) {
+          const bool some = __any(rare);
+          if (some) {
 #pragma unroll
             for (int e = 0; e < 8; ++e) {
               if (g.a.ids && qid[e] == row_id[j] && qt[e] != cand && qt[e] >= 0) v.set(e, 0.0f);
@@ -265,7 +291,7 @@ __device__ __forceinline__ void narrow_rows(const NarrowArgs& g, int wg, int wgs
             v.set(e, v[e] * w[e]);
             sum[j] += v[e];
           }
-          gf[j] = to_planes<T>(v);
+          operand(j, v, some);
         }
       }
       if constexpr (MODE != kStats) {
@@ -273,13 +299,7 @@ __device__ __forceinline__ void narrow_rows(const NarrowArgs& g, int wg, int wgs
         for (int f = 0; f < D; ++f) {
           Frag<T> c;
 #pragma unroll
-          for (int q = 0; q < P; ++q) {
-            const lds_char* at = l + tr_row + (tr_in ^ (f * 32)) + 32 * p * kNRowBytes + q * (kNTile * kNRowBytes);
-            const s16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_half*)at);
-            const s16x4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_half*)(at + 4 * kNRowBytes));
-            const s16x8 v = {lo[0], lo[1], lo[2], lo[3], hi[0], hi[1], hi[2], hi[3]};
-            c.p[q] = __builtin_bit_cast(bf16x8, v);
-          }
+          for (int q = 0; q < P; ++q) c.p[q] = turned(f, q);
 #pragma unroll
           for (int j = 0; j < F; ++j) grad[f][j] = mma(c, gf[j], grad[f][j]);
         }

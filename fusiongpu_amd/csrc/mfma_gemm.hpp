@@ -44,11 +44,15 @@ struct f32x8 {
 };
 typedef __bf16 bf16x8u __attribute__((ext_vector_type(8), aligned(2)));
 __device__ __forceinline__ f32x8 load8(const float* p) { return {load4(p), load4(p + 4)}; }
-__device__ __forceinline__ f32x8 load8(const bf16* p) {
-  const bf16x8 v = *reinterpret_cast<const bf16x8u*>(p);
+__device__ __forceinline__ f32x8 to_f32x8(const bf16x8& v) {
   const bf16x4 lo = {v[0], v[1], v[2], v[3]}, hi = {v[4], v[5], v[6], v[7]};
   return {__builtin_convertvector(lo, f32x4), __builtin_convertvector(hi, f32x4)};
 }
+__device__ __forceinline__ f32x8 load8(const bf16* p) {
+  const bf16x8 v = *reinterpret_cast<const bf16x8u*>(p);
+  return to_f32x8(v);
+}
+__device__ __forceinline__ f32x8 operator-(const f32x8& a, const f32x8& b) { return {a.lo - b.lo, a.hi - b.hi}; }
 __device__ __forceinline__ void store8(float* p, const f32x8& v) {
   store4(p, v.lo);
   store4(p + 4, v.hi);

@@ -80,3 +80,46 @@ def test_float32_products_of_one_term(m):
     dx, dw, _ = fg.linear_backward(x, torch.ones_like(x), w[:1], want=("x",))
     want = x.double() * w[0].double()
     assert ((dx.double() - want).abs() <= 6.1 * U * want.abs()).all() and dw is None
+
+
+def rounding(v):
+    """What rounding to bfloat16 takes from v."""
+    return v.bfloat16().double() - v
+
+
+def check_loss_gradient_error(nq, nc, dim, ids, weight, workspace=1.0):
+    """bfloat16 queries half way to their targets: a target's score gradient is about as large as its row's others together,
+    and no part of it may be lost.  The others are rounded, up to 2^-8 of each, with random signs: the gradients are as far
+    from the exact ones, in norm, as the result's own rounding and those together, each at its most."""
+    g = torch.Generator(device="cuda")
+    g.manual_seed(nq + dim)
+    c = torch.nn.functional.normalize(torch.randn((nc, dim), generator=g, device="cuda"))
+    t = torch.randperm(nc, generator=g, device="cuda")[:nq] if nq <= nc else torch.randint(nc, (nq,), generator=g, device="cuda")
+    if ids:  # some targets shared by several rows, near and far
+        t[1::3] = t[0:-1:3][:t[1::3].numel()]
+        t[nq // 2:nq // 2 + 5] = t[0]
+        t[-1] = t[0]
+    q = torch.nn.functional.normalize(0.35 * c[t] + 0.65 * torch.randn((nq, dim), generator=g, device="cuda") / dim**0.5)
+    q, c, t, dl = q.bfloat16(), c.bfloat16(), t.to(torch.int32), torch.full((nq,), weight, device="cuda")
+    t[::17] = -1
+    loss, lse = fg.contrastive_loss(q, c, t, 20.0)
+    size = int(fg.lib.fgpu_contrastive_loss_backward_workspace_bytes(nq, nc, dim, 1) * workspace)
+    dq, dc, _ = fg.contrastive_loss_backward(dl, q, c, t, lse, 20.0, workspace=torch.empty(size, dtype=torch.uint8, device="cuda"))
+    live, at, rows = t >= 0, t.clamp(min=0).long(), torch.arange(nq, device="cuda")
+    qd, cd = q.double(), c.double()
+    p = torch.softmax(20 * qd @ cd.t(), 1) * live[:, None] * weight
+    hot = torch.zeros_like(p)
+    hot[rows, at] = live.double() * weight
+    grad = p - hot
+    others = torch.where(hot > 0, 0.0, grad)
+    for got, want, left, side in ((dq, grad @ cd, others, cd), (dc, grad.t() @ qd, others.t(), qd)):
+        lost = (2.0**-8 * 20 * left).square() @ side.square().sum(1)
+        bound = (rounding(20 * want).square().sum() + lost.sum()).sqrt()
+        assert (got.double() - 20 * want).norm() <= 1.02 * bound
+
+
+@pytest.mark.parametrize("ids", [False, True])
+@pytest.mark.parametrize("weight", [1 / 883, 1.0, 1 / 600])
+@pytest.mark.parametrize("nq,nc,dim", [(883, 4707, 128), (1024, 1024, 96), (700, 700, 40), (3000, 30000, 61)])
+def test_loss_gradients_lose_nothing_of_the_targets(nq, nc, dim, ids, weight):
+    check_loss_gradient_error(nq, nc, dim, ids, weight)
