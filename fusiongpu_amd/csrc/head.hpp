@@ -75,6 +75,30 @@ __device__ __forceinline__ float lanes_sum(float v) {
 }
 
 // ---- products (head_gemm.hip) -------------------------------------------------
+// What the rounding of a product's bfloat16 operand left out, added to rows of D: to row m coef[c] times row r = head[m] of
+// `src` (bfloat16, rows of ld, n of it wanted), c = m, or r with `by_source`; nothing where r is not among its `rows`.  heads
+// lie `step` ints apart.  head NULL: nothing at all.
+struct Remainder {
+  const int* head = nullptr;
+  int step = 1;
+  bool by_source = false;
+  const float* coef = nullptr;
+  const uint16_t* src = nullptr;
+  int64_t ld = 0;
+  int rows = 0;
+  __device__ __forceinline__ int row_of(int m) const { return head ? head[(int64_t)m * step] : -1; }
+  __device__ __forceinline__ bool any(int r) const { return (uint32_t)r < (uint32_t)rows; }
+  __device__ __forceinline__ float coef_of(int m, int r) const { return coef[by_source ? r : m]; }
+  __device__ __forceinline__ const bf16* row(int r) const { return (const bf16*)src + r * ld; }
+  __device__ __forceinline__ void add4(f32x4& v, int m, int col) const {
+    const int r = row_of(m);
+    if (!any(r)) return;
+    const float c = coef_of(m, r);
+    const f32x4 x = load4(row(r) + col);
+#pragma unroll
+    for (int e = 0; e < 4; ++e) v[e] = fmaf(c, x[e], v[e]);
+  }
+};
 // What becomes of D: out = act(alpha D + bias) + residual, with the value before act in `pre`; out and residual [m][n].
 struct Finish {
   const void* bias = nullptr;
@@ -88,6 +112,7 @@ struct Finish {
   // result; both [m][n rounded up to 4] float32.
   const float* add = nullptr;
   float* sum = nullptr;
+  Remainder rest;  // of bfloat16 products without an activation
 };
 
 // out = act(alpha D + bias) + residual for four consecutive columns n .. n + 3 of row m (cnt of them inside).
@@ -177,6 +202,9 @@ struct LossRows {
   const int32_t* ids;
   int nq, nc;
   LossRow* rows;
+  // What head_loss.hip keeps of the targets' score gradients (NULL: nothing): gets zeros [nq], and INT_MAX [nc].
+  float* left = nullptr;
+  int* owner = nullptr;
 };
 // A copy of src [rows][cols] as an operand; rows that a mask takes out become zero.
 struct CopyJob {

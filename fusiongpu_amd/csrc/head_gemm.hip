@@ -4,13 +4,15 @@
 // plain product 1.44 to 1.6), 65536 x 4096 x 1024 with bias, GELU and the kept pre-activation 0.65 ms (0.85 PFLOP/s, 1.1 GB
 // of stores), 8192 x 4096 x 4096 in float32 214 TFLOP/s (the library's float32 product 127 to 154).
 #include <algorithm>
+#include <type_traits>
 
 #include "head.hpp"
 
 namespace fgpu {
 namespace {
 
-template <class T, int ACT>
+// REST: with Finish::rest.
+template <class T, int ACT, bool REST = false>
 struct ProductEpi {
   Finish f;
   float* part;  // [split][m][n4] in place of the result, or NULL
@@ -54,15 +56,37 @@ struct ProductEpi {
     f32x8 bias[P];
 #pragma unroll
     for (int p = 0; p < P; ++p) bias[p] = f.bias ? load8((const T*)f.bias + w.col(p)) : f32x8{{0, 0, 0, 0}, {0, 0, 0, 0}};
+    int head[G::FM];
+    if constexpr (REST) {
+#pragma unroll
+      for (int j = 0; j < G::FM; ++j) head[j] = w.row(j) < m ? f.rest.row_of(w.row(j)) : -1;
+    }
 #pragma unroll
     for (int j = 0; j < G::FM; ++j) {
       if (w.row(j) >= m) continue;
       const int64_t at = (int64_t)w.row(j) * n + w.col(0);
+      f32x8 rest[P];
+      if constexpr (REST) {
+#pragma unroll
+        for (int p = 0; p < P; ++p) rest[p] = f32x8{{0, 0, 0, 0}, {0, 0, 0, 0}};
+        if (f.rest.any(head[j])) {
+          const float c = f.rest.coef_of(w.row(j), head[j]);
+#pragma unroll
+          for (int p = 0; p < P; ++p) {
+            const f32x8 x = load8(f.rest.row(head[j]) + w.col(p));
+            rest[p] = f32x8{x.lo * c, x.hi * c};
+          }
+        }
+      }
 #pragma unroll
       for (int p = 0; p < P; ++p) {
         f32x8 v;
 #pragma unroll
-        for (int e = 0; e < 8; ++e) v.set(e, fmaf(acc[2 * p + e / 4][j][e % 4], f.alpha, bias[p][e]));
+        for (int e = 0; e < 8; ++e) {
+          float d = acc[2 * p + e / 4][j][e % 4];
+          if constexpr (REST) d += rest[p][e];
+          v.set(e, fmaf(d, f.alpha, bias[p][e]));
+        }
         if (f.pre) put<STREAM>((T*)f.pre + at + 32 * p, v);
         if (ACT != FGPU_ACT_NONE) {
 #pragma unroll
@@ -105,7 +129,8 @@ struct ProductEpi {
         const int row = t / (kCols / 4), c4 = t % (kCols / 4), col = w.first_col() + 4 * c4;
         const int gm = w.m0 + (w.wm * G::FM + j0) * 16 + row;
         if (gm >= m || col >= n) continue;
-        const f32x4 v = *reinterpret_cast<const f32x4*>(lds + row * kCols + 4 * (c4 ^ (row & (kCols / 4 - 1))));
+        f32x4 v = *reinterpret_cast<const f32x4*>(lds + row * kCols + 4 * (c4 ^ (row & (kCols / 4 - 1))));
+        if (REST && !part) f.rest.add4(v, gm, col);
         if (part)
           *reinterpret_cast<f32x4*>(part + ((int64_t)w.sp * m + gm) * n4 + col) = v;
         else
@@ -141,10 +166,12 @@ __device__ __forceinline__ void split_finish(const SplitJob& j, int block) {
   if (i >= total) return;
   const int64_t row = i / n4;
   const int col = (int)(i - row * n4) * 4;
-  if (j.f.sum)
+  if (j.f.sum) {
     *reinterpret_cast<f32x4*>(j.f.sum + i * 4) = v;
-  else
-    finish4<T>(j.f, v, row * j.n + col, col, j.n - col);
+    return;
+  }
+  j.f.rest.add4(v, (int)row, col);
+  finish4<T>(j.f, v, row * j.n + col, col, j.n - col);
 }
 
 // 16 columns x 16 groups of parts a workgroup.
@@ -268,6 +295,11 @@ fgpu_status run_tile(int tile, const GemmArgs& g, const E& e, hipStream_t s) {
 template <int PAIRS, class T>
 fgpu_status run_form(bool a_kc, bool b_kc, int tile, const GemmArgs& g, const Finish& f, float* part, hipStream_t s) {
   const ProductEpi<T, FGPU_ACT_NONE> plain{f, part, g.m, g.n};
+  if constexpr (PAIRS == 1) {
+    const ProductEpi<T, FGPU_ACT_NONE, true> rest{f, part, g.m, g.n};
+    if (f.rest.head && !part && !b_kc)
+      return a_kc ? run_tile<true, false, PAIRS>(tile, g, rest, s) : run_tile<false, false, PAIRS>(tile, g, rest, s);
+  }
   if (a_kc && !b_kc) return run_tile<true, false, PAIRS>(tile, g, plain, s);
   if (!a_kc) return run_tile<false, false, PAIRS>(tile, g, plain, s);
   if (part || f.act == FGPU_ACT_NONE) return run_tile<true, true, PAIRS>(tile, g, plain, s);
@@ -294,13 +326,23 @@ fgpu_status run_products(const ProductJob* jobs, int count, const Plan* q, int p
     f[i].stream = (int64_t)j.p.m * j.p.n * (int64_t)sizeof(O) * (j.f.pre ? 2 : 1) > (int64_t)256 << 20;
   }
   if (pair && jobs[0].asked && jobs[1].asked) {
-    const ProductEpi<O, FGPU_ACT_NONE> ex{f[0], part[0], g[0].m, g[0].n}, ew{f[1], part[1], g[1].m, g[1].n};
-    const int nx = g[0].tiles_m * g[0].tiles_n * g[0].splits, nw = g[1].tiles_m * g[1].tiles_n * g[1].splits;
-    if (pair == 128)
-      gemm_pair_kernel<Tile128, PAIRS><<<nx + nw, Tile128::threads, 0, s>>>(g[0], ex, nx, g[1], ew);
+    auto both = [&](auto rest) -> fgpu_status {
+      using E = ProductEpi<O, FGPU_ACT_NONE, decltype(rest)::value>;
+      const E ex{f[0], part[0], g[0].m, g[0].n}, ew{f[1], part[1], g[1].m, g[1].n};
+      const int nx = g[0].tiles_m * g[0].tiles_n * g[0].splits, nw = g[1].tiles_m * g[1].tiles_n * g[1].splits;
+      if (pair == 128)
+        gemm_pair_kernel<Tile128, PAIRS><<<nx + nw, Tile128::threads, 0, s>>>(g[0], ex, nx, g[1], ew);
+      else
+        gemm_pair_kernel<Tile64, PAIRS><<<nx + nw, Tile64::threads, 0, s>>>(g[0], ex, nx, g[1], ew);
+      FGPU_HIP(hipGetLastError());
+      return FGPU_OK;
+    };
+    bool rest = false;
+    for (int i = 0; i < 2; ++i) rest |= f[i].rest.head && !part[i];
+    if constexpr (PAIRS == 1)
+      FGPU_TRY(rest ? both(std::true_type{}) : both(std::false_type{}));
     else
-      gemm_pair_kernel<Tile64, PAIRS><<<nx + nw, Tile64::threads, 0, s>>>(g[0], ex, nx, g[1], ew);
-    FGPU_HIP(hipGetLastError());
+      FGPU_TRY(both(std::false_type{}));
   } else {
     for (int i = 0; i < count; ++i)
       if (jobs[i].asked) FGPU_TRY((run_form<PAIRS, O>(jobs[i].a_kc, jobs[i].b_kc, q[i].tile, g[i], f[i], part[i], s)));

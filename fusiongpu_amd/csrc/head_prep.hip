@@ -89,10 +89,14 @@ __device__ __forceinline__ void loss_row(const LossRows& r, int m) {
     o = {r.lse[m] * kLog2e, r.dloss[m], t, r.ids ? r.ids[t] : 0};
   }
   r.rows[m] = o;
+  if (r.left) r.left[m] = 0;
+}
+__device__ __forceinline__ void clear_candidates(const LossRows& r, int block, int blocks) {
+  for (int64_t c = (int64_t)block * 256 + threadIdx.x; c < r.nc; c += (int64_t)blocks * 256) r.owner[c] = INT_MAX;
 }
 
 struct Blocks {
-  int dz, copy0, copy1;
+  int dz, copy0, copy1, loss, clear;
 };
 template <class T>
 __global__ __launch_bounds__(256) void prep_kernel(Prep p, Blocks n) {
@@ -103,8 +107,10 @@ __global__ __launch_bounds__(256) void prep_kernel(Prep p, Blocks n) {
     copy_rows<T>(p.copy[0], p.loss, b, n.copy0);
   else if ((b -= n.copy0) < n.copy1)
     copy_rows<T>(p.copy[1], p.loss, b, n.copy1);
+  else if ((b -= n.copy1) < n.loss)
+    loss_row(p.loss, b * 256 + threadIdx.x);
   else
-    loss_row(p.loss, (b - n.copy1) * 256 + threadIdx.x);
+    clear_candidates(p.loss, b - n.loss, n.clear);
 }
 
 }  // namespace
@@ -118,9 +124,11 @@ fgpu_status launch_prep(const Prep& p, bool f32, hipStream_t s) {
   auto copy_blocks = [](const CopyJob& j) {
     return j.src ? (int)std::min<int64_t>(ceil_div(j.rows * (whole8(j.cols) / 4), 256), 8192) : 0;
   };
-  Blocks n{0, copy_blocks(p.copy[0]), copy_blocks(p.copy[1])};
+  Blocks n{0, copy_blocks(p.copy[0]), copy_blocks(p.copy[1]), 0, 0};
   if (p.dz.dy) n.dz = ceil_div(p.dz.cols, kDzCols) * p.dz.chunks;
-  const int total = n.dz + n.copy0 + n.copy1 + (p.loss.rows ? ceil_div(p.loss.nq, 256) : 0);
+  if (p.loss.rows) n.loss = ceil_div(p.loss.nq, 256);
+  if (p.loss.owner) n.clear = std::min(ceil_div(p.loss.nc, 1024), 1024);
+  const int total = n.dz + n.copy0 + n.copy1 + n.loss + n.clear;
   if (total == 0) return FGPU_OK;
   if (f32)
     prep_kernel<float><<<total, 256, 0, s>>>(p, n);

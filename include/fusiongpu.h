@@ -693,8 +693,11 @@ int fgpu_contrastive_loss_tile(int nq, int nc, int dim, int dtype);
  * G_ij = dloss_i (exp(s_ij - lse_i) - [j = target_i]); dq = scale G c, dc = scale
  * G^T q, dbias_j = sum_i G_ij (float32).  Each of d_dq, d_dc, d_dbias may be
  * NULL (fixed candidates need no dc).  In bfloat16, G is rounded to bfloat16
- * before the two products (not before dbias); up to 128 dims not a row's
- * element at its target, about as large as the row's others together.  Above 128 dims G is held in the
+ * before the two products (not before dbias), but for a row's element at its
+ * target, about as large as the row's others together, which loses nothing
+ * (above 128 dims, in dc: that of the first row with a target, and only for
+ * nq <= 4 nc).
+ * Above 128 dims G is held in the
  * workspace, all columns at once in the returned size (up to 2^31 elements); a
  * smaller workspace is used in chunks of columns, down to 256.  Up to 128 dims
  * G never leaves the registers, and a smaller workspace (down to the copies of

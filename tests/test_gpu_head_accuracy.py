@@ -112,7 +112,12 @@ def check_loss_gradient_error(nq, nc, dim, ids, weight, workspace=1.0):
     hot[rows, at] = live.double() * weight
     grad = p - hot
     others = torch.where(hot > 0, 0.0, grad)
-    for got, want, left, side in ((dq, grad @ cd, others, cd), (dc, grad.t() @ qd, others.t(), qd)):
+    if dim > 128:  # dc: only a target's first row
+        first = torch.full((nc,), nq, device="cuda").scatter_reduce(0, at[live], rows[live], "amin")
+        shared = torch.where((hot > 0) & (first[None, :] == rows[:, None]), 0.0, grad)
+    else:
+        shared = others
+    for got, want, left, side in ((dq, grad @ cd, others, cd), (dc, grad.t() @ qd, shared.t(), qd)):
         lost = (2.0**-8 * 20 * left).square() @ side.square().sum(1)
         bound = (rounding(20 * want).square().sum() + lost.sum()).sqrt()
         assert (got.double() - 20 * want).norm() <= 1.02 * bound
@@ -123,3 +128,12 @@ def check_loss_gradient_error(nq, nc, dim, ids, weight, workspace=1.0):
 @pytest.mark.parametrize("nq,nc,dim", [(883, 4707, 128), (1024, 1024, 96), (700, 700, 40), (3000, 30000, 61)])
 def test_loss_gradients_lose_nothing_of_the_targets(nq, nc, dim, ids, weight):
     check_loss_gradient_error(nq, nc, dim, ids, weight)
+
+
+@pytest.mark.parametrize("ids", [False, True])
+@pytest.mark.parametrize("nq,nc,dim,weight,workspace", [
+    (883, 4707, 200, 1 / 883, 1.0), (1024, 1024, 136, 1.0, 1.0), (300, 1500, 203, 1 / 600, 1.0), (3001, 30000, 256, 1 / 883, 1.0),
+    (3000, 6001, 137, 1 / 600, 1.0), (1500, 2200, 768, 1.0, 1.0), (700, 9000, 200, 1 / 883, 0.7), (3000, 20000, 136, 1.0, 0.6),
+    (2500, 700, 168, 1 / 883, 1.0)])
+def test_wide_loss_gradients_lose_nothing_of_the_targets(nq, nc, dim, weight, workspace, ids):
+    check_loss_gradient_error(nq, nc, dim, ids, weight, workspace)

@@ -146,3 +146,32 @@ def test_loss_gradients_in_chunks_down_to_the_least(nq, nc, dim, dt):
     assert least < 0.9 * full
     for size in (least, (least + full) // 2, full):
         check_loss(q, c, t, scale, bias, ids, dt, workspace=torch.empty(size, dtype=torch.uint8, device="cuda"))
+
+
+@pytest.mark.parametrize("dt", ["f32", "bf16"])
+@pytest.mark.parametrize("nq,nc,dim", [(300, 900, 72), (300, 900, 200), (1500, 2201, 136), (1501, 30011, 128)])
+def test_loss_gradients_of_some(nq, nc, dim, dt):
+    """Each gradient alone, as C callers may ask, has the bits it has among the others."""
+    q, c, t, scale, bias, ids = loss_inputs(nq, nc, dim, dt)
+    bias[::7], t[::9] = -torch.inf, -1
+    t[5:9] = t[4]
+    code, dl = int(dt == "bf16"), rnd(99, nq)
+    _, lse = fg.contrastive_loss(q, c, t, scale, bias=bias, ids=ids)
+    full = fg.contrastive_loss_backward(dl, q, c, t, lse, scale, bias=bias, ids=ids)
+    size = fg.lib.fgpu_contrastive_loss_backward_workspace_bytes(nq, nc, dim, code)
+    ws = torch.empty(size, dtype=torch.uint8, device="cuda")
+    for some in ((0,), (1,), (2,), (0, 2), (1, 2), (0, 1), ()):
+        out = [torch.full_like(g, 7) if i in some else None for i, g in enumerate(full)]
+        assert fg.lib.fgpu_contrastive_loss_backward(dl.data_ptr(), q.data_ptr(), c.data_ptr(), t.data_ptr(), lse.data_ptr(),
+                                                     bias.data_ptr(), ids.data_ptr(), nq, nc, dim, code, scale,
+                                                     *(None if o is None else o.data_ptr() for o in out), ws.data_ptr(), size,
+                                                     fg._stream()) == 0
+        assert all(o is None or torch.equal(o, g) for o, g in zip(out, full))
+
+
+@pytest.mark.parametrize("nq,nc,dim", [(5000, 3, 200), (3000, 10, 136), (9000, 300, 130), (130, 20, 200), (64, 15, 700), (9, 2, 1000)])
+def test_loss_of_few_candidates(nq, nc, dim):
+    """Many rows with one target, as a classifier has."""
+    q, c, t, scale, bias, _ = loss_inputs(nq, nc, dim, "bf16")
+    check_loss(q, c, t, scale, bias, None, "bf16")
+    check_loss(q, c, torch.full_like(t, nc - 1), scale, bias, None, "bf16")
