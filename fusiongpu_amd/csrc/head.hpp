@@ -11,46 +11,62 @@ inline int ceil_div(int64_t a, int64_t b) { return (int)((a + b - 1) / b); }
 constexpr int64_t kLaunchThreads = (int64_t)1 << 31;
 
 // ---- activations -------------------------------------------------------------
-// gelu(z) = z Phi(z).  The tail 1 - Phi(|z|) = erfc(x) / 2, x = |z| / sqrt(2), is t P(t) exp(-x^2) with t = 1 / (1 + 0.4 x):
-// t runs through (0, 1] and erfc(x) exp(x^2) / t is smooth there, so a polynomial of degree 8, fitted to its least largest
-// relative error (5.7e-8 up to |z| = 13), holds the tail to a float32 last place and a half all the way out; squaring z for
-// the exponential adds 1.5 z^2 2^-24 of it.  A sum with the tail subtracted from one, z (1 + erf(x)) / 2, would lose the
-// negative side's digits.  The exponential is the one that the derivative needs too.  (Five coefficients, good to 7.5e-8 of
-// one, not of the tail, took 639 us instead of 646 at 65536 x 4096 x 1024 in bf16.)
+// gelu(z) = z Phi(z).  The tail 1 - Phi(|z|) = erfc(x) / 2, x = |z| / sqrt(2), is t P(t) exp(-x^2) with t = 1 / (1 + c x):
+// t runs through (0, 1] and erfc(x) exp(x^2) / t is smooth there, so a polynomial fitted to its least largest relative error
+// up to |z| = 13 holds the tail's digits all the way out: of degree 8, c = 0.4, to 5.7e-8, a float32 last place and a half
+// with its roundings; of degree 6, c = 0.51, to 7.2e-7, for bfloat16 results (2^-9 at best; degree 8 there would take 646 us
+// instead of 639 at 65536 x 4096 x 1024).  Squaring z for the exponential adds 1.5 z^2 2^-24 of it.  A sum with the tail
+// subtracted from one, z (1 + erf(x)) / 2, would lose the negative side's digits.  The exponential is the one that the
+// derivative needs too.
 __device__ __forceinline__ float fast_rcp(float x) { return __builtin_amdgcn_rcpf(x); }
 __device__ __forceinline__ float fast_exp2(float x) { return __builtin_amdgcn_exp2f(x); }
 constexpr float kLog2e = 1.44269504088896341f, kLn2 = 0.69314718055994531f;
 
+template <class T>
 __device__ __forceinline__ float normal_cdf(float z, float& e) {
   e = fast_exp2(z * z * (-0.5f * kLog2e));  // exp(-z^2 / 2)
-  const float t = fast_rcp(fmaf(0.282842726f, fabsf(z), 1.0f));
-  float p = fmaf(0.0200270936f, t, -0.0672089234f);
-  p = fmaf(p, t, 0.0358143561f);
-  p = fmaf(p, t, 0.05115458f);
-  p = fmaf(p, t, 0.0348447599f);
-  p = fmaf(p, t, 0.0988777131f);
-  p = fmaf(p, t, 0.100375392f);
-  p = fmaf(p, t, 0.113302819f);
-  p = fmaf(p, t, 0.112812243f);
+  float p, t;
+  if constexpr (sizeof(T) == 4) {
+    t = fast_rcp(fmaf(0.282842726f, fabsf(z), 1.0f));
+    p = fmaf(0.0200270936f, t, -0.0672089234f);
+    p = fmaf(p, t, 0.0358143561f);
+    p = fmaf(p, t, 0.05115458f);
+    p = fmaf(p, t, 0.0348447599f);
+    p = fmaf(p, t, 0.0988777131f);
+    p = fmaf(p, t, 0.100375392f);
+    p = fmaf(p, t, 0.113302819f);
+    p = fmaf(p, t, 0.112812243f);
+  } else {
+    t = fast_rcp(fmaf(0.360624462f, fabsf(z), 1.0f));
+    p = fmaf(0.047742594f, t, -0.181245252f);
+    p = fmaf(p, t, 0.181495771f);
+    p = fmaf(p, t, 0.0259678476f);
+    p = fmaf(p, t, 0.140100196f);
+    p = fmaf(p, t, 0.141972914f);
+    p = fmaf(p, t, 0.143966064f);
+  }
   const float tail = p * t * e;
   return z < 0 ? tail : 1.0f - tail;
 }
 __device__ __forceinline__ float sigmoid(float z) { return fast_rcp(1.0f + fast_exp2(-kLog2e * z)); }
 
+// Of results (act_value) or operands and results (act_slope) of type T.
+template <class T>
 __device__ __forceinline__ float act_value(float z, int act) {
   if (act == FGPU_ACT_RELU) return z < 0 ? 0.0f : z;
   if (act == FGPU_ACT_GELU) {
     float e;
-    return z * normal_cdf(z, e);
+    return z * normal_cdf<T>(z, e);
   }
   if (act == FGPU_ACT_SILU) return z * sigmoid(z);
   return z;
 }
+template <class T>
 __device__ __forceinline__ float act_slope(float z, int act) {
   if (act == FGPU_ACT_RELU) return z > 0 ? 1.0f : 0.0f;
   if (act == FGPU_ACT_GELU) {
     float e;
-    const float c = normal_cdf(z, e);
+    const float c = normal_cdf<T>(z, e);
     return fmaf(z * 0.39894228040143268f, e, c);
   }
   if (act == FGPU_ACT_SILU) {
@@ -123,7 +139,7 @@ __device__ __forceinline__ void finish4(const Finish& f, f32x4 v, int64_t at, in
   if (f.pre) store4_n((T*)f.pre + at, v, cnt);
   if (f.act != FGPU_ACT_NONE) {
 #pragma unroll
-    for (int r = 0; r < 4; ++r) v[r] = act_value(v[r], f.act);
+    for (int r = 0; r < 4; ++r) v[r] = act_value<T>(v[r], f.act);
   }
   if (f.residual) v += load4_n((const T*)f.residual + at, cnt);
   store4_n((T*)f.out + at, v, cnt);

@@ -108,12 +108,12 @@ struct DirectRead {
       if constexpr (DZ) {
         if constexpr (sizeof(T) == 4) {
 #pragma unroll
-          for (int e = 0; e < 8; ++e) r[i].set(e, r[i].get(e) * act_slope(z[i].get(e), act));
+          for (int e = 0; e < 8; ++e) r[i].set(e, r[i].get(e) * act_slope<T>(z[i].get(e), act));
           g[i] = to_frag(r[i]);
         } else {
 #pragma unroll
           for (int e = 0; e < 8; ++e) {
-            const float v = r[i].get(e) * act_slope(z[i].get(e), act);
+            const float v = r[i].get(e) * act_slope<T>(z[i].get(e), act);
             g[i].p[0][e] = (bf16)v;
             left[i].set(e, v - (float)(bf16)v);
           }

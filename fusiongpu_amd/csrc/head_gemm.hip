@@ -90,7 +90,7 @@ struct ProductEpi {
         if (f.pre) put<STREAM>((T*)f.pre + at + 32 * p, v);
         if (ACT != FGPU_ACT_NONE) {
 #pragma unroll
-          for (int e = 0; e < 8; ++e) v.set(e, act_value(v[e], ACT));
+          for (int e = 0; e < 8; ++e) v.set(e, act_value<T>(v[e], ACT));
         }
         if (f.residual) {
           const f32x8 r = load8((const T*)f.residual + at + 32 * p);

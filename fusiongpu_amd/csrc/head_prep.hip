@@ -65,7 +65,7 @@ __device__ __forceinline__ void make_dz(const DzJob& j, int block) {
         if (j.act != FGPU_ACT_NONE) {
           const f32x4 z = load4_n((const T*)j.pre + (int64_t)r * j.cols + c, cnt);
 #pragma unroll
-          for (int k = 0; k < 4; ++k) v[k] *= act_slope(z[k], j.act);
+          for (int k = 0; k < 4; ++k) v[k] *= act_slope<T>(z[k], j.act);
         }
       }
       acc += v;
