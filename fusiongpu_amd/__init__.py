@@ -986,7 +986,8 @@ def build_ivfpq(x, nlist: int, pq_m: int, kmeans_iters: int = 20, init_mode: int
 # --------------------------------------------------------------------------- query head
 # The layers between an encoder and the index, and the loss they are trained by.  The first array decides the type:
 # bfloat16 stays, any other floating type is read as float32 (as everywhere in this package); the arrays beside it must
-# have that type already, so that no weight is converted anew at every call.
+# have that type already, so that no weight is converted anew at every call.  These are plain functions: torch's autograd
+# records nothing of them, a result of tensors that require a gradient does not; their gradients are the backward calls.
 ACTIVATIONS = {"none": 0, "relu": 1, "gelu": 2, "silu": 3}
 
 

@@ -1,7 +1,7 @@
 // head_gemm.hip -- products with a fused epilogue, and what joins split ones and column sums.
 //
 // Bound by the matrix units, and where k is short by the epilogue: 8192^3 in bf16 takes 0.82 ms (1.35 PFLOP/s; the library's
-// plain product 1.44 to 1.6), 65536 x 4096 x 1024 with bias, GELU and the kept pre-activation 0.65 ms (0.85 PFLOP/s, 1.1 GB
+// plain product 1.44 to 1.6), 65536 x 4096 x 1024 with bias, GELU and the kept pre-activation 0.64 ms (0.86 PFLOP/s, 1.1 GB
 // of stores), 8192 x 4096 x 4096 in float32 214 TFLOP/s (the library's float32 product 127 to 154).
 #include <algorithm>
 #include <type_traits>

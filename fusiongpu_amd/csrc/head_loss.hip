@@ -16,7 +16,7 @@
 // gradients, 17.9 -> 20.2 us, 8192 x 65536 x 768 2474 -> 2485).
 //
 // Above 128 dims a row's gradient no longer fits the registers beside its vector, and reading G back costs less than a
-// third product.  8192 x 65536 x 768 in bf16: statistics 0.92 ms (0.89 PFLOP/s), G 1.05 ms, dq and dc 0.70 each (1.2
+// third product.  8192 x 65536 x 768 in bf16: statistics 0.88 ms (0.94 PFLOP/s), G 0.98 ms, dq and dc 0.68 each (1.2
 // PFLOP/s): the two score products have twelve k steps a tile only, and their epilogues (an exponential an element; G's
 // stores) are not hidden, because a 256 x 256 tile leaves a CU room for one workgroup.
 #include <algorithm>

@@ -14,8 +14,8 @@
 // both gradients, 713 -> 725 us).
 //
 // Bound by the matrix units and, beside them, by the LDS (every wave reads the whole tile, once a product) and the
-// exponentials.  1000 x 100000 x 128 in float32: statistics 139 us (1.1 PFLOP/s in bf16 products), dq 265 us (1.16, the
-// score product formed again); 8192 x 65536 x 128 in bf16: forward 224 us, both gradients 650 us (0.85 PFLOP/s).
+// exponentials.  1000 x 100000 x 128 in float32: statistics 140 us (1.1 PFLOP/s in bf16 products), dq 277 us (1.1, the
+// score product formed again); 8192 x 65536 x 128 in bf16: forward 226 us, both gradients 0.70 ms (0.79 PFLOP/s).
 #include <algorithm>
 
 #include "loss_scores.hpp"

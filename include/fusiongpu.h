@@ -678,8 +678,8 @@ fgpu_status fgpu_layer_norm_backward(const void* d_dy, const void* d_x, const vo
  * candidate left has lse -infinity, loss 0 and no gradient; a row whose target
  * is masked has an infinite loss and no gradient.  d_loss, d_lse [nq] float32.
  * nq <= FGPU_LOSS_MAX_QUERIES.  Beside copies of operands that cannot be read
- * as they are, the workspace holds partial sums: at most 512 MB of them however
- * many candidates there are (above 128 dims; a few rows' worth up to 128). */
+ * as they are, the workspace holds partial sums, above 128 dims at most 512 MB
+ * and up to 128 at most 4 KB a query, however many candidates there are. */
 #define FGPU_MASK_BIAS (-8.507059173023462e37f) /* -2^126 */
 #define FGPU_LOSS_MAX_QUERIES (1 << 20)
 size_t fgpu_contrastive_loss_workspace_bytes(int nq, int nc, int dim, int dtype);
