@@ -9,9 +9,9 @@
 //
 // Bound by latency: one row x 1024 x 1024 in bf16 takes 4.6 us on the GPU, of which its 2 MB of weights are 0.4 at the
 // rate of a copy and a launch 2: 64 workgroups, four k steps a wave, which it loads two at a time, so it waits for two rounds
-// of loads and for the join; 128 x 768 x 2048 6.7 us (tiled 7.3 with the caches warm); float32 400 x 256 x 256 6.9 us (tiled, with
-// its two copies, 12).  Beyond a few rounds of tiles the fragments' loads from the caches bound it (each element is read
-// once a 32-wide tile) and the tiled products take over: head_linear.hip has the rule and both sides.
+// of loads and for the join; 128 x 768 x 2048 6.7 us (tiled 7.3 with the caches warm); float32 400 x 256 x 256 6.9 us
+// (tiled, with its two copies, 12).  Beyond a few rounds of tiles the fragments' loads from the caches bound it (each
+// element is read once a 32-wide tile) and the tiled products take over: head_linear.hip has the rule and both sides.
 #include <algorithm>
 
 #include "head.hpp"

@@ -248,7 +248,8 @@ Plan plan_at(const Product& p, int tile, int splits) {
   return q;
 }
 int64_t plan_threads(const Plan& q) {
-  return (int64_t)q.tiles_m * q.tiles_n * q.splits * (q.tile == 256 ? Tile256::threads : q.tile == 128 ? Tile128::threads : Tile64::threads);
+  const int threads = q.tile == 256 ? Tile256::threads : q.tile == 128 ? Tile128::threads : Tile64::threads;
+  return (int64_t)q.tiles_m * q.tiles_n * q.splits * threads;
 }
 // Of the plans that are one launch (2^30 rows of up to 64 columns on 64 x 64 tiles are not).
 Plan plan_of(const Product& p, int only = 0) {

@@ -18,10 +18,10 @@ DirectOperand direct(const void* p, int64_t rows, int64_t cols, const void* pre 
 
 // Whether the products of few tiles take the direct kernels (head_direct.hip): by the estimates of both, fitted to
 // measurements; a launch is priced at 2.7 us, what a caller pays for it in a row of small calls.  Measured from call
-// to call in a captured row of them (us, tiled / direct): forward bf16 1 x 1024 x 1024 (rows, in, out) 7.4 / 5.3, 128 x 1024 x 1024 9.4 / 8.0, 512 x 1024 x
-// 1024 8.5 / 12; float32 128 x 768 x 2048 22 / 11, 512 x 1024 x 1024 27 / 21, 1024^3 33 / 38; backward bf16 400 x 256 x 256
-// 11.5 / 6.1, 256 x 1024 x 1024 15 / 11, 512 x 1024 x 1024 15.7 / 16.0, 1024^3 19 / 25; float32 400 x 256 x 256 18 / 8.8,
-// 777 x 333 x 555 26 / 21, 512 x 1024 x 1024 36 / 46.
+// to call in a captured row of them, without an activation (us, tiled / direct): forward bf16 1 x 1024 x 1024 (rows, in,
+// out) 7.4 / 5.3, 128 x 1024 x 1024 9.4 / 8.0, 512 x 1024 x 1024 8.5 / 12; float32 128 x 768 x 2048 22 / 11, 512 x 1024 x
+// 1024 27 / 21, 1024^3 33 / 38; backward bf16 400 x 256 x 256 11.5 / 6.1, 256 x 1024 x 1024 15 / 11, 512 x 1024 x 1024
+// 15.7 / 16.0, 1024^3 19 / 25; float32 400 x 256 x 256 18 / 8.8, 777 x 333 x 555 26 / 21, 512 x 1024 x 1024 36 / 46.
 constexpr double kLaunch = 2.7;
 bool forward_direct(const Product& p) {
   double tiled = products_estimate_us(&p, 1);

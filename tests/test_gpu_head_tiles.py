@@ -175,3 +175,28 @@ def test_loss_of_few_candidates(nq, nc, dim):
     q, c, t, scale, bias, _ = loss_inputs(nq, nc, dim, "bf16")
     check_loss(q, c, t, scale, bias, None, "bf16")
     check_loss(q, c, torch.full_like(t, nc - 1), scale, bias, None, "bf16")
+
+
+@pytest.mark.parametrize("dt", ["f32", "bf16"])
+@pytest.mark.parametrize("nq,nc,dim", [(1500, 2201, 136), (3301, 4100, 200)])
+def test_loss_captured_and_replayed(nq, nc, dim, dt):
+    """Above 128 dims: replays on changing inputs and targets, with eager calls between, are the eager results."""
+    q, c, t, scale, bias, ids = loss_inputs(nq, nc, dim, dt)
+    dl = rnd(99, nq)
+
+    def step():
+        loss, lse = fg.contrastive_loss(q, c, t, scale, bias=bias, ids=ids)
+        return [loss, lse, *fg.contrastive_loss_backward(dl, q, c, t, lse, scale, bias=bias, ids=ids)]
+
+    step()
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = step()
+    for k in range(3):
+        q.copy_(rnd(100 + k, nq, dim, dtype=q.dtype))
+        t.copy_(t.roll(7 + k))
+        graph.replay()
+        torch.cuda.synchronize()
+        got = [o.clone() for o in out]
+        assert all(torch.equal(a, b) for a, b in zip(got, step()))
