@@ -20,8 +20,9 @@ Reference interfaces mirrored (Hello-day/FusionGPU):
   * pq_train                        -> train_residual_pq_codebooks (pq_utils.h:77-138)
   * pq_encode                       -> encode_residuals_to_pq_gpu (kmeans_gpu.cuh:450-508)
   * build_ivfpq                     -> build_global main (build_global.cu:21-258), no rebalancing
-and, without a counterpart there, the layers and the loss of a query head (linear, layer_norm, contrastive_loss and
-their backward calls), which query_head.py puts together.
+and, without a counterpart there, the layers and the loss of a query head (linear, gated_linear, layer_norm,
+contrastive_loss and their backward calls; linear_int8, gated_linear_int8 and quantize_rows for weights in 8-bit integers;
+orthogonalize for a weight's update), which query_head.py puts together.
 """
 from __future__ import annotations
 
@@ -37,7 +38,8 @@ __all__ = [
     "fixed_shift", "pq_train", "pq_encode", "build_ivfpq", "write_ivf_data", "read_ivf_data",
     "write_fvecs", "read_fvecs", "read_ivecs", "probe_counts", "rerank", "knn_exact", "graph_search",
     "stream_read", "row_gather", "FAULT_ID", "prune_probes", "graph_add_reverse", "linear", "linear_backward",
-    "layer_norm", "layer_norm_backward", "contrastive_loss", "contrastive_loss_backward",
+    "layer_norm", "layer_norm_backward", "contrastive_loss", "contrastive_loss_backward", "gated_linear",
+    "gated_linear_backward", "quantize_rows", "linear_int8", "gated_linear_int8", "orthogonalize", "int8_row",
 ]
 
 lib_path = os.path.join(os.path.dirname(os.path.abspath(__file__)), "_lib", "libfusiongpu.so")
@@ -131,6 +133,18 @@ _SIGS = {
     "fgpu_linear": (_i32, [_vp, _vp, _vp, _vp, _i64, _i32, _i32, _i32, _i32, _vp, _vp, _vp, _sz, _vp]),
     "fgpu_linear_backward_workspace_bytes": (_sz, [_i64, _i32, _i32, _i32]),
     "fgpu_linear_backward": (_i32, [_vp, _vp, _vp, _vp, _i64, _i32, _i32, _i32, _i32, _vp, _vp, _vp, _vp, _sz, _vp]),
+    "fgpu_gated_linear_tile": (_i32, [_i64, _i32, _i32, _i32]),
+    "fgpu_gated_linear_workspace_bytes": (_sz, [_i64, _i32, _i32, _i32]),
+    "fgpu_gated_linear": (_i32, [_vp, _vp, _vp, _i64, _i32, _i32, _i32, _i32, _vp, _vp, _vp, _sz, _vp]),
+    "fgpu_gated_linear_backward_workspace_bytes": (_sz, [_i64, _i32, _i32, _i32]),
+    "fgpu_gated_linear_backward": (_i32, [_vp, _vp, _vp, _vp, _i64, _i32, _i32, _i32, _i32, _vp, _vp, _vp, _vp, _sz, _vp]),
+    "fgpu_quantize_rows": (_i32, [_vp, _i64, _i32, _i32, _vp, _vp, _vp]),
+    "fgpu_linear_int8_workspace_bytes": (_sz, [_i64, _i32, _i32, _i32, _i32]),
+    "fgpu_linear_int8": (_i32, [_vp, _vp, _vp, _vp, _vp, _vp, _i64, _i32, _i32, _i32, _i32, _vp, _vp, _sz, _vp]),
+    "fgpu_gated_linear_int8_workspace_bytes": (_sz, [_i64, _i32, _i32, _i32, _i32]),
+    "fgpu_gated_linear_int8": (_i32, [_vp, _vp, _vp, _vp, _vp, _i64, _i32, _i32, _i32, _i32, _vp, _vp, _sz, _vp]),
+    "fgpu_orthogonalize_workspace_bytes": (_sz, [_i64, _i64, _i32]),
+    "fgpu_orthogonalize": (_i32, [_vp, _i64, _i64, _i32, _i32, _f32, _f32, _f32, _f32, _vp, _vp, _sz, _vp]),
     "fgpu_layer_norm": (_i32, [_vp, _vp, _vp, _i64, _i32, _i32, _f32, _vp, _vp, _vp, _vp]),
     "fgpu_layer_norm_backward_workspace_bytes": (_sz, [_i64, _i32, _i32]),
     "fgpu_layer_norm_backward": (_i32, [_vp, _vp, _vp, _vp, _vp, _i64, _i32, _i32, _vp, _vp, _vp, _vp, _sz, _vp]),
@@ -1109,6 +1123,157 @@ def linear_backward(dy, x, weight, pre=None, act: str = "none", want=("x", "weig
         _check(lib.fgpu_linear_backward(dy.data_ptr(), x.data_ptr(), w.data_ptr(), _ptr(z), rows, k, n, dt, code, _ptr(dx),
                                         _ptr(dw), _ptr(db), wp, wb, _stream()))
     return dx, dw, db
+
+
+def gated_linear(x, weight, bias=None, act: str = "silu", save_pre: bool = False, out=None, stream=None):
+    """act(x Wg^T + bg) (x Wu^T + bu) (fgpu_gated_linear): x [rows][in], weight [2 hidden][in] with Wg's rows first, bias
+    [2 hidden].  With save_pre also both factors' values before act, [rows][2 hidden], which gated_linear_backward needs:
+    (h, pre)."""
+    code = _act_code(act)
+    with _on(stream):
+        x = _head_first(x, "x")
+        (rows, k), t = x.shape, x.dtype
+        w = _head(weight, t, "weight", (None, k))
+        n = _halves(w, "weight")
+        b = _head_opt(bias, t, "bias", (2 * n,))
+        h = _head_out(out, x, (rows, n))
+        pre = _head_out(None, x, (rows, 2 * n)) if save_pre else None
+        _here(x, w, b, h)
+        dt = _dtype_code(x)
+        wp, wb, ws = _head_ws(lib.fgpu_gated_linear_workspace_bytes(rows, k, n, dt), x)
+        _check(lib.fgpu_gated_linear(x.data_ptr(), w.data_ptr(), _ptr(b), rows, k, n, dt, code, h.data_ptr(), _ptr(pre), wp,
+                                     wb, _stream()))
+    return (h, pre) if save_pre else h
+
+
+def gated_linear_backward(dh, x, weight, pre, act: str = "silu", want=("x", "weight", "bias"), stream=None):
+    """Gradients of gated_linear (fgpu_gated_linear_backward): (dx, dweight, dbias), None for those not in `want`.  pre:
+    what gated_linear(save_pre=True) returned beside h."""
+    code = _act_code(act)
+    if not set(want) <= {"x", "weight", "bias"}:
+        raise ValueError(f"want: {tuple(want)!r} names something other than x, weight and bias")
+    with _on(stream):
+        dh = _head_first(dh, "dh")
+        (rows, n), t = dh.shape, dh.dtype
+        x = _head(x, t, "x", (rows, None))
+        k = x.shape[1]
+        w = _head(weight, t, "weight", (2 * n, k))
+        z = _head(pre, t, "pre", (rows, 2 * n))
+        _here(dh, x, w, z)
+        dx = _head_out(None, dh, (rows, k)) if "x" in want else None
+        dw = _head_out(None, dh, (2 * n, k)) if "weight" in want else None
+        db = _head_out(None, dh, (2 * n,)) if "bias" in want else None
+        dt = _dtype_code(dh)
+        wp, wb, ws = _head_ws(lib.fgpu_gated_linear_backward_workspace_bytes(rows, k, n, dt), dh)
+        _check(lib.fgpu_gated_linear_backward(dh.data_ptr(), x.data_ptr(), w.data_ptr(), z.data_ptr(), rows, k, n, dt, code,
+                                              _ptr(dx), _ptr(dw), _ptr(db), wp, wb, _stream()))
+    return dx, dw, db
+
+
+def _here(*tensors):
+    """Refuses tensors of another device than the current one, whose stream the call goes to."""
+    now = _TORCH.cuda.current_device()
+    for t in tensors:
+        if t is not None and t.get_device() != now:
+            raise ValueError(f"a tensor on {t.device}, but the current device is cuda:{now}: make the call under "
+                             "torch.cuda.device(...) of its tensors")
+
+
+def _halves(w, name):
+    if w.shape[0] % 2:
+        raise ValueError(f"{name}: {w.shape[0]} rows, expected both projections' ones, an even number")
+    return w.shape[0] // 2
+
+
+def int8_row(dim: int) -> int:
+    """The bytes that quantize_rows gives a row of dim values (FGPU_INT8_ROW): whole groups of 16, zeros behind them."""
+    return (dim + 15) // 16 * 16
+
+
+def quantize_rows(x, stream=None):
+    """x [rows][dim] as 8-bit integers with a scale a row (fgpu_quantize_rows): (q int8 [rows][int8_row(dim)], scale float32
+    [rows]), x ~ q scale, zeros behind a row's dim values."""
+    torch = _torch()
+    with _on(stream):
+        x = _head_first(x, "x")
+        rows, dim = x.shape
+        _here(x)
+        q = torch.empty((rows, int8_row(dim)), dtype=torch.int8, device=x.device)
+        scale = torch.empty(rows, dtype=torch.float32, device=x.device)
+        _check(lib.fgpu_quantize_rows(x.data_ptr(), rows, dim, _dtype_code(x), q.data_ptr(), scale.data_ptr(), _stream()))
+    return q, scale
+
+
+def _int8_args(x, weight, weight_scale, x_scale, dtype):
+    """(x, its scales or None, weight, its scales, rows, in_dim, weight rows, the result's dtype)"""
+    torch = _torch()
+    if x_scale is None:
+        x = _head_first(x, "x")
+        if dtype is not None and dtype is not x.dtype:
+            raise TypeError(f"dtype: {dtype}, but x, which decides it, is {x.dtype}")
+        (rows, k), t = x.shape, x.dtype
+        xs = None
+    else:
+        t = torch.bfloat16 if dtype is None else dtype
+        if t not in (torch.bfloat16, torch.float32):
+            raise TypeError(f"dtype: {t}, expected bfloat16 or float32")
+        x = _head(x, torch.int8, "x", (None, None))
+        rows, k = x.shape
+        if k % 16:
+            raise ValueError(f"x: rows of {k} 8-bit integers, expected a multiple of 16 (quantize_rows)")
+        xs = _row(x_scale, torch.float32, "x_scale", rows)
+    w = _head(weight, torch.int8, "weight", (None, int8_row(k)))
+    return x, xs, w, _row(weight_scale, torch.float32, "weight_scale", w.shape[0]), rows, k, w.shape[0], t
+
+
+def linear_int8(x, weight, weight_scale, bias=None, residual=None, act: str = "none", x_scale=None, dtype=None, out=None,
+                stream=None):
+    """linear with a weight held as quantize_rows gives it (fgpu_linear_int8): weight int8 [out][int8_row(in)], weight_scale
+    [out].  x [rows][in] is float32 or bfloat16 and rounded row by row inside the call, or (with x_scale [rows]) int8 held
+    the same way, and then dtype names the result's type (bfloat16 by default), which bias and residual have."""
+    code = _act_code(act)
+    with _on(stream):
+        x, xs, w, ws, rows, k, n, t = _int8_args(x, weight, weight_scale, x_scale, dtype)
+        b, r = _head_opt(bias, t, "bias", (n,)), _head_opt(residual, t, "residual", (rows, n))
+        y = x.new_empty((rows, n), dtype=t) if out is None else _out(out, t, (rows, n), "out")
+        _here(x, xs, w, ws, b, r, y)
+        dt = _dtype_code(y)
+        wp, wb, hold = _head_ws(lib.fgpu_linear_int8_workspace_bytes(rows, k, n, dt, xs is not None), x)
+        _check(lib.fgpu_linear_int8(x.data_ptr(), _ptr(xs), w.data_ptr(), ws.data_ptr(), _ptr(b), _ptr(r), rows, k, n, dt, code,
+                                    y.data_ptr(), wp, wb, _stream()))
+    return y
+
+
+def gated_linear_int8(x, weight, weight_scale, bias=None, act: str = "silu", x_scale=None, dtype=None, out=None, stream=None):
+    """gated_linear with a weight held as quantize_rows gives it (fgpu_gated_linear_int8): weight int8 [2 hidden]
+    [int8_row(in)], weight_scale [2 hidden]; x, x_scale and dtype as in linear_int8."""
+    code = _act_code(act)
+    with _on(stream):
+        x, xs, w, ws, rows, k, _, t = _int8_args(x, weight, weight_scale, x_scale, dtype)
+        n = _halves(w, "weight")
+        b = _head_opt(bias, t, "bias", (2 * n,))
+        h = x.new_empty((rows, n), dtype=t) if out is None else _out(out, t, (rows, n), "out")
+        _here(x, xs, w, ws, b, h)
+        dt = _dtype_code(h)
+        wp, wb, hold = _head_ws(lib.fgpu_gated_linear_int8_workspace_bytes(rows, k, n, dt, xs is not None), x)
+        _check(lib.fgpu_gated_linear_int8(x.data_ptr(), _ptr(xs), w.data_ptr(), ws.data_ptr(), _ptr(b), rows, k, n, dt, code,
+                                          h.data_ptr(), wp, wb, _stream()))
+    return h
+
+
+def orthogonalize(x, steps: int = 5, coefficients=(3.4445, -4.7750, 2.0315), eps: float = 1e-7, out=None, stream=None):
+    """A weight's update x [rows][cols] with its singular values drawn towards one by `steps` Newton-Schulz steps s <- a s +
+    b s^3 + c s^5 (fgpu_orthogonalize), from x / (|x| + eps)."""
+    a, b, c = (float(v) for v in coefficients)
+    with _on(stream):
+        x = _head_first(x, "x")
+        rows, cols = x.shape
+        y = _head_out(out, x, (rows, cols))
+        _here(x, y)
+        dt = _dtype_code(x)
+        wp, wb, ws = _head_ws(lib.fgpu_orthogonalize_workspace_bytes(rows, cols, dt), x)
+        _check(lib.fgpu_orthogonalize(x.data_ptr(), rows, cols, dt, steps, a, b, c, eps, y.data_ptr(), wp, wb, _stream()))
+    return y
 
 
 def layer_norm(x, gamma=None, beta=None, eps: float = 1e-5, out=None, stream=None):

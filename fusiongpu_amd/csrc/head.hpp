@@ -76,6 +76,22 @@ __device__ __forceinline__ float act_slope(float z, int act) {
   return 1.0f;
 }
 
+// Both at once: the exponential is the same.
+template <class T>
+__device__ __forceinline__ void act_both(float z, int act, float& value, float& slope) {
+  value = z, slope = 1.0f;
+  if (act == FGPU_ACT_RELU) value = z < 0 ? 0.0f : z, slope = z > 0 ? 1.0f : 0.0f;
+  if (act == FGPU_ACT_GELU) {
+    float e;
+    const float c = normal_cdf<T>(z, e);
+    value = z * c, slope = fmaf(z * 0.39894228040143268f, e, c);
+  }
+  if (act == FGPU_ACT_SILU) {
+    const float s = sigmoid(z);
+    value = z * s, slope = s * fmaf(z, 1.0f - s, 1.0f);
+  }
+}
+
 // ---- sums across lanes -----------------------------------------------------------
 // Sum over aligned groups of N lanes (16, 32 or 64), the same bits in all of them.  Four exchanges inside a row of 16
 // lanes (pairs, quads, then the mirrored half and the mirrored row, whose sums are already alike), two swaps beyond.
@@ -145,12 +161,37 @@ __device__ __forceinline__ void finish4(const Finish& f, f32x4 v, int64_t at, in
   store4_n((T*)f.out + at, v, cnt);
 }
 
+// h = act(g) u with g and u = D's two halves + bias [2 n], for four consecutive columns col .. col + 3 of a row (cnt of
+// them inside); both halves kept in `pre` [m][2 n] where wanted, h in `out` [m][n].
+template <class T>
+__device__ __forceinline__ void finish4_gated(const Finish& f, f32x4 g, f32x4 u, int64_t row, int n, int col, int cnt) {
+  if (f.bias) {
+    g += load4_n((const T*)f.bias + col, cnt);
+    u += load4_n((const T*)f.bias + n + col, cnt);
+  }
+  if (f.pre) {
+    T* pre = (T*)f.pre + row * 2 * n + col;
+    store4_n(pre, g, cnt);
+    store4_n(pre + n, u, cnt);
+  }
+#pragma unroll
+  for (int r = 0; r < 4; ++r) u[r] *= act_value<T>(g[r], f.act);
+  store4_n((T*)f.out + row * n + col, u, cnt);
+}
+
 // A product of m x n over k, of bf16 operands and results, or (f32) of split planes and float32 results.
 struct Product {
   int m, n, k;
   bool f32;
   bool chunked = false;
+  int pairs = 0;  // plane products of a step of k, 0: six of float32, one of bf16
 };
+// How a product is cut: tiles of `tile` squared, k in `splits` parts; tile 0: no cut is one launch.
+struct Plan {
+  int tile, tiles_m, tiles_n, splits, k_per_split;
+  double us;
+};
+Plan plan_product(const Product& p, bool may_split);
 // One product and where its result goes.
 struct ProductJob {
   Product p;
@@ -237,6 +278,9 @@ struct DzJob {
   int act = 0, rows = 0, cols = 0, chunks = 0;
   GemmOperand dst{};
   float* part = nullptr;
+  // Of a gated layer h = act(g) u: dy is dh [rows][cols], pre [g | u] [rows][2 cols], and dz [dh u act'(g) | dh act(g)]
+  // with its sums [chunk][2 cols].
+  bool gated = false;
 };
 int dz_chunks(int rows, int cols);
 struct Prep {
@@ -253,6 +297,7 @@ struct DirectOperand {
   const void* p;
   int64_t ld, count;
   const void* pre;
+  int up = 0;  // gated products: rows from one of the operand to the one that its product goes with
 };
 struct DirectJob {
   DirectOperand a, b;
@@ -263,6 +308,8 @@ struct DirectJob {
 };
 // D = A B^T, both with k contiguous.
 fgpu_status launch_direct_forward(const DirectJob& j, bool f32, hipStream_t s);
+// A gated layer's: n hidden columns, b.up = n.
+fgpu_status launch_direct_gated(const DirectJob& j, bool f32, hipStream_t s);
 // In one launch: x (A with k contiguous, B strided), w (both strided); either may be NULL.
 fgpu_status launch_direct_backward(const DirectJob* x, const DirectJob* w, bool f32, hipStream_t s);
 // The times that the rule between these and the tiled products goes by.

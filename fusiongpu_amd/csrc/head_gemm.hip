@@ -223,10 +223,6 @@ __global__ __launch_bounds__(256) void join_kernel(SplitJob a, int a_blocks, Spl
 }
 constexpr int kJoinGrid = 1 << 16;  // workgroups at most: a block's result is the same whichever takes it
 
-struct Plan {
-  int tile, tiles_m, tiles_n, splits, k_per_split;
-  double us;
-};
 // Microseconds of a product on `tile` tiles with k in `splits` parts.  A workgroup's k step takes `alone` while few share
 // a CU and `shared` for each that does (measured: 256 x 256 1.6 / 1.6 at one a CU, 128 x 128 0.64 / 0.5 at two, 64 x 64
 // 0.35 / 0.21 at five; float32's six plane products six times that, but 1.2 / 0.63 at three for 64 x 64, which holds all
@@ -241,7 +237,7 @@ Plan plan_at(const Product& p, int tile, int splits) {
   const double fixed = tile == 256 ? 8 : tile == 128 ? 4 : 3;
   const int most = tile == 256 ? 1 : tile == 128 ? 2 : p.f32 ? 3 : 5;
   const int64_t wgs = (int64_t)q.tiles_m * q.tiles_n * q.splits, full = wgs / (256 * most), rest = wgs % (256 * most);
-  const double k = (double)per * (p.f32 ? 6 : 1);
+  const double k = (double)per * (p.pairs ? p.pairs : p.f32 ? 6 : 1);
   q.us = full * (k * std::max(alone, most * shared) + fixed);
   if (rest) q.us += k * std::max(alone, ceil_div(rest, 256) * shared) + fixed;
   if (q.splits > 1) q.us += 3 + 8.0 * q.splits * p.m * ((p.n + 3) & ~3) / 6e6;
@@ -252,12 +248,12 @@ int64_t plan_threads(const Plan& q) {
   return (int64_t)q.tiles_m * q.tiles_n * q.splits * threads;
 }
 // Of the plans that are one launch (2^30 rows of up to 64 columns on 64 x 64 tiles are not).
-Plan plan_of(const Product& p, int only = 0) {
+Plan plan_of(const Product& p, int only = 0, bool may_split = true) {
   Plan best{};
   for (int tile : {256, 128, 64}) {
     if (only && tile != only) continue;
     for (int splits : {1, 2, 3, 4, 6, 8, 12, 16, 24, 32, 48, 64}) {
-      if (splits > 1 && splits > ceil_div(p.k, 2 * kGemmBK)) break;
+      if (splits > 1 && (!may_split || splits > ceil_div(p.k, 2 * kGemmBK))) break;
       const Plan q = plan_at(p, tile, splits);
       if (plan_threads(q) >= 2 * kLaunchThreads) continue;
       if (!best.tile || q.us < best.us) best = q;
@@ -369,6 +365,8 @@ fgpu_status launch_join(const SplitJob& a, const SplitJob& b, const ColumnSum* s
   FGPU_HIP(hipGetLastError());
   return FGPU_OK;
 }
+
+Plan plan_product(const Product& p, bool may_split) { return plan_of(p, 0, may_split); }
 
 size_t products_workspace_bytes(const Product* p, int count) {
   Plan q[2];

@@ -85,6 +85,81 @@ __device__ __forceinline__ void make_dz(const DzJob& j, int block) {
   }
 }
 
+// Four elements of an operand's row at any address, the first n of them.
+template <class T>
+__device__ __forceinline__ void put4_n(uint16_t* d, int64_t plane, const f32x4& v, int n) {
+  if constexpr (sizeof(T) == 2) {
+    store4_n((bf16*)d, v, n);
+  } else {
+    bf16x4 p[3];
+    split4(v, p[0], p[1], p[2]);
+#pragma unroll
+    for (int q = 0; q < 3; ++q) {
+      bf16* at = (bf16*)d + q * plane;
+      if (n >= 4) {
+        *reinterpret_cast<bf16x4u*>(at) = p[q];
+      } else {
+#pragma unroll
+        for (int e = 0; e < 3; ++e)
+          if (e < n) at[e] = p[q][e];
+      }
+    }
+  }
+}
+
+// The same of a gated layer: a thread four hidden columns, both halves of dz.
+template <class T>
+__device__ __forceinline__ void make_gated_dz(const DzJob& j, int block) {
+  __shared__ f32x4 sum[2][4][64];
+  const int across = (j.cols + kDzCols - 1) / kDzCols, chunk = block / across;
+  const int lane = threadIdx.x & 63, w = threadIdx.x >> 6;
+  const int c = block % across * kDzCols + lane * 4, cnt = min(j.cols - c, 4);
+  const int per = (j.rows + j.chunks - 1) / j.chunks, r0 = chunk * per, r1 = min(j.rows, r0 + per);
+  uint16_t* dst = const_cast<uint16_t*>(j.dst.p);
+  f32x4 ag = {0, 0, 0, 0}, au = {0, 0, 0, 0};
+  if (cnt > 0) {
+    const int pad = c + 4 >= j.cols ? (int)whole8(2 * j.cols) - 2 * j.cols : 0;  // zeros behind the row
+#pragma unroll 2
+    for (int r = r0 + w; r < r1; r += 4) {
+      const T* pre = (const T*)j.pre + (int64_t)r * 2 * j.cols + c;
+      const f32x4 d = load4_n((const T*)j.dy + (int64_t)r * j.cols + c, cnt);
+      const f32x4 g = load4_n(pre, cnt), u = load4_n(pre + j.cols, cnt);
+      f32x4 dg, du;
+#pragma unroll
+      for (int k = 0; k < 4; ++k) {
+        float value, slope;
+        act_both<T>(g[k], j.act, value, slope);
+        dg[k] = d[k] * u[k] * slope;
+        du[k] = d[k] * value;
+      }
+      if (cnt < 4) {
+#pragma unroll
+        for (int k = 1; k < 4; ++k)
+          if (k >= cnt) dg[k] = du[k] = 0;
+      }
+      ag += dg, au += du;
+      if (dst) {
+        uint16_t* at = dst + (int64_t)r * j.dst.ld + c;
+        put4_n<T>(at, j.dst.plane, dg, cnt);
+        put4_n<T>(at + j.cols, j.dst.plane, du, cnt);
+        for (int e = 0; e < pad; ++e)
+          for (int q = 0; q < Frag<T>::planes; ++q) at[j.cols + cnt + e + q * j.dst.plane] = 0;
+      }
+    }
+  }
+  if (!j.part) return;
+  sum[0][w][lane] = ag, sum[1][w][lane] = au;
+  __syncthreads();
+  if (w < 2 && cnt > 0) {
+    f32x4 v = sum[w][0][lane];
+    for (int k = 1; k < 4; ++k) v += sum[w][k][lane];
+    float* d = j.part + ((int64_t)chunk * 2 + w) * j.cols + c;
+#pragma unroll
+    for (int k = 0; k < 4; ++k)
+      if (k < cnt) d[k] = v[k];
+  }
+}
+
 __device__ __forceinline__ void loss_row(const LossRows& r, int m) {
   if (m >= r.nq) return;
   LossRow o{INFINITY, 0.0f, -1, 0};
@@ -107,7 +182,7 @@ template <class T>
 __global__ __launch_bounds__(256) void prep_kernel(Prep p, Blocks n) {
   int b = blockIdx.x;
   if (b < n.dz)
-    make_dz<T>(p.dz, b);
+    p.dz.gated ? make_gated_dz<T>(p.dz, b) : make_dz<T>(p.dz, b);
   else if ((b -= n.dz) < n.copy0)
     copy_rows<T>(p.copy[0], p.loss, b, n.copy0);
   else if ((b -= n.copy0) < n.copy1)

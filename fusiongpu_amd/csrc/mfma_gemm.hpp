@@ -1,10 +1,13 @@
-// mfma_gemm.hpp -- the matrix-product core of the query head's operators (head_linear.hip, head_loss.hip).
+// mfma_gemm.hpp -- the matrix-product core of the query head's operators (head_linear.hip, head_gated.hip, head_int8.hip,
+// head_ortho.hip, head_loss.hip).
 //
-// D[m][n] = sum_k A(m, k) B(n, k) on bf16 MFMA with float32 accumulators.  Each operand is read either with k contiguous
+// D[m][n] = sum_k A(m, k) B(n, k) on MFMA, bf16 with float32 accumulators unless said otherwise (OfHalf, OfInt8).  Each operand is read either with k contiguous
 // (rows of k) or with k strided (rows of m or n, one row a k), so the forward product x W^T and both gradients dz W and
 // dz^T x come from one kernel without a transposed copy.  float32 operands are held as three bf16 planes (split2
 // below) and the k loop walks the six plane pairs that are more than 2^-22 of the whole.
 #pragma once
+
+#include <type_traits>
 
 #include "common.hpp"
 
@@ -17,6 +20,8 @@ typedef float f32x2 __attribute__((ext_vector_type(2)));
 typedef float f32x4 __attribute__((ext_vector_type(4)));
 typedef short s16x4 __attribute__((ext_vector_type(4)));
 typedef short s16x8 __attribute__((ext_vector_type(8)));
+typedef int i32x4 __attribute__((ext_vector_type(4)));
+typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
 
 using bf16 = __bf16;
 
@@ -139,6 +144,29 @@ struct GemmArgs {
   int tiles_m, tiles_n;
   int splits;       // workgroups a tile, each on its own part of k
   int k_per_split;  // a multiple of kGemmBK
+  int64_t up = 0;   // gated products: elements from a row of B to the one that its product goes with
+};
+
+// What the elements are: operands always move as 16-byte vectors of 16-bit units, eight of a row in a lane, and only the
+// matrix instruction tells them apart.
+struct OfBf16 {
+  using Acc = f32x4;
+  static __device__ __forceinline__ Acc mma(const bf16x8& n, const bf16x8& m, Acc c) {
+    return __builtin_amdgcn_mfma_f32_16x16x32_bf16(n, m, c, 0, 0, 0);
+  }
+};
+struct OfHalf {
+  using Acc = f32x4;
+  static __device__ __forceinline__ Acc mma(const bf16x8& n, const bf16x8& m, Acc c) {
+    return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(f16x8, n), __builtin_bit_cast(f16x8, m), c, 0, 0, 0);
+  }
+};
+// Two 8-bit integers a unit: k counts pairs, and sums are exact up to 2^17 products.
+struct OfInt8 {
+  using Acc = i32x4;
+  static __device__ __forceinline__ Acc mma(const bf16x8& n, const bf16x8& m, Acc c) {
+    return __builtin_amdgcn_mfma_i32_16x16x64_i8(__builtin_bit_cast(i32x4, n), __builtin_bit_cast(i32x4, m), c, 0, 0, 0);
+  }
 };
 
 // A lane's eight k of one row as MFMA operands: one bf16 vector, or the three planes of float32.
@@ -172,9 +200,11 @@ __device__ __forceinline__ f32x4 mma(const Frag<float>& n, const Frag<float>& m,
 
 constexpr int kGemmBK = 64;
 
-// Plane pairs (a, b) in the order they are accumulated: the smallest products first.
-__device__ __forceinline__ int pair_a(int p) { return (0x201100 >> (4 * (5 - p))) & 0xF; }
-__device__ __forceinline__ int pair_b(int p) { return (0x021010 >> (4 * (5 - p))) & 0xF; }
+// Plane pairs (a, b) in the order they are accumulated, the smallest products first: of three planes six, of two three.
+template <int PAIRS = 6>
+__device__ __forceinline__ int pair_a(int p) { return PAIRS == 3 ? p == 0 : (0x201100 >> (4 * (5 - p))) & 0xF; }
+template <int PAIRS = 6>
+__device__ __forceinline__ int pair_b(int p) { return PAIRS == 3 ? p == 1 : (0x021010 >> (4 * (5 - p))) & 0xF; }
 
 // Tiles: BM x BN a workgroup of WM x WN waves, each wave (BM / WM) x (BN / WN) in 16 x 16 MFMA tiles.
 template <int BM_, int BN_, int WM_, int WN_>
@@ -270,6 +300,33 @@ struct TileLoad {
   }
 };
 
+// The same for the B operand of a gated product, k contiguous: of each 64 rows of the tile the first half are rows of B, the
+// second half the ones `up` elements further on that their products go with.  A wave's lanes fill rows of one half.
+template <int R, int NT, int BK = kGemmBK>
+struct GatedTileLoad : TileLoad<R, NT, true, true, BK> {
+  using Base = TileLoad<R, NT, true, true, BK>;
+  static constexpr int wave_rows = kWave * 16 / Base::row_bytes;
+  __device__ void init(int64_t ld, int tid) {
+    Base::init(ld, tid);
+    this->voff -= (uint32_t)((int64_t)(tid / kWave * wave_rows) * ld * 2);  // from the wave's first row
+  }
+  __device__ __forceinline__ void issue(const GemmOperand& o, int64_t up, int plane, int r0, int nr, int k0, int nk,
+                                        lds_char* lds, int wave, bool live = true) const {
+    const uint16_t* base = o.p + plane * o.plane + (int64_t)r0 * o.ld + k0;
+    const int64_t last = (int64_t)(min(nr - r0, R / 2) - 1) * o.ld + min(((nk + 7) & ~7) - k0, BK);
+    const uint32_t off = this->kc >= nk - k0 ? 0x80000000u : this->voff;
+#pragma unroll
+    for (int i = 0; i < Base::loads; ++i) {
+      const int row = i * Base::rows_a_load + wave * wave_rows;  // of the tile, the wave's first
+      auto rsrc = __builtin_amdgcn_make_buffer_rsrc(const_cast<uint16_t*>(base + (row & 32 ? up : 0)), 0,
+                                                    live ? (int)(last * 2) : 0, 0x00027000);
+      const uint32_t at = (uint32_t)((row >> 6) * 32 + (row & 31)) * (uint32_t)(o.ld * 2);
+      __builtin_amdgcn_raw_ptr_buffer_load_lds(rsrc, (lds_void*)(lds + i * (NT * 16) + wave * (kWave * 16)), 16, off + at, 0,
+                                               0, 0);
+    }
+  }
+};
+
 // A lane's fragments of 16 rows x 32 k (k half kk of the 64) from the tile at `lds`.
 template <int R, bool KC, bool ISB, int BK = kGemmBK>
 struct TileRead {
@@ -337,6 +394,9 @@ struct GemmWave {
 };
 // acc[f][j]: a lane holds columns col(p) .. col(p) + 7 of row(j) in acc[2 p][j] and acc[2 p + 1][j].
 
+template <class T, bool BKC, bool GATED, int BK = kGemmBK>
+using GemmLoadB = std::conditional_t<GATED, GatedTileLoad<T::BN, T::threads, BK>, TileLoad<T::BN, T::threads, BKC, true, BK>>;
+
 // One workgroup a tile.  Of a k step's 64, the fragments of one half are read while the other half's products run, so the
 // LDS's latency passes behind the matrix instructions; the step's only barrier lies between its halves, when every wave
 // holds the last fragments of this buffer and the next one's loads, issued a whole step before, have to have landed.
@@ -349,9 +409,12 @@ struct GemmWave {
 // 2.1 while a workgroup has its CU to itself).
 constexpr int kPlanesBK = 32;
 template <class T, int PAIRS>
-constexpr bool gemm_planes() { return PAIRS == 6 && T::BM == 64; }
+constexpr bool gemm_planes() { return PAIRS > 1 && T::BM == 64; }
+constexpr int planes_of(int pairs) { return pairs == 6 ? 3 : pairs == 3 ? 2 : 1; }
 template <class T, int PAIRS>
-constexpr int gemm_stage() { return gemm_planes<T, PAIRS>() ? 3 * (T::BM + T::BN) * kPlanesBK * 2 : T::stage_bytes; }
+constexpr int gemm_stage() {
+  return gemm_planes<T, PAIRS>() ? planes_of(PAIRS) * (T::BM + T::BN) * kPlanesBK * 2 : T::stage_bytes;
+}
 
 // k contiguous in both operands: a third buffer, so that two stages' loads are in flight (1000 x 385 x 771 forward 22.8 ->
 // 19.4 us, 4096 x 1024 x 1024 79 -> 76; with strided operands, whose fragments take twice the LDS loads, a third of the CU's
@@ -359,13 +422,14 @@ constexpr int gemm_stage() { return gemm_planes<T, PAIRS>() ? 3 * (T::BM + T::BN
 template <class T, int PAIRS, bool KC>
 constexpr int gemm_third() { return gemm_planes<T, PAIRS>() && KC ? gemm_stage<T, PAIRS>() : 16; }
 
-template <class T, bool AKC, bool BKC, class Acc>
+template <class T, bool AKC, bool BKC, int PAIRS, class Num, bool GATED, class Acc>
 __device__ __forceinline__ void planes_products(const GemmArgs& g, Acc& acc, int m0, int n0, int kbeg, int kend, int wm, int wn,
-                                                char (&s0)[gemm_stage<T, 6>()], char (&s1)[gemm_stage<T, 6>()],
-                                                char (&s2)[gemm_third<T, 6, AKC && BKC>()]) {
+                                                char (&s0)[gemm_stage<T, PAIRS>()], char (&s1)[gemm_stage<T, PAIRS>()],
+                                                char (&s2)[gemm_third<T, PAIRS, AKC && BKC>()]) {
+  constexpr int P = planes_of(PAIRS);
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   TileLoad<T::BM, T::threads, AKC, false, kPlanesBK> la;
-  TileLoad<T::BN, T::threads, BKC, true, kPlanesBK> lb;
+  GemmLoadB<T, BKC, GATED, kPlanesBK> lb;
   la.init(g.a.ld, tid);
   lb.init(g.b.ld, tid);
   TileRead<T::BM, AKC, false, kPlanesBK> ra;
@@ -381,26 +445,30 @@ __device__ __forceinline__ void planes_products(const GemmArgs& g, Acc& acc, int
     const bool live = k < kend;
     k = min(k, klast);
 #pragma unroll
-    for (int p = 0; p < 3; ++p) {
+    for (int p = 0; p < P; ++p) {
       la.issue(g.a, p, m0, g.m, k, g.k, (lds_char*)s + p * pa, wave, live);
-      lb.issue(g.b, p, n0, g.n, k, g.k, (lds_char*)s + 3 * pa + p * pb, wave, live);
+      if constexpr (GATED) lb.issue(g.b, g.up, p, n0, g.n, k, g.k, (lds_char*)s + P * pa + p * pb, wave, live);
+      else lb.issue(g.b, p, n0, g.n, k, g.k, (lds_char*)s + P * pa + p * pb, wave, live);
     }
   };
   auto work = [&](char* s) {
-    Frag<float> a[T::FM], b[T::FN];
+    bf16x8 a[T::FM][P], b[T::FN][P];
 #pragma unroll
-    for (int p = 0; p < 3; ++p) {
+    for (int p = 0; p < P; ++p) {
 #pragma unroll
-      for (int i = 0; i < T::FN; ++i) b[i].p[p] = rb.get((const lds_char*)s + 3 * pa + p * pb, i, 0);
+      for (int i = 0; i < T::FN; ++i) b[i][p] = rb.get((const lds_char*)s + P * pa + p * pb, i, 0);
 #pragma unroll
-      for (int j = 0; j < T::FM; ++j) a[j].p[p] = ra.get((const lds_char*)s + p * pa, j, 0);
+      for (int j = 0; j < T::FM; ++j) a[j][p] = ra.get((const lds_char*)s + p * pa, j, 0);
     }
 #pragma unroll
     for (int j = 0; j < T::FM; ++j)
 #pragma unroll
-      for (int i = 0; i < T::FN; ++i) acc[i][j] = mma(b[i], a[j], acc[i][j]);
+      for (int i = 0; i < T::FN; ++i)
+#pragma unroll
+        for (int q = 0; q < PAIRS; ++q)
+          acc[i][j] = Num::mma(b[i][pair_b<PAIRS>(q)], a[j][pair_a<PAIRS>(q)], acc[i][j]);
   };
-  constexpr int B = kPlanesBK, in_flight = 3 * (decltype(la)::loads + decltype(lb)::loads);  // of one stage
+  constexpr int B = kPlanesBK, in_flight = P * (decltype(la)::loads + decltype(lb)::loads);  // of one stage
   if constexpr (!(AKC && BKC)) {
     issue(s0, kbeg);
     int k = kbeg;
@@ -439,29 +507,29 @@ __device__ __forceinline__ void planes_products(const GemmArgs& g, Acc& acc, int
   }
 }
 
-template <class T, bool AKC, bool BKC, int PAIRS, class Epi>
+template <class T, bool AKC, bool BKC, int PAIRS, class Num, bool GATED, class Epi>
 __device__ __forceinline__ void gemm_tile(const GemmArgs& g, const Epi& epi, int wg, int wgs, char (&s0)[gemm_stage<T, PAIRS>()],
                                           char (&s1)[gemm_stage<T, PAIRS>()], char (&s2)[gemm_third<T, PAIRS, AKC && BKC>()]) {
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int wm = wave / T::WN, wn = wave % T::WN;
   int tm, tn, sp;
   gemm_tile_of(g, wg, wgs, tm, tn, sp);
-  const int m0 = tm * T::BM, n0 = tn * T::BN;
+  const int m0 = tm * T::BM, n0 = tn * (GATED ? T::BN / 2 : T::BN);
   const int kbeg = sp * g.k_per_split, kend = min(g.k, kbeg + g.k_per_split);
-  f32x4 acc[T::FN][T::FM];
+  typename Num::Acc acc[T::FN][T::FM];
 #pragma unroll
   for (int i = 0; i < T::FN; ++i)
 #pragma unroll
-    for (int j = 0; j < T::FM; ++j) acc[i][j] = f32x4{0, 0, 0, 0};
+    for (int j = 0; j < T::FM; ++j) acc[i][j] = typename Num::Acc{0, 0, 0, 0};
   typename Epi::template Side<T> side;
   if constexpr (gemm_planes<T, PAIRS>()) {
     side.fetch(epi, m0, n0, tid);
-    planes_products<T, AKC, BKC>(g, acc, m0, n0, kbeg, kend, wm, wn, s0, s1, s2);
+    planes_products<T, AKC, BKC, PAIRS, Num, GATED>(g, acc, m0, n0, kbeg, kend, wm, wn, s0, s1, s2);
   } else {
     const int steps = max(0, (kend - kbeg + kGemmBK - 1) / kGemmBK) * PAIRS;
 
     TileLoad<T::BM, T::threads, AKC, false> la;
-    TileLoad<T::BN, T::threads, BKC, true> lb;
+    GemmLoadB<T, BKC, GATED> lb;
     la.init(g.a.ld, tid);
     lb.init(g.b.ld, tid);
     TileRead<T::BM, AKC, false> ra;
@@ -473,9 +541,10 @@ __device__ __forceinline__ void gemm_tile(const GemmArgs& g, const Epi& epi, int
     int pk = kbeg, pp = 0;  // the next stage to load
     // The pairs of one k step follow one another, so a plane's tile is read again while it is in the L2.
     auto issue = [&](char* s) {
-      const int qa = PAIRS == 1 ? 0 : pair_a(pp), qb = PAIRS == 1 ? 0 : pair_b(pp);
+      const int qa = PAIRS == 1 ? 0 : pair_a<PAIRS>(pp), qb = PAIRS == 1 ? 0 : pair_b<PAIRS>(pp);
       la.issue(g.a, qa, m0, g.m, pk, g.k, (lds_char*)s, wave);
-      lb.issue(g.b, qb, n0, g.n, pk, g.k, (lds_char*)s + boff, wave);
+      if constexpr (GATED) lb.issue(g.b, g.up, qb, n0, g.n, pk, g.k, (lds_char*)s + boff, wave);
+      else lb.issue(g.b, qb, n0, g.n, pk, g.k, (lds_char*)s + boff, wave);
       if (PAIRS == 1 || ++pp == PAIRS) {
         pp = 0;
         pk += kGemmBK;
@@ -495,7 +564,7 @@ __device__ __forceinline__ void gemm_tile(const GemmArgs& g, const Epi& epi, int
       for (int j = 0; j < T::FM; ++j)
 #pragma unroll
         for (int i = 0; i < T::FN; ++i)
-          acc[i][j] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(h.b[i], h.a[j], acc[i][j], 0, 0, 0);
+          acc[i][j] = Num::mma(h.b[i], h.a[j], acc[i][j]);
     };
     Half h0, h1;
     // One step: the buffer `cur` holds it, `next` the following one; `more`: the one after that exists.
@@ -529,12 +598,12 @@ __device__ __forceinline__ void gemm_tile(const GemmArgs& g, const Epi& epi, int
 }
 
 // Registers for two waves a SIMD: one workgroup of 256 x 256 a CU, two of 128 x 128.
-template <class T, bool AKC, bool BKC, int PAIRS, class Epi>
+template <class T, bool AKC, bool BKC, int PAIRS, class Epi, class Num = OfBf16, bool GATED = false>
 __global__ __launch_bounds__(T::threads, 2) void gemm_kernel(GemmArgs g, Epi epi) {
   __shared__ __attribute__((aligned(1024))) char s0[gemm_stage<T, PAIRS>()];
   __shared__ __attribute__((aligned(1024))) char s1[gemm_stage<T, PAIRS>()];
   __shared__ __attribute__((aligned(1024))) char s2[gemm_third<T, PAIRS, AKC && BKC>()];
-  gemm_tile<T, AKC, BKC, PAIRS>(g, epi, blockIdx.x, gridDim.x, s0, s1, s2);
+  gemm_tile<T, AKC, BKC, PAIRS, Num, GATED>(g, epi, blockIdx.x, gridDim.x, s0, s1, s2);
 }
 
 // Both gradients of a small layer in one launch: the first x_wgs workgroups form x (A with k contiguous, B strided), the
@@ -546,9 +615,9 @@ __global__ __launch_bounds__(T::threads, 2) void gemm_pair_kernel(GemmArgs x, Ep
   __shared__ __attribute__((aligned(1024))) char s2[gemm_third<T, PAIRS, false>()];
   const int b = blockIdx.x;
   if (b < x_wgs)
-    gemm_tile<T, true, false, PAIRS>(x, ex, b, x_wgs, s0, s1, s2);
+    gemm_tile<T, true, false, PAIRS, OfBf16, false>(x, ex, b, x_wgs, s0, s1, s2);
   else
-    gemm_tile<T, false, false, PAIRS>(w, ew, b - x_wgs, gridDim.x - x_wgs, s0, s1, s2);
+    gemm_tile<T, false, false, PAIRS, OfBf16, false>(w, ew, b - x_wgs, gridDim.x - x_wgs, s0, s1, s2);
 }
 
 }  // namespace fgpu

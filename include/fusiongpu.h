@@ -649,6 +649,66 @@ fgpu_status fgpu_linear_backward(const void* d_dy, const void* d_x, const void* 
 #define FGPU_TILE_PAIR 1024
 int fgpu_linear_tile(int64_t rows, int in_dim, int out_dim, int dtype, int product);
 
+/* The gated layer h [rows][hidden] = act(g) u with g = x w_g^T + bias_g and u =
+ * x w_u^T + bias_u, in one product: w [2 hidden][in_dim] holds w_g's rows, then
+ * w_u's, d_bias [2 hidden] (may be NULL) both biases.  d_pre [rows][2 hidden]
+ * (may be NULL) gets [g | u], which the backward pass needs.  hidden <= 2^15. */
+size_t fgpu_gated_linear_workspace_bytes(int64_t rows, int in_dim, int hidden, int dtype);
+fgpu_status fgpu_gated_linear(const void* d_x, const void* d_w, const void* d_bias, int64_t rows, int in_dim, int hidden,
+                              int dtype, int act, void* d_h, void* d_pre, void* d_workspace, size_t workspace_bytes,
+                              void* stream);
+/* Its gradients for dh [rows][hidden] from the kept d_pre: with dz = [dh u
+ * act'(g) | dh act(g)], dx = dz w, dw = dz^T x, db = the column sums of dz.  Each
+ * of d_dx, d_dw, d_db may be NULL (not wanted); d_w is read for dx, d_x for dw.
+ * In bfloat16, dz is rounded to bfloat16 before the two products (not before
+ * db).  d_dh and d_pre need their element's alignment only. */
+size_t fgpu_gated_linear_backward_workspace_bytes(int64_t rows, int in_dim, int hidden, int dtype);
+fgpu_status fgpu_gated_linear_backward(const void* d_dh, const void* d_x, const void* d_w, const void* d_pre, int64_t rows,
+                                       int in_dim, int hidden, int dtype, int act, void* d_dx, void* d_dw, void* d_db,
+                                       void* d_workspace, size_t workspace_bytes, void* stream);
+/* As fgpu_linear_tile, of the forward product. */
+int fgpu_gated_linear_tile(int64_t rows, int in_dim, int hidden, int dtype);
+
+/* Rows as 8-bit integers with a scale each: with m the largest magnitude of a
+ * row of x [rows][dim], q = x 127 / m rounded to the nearest whole number as the
+ * real number it is (ties to even), and scale = m / 127 (float32).  A row of zeros
+ * has scale 0; of a row that holds something not finite the scale is NaN and q
+ * zero.  d_q [rows][FGPU_INT8_ROW(dim)] gets zeros behind a row's values and must
+ * be 16-byte aligned; d_x needs its element's alignment. */
+#define FGPU_INT8_ROW(dim) (((dim) + 15) / 16 * 16)
+fgpu_status fgpu_quantize_rows(const void* d_x, int64_t rows, int dim, int dtype, int8_t* d_q, float* d_scale, void* stream);
+
+/* fgpu_linear with a weight held so: d_w [out_dim][FGPU_INT8_ROW(in_dim)] and
+ * d_w_scale [out_dim].  x is of `dtype` (d_x_scale NULL) and rounded row by row
+ * as above inside the call, or held so already: [rows][FGPU_INT8_ROW(in_dim)]
+ * with d_x_scale [rows] (behind the values, x's or w's bytes are zeros).  z =
+ * x_scale w_scale sum q_x q_w + bias, the sum exact in 32 bits; bias, residual
+ * and y are of `dtype`.  d_residual may be d_y itself. */
+size_t fgpu_linear_int8_workspace_bytes(int64_t rows, int in_dim, int out_dim, int dtype, int quantized_x);
+fgpu_status fgpu_linear_int8(const void* d_x, const float* d_x_scale, const int8_t* d_w, const float* d_w_scale,
+                             const void* d_bias, const void* d_residual, int64_t rows, int in_dim, int out_dim, int dtype,
+                             int act, void* d_y, void* d_workspace, size_t workspace_bytes, void* stream);
+/* fgpu_gated_linear likewise: d_w [2 hidden][FGPU_INT8_ROW(in_dim)], d_w_scale
+ * [2 hidden]. */
+size_t fgpu_gated_linear_int8_workspace_bytes(int64_t rows, int in_dim, int hidden, int dtype, int quantized_x);
+fgpu_status fgpu_gated_linear_int8(const void* d_x, const float* d_x_scale, const int8_t* d_w, const float* d_w_scale,
+                                   const void* d_bias, int64_t rows, int in_dim, int hidden, int dtype, int act, void* d_h,
+                                   void* d_workspace, size_t workspace_bytes, void* stream);
+
+/* A weight's update x [rows][cols] with its singular values drawn towards one:
+ * X = x / (|x| + eps), |x| the Frobenius norm, then `steps` times X <- a X + (b A
+ * + c A^2) X with A = X X^T (of more rows than columns, the same from the other
+ * side): each singular value s becomes a s + b s^3 + c s^5.  y = X.  A matrix of
+ * zeros stays zero; something not finite makes all of y NaN.  Between the
+ * products X, A and b A + c A^2 are held to 2^-23 of their value and 2^-35 of
+ * one, and must stay below 64 in magnitude (coefficients that keep the singular
+ * values below about two do).  rows and cols up to 2^16; d_y may be d_x; d_x and
+ * d_y need their element's alignment. */
+#define FGPU_ORTHO_MAX_STEPS 64
+size_t fgpu_orthogonalize_workspace_bytes(int64_t rows, int64_t cols, int dtype);
+fgpu_status fgpu_orthogonalize(const void* d_x, int64_t rows, int64_t cols, int dtype, int steps, float a, float b, float c,
+                               float eps, void* d_y, void* d_workspace, size_t workspace_bytes, void* stream);
+
 /* y = (x - mean) rstd gamma + beta for each row of x [rows][dim], mean and
  * rstd = 1 / sqrt(variance + eps) its own (biased variance, about the mean).
  * d_gamma, d_beta [dim] may be NULL (one, zero); d_mean, d_rstd [rows] float32
