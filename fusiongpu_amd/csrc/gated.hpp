@@ -66,29 +66,32 @@ struct GatedEpi {
   // STREAM: results past the caches.
   template <bool STREAM, class G, class A>
   __device__ __forceinline__ void rows(A (&acc)[G::FN][G::FM], const GemmWave<G>& w) const {
-    static_assert(G::FN == 4, "32 hidden columns a wave");
+    static_assert(G::FN % 4 == 0, "groups of 32 hidden columns");
     constexpr bool kInt = std::is_same_v<A, i32x4>;
-    const int c = w.n0 + w.wn * 32 + 8 * (w.lane >> 4), cnt = n - c;
-    if (cnt <= 0) return;
     const f32x8 zero{{0, 0, 0, 0}, {0, 0, 0, 0}};
-    f32x8 bg = zero, bu = zero, sg = zero, su = zero;
-    if (f.bias) bg = load8_n((const T*)f.bias + c, cnt), bu = load8_n((const T*)f.bias + n + c, cnt);
-    if (kInt) sg = load8_n(s.col + c, cnt), su = load8_n(s.col + n + c, cnt);
 #pragma unroll
-    for (int j = 0; j < G::FM; ++j) {
-      const int64_t row = w.row(j);
-      if (row >= m) continue;
-      const float sr = kInt ? s.row[row] : 1.0f;
-      f32x8 g = eight(acc[0][j], acc[1][j], sr, sg), u = eight(acc[2][j], acc[3][j], sr, su);
-      g.lo += bg.lo, g.hi += bg.hi, u.lo += bu.lo, u.hi += bu.hi;
-      if (f.pre) {
-        T* pre = (T*)f.pre + row * 2 * n + c;
-        store8_n<STREAM>(pre, g, cnt);
-        store8_n<STREAM>(pre + n, u, cnt);
+    for (int q = 0; q < G::FN / 4; ++q) {
+      const int c = w.n0 + (w.wn * (G::FN / 4) + q) * 32 + 8 * (w.lane >> 4), cnt = n - c;
+      if (cnt <= 0) continue;
+      f32x8 bg = zero, bu = zero, sg = zero, su = zero;
+      if (f.bias) bg = load8_n((const T*)f.bias + c, cnt), bu = load8_n((const T*)f.bias + n + c, cnt);
+      if (kInt) sg = load8_n(s.col + c, cnt), su = load8_n(s.col + n + c, cnt);
+#pragma unroll
+      for (int j = 0; j < G::FM; ++j) {
+        const int64_t row = w.row(j);
+        if (row >= m) continue;
+        const float sr = kInt ? s.row[row] : 1.0f;
+        f32x8 g = eight(acc[4 * q][j], acc[4 * q + 1][j], sr, sg), u = eight(acc[4 * q + 2][j], acc[4 * q + 3][j], sr, su);
+        g.lo += bg.lo, g.hi += bg.hi, u.lo += bu.lo, u.hi += bu.hi;
+        if (f.pre) {
+          T* pre = (T*)f.pre + row * 2 * n + c;
+          store8_n<STREAM>(pre, g, cnt);
+          store8_n<STREAM>(pre + n, u, cnt);
+        }
+#pragma unroll
+        for (int e = 0; e < 8; ++e) u.set(e, act_value<T>(g[e], ACT) * u[e]);
+        store8_n<STREAM>((T*)f.out + row * n + c, u, cnt);
       }
-#pragma unroll
-      for (int e = 0; e < 8; ++e) u.set(e, act_value<T>(g[e], ACT) * u[e]);
-      store8_n<STREAM>((T*)f.out + row * n + c, u, cnt);
     }
   }
 };
@@ -101,9 +104,9 @@ template <int PAIRS, class Num, class T, int ACT>
 fgpu_status run_gated(const GemmArgs& g, int tile, const GatedEpi<T, ACT>& e, hipStream_t s) {
   const int grid = g.tiles_m * g.tiles_n;
   using E = GatedEpi<T, ACT>;
-  if (tile == 256) gemm_kernel<GatedTile256, true, true, PAIRS, E, Num, true><<<grid, GatedTile256::threads, 0, s>>>(g, e);
-  else if (tile == 128) gemm_kernel<GatedTile128, true, true, PAIRS, E, Num, true><<<grid, GatedTile128::threads, 0, s>>>(g, e);
-  else gemm_kernel<GatedTile64, true, true, PAIRS, E, Num, true><<<grid, GatedTile64::threads, 0, s>>>(g, e);
+  if (tile == 256) gemm_kernel<GatedTile256, true, true, PAIRS, E, Num, kGated><<<grid, GatedTile256::threads, 0, s>>>(g, e);
+  else if (tile == 128) gemm_kernel<GatedTile128, true, true, PAIRS, E, Num, kGated><<<grid, GatedTile128::threads, 0, s>>>(g, e);
+  else gemm_kernel<GatedTile64, true, true, PAIRS, E, Num, kGated><<<grid, GatedTile64::threads, 0, s>>>(g, e);
   FGPU_HIP(hipGetLastError());
   return FGPU_OK;
 }

@@ -96,14 +96,18 @@ struct OrthoFinish {
   Planes c, to;
   void* out = nullptr;
   int m = 0, n = 0;
-  template <class T>
-  __device__ __forceinline__ void put(f32x8 v, int64_t row, int col) const {
+  __device__ __forceinline__ f32x8 value(f32x8 v, int64_t row, int col, bool inside) const {
     v.lo *= alpha, v.hi *= alpha;
-    if (c.p) {
+    if (c.p && inside) {
       const f32x8 o = planes8(c, row * c.ld + col);
 #pragma unroll
       for (int e = 0; e < 8; ++e) v.set(e, fmaf(beta, o[e], v[e]));
     }
+    return v;
+  }
+  template <class T>
+  __device__ __forceinline__ void put(f32x8 v, int64_t row, int col) const {
+    v = value(v, row, col, true);
     if (out) store8_n<false>((T*)out + row * n + col, v, n - col);
     else put_planes8(to, row * to.ld + col, v);
   }
@@ -111,7 +115,6 @@ struct OrthoFinish {
 template <class T>
 struct OrthoEpi {
   OrthoFinish f;
-  float* part;  // [split][m][n8]: the product alone, to be joined; or NULL
 
   template <class G>
   struct Side {
@@ -127,63 +130,165 @@ struct OrthoEpi {
 #pragma unroll
       for (int j = 0; j < G::FM; ++j) {
         const int64_t row = w.row(j);
-        if (row >= f.m) continue;
-        if (part) {
-          float* d = part + ((int64_t)w.sp * f.m + row) * n8 + col;
-          *reinterpret_cast<f32x4*>(d) = acc[2 * p][j];
-          *reinterpret_cast<f32x4*>(d + 4) = acc[2 * p + 1][j];
-        } else {
-          f.put<T>(f32x8{acc[2 * p][j], acc[2 * p + 1][j]}, row, col);
-        }
+        if (row < f.m) f.put<T>(f32x8{acc[2 * p][j], acc[2 * p + 1][j]}, row, col);
       }
     }
   }
 };
-// The parts of a split product added in their order, eight columns a thread.
-template <class T>
-__global__ __launch_bounds__(256) void ortho_join_kernel(OrthoFinish f, const float* part, int splits) {
-  const int n8 = (f.n + 7) & ~7, per = n8 / 8;
-  const int64_t total = (int64_t)f.m * per;
-  for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < total; i += (int64_t)gridDim.x * 256) {
+// A symmetric product's tiles on and below the diagonal as they are, [split][tile][row][column].
+struct TriangleEpi {
+  float* part;
+  int tiles;
+
+  template <class G>
+  struct Side {
+    __device__ void fetch(const TriangleEpi&, int, int, int) {}
+  };
+  template <class G>
+  __device__ __forceinline__ void finish(f32x4 (&acc)[G::FN][G::FM], const GemmWave<G>& w, char*, const Side<G>&) const {
+    float* tile = part + ((int64_t)w.sp * tiles + triangle_tiles(w.tm) + w.tn) * (G::BM * G::BN);
+#pragma unroll
+    for (int p = 0; p < G::FN / 2; ++p)
+#pragma unroll
+      for (int j = 0; j < G::FM; ++j) {
+        float* d = tile + (w.row(j) - w.m0) * G::BN + w.col(p) - w.n0;
+        *reinterpret_cast<f32x4*>(d) = acc[2 * p][j];
+        *reinterpret_cast<f32x4*>(d + 4) = acc[2 * p + 1][j];
+      }
+  }
+};
+// Their parts added in their order and finished, as planes on both sides of the diagonal: a workgroup 64 x 64, which it turns
+// in LDS.
+__global__ __launch_bounds__(256) void triangle_join_kernel(OrthoFinish f, const float* part, int splits, int tiles, int tile) {
+  __shared__ float turned[64][65];
+  const int side = tile / 64, patch = blockIdx.x % (side * side), t = blockIdx.x / (side * side);
+  int tm, tn;
+  triangle_at(t, tm, tn);
+  const int pm = patch / side, pn = patch % side, r0 = tm * tile + pm * 64, c0 = tn * tile + pn * 64;
+  if (c0 > r0 || r0 >= f.n) return;  // in a tile on the diagonal; beyond the matrix
+  const int n8 = (f.n + 7) & ~7, c = threadIdx.x % 8 * 8;
+#pragma unroll
+  for (int h = 0; h < 2; ++h) {
+    const int r = threadIdx.x / 8 + 32 * h;
     f32x8 v{{0, 0, 0, 0}, {0, 0, 0, 0}};
+    const float* at = part + (int64_t)t * tile * tile + (pm * 64 + r) * tile + pn * 64 + c;
 #pragma unroll 4
     for (int s = 0; s < splits; ++s) {
-      const f32x8 q = load8(part + ((int64_t)s * total + i) * 8);
+      const f32x8 q = load8(at + (int64_t)s * tiles * tile * tile);
       v.lo += q.lo, v.hi += q.hi;
     }
-    const int64_t row = i / per;
-    f.put<T>(v, row, (int)(i - row * per) * 8);
+    v = f.value(v, r0 + r, c0 + c, r0 + r < f.n && c0 + c < n8);
+    if (r0 + r < f.n && c0 + c < n8) put_planes8(f.to, (int64_t)(r0 + r) * f.to.ld + c0 + c, v);
+#pragma unroll
+    for (int e = 0; e < 8; ++e) turned[c + e][r] = v[e];
+  }
+  if (c0 == r0) return;
+  __syncthreads();
+#pragma unroll
+  for (int h = 0; h < 2; ++h) {
+    const int r = threadIdx.x / 8 + 32 * h;
+    if (c0 + r >= f.n || r0 + c >= n8) continue;
+    f32x8 v;
+#pragma unroll
+    for (int e = 0; e < 8; ++e) v.set(e, turned[r][c + e]);
+    put_planes8(f.to, (int64_t)(c0 + r) * f.to.ld + r0 + c, v);
   }
 }
 
-constexpr int kPairs = 3;
-Plan plan_ortho(int m, int n, int k) {
-  Product p{m, n, k, false};
-  p.pairs = kPairs;
-  return plan_product(p, true);
+// ---- how a product is cut ------------------------------------------------------------
+// Microseconds, fitted over 1024 x 1024 over 1024 and 8192 and 8192 x 1024 over 1024: a step of k (64 of one plane, 32 of two)
+// of a workgroup while it has its CU to itself, for each of those that share one, and how many do.
+struct StepTime {
+  double alone, shared;
+  int most;
+};
+StepTime step_time(int tile, int pairs) {
+  if (pairs == 1) return tile == 256 ? StepTime{1.5, 1.5, 1} : tile == 128 ? StepTime{0.6, 0.43, 2} : StepTime{0.3, 0.2, 5};
+  return tile == 256 ? StepTime{2.0, 2.0, 1} : tile == 128 ? StepTime{0.75, 0.6, 2} : StepTime{0.26, 0.2, 3};
 }
-size_t ortho_part_bytes(int m, int n, const Plan& q) {
-  return q.splits > 1 ? carve_bytes<float>((size_t)q.splits * m * ((n + 7) & ~7)) : 0;
+struct Cut {
+  int tile = 0, splits = 1, k_per_split = 0;
+  double us = 0;
+};
+double cut_us(const Cut& q, int pairs, int64_t tiles) {
+  const StepTime t = step_time(q.tile, pairs);
+  const int steps = ceil_div(q.k_per_split, pairs == 1 ? kGemmBK : kPlanesBK), round = 256 * t.most;
+  const double fixed = q.tile == 256 ? 6 : q.tile == 128 ? 3.5 : 2.5;
+  const int64_t wgs = tiles * q.splits, full = wgs / round, rest = wgs % round;
+  double us = full * (steps * std::max(t.alone, t.most * t.shared) + fixed);
+  if (rest) us += steps * std::max(t.alone, ceil_div(rest, 256) * t.shared) + fixed;
+  return us;
+}
+// A product of m x n over k, whole.
+Cut cut_product(int m, int n, int k, int pairs) {
+  Cut best;
+  for (int tile : {256, 128, 64}) {
+    const int64_t tiles = (int64_t)ceil_div(m, tile) * ceil_div(n, tile);
+    Cut q{tile, 1, ceil_div(k, kGemmBK) * kGemmBK};
+    q.us = cut_us(q, pairs, tiles);
+    if (!best.tile || q.us < best.us) best = q;
+  }
+  return best;
+}
+// A symmetric product of n x n over k: whole, or (splits > 0 in `part`) its triangle in parts, joined by a launch more.
+struct SymmetricCut {
+  Cut whole, part;
+  bool joined;
+  size_t part_bytes(int n) const {
+    return joined ? carve_bytes<float>((size_t)part.splits * triangle_tiles(ceil_div(n, part.tile)) * part.tile * part.tile) : 0;
+  }
+};
+SymmetricCut cut_symmetric(int n, int k, int pairs) {
+  SymmetricCut c;
+  c.whole = cut_product(n, n, k, pairs);
+  for (int tile : {256, 128, 64}) {
+    const int64_t tiles = triangle_tiles(ceil_div(n, tile));
+    for (int splits = 1; splits <= 64; ++splits) {
+      if (splits > 1 && (splits > ceil_div(k, 2 * kGemmBK) || tiles * splits > 2048)) break;
+      Cut q{tile, splits, ceil_div(ceil_div(k, kGemmBK), splits) * kGemmBK};
+      if (ceil_div(k, q.k_per_split) != splits) continue;
+      q.us = cut_us(q, pairs, tiles) + 4 + tiles * splits * tile * tile * 8.0 / 5e6;
+      if (!c.part.tile || q.us < c.part.us) c.part = q;
+    }
+  }
+  c.joined = c.part.us < c.whole.us;
+  return c;
 }
 
-template <class T, bool AKC, bool BKC>
-fgpu_status ortho_product(const Planes& a, const Planes& b, int k, const OrthoFinish& f, float* part, hipStream_t s) {
-  const Plan q = plan_ortho(f.m, f.n, k);
-  FGPU_CHECK(q.tile, FGPU_ERR_UNSUPPORTED, "orthogonalize: more tiles than one launch takes");
-  const GemmArgs g{{a.p, a.ld, a.plane}, {b.p, b.ld, b.plane}, f.m, f.n, k, q.tiles_m, q.tiles_n, q.splits, q.k_per_split};
-  const OrthoEpi<T> e{f, q.splits > 1 ? part : nullptr};
-  const int grid = q.tiles_m * q.tiles_n * q.splits;
-  if (q.tile == 256) gemm_kernel<Tile256, AKC, BKC, kPairs, OrthoEpi<T>, OfHalf><<<grid, Tile256::threads, 0, s>>>(g, e);
-  else if (q.tile == 128) gemm_kernel<Tile128, AKC, BKC, kPairs, OrthoEpi<T>, OfHalf><<<grid, Tile128::threads, 0, s>>>(g, e);
-  else gemm_kernel<Tile64, AKC, BKC, kPairs, OrthoEpi<T>, OfHalf><<<grid, Tile64::threads, 0, s>>>(g, e);
+template <int PAIRS, bool AKC, bool BKC, int FORM, class E>
+fgpu_status run_cut(const GemmArgs& g, int tile, int grid, const E& e, hipStream_t s) {
+  if (tile == 256) gemm_kernel<Tile256, AKC, BKC, PAIRS, E, OfHalf, FORM><<<grid, Tile256::threads, 0, s>>>(g, e);
+  else if (tile == 128) gemm_kernel<Tile128, AKC, BKC, PAIRS, E, OfHalf, FORM><<<grid, Tile128::threads, 0, s>>>(g, e);
+  else gemm_kernel<Tile64, AKC, BKC, PAIRS, E, OfHalf, FORM><<<grid, Tile64::threads, 0, s>>>(g, e);
   FGPU_HIP(hipGetLastError());
-  if (q.splits > 1) {
-    const int blocks = (int)std::min<int64_t>(((int64_t)f.m * ((f.n + 7) / 8) + 255) / 256, 256 * 16);
-    ortho_join_kernel<T><<<blocks, 256, 0, s>>>(f, part, q.splits);
-    FGPU_HIP(hipGetLastError());
-  }
   return FGPU_OK;
 }
+template <class T, int PAIRS, bool AKC, bool BKC>
+fgpu_status run_whole(const Planes& a, const Planes& b, int k, const OrthoFinish& f, const Cut& q, hipStream_t s) {
+  const GemmArgs g{{a.p, a.ld, a.plane}, {b.p, b.ld, b.plane}, f.m, f.n, k, ceil_div(f.m, q.tile), ceil_div(f.n, q.tile), 1,
+                   q.k_per_split};
+  return run_cut<PAIRS, AKC, BKC, kPlain>(g, q.tile, g.tiles_m * g.tiles_n, OrthoEpi<T>{f}, s);
+}
+// a a^T of n rows (KC: k contiguous).
+template <class T, int PAIRS, bool KC>
+fgpu_status run_symmetric(const Planes& a, int k, const OrthoFinish& f, float* part, hipStream_t s) {
+  const SymmetricCut c = cut_symmetric(f.n, k, PAIRS);
+  if (!c.joined) return run_whole<T, PAIRS, KC, KC>(a, a, k, f, c.whole, s);
+  const Cut& q = c.part;
+  const int t = ceil_div(f.n, q.tile), tiles = triangle_tiles(t);
+  const GemmArgs g{{a.p, a.ld, a.plane}, {a.p, a.ld, a.plane}, f.n, f.n, k, t, t, q.splits, q.k_per_split};
+  FGPU_TRY((run_cut<PAIRS, KC, KC, kTriangle>(g, q.tile, tiles * q.splits, TriangleEpi{part, tiles}, s)));
+  triangle_join_kernel<<<tiles * (q.tile / 64) * (q.tile / 64), 256, 0, s>>>(f, part, q.splits, tiles, q.tile);
+  FGPU_HIP(hipGetLastError());
+  return FGPU_OK;
+}
+
+// Products of bfloat16 updates in fewer pieces.  X is held in two planes throughout, but A takes one of them always, and P and
+// the product with it do in the first two steps: what those roundings leave lies in the directions of large singular
+// values, which the later steps do not multiply.  Against 64 bits (64 to 512 rows, singular values even, normal, as i^-1/2
+// to i^-2) the result is then off by at most 1.3e-3 of its norm, mostly below 6e-4, before it is rounded to bfloat16
+// (1.7e-3); with one plane in every product 2.7e-3, with X in one plane as well up to 8e-3.
+constexpr int kOnePlaneSteps = 2;
 
 struct Shape {
   int rows, cols, small, large;
@@ -191,11 +296,10 @@ struct Shape {
   Shape(int r, int c) : rows(r), cols(c), small(std::min(r, c)), large(std::max(r, c)), tall(r > c) {}
   size_t x_bytes() const { return carve_bytes<uint16_t>((size_t)rows * packed_ld(cols) * 2); }
   size_t a_bytes() const { return carve_bytes<uint16_t>((size_t)small * packed_ld(small) * 2); }
-  size_t part_bytes() const {
-    const int m = tall ? rows : small, n = tall ? small : cols;
-    return std::max({ortho_part_bytes(small, small, plan_ortho(small, small, large)),
-                     ortho_part_bytes(small, small, plan_ortho(small, small, small)),
-                     ortho_part_bytes(m, n, plan_ortho(m, n, small))});
+  size_t part_bytes(bool f32) const {
+    const int few = f32 ? 3 : 1;
+    return std::max({cut_symmetric(small, large, few).part_bytes(small), cut_symmetric(small, small, few).part_bytes(small),
+                     cut_symmetric(small, small, 3).part_bytes(small)});
   }
 };
 Planes planes_at(void* p, int rows, int cols) { return {(uint16_t*)p, packed_ld(cols), rows * packed_ld(cols)}; }
@@ -207,13 +311,25 @@ fgpu_status check_common(int64_t rows, int64_t cols, int dtype) {
   return FGPU_OK;
 }
 
+template <class T, int PAIRS>
+fgpu_status gram(const Planes& x, const Shape& sh, const OrthoFinish& f, float* part, hipStream_t s) {
+  return sh.tall ? run_symmetric<T, PAIRS, false>(x, sh.large, f, part, s) : run_symmetric<T, PAIRS, true>(x, sh.large, f, part, s);
+}
+template <class T, int PAIRS>
+fgpu_status step(const Planes& x, const Planes& a, const Planes& p, const Shape& sh, const OrthoFinish& fp,
+                 const OrthoFinish& fx, float* part, hipStream_t s) {
+  FGPU_TRY((run_symmetric<T, PAIRS, true>(a, sh.small, fp, part, s)));
+  const Cut q = cut_product(fx.m, fx.n, sh.small, PAIRS);
+  return sh.tall ? run_whole<T, PAIRS, true, true>(x, p, sh.small, fx, q, s) : run_whole<T, PAIRS, true, false>(p, x, sh.small, fx, q, s);
+}
+
 template <class T>
 fgpu_status run_ortho(const T* x, const Shape& sh, int steps, float a, float b, float c, float eps, T* out, Carve& ws,
                       hipStream_t s) {
   Planes xs[2] = {planes_at(ws.take<char>(sh.x_bytes()), sh.rows, sh.cols), planes_at(ws.take<char>(sh.x_bytes()), sh.rows, sh.cols)};
   const Planes ga = planes_at(ws.take<char>(sh.a_bytes()), sh.small, sh.small);
   const Planes gp = planes_at(ws.take<char>(sh.a_bytes()), sh.small, sh.small);
-  float* part = (float*)ws.take<char>(sh.part_bytes());
+  float* part = (float*)ws.take<char>(sh.part_bytes(sizeof(T) == 4));
   double* norm = ws.take<double>(kNormBlocks);
   FGPU_CHECK(ws.held(), FGPU_ERR_WORKSPACE, "orthogonalize: workspace smaller than fgpu_orthogonalize_workspace_bytes");
   const int64_t count = (int64_t)sh.rows * sh.cols;
@@ -231,15 +347,9 @@ fgpu_status run_ortho(const T* x, const Shape& sh, int steps, float a, float b, 
     fp.alpha = c / kHeld, fp.beta = b, fp.c = ga, fp.to = gp, fp.m = fp.n = n;
     fx.alpha = 1 / kHeld, fx.beta = a, fx.c = from, fx.to = to, fx.m = sh.rows, fx.n = sh.cols;
     if (last) fx.out = out, fx.alpha /= kHeld, fx.beta /= kHeld;
-    if (sh.tall) {
-      FGPU_TRY((ortho_product<T, false, false>(from, from, sh.large, fa, part, s)));
-      FGPU_TRY((ortho_product<T, true, true>(ga, ga, n, fp, part, s)));
-      FGPU_TRY((ortho_product<T, true, true>(from, gp, n, fx, part, s)));
-    } else {
-      FGPU_TRY((ortho_product<T, true, true>(from, from, sh.large, fa, part, s)));
-      FGPU_TRY((ortho_product<T, true, true>(ga, ga, n, fp, part, s)));
-      FGPU_TRY((ortho_product<T, true, false>(gp, from, n, fx, part, s)));
-    }
+    const bool one = sizeof(T) == 2 && i < kOnePlaneSteps;
+    FGPU_TRY((sizeof(T) == 2 ? gram<T, 1>(from, sh, fa, part, s) : gram<T, 3>(from, sh, fa, part, s)));
+    FGPU_TRY((one ? step<T, 1>(from, ga, gp, sh, fp, fx, part, s) : step<T, 3>(from, ga, gp, sh, fp, fx, part, s)));
   }
   return FGPU_OK;
 }
@@ -254,7 +364,7 @@ extern "C" {
 size_t fgpu_orthogonalize_workspace_bytes(int64_t rows, int64_t cols, int dtype) {
   if (check_common(rows, cols, dtype) != FGPU_OK || rows == 0 || cols == 0) return 0;
   const Shape sh((int)rows, (int)cols);
-  return 2 * (sh.x_bytes() + sh.a_bytes()) + sh.part_bytes() + carve_bytes<double>(kNormBlocks);
+  return 2 * (sh.x_bytes() + sh.a_bytes()) + sh.part_bytes(dtype == FGPU_DTYPE_F32) + carve_bytes<double>(kNormBlocks);
 }
 
 fgpu_status fgpu_orthogonalize(const void* d_x, int64_t rows, int64_t cols, int dtype, int steps, float a, float b, float c,

@@ -138,6 +138,10 @@ struct GemmOperand {
   int64_t plane;
 };
 
+// What a product's tiles are: all of D; (gated) columns of both factors in each; (triangle) of a symmetric D the ones on and
+// below the diagonal.
+enum GemmForm { kPlain, kGated, kTriangle };
+
 struct GemmArgs {
   GemmOperand a, b;
   int m, n, k;
@@ -380,6 +384,22 @@ __device__ __forceinline__ void gemm_tile_of(const GemmArgs& g, int wg, int tota
   tn = in / gm;
 }
 
+// The same over the t (t + 1) / 2 tiles on and below the diagonal, row by row.
+__host__ __device__ __forceinline__ int triangle_tiles(int t) { return t * (t + 1) / 2; }
+__device__ __forceinline__ void triangle_at(int t, int& tm, int& tn) {
+  tm = (int)((sqrtf(8.0f * t + 1.0f) - 1.0f) * 0.5f);
+  if (triangle_tiles(tm + 1) <= t) ++tm;
+  if (triangle_tiles(tm) > t) --tm;
+  tn = t - triangle_tiles(tm);
+}
+__device__ __forceinline__ void gemm_triangle_of(const GemmArgs& g, int wg, int total, int& tm, int& tn, int& sp) {
+  constexpr int kXcd = 8;
+  const int per = total / kXcd, rest = total % kXcd, x = wg % kXcd;
+  const int t = x * per + min(x, rest) + wg / kXcd, tiles = triangle_tiles(g.tiles_m);
+  sp = t / tiles;
+  triangle_at(t - sp * tiles, tm, tn);
+}
+
 // Where a wave's part of a tile lies, for its epilogue.
 template <class T>
 struct GemmWave {
@@ -394,8 +414,8 @@ struct GemmWave {
 };
 // acc[f][j]: a lane holds columns col(p) .. col(p) + 7 of row(j) in acc[2 p][j] and acc[2 p + 1][j].
 
-template <class T, bool BKC, bool GATED, int BK = kGemmBK>
-using GemmLoadB = std::conditional_t<GATED, GatedTileLoad<T::BN, T::threads, BK>, TileLoad<T::BN, T::threads, BKC, true, BK>>;
+template <class T, bool BKC, int FORM, int BK = kGemmBK>
+using GemmLoadB = std::conditional_t<FORM == kGated, GatedTileLoad<T::BN, T::threads, BK>, TileLoad<T::BN, T::threads, BKC, true, BK>>;
 
 // One workgroup a tile.  Of a k step's 64, the fragments of one half are read while the other half's products run, so the
 // LDS's latency passes behind the matrix instructions; the step's only barrier lies between its halves, when every wave
@@ -406,10 +426,11 @@ using GemmLoadB = std::conditional_t<GATED, GatedTileLoad<T::BN, T::threads, BK>
 //
 // The smallest tiles hold all three planes of float32 operands for 32 k at a time and form the six products from them:
 // a barrier for 24 matrix instructions a wave instead of eight, and half the loads (a 64-wide step of k 1.2 us instead of
-// 2.1 while a workgroup has its CU to itself).
+// 2.1 while a workgroup has its CU to itself).  Of two planes every tile holds both: the three products read each plane's
+// fragments once instead of three times in two (8192 x 1024 x 1024 on 128 x 128 44 -> 41 us, on 256 x 256 61 -> 57).
 constexpr int kPlanesBK = 32;
 template <class T, int PAIRS>
-constexpr bool gemm_planes() { return PAIRS > 1 && T::BM == 64; }
+constexpr bool gemm_planes() { return PAIRS == 3 || (PAIRS > 1 && T::BM == 64); }
 constexpr int planes_of(int pairs) { return pairs == 6 ? 3 : pairs == 3 ? 2 : 1; }
 template <class T, int PAIRS>
 constexpr int gemm_stage() {
@@ -420,16 +441,16 @@ constexpr int gemm_stage() {
 // 19.4 us, 4096 x 1024 x 1024 79 -> 76; with strided operands, whose fragments take twice the LDS loads, a third of the CU's
 // workgroups less costs as much as it gives: 16384 x 768 x 128 backward 86 -> 91).
 template <class T, int PAIRS, bool KC>
-constexpr int gemm_third() { return gemm_planes<T, PAIRS>() && KC ? gemm_stage<T, PAIRS>() : 16; }
+constexpr int gemm_third() { return gemm_planes<T, PAIRS>() && KC && T::BM == 64 ? gemm_stage<T, PAIRS>() : 16; }
 
-template <class T, bool AKC, bool BKC, int PAIRS, class Num, bool GATED, class Acc>
+template <class T, bool AKC, bool BKC, int PAIRS, class Num, int FORM, class Acc>
 __device__ __forceinline__ void planes_products(const GemmArgs& g, Acc& acc, int m0, int n0, int kbeg, int kend, int wm, int wn,
                                                 char (&s0)[gemm_stage<T, PAIRS>()], char (&s1)[gemm_stage<T, PAIRS>()],
                                                 char (&s2)[gemm_third<T, PAIRS, AKC && BKC>()]) {
   constexpr int P = planes_of(PAIRS);
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   TileLoad<T::BM, T::threads, AKC, false, kPlanesBK> la;
-  GemmLoadB<T, BKC, GATED, kPlanesBK> lb;
+  GemmLoadB<T, BKC, FORM, kPlanesBK> lb;
   la.init(g.a.ld, tid);
   lb.init(g.b.ld, tid);
   TileRead<T::BM, AKC, false, kPlanesBK> ra;
@@ -447,7 +468,7 @@ __device__ __forceinline__ void planes_products(const GemmArgs& g, Acc& acc, int
 #pragma unroll
     for (int p = 0; p < P; ++p) {
       la.issue(g.a, p, m0, g.m, k, g.k, (lds_char*)s + p * pa, wave, live);
-      if constexpr (GATED) lb.issue(g.b, g.up, p, n0, g.n, k, g.k, (lds_char*)s + P * pa + p * pb, wave, live);
+      if constexpr (FORM == kGated) lb.issue(g.b, g.up, p, n0, g.n, k, g.k, (lds_char*)s + P * pa + p * pb, wave, live);
       else lb.issue(g.b, p, n0, g.n, k, g.k, (lds_char*)s + P * pa + p * pb, wave, live);
     }
   };
@@ -469,7 +490,7 @@ __device__ __forceinline__ void planes_products(const GemmArgs& g, Acc& acc, int
           acc[i][j] = Num::mma(b[i][pair_b<PAIRS>(q)], a[j][pair_a<PAIRS>(q)], acc[i][j]);
   };
   constexpr int B = kPlanesBK, in_flight = P * (decltype(la)::loads + decltype(lb)::loads);  // of one stage
-  if constexpr (!(AKC && BKC)) {
+  if constexpr (!(AKC && BKC) || T::BM > 64) {
     issue(s0, kbeg);
     int k = kbeg;
     for (; k + B < kend; k += 2 * B) {
@@ -507,14 +528,15 @@ __device__ __forceinline__ void planes_products(const GemmArgs& g, Acc& acc, int
   }
 }
 
-template <class T, bool AKC, bool BKC, int PAIRS, class Num, bool GATED, class Epi>
+template <class T, bool AKC, bool BKC, int PAIRS, class Num, int FORM, class Epi>
 __device__ __forceinline__ void gemm_tile(const GemmArgs& g, const Epi& epi, int wg, int wgs, char (&s0)[gemm_stage<T, PAIRS>()],
                                           char (&s1)[gemm_stage<T, PAIRS>()], char (&s2)[gemm_third<T, PAIRS, AKC && BKC>()]) {
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int wm = wave / T::WN, wn = wave % T::WN;
   int tm, tn, sp;
-  gemm_tile_of(g, wg, wgs, tm, tn, sp);
-  const int m0 = tm * T::BM, n0 = tn * (GATED ? T::BN / 2 : T::BN);
+  if constexpr (FORM == kTriangle) gemm_triangle_of(g, wg, wgs, tm, tn, sp);
+  else gemm_tile_of(g, wg, wgs, tm, tn, sp);
+  const int m0 = tm * T::BM, n0 = tn * (FORM == kGated ? T::BN / 2 : T::BN);
   const int kbeg = sp * g.k_per_split, kend = min(g.k, kbeg + g.k_per_split);
   typename Num::Acc acc[T::FN][T::FM];
 #pragma unroll
@@ -524,12 +546,12 @@ __device__ __forceinline__ void gemm_tile(const GemmArgs& g, const Epi& epi, int
   typename Epi::template Side<T> side;
   if constexpr (gemm_planes<T, PAIRS>()) {
     side.fetch(epi, m0, n0, tid);
-    planes_products<T, AKC, BKC, PAIRS, Num, GATED>(g, acc, m0, n0, kbeg, kend, wm, wn, s0, s1, s2);
+    planes_products<T, AKC, BKC, PAIRS, Num, FORM>(g, acc, m0, n0, kbeg, kend, wm, wn, s0, s1, s2);
   } else {
     const int steps = max(0, (kend - kbeg + kGemmBK - 1) / kGemmBK) * PAIRS;
 
     TileLoad<T::BM, T::threads, AKC, false> la;
-    GemmLoadB<T, BKC, GATED> lb;
+    GemmLoadB<T, BKC, FORM> lb;
     la.init(g.a.ld, tid);
     lb.init(g.b.ld, tid);
     TileRead<T::BM, AKC, false> ra;
@@ -543,7 +565,7 @@ __device__ __forceinline__ void gemm_tile(const GemmArgs& g, const Epi& epi, int
     auto issue = [&](char* s) {
       const int qa = PAIRS == 1 ? 0 : pair_a<PAIRS>(pp), qb = PAIRS == 1 ? 0 : pair_b<PAIRS>(pp);
       la.issue(g.a, qa, m0, g.m, pk, g.k, (lds_char*)s, wave);
-      if constexpr (GATED) lb.issue(g.b, g.up, qb, n0, g.n, pk, g.k, (lds_char*)s + boff, wave);
+      if constexpr (FORM == kGated) lb.issue(g.b, g.up, qb, n0, g.n, pk, g.k, (lds_char*)s + boff, wave);
       else lb.issue(g.b, qb, n0, g.n, pk, g.k, (lds_char*)s + boff, wave);
       if (PAIRS == 1 || ++pp == PAIRS) {
         pp = 0;
@@ -598,12 +620,12 @@ __device__ __forceinline__ void gemm_tile(const GemmArgs& g, const Epi& epi, int
 }
 
 // Registers for two waves a SIMD: one workgroup of 256 x 256 a CU, two of 128 x 128.
-template <class T, bool AKC, bool BKC, int PAIRS, class Epi, class Num = OfBf16, bool GATED = false>
+template <class T, bool AKC, bool BKC, int PAIRS, class Epi, class Num = OfBf16, int FORM = kPlain>
 __global__ __launch_bounds__(T::threads, 2) void gemm_kernel(GemmArgs g, Epi epi) {
   __shared__ __attribute__((aligned(1024))) char s0[gemm_stage<T, PAIRS>()];
   __shared__ __attribute__((aligned(1024))) char s1[gemm_stage<T, PAIRS>()];
   __shared__ __attribute__((aligned(1024))) char s2[gemm_third<T, PAIRS, AKC && BKC>()];
-  gemm_tile<T, AKC, BKC, PAIRS, Num, GATED>(g, epi, blockIdx.x, gridDim.x, s0, s1, s2);
+  gemm_tile<T, AKC, BKC, PAIRS, Num, FORM>(g, epi, blockIdx.x, gridDim.x, s0, s1, s2);
 }
 
 // Both gradients of a small layer in one launch: the first x_wgs workgroups form x (A with k contiguous, B strided), the
@@ -615,9 +637,9 @@ __global__ __launch_bounds__(T::threads, 2) void gemm_pair_kernel(GemmArgs x, Ep
   __shared__ __attribute__((aligned(1024))) char s2[gemm_third<T, PAIRS, false>()];
   const int b = blockIdx.x;
   if (b < x_wgs)
-    gemm_tile<T, true, false, PAIRS, OfBf16, false>(x, ex, b, x_wgs, s0, s1, s2);
+    gemm_tile<T, true, false, PAIRS, OfBf16, kPlain>(x, ex, b, x_wgs, s0, s1, s2);
   else
-    gemm_tile<T, false, false, PAIRS, OfBf16, false>(w, ew, b - x_wgs, gridDim.x - x_wgs, s0, s1, s2);
+    gemm_tile<T, false, false, PAIRS, OfBf16, kPlain>(w, ew, b - x_wgs, gridDim.x - x_wgs, s0, s1, s2);
 }
 
 }  // namespace fgpu
