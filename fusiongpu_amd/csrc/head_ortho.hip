@@ -90,9 +90,9 @@ __global__ __launch_bounds__(256) void start_kernel(const T* x, int64_t rows, in
 }
 
 // ---- the products ------------------------------------------------------------------
-// alpha D + beta C, as planes or (out) as the result.
+// alpha D + beta C + diagonal I, as planes or (out) as the result.
 struct OrthoFinish {
-  float alpha = 0, beta = 0;
+  float alpha = 0, beta = 0, diagonal = 0;
   Planes c, to;
   void* out = nullptr;
   int m = 0, n = 0;
@@ -102,6 +102,10 @@ struct OrthoFinish {
       const f32x8 o = planes8(c, row * c.ld + col);
 #pragma unroll
       for (int e = 0; e < 8; ++e) v.set(e, fmaf(beta, o[e], v[e]));
+    }
+    if (diagonal != 0) {
+#pragma unroll
+      for (int e = 0; e < 8; ++e) v.set(e, v[e] + (row == col + e ? diagonal : 0.0f));
     }
     return v;
   }
@@ -283,12 +287,26 @@ fgpu_status run_symmetric(const Planes& a, int k, const OrthoFinish& f, float* p
   return FGPU_OK;
 }
 
-// Products of bfloat16 updates in fewer pieces.  X is held in two planes throughout, but A takes one of them always, and P and
-// the product with it do in the first two steps: what those roundings leave lies in the directions of large singular
-// values, which the later steps do not multiply.  Against 64 bits (64 to 512 rows, singular values even, normal, as i^-1/2
-// to i^-2) the result is then off by at most 1.3e-3 of its norm, mostly below 6e-4, before it is rounded to bfloat16
-// (1.7e-3); with one plane in every product 2.7e-3, with X in one plane as well up to 8e-3.
-constexpr int kOnePlaneSteps = 2;
+// How a step forms a X + P X.  In two planes as (a I + P) X, in one with X added apart, from both of its planes: a X + P X, or,
+// near the end, X + (P + (a - 1) I) X, whose second factor is small in the directions whose singular values have arrived.
+//
+// Of bfloat16 updates A takes one plane of X, and the first two and the last two steps one plane in the other products too:
+// what the first roundings leave lies in the directions of large singular values, which the later steps do not multiply,
+// and the last ones' is little, as said.  Against 64 bits (64 to 512 rows; singular values even, of normal numbers, as i^-1/2 to
+// i^-2; four to eight steps) the result is then off by at most 1.4e-3 of its norm, mostly below 7e-4, before it is rounded to
+// bfloat16 (1.7e-3); with one plane in every product and P as it is 2.7e-3, with X in one plane as well up to 8e-3.  Of more
+// steps A's rounding leaves up to 1.9e-3, and coefficients larger than the usual ones more than that: those take two.
+struct Form {
+  int gram, rest;  // plane products of A, of the product with P; P itself takes three but in the first two steps
+  bool apart, near_one;
+};
+Form form_of(bool f32, int i, int steps, float a, float b, float c) {
+  if (f32 || std::fabs(a) + std::fabs(b) + std::fabs(c) > 10.5f) return {3, 3, false, false};
+  const int gram = steps <= 8 ? 1 : 3;
+  if (i < 2) return {gram, 1, true, false};
+  if (i >= steps - 2) return {gram, 1, true, true};
+  return {gram, 3, false, false};
+}
 
 struct Shape {
   int rows, cols, small, large;
@@ -296,10 +314,11 @@ struct Shape {
   Shape(int r, int c) : rows(r), cols(c), small(std::min(r, c)), large(std::max(r, c)), tall(r > c) {}
   size_t x_bytes() const { return carve_bytes<uint16_t>((size_t)rows * packed_ld(cols) * 2); }
   size_t a_bytes() const { return carve_bytes<uint16_t>((size_t)small * packed_ld(small) * 2); }
-  size_t part_bytes(bool f32) const {
-    const int few = f32 ? 3 : 1;
-    return std::max({cut_symmetric(small, large, few).part_bytes(small), cut_symmetric(small, small, few).part_bytes(small),
-                     cut_symmetric(small, small, 3).part_bytes(small)});
+  size_t part_bytes() const {
+    size_t b = 0;
+    for (int pairs : {1, 3})
+      for (int k : {small, large}) b = std::max(b, cut_symmetric(small, k, pairs).part_bytes(small));
+    return b;
   }
 };
 Planes planes_at(void* p, int rows, int cols) { return {(uint16_t*)p, packed_ld(cols), rows * packed_ld(cols)}; }
@@ -316,11 +335,9 @@ fgpu_status gram(const Planes& x, const Shape& sh, const OrthoFinish& f, float* 
   return sh.tall ? run_symmetric<T, PAIRS, false>(x, sh.large, f, part, s) : run_symmetric<T, PAIRS, true>(x, sh.large, f, part, s);
 }
 template <class T, int PAIRS>
-fgpu_status step(const Planes& x, const Planes& a, const Planes& p, const Shape& sh, const OrthoFinish& fp,
-                 const OrthoFinish& fx, float* part, hipStream_t s) {
-  FGPU_TRY((run_symmetric<T, PAIRS, true>(a, sh.small, fp, part, s)));
-  const Cut q = cut_product(fx.m, fx.n, sh.small, PAIRS);
-  return sh.tall ? run_whole<T, PAIRS, true, true>(x, p, sh.small, fx, q, s) : run_whole<T, PAIRS, true, false>(p, x, sh.small, fx, q, s);
+fgpu_status step(const Planes& x, const Planes& p, const Shape& sh, const OrthoFinish& f, hipStream_t s) {
+  const Cut q = cut_product(f.m, f.n, sh.small, PAIRS);
+  return sh.tall ? run_whole<T, PAIRS, true, true>(x, p, sh.small, f, q, s) : run_whole<T, PAIRS, true, false>(p, x, sh.small, f, q, s);
 }
 
 template <class T>
@@ -329,7 +346,7 @@ fgpu_status run_ortho(const T* x, const Shape& sh, int steps, float a, float b, 
   Planes xs[2] = {planes_at(ws.take<char>(sh.x_bytes()), sh.rows, sh.cols), planes_at(ws.take<char>(sh.x_bytes()), sh.rows, sh.cols)};
   const Planes ga = planes_at(ws.take<char>(sh.a_bytes()), sh.small, sh.small);
   const Planes gp = planes_at(ws.take<char>(sh.a_bytes()), sh.small, sh.small);
-  float* part = (float*)ws.take<char>(sh.part_bytes(sizeof(T) == 4));
+  float* part = (float*)ws.take<char>(sh.part_bytes());
   double* norm = ws.take<double>(kNormBlocks);
   FGPU_CHECK(ws.held(), FGPU_ERR_WORKSPACE, "orthogonalize: workspace smaller than fgpu_orthogonalize_workspace_bytes");
   const int64_t count = (int64_t)sh.rows * sh.cols;
@@ -342,14 +359,18 @@ fgpu_status run_ortho(const T* x, const Shape& sh, int steps, float a, float b, 
   for (int i = 0; i < steps; ++i) {
     const Planes &from = xs[i & 1], &to = xs[i + 1 & 1];
     const bool last = i + 1 == steps;
+    const Form m = form_of(sizeof(T) == 4, i, steps, a, b, c);
     OrthoFinish fa, fp, fx;
     fa.alpha = 1 / kHeld, fa.to = ga, fa.m = fa.n = n;
     fp.alpha = c / kHeld, fp.beta = b, fp.c = ga, fp.to = gp, fp.m = fp.n = n;
-    fx.alpha = 1 / kHeld, fx.beta = a, fx.c = from, fx.to = to, fx.m = sh.rows, fx.n = sh.cols;
+    fp.diagonal = kHeld * (!m.apart ? a : m.near_one ? a - 1 : 0);
+    fx.alpha = 1 / kHeld, fx.to = to, fx.m = sh.rows, fx.n = sh.cols;
+    if (m.apart) fx.beta = m.near_one ? 1 : a, fx.c = from;
     if (last) fx.out = out, fx.alpha /= kHeld, fx.beta /= kHeld;
-    const bool one = sizeof(T) == 2 && i < kOnePlaneSteps;
-    FGPU_TRY((sizeof(T) == 2 ? gram<T, 1>(from, sh, fa, part, s) : gram<T, 3>(from, sh, fa, part, s)));
-    FGPU_TRY((one ? step<T, 1>(from, ga, gp, sh, fp, fx, part, s) : step<T, 3>(from, ga, gp, sh, fp, fx, part, s)));
+    FGPU_TRY((m.gram == 1 ? gram<T, 1>(from, sh, fa, part, s) : gram<T, 3>(from, sh, fa, part, s)));
+    const bool early = m.rest == 1 && !m.near_one;
+    FGPU_TRY((early ? run_symmetric<T, 1, true>(ga, n, fp, part, s) : run_symmetric<T, 3, true>(ga, n, fp, part, s)));
+    FGPU_TRY((m.rest == 1 ? step<T, 1>(from, gp, sh, fx, s) : step<T, 3>(from, gp, sh, fx, s)));
   }
   return FGPU_OK;
 }
@@ -364,7 +385,7 @@ extern "C" {
 size_t fgpu_orthogonalize_workspace_bytes(int64_t rows, int64_t cols, int dtype) {
   if (check_common(rows, cols, dtype) != FGPU_OK || rows == 0 || cols == 0) return 0;
   const Shape sh((int)rows, (int)cols);
-  return 2 * (sh.x_bytes() + sh.a_bytes()) + sh.part_bytes(dtype == FGPU_DTYPE_F32) + carve_bytes<double>(kNormBlocks);
+  return 2 * (sh.x_bytes() + sh.a_bytes()) + sh.part_bytes() + carve_bytes<double>(kNormBlocks);
 }
 
 fgpu_status fgpu_orthogonalize(const void* d_x, int64_t rows, int64_t cols, int dtype, int steps, float a, float b, float c,
