@@ -199,9 +199,122 @@ __global__ __launch_bounds__(256) void triangle_join_kernel(OrthoFinish f, const
   }
 }
 
+// Few tiles: eight or sixteen waves share 32 x 32, each with its part of k and its fragments straight from the planes (whose
+// ends are zeros), as in head_direct.hpp; the partial tiles meet in LDS.  One launch, no parts in memory.
+constexpr int kFewTile = 32, kFewBK = 32;
+inline int few_waves(int k) { return k > 512 ? 16 : 8; }
+template <int PAIRS, bool KC, bool ISB>
+struct FewRead {
+  static constexpr int P = planes_of(PAIRS), lds_bytes = KC ? 0 : P * kFewBK * kFewTile * 2;
+  bf16x8 r[P][2];
+  __device__ __forceinline__ void load(const Planes& o, int r0, int nr, int k0, int nk, int lane) {
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      int64_t at;
+      bool in;
+      if constexpr (KC) {
+        const int l = lane & 15, row = r0 + (ISB ? 8 * (l >> 2) + 4 * i + (l & 3) : 16 * i + l), k = k0 + 8 * (lane >> 4);
+        at = row * o.ld + k, in = row < nr && k < nk;
+      } else {
+        const int t = lane + kWave * i, k = k0 + t / 4, col = r0 + t % 4 * 8;
+        at = k * o.ld + col, in = k < nk && col < nr;
+      }
+#pragma unroll
+      for (int p = 0; p < P; ++p)
+        r[p][i] = in ? *reinterpret_cast<const bf16x8*>(o.p + p * o.plane + at) : bf16x8{0, 0, 0, 0, 0, 0, 0, 0};
+    }
+  }
+  // Strided: through the wave's own LDS and its transposing load.
+  __device__ __forceinline__ void frags(bf16x8 (&f)[2][P], char* lds, int lane) const {
+    if constexpr (KC) {
+#pragma unroll
+      for (int p = 0; p < P; ++p) f[0][p] = r[p][0], f[1][p] = r[p][1];
+    } else {
+      typedef __attribute__((address_space(3))) s16x4 lds_half;
+      constexpr int row_bytes = kFewTile * 2;
+      wave_lds_order();
+#pragma unroll
+      for (int p = 0; p < P; ++p)
+#pragma unroll
+        for (int i = 0; i < 2; ++i) *reinterpret_cast<bf16x8*>(lds + p * kFewBK * row_bytes + (lane + kWave * i) * 16) = r[p][i];
+      wave_lds_order();
+      const int l = lane & 15, g = lane >> 4;
+#pragma unroll
+      for (int p = 0; p < P; ++p)
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+          char* at = lds + (p * kFewBK + 8 * g + (l >> 2)) * row_bytes + (ISB ? (l & 3) * 16 + i * 8 : i * 32 + (l & 3) * 8);
+          const s16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_half*)(lds_char*)at);
+          const s16x4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_half*)(lds_char*)(at + 4 * row_bytes));
+          const s16x8 v = {lo[0], lo[1], lo[2], lo[3], hi[0], hi[1], hi[2], hi[3]};
+          f[i][p] = __builtin_bit_cast(bf16x8, v);
+        }
+      wave_lds_order();
+    }
+  }
+};
+template <class T, int PAIRS, bool AKC, bool BKC, int kFewWaves>
+__global__ __launch_bounds__(kFewWaves * kWave) void few_tiles_kernel(Planes a, Planes b, int k, OrthoFinish f) {
+  using RA = FewRead<PAIRS, AKC, false>;
+  using RB = FewRead<PAIRS, BKC, true>;
+  constexpr int stage = kFewWaves * (RA::lds_bytes + RB::lds_bytes), joined = kFewWaves * 4 * kWave * 16;
+  __shared__ __attribute__((aligned(1024))) char lds[stage > joined ? stage : joined];
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int across = (f.n + kFewTile - 1) / kFewTile;
+  const int m0 = blockIdx.x / across * kFewTile, n0 = blockIdx.x % across * kFewTile;
+  const int steps = (k + kFewBK - 1) / kFewBK, per = (steps + kFewWaves - 1) / kFewWaves;
+  const int s0 = wave * per, s1 = min(steps, s0 + per);
+  char* la = lds + wave * (RA::lds_bytes + RB::lds_bytes);
+  f32x4 acc[2][2];
+#pragma unroll
+  for (int i = 0; i < 2; ++i) acc[i][0] = acc[i][1] = f32x4{0, 0, 0, 0};
+  auto work = [&](const RA& ra, const RB& rb) {
+    bf16x8 fa[2][RA::P], fb[2][RB::P];
+    ra.frags(fa, la, lane);
+    rb.frags(fb, la + RA::lds_bytes, lane);
+#pragma unroll
+    for (int j = 0; j < 2; ++j)
+#pragma unroll
+      for (int i = 0; i < 2; ++i)
+#pragma unroll
+        for (int q = 0; q < PAIRS; ++q)
+          acc[i][j] = OfHalf::mma(fb[i][PAIRS == 1 ? 0 : pair_b<PAIRS>(q)], fa[j][PAIRS == 1 ? 0 : pair_a<PAIRS>(q)], acc[i][j]);
+  };
+  for (int s = s0; s < s1; s += 2) {  // two steps' loads in flight
+    RA a0, a1;
+    RB b0, b1;
+    a0.load(a, m0, f.m, s * kFewBK, k, lane);
+    b0.load(b, n0, f.n, s * kFewBK, k, lane);
+    const bool two = s + 1 < s1;
+    if (two) {
+      a1.load(a, m0, f.m, (s + 1) * kFewBK, k, lane);
+      b1.load(b, n0, f.n, (s + 1) * kFewBK, k, lane);
+    }
+    work(a0, b0);
+    if (two) work(a1, b1);
+  }
+  __syncthreads();
+  f32x4* join = reinterpret_cast<f32x4*>(lds);  // [wave][row fragment][column fragment][lane]
+#pragma unroll
+  for (int j = 0; j < 2; ++j)
+#pragma unroll
+    for (int i = 0; i < 2; ++i) join[((wave * 2 + j) * 2 + i) * kWave + lane] = acc[i][j];
+  __syncthreads();
+  if (threadIdx.x >= 2 * kWave) return;
+  const int j = threadIdx.x / kWave, row = m0 + 16 * j + (lane & 15), col = n0 + 8 * (lane >> 4);
+  f32x8 v{{0, 0, 0, 0}, {0, 0, 0, 0}};
+#pragma unroll
+  for (int w = 0; w < kFewWaves; ++w) {
+    v.lo += join[((w * 2 + j) * 2) * kWave + lane];
+    v.hi += join[((w * 2 + j) * 2 + 1) * kWave + lane];
+  }
+  if (row < f.m && col < ((f.n + 7) & ~7)) f.put<T>(v, row, col);
+}
+
 // ---- how a product is cut ------------------------------------------------------------
-// Microseconds, fitted over 1024 x 1024 over 1024 and 8192 and 8192 x 1024 over 1024: a step of k (64 of one plane, 32 of two)
-// of a workgroup while it has its CU to itself, for each of those that share one, and how many do.
+// Microseconds, fitted over sides of 64 to 4096 and k to 8192: a step of k (64 of one plane, 32 of two) of a workgroup while
+// it has its CU to itself, for each of those that share one, and how many do; both operands k contiguous (a strided one takes
+// 1.3 times as long).
 struct StepTime {
   double alone, shared;
   int most;
@@ -214,23 +327,32 @@ struct Cut {
   int tile = 0, splits = 1, k_per_split = 0;
   double us = 0;
 };
-double cut_us(const Cut& q, int pairs, int64_t tiles) {
+double cut_us(const Cut& q, int pairs, bool strided, int64_t tiles, double fixed) {
   const StepTime t = step_time(q.tile, pairs);
   const int steps = ceil_div(q.k_per_split, pairs == 1 ? kGemmBK : kPlanesBK), round = 256 * t.most;
-  const double fixed = q.tile == 256 ? 6 : q.tile == 128 ? 3.5 : 2.5;
+  const double k = steps * (strided ? 1.3 : 1.0);
   const int64_t wgs = tiles * q.splits, full = wgs / round, rest = wgs % round;
-  double us = full * (steps * std::max(t.alone, t.most * t.shared) + fixed);
-  if (rest) us += steps * std::max(t.alone, ceil_div(rest, 256) * t.shared) + fixed;
+  double us = full * (k * std::max(t.alone, t.most * t.shared) + fixed);
+  if (rest) us += k * std::max(t.alone, ceil_div(rest, 256) * t.shared) + fixed;
   return us;
 }
-// A product of m x n over k, whole.
-Cut cut_product(int m, int n, int k, int pairs) {
-  Cut best;
+// The kernel of few tiles, whose waves take their steps one after the other; strided: how many operands are.
+double few_us(int m, int n, int k, int pairs, int strided) {
+  const int steps = ceil_div(ceil_div(k, kFewBK), few_waves(k));
+  const double all = (double)ceil_div(m, kFewTile) * ceil_div(n, kFewTile) * steps / 256;
+  const double more = few_waves(k) == 16 ? 1.75 : 1;
+  const double alone = (strided == 2 ? 0.42 : strided ? 0.5 : 0.6) * more;
+  const double shared = (strided == 2 ? 0.65 : strided ? 0.83 : 1.09) * more;
+  return 2.6 + std::max(steps * alone, all * shared) * (pairs == 1 ? 1 : 1.9);
+}
+// A product of m x n over k, whole: tile 32 for the kernel of few tiles.
+Cut cut_product(int m, int n, int k, int pairs, int strided) {
+  Cut best{kFewTile, 1, 0, few_us(m, n, k, pairs, strided)};
   for (int tile : {256, 128, 64}) {
     const int64_t tiles = (int64_t)ceil_div(m, tile) * ceil_div(n, tile);
     Cut q{tile, 1, ceil_div(k, kGemmBK) * kGemmBK};
-    q.us = cut_us(q, pairs, tiles);
-    if (!best.tile || q.us < best.us) best = q;
+    q.us = cut_us(q, pairs, strided == 2, tiles, tile == 256 ? 9 : tile == 128 ? 5 : 3);
+    if (q.us < best.us) best = q;
   }
   return best;
 }
@@ -242,16 +364,16 @@ struct SymmetricCut {
     return joined ? carve_bytes<float>((size_t)part.splits * triangle_tiles(ceil_div(n, part.tile)) * part.tile * part.tile) : 0;
   }
 };
-SymmetricCut cut_symmetric(int n, int k, int pairs) {
+SymmetricCut cut_symmetric(int n, int k, int pairs, bool strided) {
   SymmetricCut c;
-  c.whole = cut_product(n, n, k, pairs);
+  c.whole = cut_product(n, n, k, pairs, strided ? 2 : 0);
   for (int tile : {256, 128, 64}) {
     const int64_t tiles = triangle_tiles(ceil_div(n, tile));
     for (int splits = 1; splits <= 64; ++splits) {
       if (splits > 1 && (splits > ceil_div(k, 2 * kGemmBK) || tiles * splits > 2048)) break;
       Cut q{tile, splits, ceil_div(ceil_div(k, kGemmBK), splits) * kGemmBK};
       if (ceil_div(k, q.k_per_split) != splits) continue;
-      q.us = cut_us(q, pairs, tiles) + 4 + tiles * splits * tile * tile * 8.0 / 5e6;
+      q.us = cut_us(q, pairs, strided, tiles, tile == 256 ? 6 : tile == 128 ? 3.5 : 2.5) + 4 + tiles * splits * tile * tile * 8.0 / 5e6;
       if (!c.part.tile || q.us < c.part.us) c.part = q;
     }
   }
@@ -269,6 +391,13 @@ fgpu_status run_cut(const GemmArgs& g, int tile, int grid, const E& e, hipStream
 }
 template <class T, int PAIRS, bool AKC, bool BKC>
 fgpu_status run_whole(const Planes& a, const Planes& b, int k, const OrthoFinish& f, const Cut& q, hipStream_t s) {
+  if (q.tile == kFewTile) {
+    const int tiles = ceil_div(f.m, kFewTile) * ceil_div(f.n, kFewTile);
+    if (few_waves(k) == 16) few_tiles_kernel<T, PAIRS, AKC, BKC, 16><<<tiles, 16 * kWave, 0, s>>>(a, b, k, f);
+    else few_tiles_kernel<T, PAIRS, AKC, BKC, 8><<<tiles, 8 * kWave, 0, s>>>(a, b, k, f);
+    FGPU_HIP(hipGetLastError());
+    return FGPU_OK;
+  }
   const GemmArgs g{{a.p, a.ld, a.plane}, {b.p, b.ld, b.plane}, f.m, f.n, k, ceil_div(f.m, q.tile), ceil_div(f.n, q.tile), 1,
                    q.k_per_split};
   return run_cut<PAIRS, AKC, BKC, kPlain>(g, q.tile, g.tiles_m * g.tiles_n, OrthoEpi<T>{f}, s);
@@ -276,7 +405,7 @@ fgpu_status run_whole(const Planes& a, const Planes& b, int k, const OrthoFinish
 // a a^T of n rows (KC: k contiguous).
 template <class T, int PAIRS, bool KC>
 fgpu_status run_symmetric(const Planes& a, int k, const OrthoFinish& f, float* part, hipStream_t s) {
-  const SymmetricCut c = cut_symmetric(f.n, k, PAIRS);
+  const SymmetricCut c = cut_symmetric(f.n, k, PAIRS, !KC);
   if (!c.joined) return run_whole<T, PAIRS, KC, KC>(a, a, k, f, c.whole, s);
   const Cut& q = c.part;
   const int t = ceil_div(f.n, q.tile), tiles = triangle_tiles(t);
@@ -317,7 +446,7 @@ struct Shape {
   size_t part_bytes() const {
     size_t b = 0;
     for (int pairs : {1, 3})
-      for (int k : {small, large}) b = std::max(b, cut_symmetric(small, k, pairs).part_bytes(small));
+      b = std::max({b, cut_symmetric(small, large, pairs, tall).part_bytes(small), cut_symmetric(small, small, pairs, false).part_bytes(small)});
     return b;
   }
 };
@@ -336,7 +465,7 @@ fgpu_status gram(const Planes& x, const Shape& sh, const OrthoFinish& f, float* 
 }
 template <class T, int PAIRS>
 fgpu_status step(const Planes& x, const Planes& p, const Shape& sh, const OrthoFinish& f, hipStream_t s) {
-  const Cut q = cut_product(f.m, f.n, sh.small, PAIRS);
+  const Cut q = cut_product(f.m, f.n, sh.small, PAIRS, sh.tall ? 0 : 1);
   return sh.tall ? run_whole<T, PAIRS, true, true>(x, p, sh.small, f, q, s) : run_whole<T, PAIRS, true, false>(p, x, sh.small, f, q, s);
 }
 
