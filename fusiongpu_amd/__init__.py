@@ -28,6 +28,7 @@ from __future__ import annotations
 
 import contextlib
 import ctypes
+import functools
 import os
 import sys
 
@@ -1138,11 +1139,11 @@ def gated_linear(x, weight, bias=None, act: str = "silu", save_pre: bool = False
         b = _head_opt(bias, t, "bias", (2 * n,))
         h = _head_out(out, x, (rows, n))
         pre = _head_out(None, x, (rows, 2 * n)) if save_pre else None
-        _here(x, w, b, h)
+        stream = _stream_here(x, w, b, h)
         dt = _dtype_code(x)
-        wp, wb, ws = _head_ws(lib.fgpu_gated_linear_workspace_bytes(rows, k, n, dt), x)
+        wp, wb, ws = _head_ws(_ws_bytes("fgpu_gated_linear_workspace_bytes", rows, k, n, dt), x)
         _check(lib.fgpu_gated_linear(x.data_ptr(), w.data_ptr(), _ptr(b), rows, k, n, dt, code, h.data_ptr(), _ptr(pre), wp,
-                                     wb, _stream()))
+                                     wb, stream))
     return (h, pre) if save_pre else h
 
 
@@ -1159,24 +1160,33 @@ def gated_linear_backward(dh, x, weight, pre, act: str = "silu", want=("x", "wei
         k = x.shape[1]
         w = _head(weight, t, "weight", (2 * n, k))
         z = _head(pre, t, "pre", (rows, 2 * n))
-        _here(dh, x, w, z)
+        stream = _stream_here(dh, x, w, z)
         dx = _head_out(None, dh, (rows, k)) if "x" in want else None
         dw = _head_out(None, dh, (2 * n, k)) if "weight" in want else None
         db = _head_out(None, dh, (2 * n,)) if "bias" in want else None
         dt = _dtype_code(dh)
-        wp, wb, ws = _head_ws(lib.fgpu_gated_linear_backward_workspace_bytes(rows, k, n, dt), dh)
+        wp, wb, ws = _head_ws(_ws_bytes("fgpu_gated_linear_backward_workspace_bytes", rows, k, n, dt), dh)
         _check(lib.fgpu_gated_linear_backward(dh.data_ptr(), x.data_ptr(), w.data_ptr(), z.data_ptr(), rows, k, n, dt, code,
-                                              _ptr(dx), _ptr(dw), _ptr(db), wp, wb, _stream()))
+                                              _ptr(dx), _ptr(dw), _ptr(db), wp, wb, stream))
     return dx, dw, db
 
 
-def _here(*tensors):
-    """Refuses tensors of another device than the current one, whose stream the call goes to."""
-    now = _TORCH.cuda.current_device()
+def _stream_here(*tensors):
+    """The handle of the current stream, for a call on `tensors`: refuses those of another device than the current one, whose
+    stream it is."""
+    cuda = _TORCH.cuda
+    now = cuda.current_device()
     for t in tensors:
         if t is not None and t.get_device() != now:
             raise ValueError(f"a tensor on {t.device}, but the current device is cuda:{now}: make the call under "
                              "torch.cuda.device(...) of its tensors")
+    return _raw_stream(now) if _raw_stream is not None else cuda.current_stream().cuda_stream
+
+
+@functools.lru_cache(maxsize=1024)
+def _ws_bytes(name, *sizes):
+    """The library's answer to how many bytes a call of these sizes needs, asked once."""
+    return getattr(lib, name)(*sizes)
 
 
 def _halves(w, name):
@@ -1197,10 +1207,10 @@ def quantize_rows(x, stream=None):
     with _on(stream):
         x = _head_first(x, "x")
         rows, dim = x.shape
-        _here(x)
+        stream = _stream_here(x)
         q = torch.empty((rows, int8_row(dim)), dtype=torch.int8, device=x.device)
         scale = torch.empty(rows, dtype=torch.float32, device=x.device)
-        _check(lib.fgpu_quantize_rows(x.data_ptr(), rows, dim, _dtype_code(x), q.data_ptr(), scale.data_ptr(), _stream()))
+        _check(lib.fgpu_quantize_rows(x.data_ptr(), rows, dim, _dtype_code(x), q.data_ptr(), scale.data_ptr(), stream))
     return q, scale
 
 
@@ -1236,11 +1246,11 @@ def linear_int8(x, weight, weight_scale, bias=None, residual=None, act: str = "n
         x, xs, w, ws, rows, k, n, t = _int8_args(x, weight, weight_scale, x_scale, dtype)
         b, r = _head_opt(bias, t, "bias", (n,)), _head_opt(residual, t, "residual", (rows, n))
         y = x.new_empty((rows, n), dtype=t) if out is None else _out(out, t, (rows, n), "out")
-        _here(x, xs, w, ws, b, r, y)
+        stream = _stream_here(x, xs, w, ws, b, r, y)
         dt = _dtype_code(y)
-        wp, wb, hold = _head_ws(lib.fgpu_linear_int8_workspace_bytes(rows, k, n, dt, xs is not None), x)
+        wp, wb, hold = _head_ws(_ws_bytes("fgpu_linear_int8_workspace_bytes", rows, k, n, dt, xs is not None), x)
         _check(lib.fgpu_linear_int8(x.data_ptr(), _ptr(xs), w.data_ptr(), ws.data_ptr(), _ptr(b), _ptr(r), rows, k, n, dt, code,
-                                    y.data_ptr(), wp, wb, _stream()))
+                                    y.data_ptr(), wp, wb, stream))
     return y
 
 
@@ -1253,11 +1263,11 @@ def gated_linear_int8(x, weight, weight_scale, bias=None, act: str = "silu", x_s
         n = _halves(w, "weight")
         b = _head_opt(bias, t, "bias", (2 * n,))
         h = x.new_empty((rows, n), dtype=t) if out is None else _out(out, t, (rows, n), "out")
-        _here(x, xs, w, ws, b, h)
+        stream = _stream_here(x, xs, w, ws, b, h)
         dt = _dtype_code(h)
-        wp, wb, hold = _head_ws(lib.fgpu_gated_linear_int8_workspace_bytes(rows, k, n, dt, xs is not None), x)
+        wp, wb, hold = _head_ws(_ws_bytes("fgpu_gated_linear_int8_workspace_bytes", rows, k, n, dt, xs is not None), x)
         _check(lib.fgpu_gated_linear_int8(x.data_ptr(), _ptr(xs), w.data_ptr(), ws.data_ptr(), _ptr(b), rows, k, n, dt, code,
-                                          h.data_ptr(), wp, wb, _stream()))
+                                          h.data_ptr(), wp, wb, stream))
     return h
 
 
@@ -1269,10 +1279,10 @@ def orthogonalize(x, steps: int = 5, coefficients=(3.4445, -4.7750, 2.0315), eps
         x = _head_first(x, "x")
         rows, cols = x.shape
         y = _head_out(out, x, (rows, cols))
-        _here(x, y)
+        stream = _stream_here(x, y)
         dt = _dtype_code(x)
-        wp, wb, ws = _head_ws(lib.fgpu_orthogonalize_workspace_bytes(rows, cols, dt), x)
-        _check(lib.fgpu_orthogonalize(x.data_ptr(), rows, cols, dt, steps, a, b, c, eps, y.data_ptr(), wp, wb, _stream()))
+        wp, wb, ws = _head_ws(_ws_bytes("fgpu_orthogonalize_workspace_bytes", rows, cols, dt), x)
+        _check(lib.fgpu_orthogonalize(x.data_ptr(), rows, cols, dt, steps, a, b, c, eps, y.data_ptr(), wp, wb, stream))
     return y
 
 

@@ -16,27 +16,6 @@ struct Scales {
   const float* row = nullptr;
   const float* col = nullptr;
 };
-// Eight consecutive values from p on, the first cnt of them.
-template <class T>
-__device__ __forceinline__ f32x8 load8_n(const T* p, int cnt) {
-  if (cnt >= 8) return load8(p);
-  f32x8 v{{0, 0, 0, 0}, {0, 0, 0, 0}};
-#pragma unroll
-  for (int e = 0; e < 7; ++e)
-    if (e < cnt) v.set(e, to_f32(p[e]));
-  return v;
-}
-template <bool STREAM, class T>
-__device__ __forceinline__ void store8_n(T* p, const f32x8& v, int cnt) {
-  if (cnt >= 8) {
-    if constexpr (STREAM) stream8(p, v);
-    else store8(p, v);
-    return;
-  }
-#pragma unroll
-  for (int e = 0; e < 7; ++e)
-    if (e < cnt) p[e] = (T)v[e];
-}
 // Eight columns of a row from two fragments' accumulators, scaled where they are integers.
 template <class A>
 __device__ __forceinline__ f32x8 eight(const A& lo, const A& hi, float row, const f32x8& col) {
@@ -51,6 +30,7 @@ __device__ __forceinline__ f32x8 eight(const A& lo, const A& hi, float row, cons
 
 template <class T, int ACT>
 struct GatedEpi {
+  static constexpr bool kStagger = true;
   Finish f;  // bias [2 n], out [m][n], pre [m][2 n], stream
   Scales s;
   int m, n;
@@ -99,6 +79,11 @@ struct GatedEpi {
 // Results of more than the last-level cache's 256 MB go past it (head_gemm.hip has both sides).
 inline bool past_caches(int64_t bytes) { return bytes > (int64_t)256 << 20; }
 
+// Where 256 x 256 tiles, one a CU, come in eight rounds and more: 17 us from the first to the last start, about half a tile of
+// 1024 k (65536 x 4096 x 1024 with both factors kept 1111 -> 1068 us, 8-bit 628 -> 565; 9 us 1078 and 569, 34 us 1084 and
+// 595; two workgroups a CU of 128 x 128 gain nothing).
+inline int stagger_of(const Plan& q) { return q.tile == 256 && (int64_t)q.tiles_m * q.tiles_n >= 8 * 256 ? 64 : 0; }
+
 // n hidden columns over k units (OfInt8: pairs), by the plan of a product of 2 n columns.
 template <int PAIRS, class Num, class T, int ACT>
 fgpu_status run_gated(const GemmArgs& g, int tile, const GatedEpi<T, ACT>& e, hipStream_t s) {
@@ -113,7 +98,7 @@ fgpu_status run_gated(const GemmArgs& g, int tile, const GatedEpi<T, ACT>& e, hi
 template <int PAIRS, class Num, class T>
 fgpu_status run_gated(const GemmOperand& a, const GemmOperand& b, int64_t up, int m, int n, int k, const Plan& q, Finish f,
                       const Scales& sc, hipStream_t s) {
-  const GemmArgs g{a, b, m, n, k, q.tiles_m, q.tiles_n, 1, ceil_div(k, kGemmBK) * kGemmBK, up};
+  const GemmArgs g{a, b, m, n, k, q.tiles_m, q.tiles_n, 1, ceil_div(k, kGemmBK) * kGemmBK, stagger_of(q), up};
   f.stream = past_caches((int64_t)m * n * (f.pre ? 3 : 1) * (int64_t)sizeof(T));
   switch (f.act) {
     case FGPU_ACT_NONE: return run_gated<PAIRS, Num>(g, q.tile, GatedEpi<T, FGPU_ACT_NONE>{f, sc, m, n}, s);

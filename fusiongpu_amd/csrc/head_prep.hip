@@ -85,78 +85,73 @@ __device__ __forceinline__ void make_dz(const DzJob& j, int block) {
   }
 }
 
-// Four elements of an operand's row at any address, the first n of them.
+// Eight elements of an operand's row at any address, the first n of them.
 template <class T>
-__device__ __forceinline__ void put4_n(uint16_t* d, int64_t plane, const f32x4& v, int n) {
-  if constexpr (sizeof(T) == 2) {
-    store4_n((bf16*)d, v, n);
-  } else {
-    bf16x4 p[3];
-    split4(v, p[0], p[1], p[2]);
+__device__ __forceinline__ void put8_n(uint16_t* d, int64_t plane, const f32x8& v, int n) {
+  bf16x8 p[Frag<T>::planes];
+  if constexpr (sizeof(T) == 2) p[0] = to_bf16x8(v);
+  else split8(v, p[0], p[1], p[2]);
 #pragma unroll
-    for (int q = 0; q < 3; ++q) {
-      bf16* at = (bf16*)d + q * plane;
-      if (n >= 4) {
-        *reinterpret_cast<bf16x4u*>(at) = p[q];
-      } else {
+  for (int q = 0; q < Frag<T>::planes; ++q) {
+    bf16* at = (bf16*)d + q * plane;
+    if (n >= 8) {
+      *reinterpret_cast<bf16x8u*>(at) = p[q];
+    } else {
 #pragma unroll
-        for (int e = 0; e < 3; ++e)
-          if (e < n) at[e] = p[q][e];
-      }
+      for (int e = 0; e < 7; ++e)
+        if (e < n) at[e] = p[q][e];
     }
   }
 }
 
-// The same of a gated layer: a thread four hidden columns, both halves of dz.
+// The same of a gated layer: a thread eight hidden columns, both halves of dz.
 template <class T>
 __device__ __forceinline__ void make_gated_dz(const DzJob& j, int block) {
-  __shared__ f32x4 sum[2][4][64];
-  const int across = (j.cols + kDzCols - 1) / kDzCols, chunk = block / across;
+  __shared__ float sum[2][3][512];
+  const int across = (j.cols + 2 * kDzCols - 1) / (2 * kDzCols), chunk = block / across;
   const int lane = threadIdx.x & 63, w = threadIdx.x >> 6;
-  const int c = block % across * kDzCols + lane * 4, cnt = min(j.cols - c, 4);
+  const int c = block % across * 2 * kDzCols + lane * 8, cnt = min(j.cols - c, 8);
   const int per = (j.rows + j.chunks - 1) / j.chunks, r0 = chunk * per, r1 = min(j.rows, r0 + per);
   uint16_t* dst = const_cast<uint16_t*>(j.dst.p);
-  f32x4 ag = {0, 0, 0, 0}, au = {0, 0, 0, 0};
+  f32x8 ag{{0, 0, 0, 0}, {0, 0, 0, 0}}, au = ag;
   if (cnt > 0) {
-    const int pad = c + 4 >= j.cols ? (int)whole8(2 * j.cols) - 2 * j.cols : 0;  // zeros behind the row
+    const int pad = c + 8 >= j.cols ? (int)whole8(2 * j.cols) - 2 * j.cols : 0;  // zeros behind the row
 #pragma unroll 2
     for (int r = r0 + w; r < r1; r += 4) {
       const T* pre = (const T*)j.pre + (int64_t)r * 2 * j.cols + c;
-      const f32x4 d = load4_n((const T*)j.dy + (int64_t)r * j.cols + c, cnt);
-      const f32x4 g = load4_n(pre, cnt), u = load4_n(pre + j.cols, cnt);
-      f32x4 dg, du;
+      const f32x8 d = load8_n((const T*)j.dy + (int64_t)r * j.cols + c, cnt);
+      const f32x8 g = load8_n(pre, cnt), u = load8_n(pre + j.cols, cnt);
+      f32x8 dg, du;
 #pragma unroll
-      for (int k = 0; k < 4; ++k) {
+      for (int k = 0; k < 8; ++k) {
         float value, slope;
         act_both<T>(g[k], j.act, value, slope);
-        dg[k] = d[k] * u[k] * slope;
-        du[k] = d[k] * value;
+        dg.set(k, d[k] * u[k] * slope);
+        du.set(k, d[k] * value);
       }
-      if (cnt < 4) {
-#pragma unroll
-        for (int k = 1; k < 4; ++k)
-          if (k >= cnt) dg[k] = du[k] = 0;
-      }
-      ag += dg, au += du;
+      ag.lo += dg.lo, ag.hi += dg.hi, au.lo += du.lo, au.hi += du.hi;
       if (dst) {
         uint16_t* at = dst + (int64_t)r * j.dst.ld + c;
-        put4_n<T>(at, j.dst.plane, dg, cnt);
-        put4_n<T>(at + j.cols, j.dst.plane, du, cnt);
+        put8_n<T>(at, j.dst.plane, dg, cnt);
+        put8_n<T>(at + j.cols, j.dst.plane, du, cnt);
         for (int e = 0; e < pad; ++e)
           for (int q = 0; q < Frag<T>::planes; ++q) at[j.cols + cnt + e + q * j.dst.plane] = 0;
       }
     }
   }
   if (!j.part) return;
-  sum[0][w][lane] = ag, sum[1][w][lane] = au;
-  __syncthreads();
-  if (w < 2 && cnt > 0) {
-    f32x4 v = sum[w][0][lane];
-    for (int k = 1; k < 4; ++k) v += sum[w][k][lane];
-    float* d = j.part + ((int64_t)chunk * 2 + w) * j.cols + c;
+  if (w) {
 #pragma unroll
-    for (int k = 0; k < 4; ++k)
-      if (k < cnt) d[k] = v[k];
+    for (int k = 0; k < 8; ++k) sum[0][w - 1][lane + 64 * k] = ag[k], sum[1][w - 1][lane + 64 * k] = au[k];
+  }
+  __syncthreads();
+  if (w || cnt <= 0) return;
+  float* d = j.part + (int64_t)chunk * 2 * j.cols + c;
+#pragma unroll
+  for (int k = 0; k < 8; ++k) {
+    float g = ag[k], u = au[k];
+    for (int v = 0; v < 3; ++v) g += sum[0][v][lane + 64 * k], u += sum[1][v][lane + 64 * k];
+    if (k < cnt) d[k] = g, d[j.cols + k] = u;
   }
 }
 
@@ -205,7 +200,7 @@ fgpu_status launch_prep(const Prep& p, bool f32, hipStream_t s) {
     return j.src ? (int)std::min<int64_t>(ceil_div(j.rows * (whole8(j.cols) / 4), 256), 8192) : 0;
   };
   Blocks n{0, copy_blocks(p.copy[0]), copy_blocks(p.copy[1]), 0, 0};
-  if (p.dz.dy) n.dz = ceil_div(p.dz.cols, kDzCols) * p.dz.chunks;
+  if (p.dz.dy) n.dz = ceil_div(p.dz.cols, p.dz.gated ? 2 * kDzCols : kDzCols) * p.dz.chunks;
   if (p.loss.rows) n.loss = ceil_div(p.loss.nq, 256);
   if (p.loss.owner) n.clear = std::min(ceil_div(p.loss.nc, 1024), 1024);
   const int total = n.dz + n.copy0 + n.copy1 + n.loss + n.clear;
