@@ -30,7 +30,6 @@ __device__ __forceinline__ f32x8 eight(const A& lo, const A& hi, float row, cons
 
 template <class T, int ACT>
 struct GatedEpi {
-  static constexpr bool kStagger = true;
   Finish f;  // bias [2 n], out [m][n], pre [m][2 n], stream
   Scales s;
   int m, n;
@@ -79,11 +78,6 @@ struct GatedEpi {
 // Results of more than the last-level cache's 256 MB go past it (head_gemm.hip has both sides).
 inline bool past_caches(int64_t bytes) { return bytes > (int64_t)256 << 20; }
 
-// Where 256 x 256 tiles, one a CU, come in eight rounds and more: 17 us from the first to the last start, about half a tile of
-// 1024 k (65536 x 4096 x 1024 with both factors kept 1111 -> 1068 us, 8-bit 628 -> 565; 9 us 1078 and 569, 34 us 1084 and
-// 595; two workgroups a CU of 128 x 128 gain nothing).
-inline int stagger_of(const Plan& q) { return q.tile == 256 && (int64_t)q.tiles_m * q.tiles_n >= 8 * 256 ? 64 : 0; }
-
 // n hidden columns over k units (OfInt8: pairs), by the plan of a product of 2 n columns.
 template <int PAIRS, class Num, class T, int ACT>
 fgpu_status run_gated(const GemmArgs& g, int tile, const GatedEpi<T, ACT>& e, hipStream_t s) {
@@ -98,7 +92,7 @@ fgpu_status run_gated(const GemmArgs& g, int tile, const GatedEpi<T, ACT>& e, hi
 template <int PAIRS, class Num, class T>
 fgpu_status run_gated(const GemmOperand& a, const GemmOperand& b, int64_t up, int m, int n, int k, const Plan& q, Finish f,
                       const Scales& sc, hipStream_t s) {
-  const GemmArgs g{a, b, m, n, k, q.tiles_m, q.tiles_n, 1, ceil_div(k, kGemmBK) * kGemmBK, stagger_of(q), up};
+  const GemmArgs g{a, b, m, n, k, q.tiles_m, q.tiles_n, 1, ceil_div(k, kGemmBK) * kGemmBK, up};
   f.stream = past_caches((int64_t)m * n * (f.pre ? 3 : 1) * (int64_t)sizeof(T));
   switch (f.act) {
     case FGPU_ACT_NONE: return run_gated<PAIRS, Num>(g, q.tile, GatedEpi<T, FGPU_ACT_NONE>{f, sc, m, n}, s);

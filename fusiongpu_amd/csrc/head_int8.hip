@@ -125,7 +125,6 @@ fgpu_status quantize(const void* x, int64_t rows, int dim, bool f32, int8_t* q, 
 // ---- the linear layer's epilogue --------------------------------------------------
 template <class T, int ACT>
 struct Int8Epi {
-  static constexpr bool kStagger = true;
   Finish f;
   Scales s;
   int m, n;
@@ -335,7 +334,7 @@ fgpu_status run_layer(const void* x, const float* x_scale, const int8_t* w, cons
   const GemmOperand a{(const uint16_t*)x, ld / 2, 0}, b{(const uint16_t*)w, ld / 2, 0};
   const Scales sc{x_scale, w_scale};
   if (gated) return run_gated<1, OfInt8, T>(a, b, (int64_t)n * b.ld, p.m, n, p.k, q, f, sc, s);
-  const GemmArgs g{a, b, p.m, n, p.k, q.tiles_m, q.tiles_n, 1, ceil_div(p.k, kGemmBK) * kGemmBK, stagger_of(q)};
+  const GemmArgs g{a, b, p.m, n, p.k, q.tiles_m, q.tiles_n, 1, ceil_div(p.k, kGemmBK) * kGemmBK};
   f.stream = past_caches(rows * n * (int64_t)sizeof(T));
   switch (f.act) {
     case FGPU_ACT_NONE: return run_linear(g, q.tile, Int8Epi<T, FGPU_ACT_NONE>{f, sc, p.m, n}, s);

@@ -170,7 +170,6 @@ struct GemmArgs {
   int tiles_m, tiles_n;
   int splits;       // workgroups a tile, each on its own part of k
   int k_per_split;  // a multiple of kGemmBK
-  int stagger = 0;  // see below
   int64_t up = 0;   // gated products: elements from a row of B to the one that its product goes with
 };
 
@@ -642,27 +641,12 @@ __device__ __forceinline__ void gemm_tile(const GemmArgs& g, const Epi& epi, int
   epi.template finish<T>(acc, w, s1, side);
 }
 
-// Epilogues that store much run in step on all CUs where nothing sets them apart: all compute while the memory is idle, then all
-// wait for it.  With `kStagger` the first workgroups of a long grid start one after the other within an XCD, spread over
-// g.stagger sleeps of 640 cycles, and what follows on their CUs stays apart.
-template <class Epi, class = void>
-struct Staggers : std::false_type {};
-template <class Epi>
-struct Staggers<Epi, std::void_t<decltype(Epi::kStagger)>> : std::true_type {};
-template <class Epi>
-__device__ __forceinline__ void stagger(const GemmArgs& g, int wg) {
-  constexpr int kXcd = 8, kCus = 32;
-  if (!g.stagger || wg >= kXcd * kCus) return;
-  for (int n = wg / kXcd * g.stagger / kCus; n > 0; --n) __builtin_amdgcn_s_sleep(10);
-}
-
 // Registers for two waves a SIMD: one workgroup of 256 x 256 a CU, two of 128 x 128.
 template <class T, bool AKC, bool BKC, int PAIRS, class Epi, class Num = OfBf16, int FORM = kPlain>
 __global__ __launch_bounds__(T::threads, 2) void gemm_kernel(GemmArgs g, Epi epi) {
   __shared__ __attribute__((aligned(1024))) char s0[gemm_stage<T, PAIRS>()];
   __shared__ __attribute__((aligned(1024))) char s1[gemm_stage<T, PAIRS>()];
   __shared__ __attribute__((aligned(1024))) char s2[gemm_third<T, PAIRS, AKC && BKC>()];
-  if constexpr (Staggers<Epi>::value) stagger<Epi>(g, blockIdx.x);
   gemm_tile<T, AKC, BKC, PAIRS, Num, FORM>(g, epi, blockIdx.x, gridDim.x, s0, s1, s2);
 }
 
