@@ -203,20 +203,20 @@ __global__ __launch_bounds__(256) void triangle_join_kernel(OrthoFinish f, const
 // ends are zeros), as in head_direct.hpp; the partial tiles meet in LDS.  One launch, no parts in memory.
 constexpr int kFewTile = 32, kFewBK = 32;
 inline int few_waves(int k) { return k > 512 ? 16 : 8; }
-template <int PAIRS, bool KC, bool ISB>
+template <int PAIRS, bool KC, bool ISB, int F = 2>
 struct FewRead {
-  static constexpr int P = planes_of(PAIRS), lds_bytes = KC ? 0 : P * kFewBK * kFewTile * 2;
-  bf16x8 r[P][2];
+  static constexpr int P = planes_of(PAIRS), lds_bytes = KC ? 0 : P * kFewBK * F * 32;
+  bf16x8 r[P][F];
   __device__ __forceinline__ void load(const Planes& o, int r0, int nr, int k0, int nk, int lane) {
 #pragma unroll
-    for (int i = 0; i < 2; ++i) {
+    for (int i = 0; i < F; ++i) {
       int64_t at;
       bool in;
       if constexpr (KC) {
         const int l = lane & 15, row = r0 + (ISB ? 8 * (l >> 2) + 4 * i + (l & 3) : 16 * i + l), k = k0 + 8 * (lane >> 4);
         at = row * o.ld + k, in = row < nr && k < nk;
       } else {
-        const int t = lane + kWave * i, k = k0 + t / 4, col = r0 + t % 4 * 8;
+        const int t = lane + kWave * i, k = k0 + t / (2 * F), col = r0 + t % (2 * F) * 8;
         at = k * o.ld + col, in = k < nk && col < nr;
       }
 #pragma unroll
@@ -225,24 +225,26 @@ struct FewRead {
     }
   }
   // Strided: through the wave's own LDS and its transposing load.
-  __device__ __forceinline__ void frags(bf16x8 (&f)[2][P], char* lds, int lane) const {
+  __device__ __forceinline__ void frags(bf16x8 (&f)[F][P], char* lds, int lane) const {
     if constexpr (KC) {
 #pragma unroll
-      for (int p = 0; p < P; ++p) f[0][p] = r[p][0], f[1][p] = r[p][1];
+      for (int p = 0; p < P; ++p)
+#pragma unroll
+        for (int i = 0; i < F; ++i) f[i][p] = r[p][i];
     } else {
       typedef __attribute__((address_space(3))) s16x4 lds_half;
-      constexpr int row_bytes = kFewTile * 2;
+      constexpr int row_bytes = F * 32;
       wave_lds_order();
 #pragma unroll
       for (int p = 0; p < P; ++p)
 #pragma unroll
-        for (int i = 0; i < 2; ++i) *reinterpret_cast<bf16x8*>(lds + p * kFewBK * row_bytes + (lane + kWave * i) * 16) = r[p][i];
+        for (int i = 0; i < F; ++i) *reinterpret_cast<bf16x8*>(lds + p * kFewBK * row_bytes + (lane + kWave * i) * 16) = r[p][i];
       wave_lds_order();
       const int l = lane & 15, g = lane >> 4;
 #pragma unroll
       for (int p = 0; p < P; ++p)
 #pragma unroll
-        for (int i = 0; i < 2; ++i) {
+        for (int i = 0; i < F; ++i) {
           char* at = lds + (p * kFewBK + 8 * g + (l >> 2)) * row_bytes + (ISB ? (l & 3) * 16 + i * 8 : i * 32 + (l & 3) * 8);
           const s16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_half*)(lds_char*)at);
           const s16x4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_half*)(lds_char*)(at + 4 * row_bytes));
@@ -253,27 +255,27 @@ struct FewRead {
     }
   }
 };
-template <class T, int PAIRS, bool AKC, bool BKC, int kFewWaves>
+template <class T, int PAIRS, bool AKC, bool BKC, int kFewWaves, int FM>
 __global__ __launch_bounds__(kFewWaves * kWave) void few_tiles_kernel(Planes a, Planes b, int k, OrthoFinish f) {
-  using RA = FewRead<PAIRS, AKC, false>;
+  using RA = FewRead<PAIRS, AKC, false, FM>;
   using RB = FewRead<PAIRS, BKC, true>;
-  constexpr int stage = kFewWaves * (RA::lds_bytes + RB::lds_bytes), joined = kFewWaves * 4 * kWave * 16;
+  constexpr int stage = kFewWaves * (RA::lds_bytes + RB::lds_bytes), joined = kFewWaves * FM * 2 * kWave * 16;
   __shared__ __attribute__((aligned(1024))) char lds[stage > joined ? stage : joined];
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int across = (f.n + kFewTile - 1) / kFewTile;
-  const int m0 = blockIdx.x / across * kFewTile, n0 = blockIdx.x % across * kFewTile;
+  const int m0 = blockIdx.x / across * 16 * FM, n0 = blockIdx.x % across * kFewTile;
   const int steps = (k + kFewBK - 1) / kFewBK, per = (steps + kFewWaves - 1) / kFewWaves;
   const int s0 = wave * per, s1 = min(steps, s0 + per);
   char* la = lds + wave * (RA::lds_bytes + RB::lds_bytes);
-  f32x4 acc[2][2];
+  f32x4 acc[2][FM];
 #pragma unroll
-  for (int i = 0; i < 2; ++i) acc[i][0] = acc[i][1] = f32x4{0, 0, 0, 0};
+  for (int j = 0; j < FM; ++j) acc[0][j] = acc[1][j] = f32x4{0, 0, 0, 0};
   auto work = [&](const RA& ra, const RB& rb) {
-    bf16x8 fa[2][RA::P], fb[2][RB::P];
+    bf16x8 fa[FM][RA::P], fb[2][RB::P];
     ra.frags(fa, la, lane);
     rb.frags(fb, la + RA::lds_bytes, lane);
 #pragma unroll
-    for (int j = 0; j < 2; ++j)
+    for (int j = 0; j < FM; ++j)
 #pragma unroll
       for (int i = 0; i < 2; ++i)
 #pragma unroll
@@ -296,17 +298,17 @@ __global__ __launch_bounds__(kFewWaves * kWave) void few_tiles_kernel(Planes a, 
   __syncthreads();
   f32x4* join = reinterpret_cast<f32x4*>(lds);  // [wave][row fragment][column fragment][lane]
 #pragma unroll
-  for (int j = 0; j < 2; ++j)
+  for (int j = 0; j < FM; ++j)
 #pragma unroll
-    for (int i = 0; i < 2; ++i) join[((wave * 2 + j) * 2 + i) * kWave + lane] = acc[i][j];
+    for (int i = 0; i < 2; ++i) join[((wave * FM + j) * 2 + i) * kWave + lane] = acc[i][j];
   __syncthreads();
-  if (threadIdx.x >= 2 * kWave) return;
+  if (threadIdx.x >= FM * kWave) return;
   const int j = threadIdx.x / kWave, row = m0 + 16 * j + (lane & 15), col = n0 + 8 * (lane >> 4);
   f32x8 v{{0, 0, 0, 0}, {0, 0, 0, 0}};
 #pragma unroll
   for (int w = 0; w < kFewWaves; ++w) {
-    v.lo += join[((w * 2 + j) * 2) * kWave + lane];
-    v.hi += join[((w * 2 + j) * 2 + 1) * kWave + lane];
+    v.lo += join[((w * FM + j) * 2) * kWave + lane];
+    v.hi += join[((w * FM + j) * 2 + 1) * kWave + lane];
   }
   if (row < f.m && col < ((f.n + 7) & ~7)) f.put<T>(v, row, col);
 }
@@ -341,7 +343,8 @@ double few_us(int m, int n, int k, int pairs, int strided) {
   const int steps = ceil_div(ceil_div(k, kFewBK), few_waves(k));
   const double all = (double)ceil_div(m, kFewTile) * ceil_div(n, kFewTile) * steps / 256;
   const double more = few_waves(k) == 16 ? 1.75 : 1;
-  const double alone = (strided == 2 ? 0.42 : strided ? 0.5 : 0.6) * more;
+  const double half = ceil_div(m, 16) * (int64_t)ceil_div(n, kFewTile) <= 256 ? 0.7 : 1;
+  const double alone = (strided == 2 ? 0.42 : strided ? 0.5 : 0.6) * more * half;
   const double shared = (strided == 2 ? 0.65 : strided ? 0.83 : 1.09) * more;
   return 2.6 + std::max(steps * alone, all * shared) * (pairs == 1 ? 1 : 1.9);
 }
@@ -392,9 +395,16 @@ fgpu_status run_cut(const GemmArgs& g, int tile, int grid, const E& e, hipStream
 template <class T, int PAIRS, bool AKC, bool BKC>
 fgpu_status run_whole(const Planes& a, const Planes& b, int k, const OrthoFinish& f, const Cut& q, hipStream_t s) {
   if (q.tile == kFewTile) {
-    const int tiles = ceil_div(f.m, kFewTile) * ceil_div(f.n, kFewTile);
-    if (few_waves(k) == 16) few_tiles_kernel<T, PAIRS, AKC, BKC, 16><<<tiles, 16 * kWave, 0, s>>>(a, b, k, f);
-    else few_tiles_kernel<T, PAIRS, AKC, BKC, 8><<<tiles, 8 * kWave, 0, s>>>(a, b, k, f);
+    // Half the rows a workgroup while that leaves CUs without one.
+    const int across = ceil_div(f.n, kFewTile);
+    const bool half = ceil_div(f.m, 16) * across <= 256, many = few_waves(k) == 16;
+    auto go = [&](auto waves, auto fm) {
+      constexpr int W = decltype(waves)::value, FM = decltype(fm)::value;
+      few_tiles_kernel<T, PAIRS, AKC, BKC, W, FM><<<ceil_div(f.m, 16 * FM) * across, W * kWave, 0, s>>>(a, b, k, f);
+    };
+    using std::integral_constant;
+    if (many) half ? go(integral_constant<int, 16>{}, integral_constant<int, 1>{}) : go(integral_constant<int, 16>{}, integral_constant<int, 2>{});
+    else half ? go(integral_constant<int, 8>{}, integral_constant<int, 1>{}) : go(integral_constant<int, 8>{}, integral_constant<int, 2>{});
     FGPU_HIP(hipGetLastError());
     return FGPU_OK;
   }
