@@ -191,7 +191,7 @@ struct Plan {
   int tile, tiles_m, tiles_n, splits, k_per_split;
   double us;
 };
-Plan plan_product(const Product& p, bool may_split);
+Plan plan_product(const Product& p, bool may_split, int only_tile = 0);
 // One product and where its result goes.
 struct ProductJob {
   Product p;

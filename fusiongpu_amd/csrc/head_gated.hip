@@ -4,6 +4,7 @@
 // 32 of Wu that belong to the same hidden columns (GatedTileLoad), so a lane's accumulators hold g and u of the same
 // columns and act(g) u is formed before anything is stored.
 #include <algorithm>
+#include <cmath>
 
 #include "gated.hpp"
 
@@ -11,6 +12,133 @@ namespace fgpu {
 namespace {
 
 constexpr int kMaxHidden = FGPU_HEAD_MAX_DIM / 2;
+
+// ---- float32, planes formed on the way to LDS -----------------------------------------
+// Mid-size float32 layers: a launch that copies both operands into planes first costs as much as a third of the product, and what
+// it wrote comes back through other XCDs' caches.  Here a thread loads eight values of a row as they lie (any alignment),
+// two steps ahead, splits them in registers and writes the three planes; each value is split once a tile instead of once.
+struct SplitJob32 {
+  const float* x;
+  const float* w;
+  int m, n, k;
+  int tiles_n;
+};
+struct Eight {
+  f32x8 v;
+  // Eight values of row `row` from k on; zeros outside.
+  __device__ __forceinline__ void load(const float* p, int64_t row, bool in, int k, int nk) {
+    v = f32x8{{0, 0, 0, 0}, {0, 0, 0, 0}};
+    if (in && k < nk) v = load8_n(p + row * nk + k, nk - k);
+  }
+};
+template <class T, int ACT>
+__global__ __launch_bounds__(T::threads, 2) void gated_split_kernel(SplitJob32 j, GatedEpi<float, ACT> epi) {
+  constexpr int B = kPlanesBK, pa = T::BM * B * 2, pb = T::BN * B * 2, kb = T::BN * 4 / T::threads;
+  static_assert(T::BM * 4 == T::threads && kb * T::threads == T::BN * 4, "whole chunks a thread");
+  __shared__ __attribute__((aligned(1024))) char s0[3 * (pa + pb)];
+  __shared__ __attribute__((aligned(1024))) char s1[3 * (pa + pb)];
+  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int wm = wave / T::WN, wn = wave % T::WN;
+  GemmArgs g{};
+  g.tiles_n = j.tiles_n, g.tiles_m = gridDim.x / j.tiles_n;
+  int tm, tn, sp;
+  gemm_tile_of(g, blockIdx.x, gridDim.x, tm, tn, sp);
+  const int m0 = tm * T::BM, n0 = tn * (T::BN / 2), chunk = tid & 3, row = tid >> 2;
+  TileRead<T::BM, true, false, B> ra;
+  TileRead<T::BN, true, true, B> rb;
+  ra.init(lane, wm * (T::BM / T::WM));
+  rb.init(lane, wn * (T::BN / T::WN));
+  struct Stage {
+    Eight a, b[kb];
+  };
+  auto load = [&](Stage& t, int k) {
+    t.a.load(j.x, m0 + row, m0 + row < j.m, k + chunk * 8, j.k);
+#pragma unroll
+    for (int i = 0; i < kb; ++i) {
+      const int r = row + i * (T::threads / 4), h = n0 + (r >> 6) * 32 + (r & 31);
+      t.b[i].load(j.w, (r & 32) ? (int64_t)h + j.n : h, h < j.n, k + chunk * 8, j.k);
+    }
+  };
+  auto put = [&](char* at, int plane, const Eight& e) {
+    bf16x8 p[3];
+    split8(e.v, p[0], p[1], p[2]);
+#pragma unroll
+    for (int q = 0; q < 3; ++q) *reinterpret_cast<bf16x8*>(at + q * plane) = p[q];
+  };
+  auto store = [&](const Stage& t, char* s) {
+    put(s + row * (B * 2) + (chunk ^ tile_swizzle<true, false, 4>(row)) * 16, pa, t.a);
+#pragma unroll
+    for (int i = 0; i < kb; ++i) {
+      const int r = row + i * (T::threads / 4);
+      put(s + 3 * pa + r * (B * 2) + (chunk ^ tile_swizzle<true, true, 4>(r)) * 16, pb, t.b[i]);
+    }
+  };
+  f32x4 acc[T::FN][T::FM];
+#pragma unroll
+  for (int i = 0; i < T::FN; ++i)
+#pragma unroll
+    for (int q = 0; q < T::FM; ++q) acc[i][q] = f32x4{0, 0, 0, 0};
+  auto work = [&](const char* s) {
+    bf16x8 a[T::FM][3], b[T::FN][3];
+#pragma unroll
+    for (int p = 0; p < 3; ++p) {
+#pragma unroll
+      for (int i = 0; i < T::FN; ++i) b[i][p] = rb.get((const lds_char*)s + 3 * pa + p * pb, i, 0);
+#pragma unroll
+      for (int q = 0; q < T::FM; ++q) a[q][p] = ra.get((const lds_char*)s + p * pa, q, 0);
+    }
+#pragma unroll
+    for (int q = 0; q < T::FM; ++q)
+#pragma unroll
+      for (int i = 0; i < T::FN; ++i)
+#pragma unroll
+        for (int c = 0; c < 6; ++c) acc[i][q] = OfBf16::mma(b[i][pair_b(c)], a[q][pair_a(c)], acc[i][q]);
+  };
+  // Behind the barrier of step i its planes are in `cur`, nobody reads `other`, and the values of i + 1 and i + 2 are on the way.
+  Stage t0, t1;
+  load(t0, 0);
+  load(t1, B);
+  store(t0, s0);
+  load(t0, 2 * B);
+  for (int k = 0; k < j.k; k += 2 * B) {
+    __syncthreads();
+    work(s0);
+    if (k + B >= j.k) break;
+    store(t1, s1);
+    load(t1, k + 3 * B);
+    __syncthreads();
+    work(s1);
+    store(t0, s0);
+    load(t0, k + 4 * B);
+  }
+  const GemmWave<T> w{m0, n0, tm, tn, 0, wm, wn, lane, s1};
+  epi.template finish<T>(acc, w, s1, typename GatedEpi<float, ACT>::template Side<T>{});
+}
+using WideSplitTile = GemmTile<64, 128, 2, 2>;
+template <class T>
+fgpu_status run_split(SplitJob32 j, const Finish& f, hipStream_t s) {
+  j.tiles_n = ceil_div(j.n, T::BN / 2);
+  auto go = [&](auto act) {
+    constexpr int ACT = decltype(act)::value;
+    gated_split_kernel<T, ACT><<<ceil_div(j.m, T::BM) * j.tiles_n, T::threads, 0, s>>>(j, GatedEpi<float, ACT>{f, {}, j.m, j.n});
+  };
+  using std::integral_constant;
+  switch (f.act) {
+    case FGPU_ACT_NONE: go(integral_constant<int, FGPU_ACT_NONE>{}); break;
+    case FGPU_ACT_RELU: go(integral_constant<int, FGPU_ACT_RELU>{}); break;
+    case FGPU_ACT_GELU: go(integral_constant<int, FGPU_ACT_GELU>{}); break;
+    default: go(integral_constant<int, FGPU_ACT_SILU>{});
+  }
+  FGPU_HIP(hipGetLastError());
+  return FGPU_OK;
+}
+// Microseconds, fitted over 100 to 8000 rows, 96 to 2048 hidden and 96 to 2048 k: a step of 32 k of a workgroup alone on its CU,
+// and of each of several.
+double split_us(int m, int n, int k, int width) {
+  const int64_t each = ceil_div((int64_t)ceil_div(m, 64) * ceil_div(n, width / 2), 256);
+  const double alone = width == 64 ? 0.72 : 1.08, shared = width == 64 ? 0.56 : 0.88;
+  return 3.3 + ceil_div(k, kPlanesBK) * (each == 1 ? alone : each * shared);
+}
 
 fgpu_status check_common(int64_t rows, int in_dim, int hidden, int dtype, int act) {
   FGPU_CHECK(dtype == FGPU_DTYPE_F32 || dtype == FGPU_DTYPE_BF16, FGPU_ERR_ARG, "gated linear: unknown dtype");
@@ -22,11 +150,32 @@ fgpu_status check_common(int64_t rows, int in_dim, int hidden, int dtype, int ac
 }
 bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
 
-// Between the kernel of few tiles and the tiled ones, by the estimates that the linear layer of 2 hidden columns goes by.
-bool forward_direct(const Product& p, const Plan& q) {
-  double tiled = q.us;
-  if (needs_pack(p.k, p.f32)) tiled += 5.7 + ((double)p.m + p.n) * p.k * (p.f32 ? 10 : 4) / 4e6;
-  return !q.tile || direct_forward_estimate_us(p) < tiled;
+// Which kernel a forward call takes, by estimates: that of few tiles, tiles whose planes are formed on the way (float32), or tiles
+// of operands as they are or packed (a launch more).  us, few / on the way / packed: float32 1000 x 771 x 385 (rows, hidden, in)
+// - / 18.8 / 25.9, 2000 x 771 x 385 - / 26.6 / 42.7, 300 x 771 x 1024 20.6 / 26.7 / -, 4000 x 2048 x 1024 - / 202 / 167.
+struct Choice {
+  bool direct = false;
+  int split = 0;  // the width of its tiles
+  Plan plan;
+};
+Choice choose(int m, int n, int k, bool f32) {
+  const Product p{m, 2 * n, k, f32};
+  Choice c;
+  c.plan = plan_product(p, false, f32 ? 256 : 0);
+  if (f32) {  // packed tiles of 128 are faster nowhere
+    const Plan q = plan_product(p, false, 64);
+    if (!c.plan.tile || (q.tile && q.us < c.plan.us)) c.plan = q;
+  }
+  double us = c.plan.tile ? c.plan.us : INFINITY;
+  if (needs_pack(k, f32)) us += 5.7 + ((double)p.m + p.n) * k * (f32 ? 10 : 4) / 4e6;
+  if (f32 && (int64_t)ceil_div(m, 64) * ceil_div(n, 32) * GatedTile64::threads < kLaunchThreads) {
+    for (int width : {64, 128}) {
+      const double t = split_us(m, n, k, width);
+      if (t < us) us = t, c.split = width;
+    }
+  }
+  if (direct_forward_estimate_us(p) < us) c.direct = true, c.split = 0;
+  return c;
 }
 
 }  // namespace
@@ -38,16 +187,16 @@ extern "C" {
 
 int fgpu_gated_linear_tile(int64_t rows, int in_dim, int hidden, int dtype) {
   if (check_common(rows, in_dim, hidden, dtype, 0) != FGPU_OK || rows == 0) return -1;
-  const Product p{(int)rows, 2 * hidden, in_dim, dtype == FGPU_DTYPE_F32};
-  const Plan q = plan_product(p, false);
-  return forward_direct(p, q) ? 0 : q.tile;
+  const Choice c = choose((int)rows, hidden, in_dim, dtype == FGPU_DTYPE_F32);
+  return c.direct ? 0 : c.split ? c.split + FGPU_TILE_SPLIT : c.plan.tile ? c.plan.tile : -1;
 }
 
 size_t fgpu_gated_linear_workspace_bytes(int64_t rows, int in_dim, int hidden, int dtype) {
   if (check_common(rows, in_dim, hidden, dtype, 0) != FGPU_OK || rows == 0) return 0;
   const bool f32 = dtype == FGPU_DTYPE_F32;
-  const Product p{(int)rows, 2 * hidden, in_dim, f32};
-  if (!needs_pack(in_dim, f32) || forward_direct(p, plan_product(p, false))) return 0;
+  if (!needs_pack(in_dim, f32)) return 0;
+  const Choice c = choose((int)rows, hidden, in_dim, f32);
+  if (c.direct || c.split) return 0;
   return packed_bytes(rows, in_dim, f32) + packed_bytes(2 * hidden, in_dim, f32);
 }
 
@@ -61,16 +210,21 @@ fgpu_status fgpu_gated_linear(const void* d_x, const void* d_w, const void* d_bi
              "gated linear: x, weight and workspace must be 16-byte aligned");
   const bool f32 = dtype == FGPU_DTYPE_F32;
   hipStream_t s = as_stream(stream);
-  const Product p{(int)rows, 2 * hidden, in_dim, f32};
-  const Plan q = plan_product(p, false);
+  const int m = (int)rows;
+  const Choice c = choose(m, hidden, in_dim, f32);
   Finish f;
   f.bias = d_bias, f.out = d_h, f.pre = d_pre, f.act = act;
-  if (forward_direct(p, q)) {
-    DirectJob j{{d_x, in_dim, rows * in_dim, nullptr}, {d_w, in_dim, (int64_t)2 * hidden * in_dim, nullptr}, p.m, hidden, in_dim,
-                0, f, nullptr};
+  if (c.direct) {
+    DirectJob j{{d_x, in_dim, rows * in_dim, nullptr}, {d_w, in_dim, (int64_t)2 * hidden * in_dim, nullptr}, m, hidden, in_dim, 0, f,
+                nullptr};
     j.b.up = hidden;
     return launch_direct_gated(j, f32, s);
   }
+  if (c.split) {
+    const SplitJob32 j{(const float*)d_x, (const float*)d_w, m, hidden, in_dim, 0};
+    return c.split == 64 ? run_split<GatedTile64>(j, f, s) : run_split<WideSplitTile>(j, f, s);
+  }
+  FGPU_CHECK(c.plan.tile, FGPU_ERR_UNSUPPORTED, "gated linear: more tiles than one launch takes (2^39 results)");
   Carve ws(d_workspace, workspace_bytes);
   GemmOperand a = as_is(d_x, in_dim), b = as_is(d_w, in_dim);
   Prep prep;
@@ -82,8 +236,8 @@ fgpu_status fgpu_gated_linear(const void* d_x, const void* d_w, const void* d_bi
   }
   FGPU_CHECK(ws.held(), FGPU_ERR_WORKSPACE, "gated linear: workspace smaller than fgpu_gated_linear_workspace_bytes");
   FGPU_TRY(launch_prep(prep, f32, s));
-  if (f32) return run_gated<6, OfBf16, float>(a, b, hidden * b.ld, p.m, hidden, in_dim, q, f, {}, s);
-  return run_gated<1, OfBf16, bf16>(a, b, hidden * b.ld, p.m, hidden, in_dim, q, f, {}, s);
+  if (f32) return run_gated<6, OfBf16, float>(a, b, hidden * b.ld, m, hidden, in_dim, c.plan, f, {}, s);
+  return run_gated<1, OfBf16, bf16>(a, b, hidden * b.ld, m, hidden, in_dim, c.plan, f, {}, s);
 }
 
 size_t fgpu_gated_linear_backward_workspace_bytes(int64_t rows, int in_dim, int hidden, int dtype) {

@@ -366,7 +366,7 @@ fgpu_status launch_join(const SplitJob& a, const SplitJob& b, const ColumnSum* s
   return FGPU_OK;
 }
 
-Plan plan_product(const Product& p, bool may_split) { return plan_of(p, 0, may_split); }
+Plan plan_product(const Product& p, bool may_split, int only_tile) { return plan_of(p, only_tile, may_split); }
 
 size_t products_workspace_bytes(const Product* p, int count) {
   Plan q[2];

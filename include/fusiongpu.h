@@ -666,7 +666,9 @@ size_t fgpu_gated_linear_backward_workspace_bytes(int64_t rows, int in_dim, int 
 fgpu_status fgpu_gated_linear_backward(const void* d_dh, const void* d_x, const void* d_w, const void* d_pre, int64_t rows,
                                        int in_dim, int hidden, int dtype, int act, void* d_dx, void* d_dw, void* d_db,
                                        void* d_workspace, size_t workspace_bytes, void* stream);
-/* As fgpu_linear_tile, of the forward product. */
+/* As fgpu_linear_tile, of the forward product; plus FGPU_TILE_SPLIT where float32
+ * operands become planes inside the product's kernel. */
+#define FGPU_TILE_SPLIT 2048
 int fgpu_gated_linear_tile(int64_t rows, int in_dim, int hidden, int dtype);
 
 /* Rows as 8-bit integers with a scale each: with m the largest magnitude of a

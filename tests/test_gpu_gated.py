@@ -92,11 +92,13 @@ def test_activations(act, dt, m):
 def test_every_tile(act, dt):
     """A size that takes each kernel, with rows and columns that end inside a tile and a k that ends inside a step."""
     seen = set()
-    sizes = [(15, 200, 70), (70, 200, 100), (1500, 200, 999), (2500, 72, 700), (5000, 328, 1030), (20000, 72, 1030), (3000, 520, 1000)]
+    sizes = [(15, 200, 70), (70, 200, 100), (1500, 200, 999), (2500, 72, 700), (5000, 328, 1030), (20000, 72, 1030), (3000, 520, 1000),
+             (960, 643, 577), (4555, 291, 1556)]
     for m, k, n in sizes:
         seen.add(fg.lib.fgpu_gated_linear_tile(m, k, n, int(dt == "bf16")))
         check_gated(m, k, n, dt, act, True, True, seed=m)
-    assert seen >= {0, 64, 128, 256}, seen
+    split = 2048  # planes formed on the way: 64 and 128 wide
+    assert seen >= ({0, 64, 256, split + 64, split + 128} if dt == "f32" else {0, 64, 128, 256}), seen
 
 
 @pytest.mark.parametrize("dt", ["f32", "bf16"])
