@@ -16,14 +16,14 @@ struct Scales {
   const float* row = nullptr;
   const float* col = nullptr;
 };
-// Eight columns of a row from two fragments' accumulators, scaled where they are integers.
+// Eight columns of a row from two fragments' accumulators, scaled where they are integers, with the bias.
 template <class A>
-__device__ __forceinline__ f32x8 eight(const A& lo, const A& hi, float row, const f32x8& col) {
+__device__ __forceinline__ f32x8 eight(const A& lo, const A& hi, float row, const f32x8& col, const f32x8& bias) {
   f32x8 v;
 #pragma unroll
   for (int e = 0; e < 8; ++e) {
-    if constexpr (std::is_same_v<A, i32x4>) v.set(e, (float)(e < 4 ? lo[e] : hi[e - 4]) * row * col[e]);
-    else v.set(e, e < 4 ? lo[e] : hi[e - 4]);
+    if constexpr (std::is_same_v<A, i32x4>) v.set(e, fmaf((float)(e < 4 ? lo[e] : hi[e - 4]) * col[e], row, bias[e]));
+    else v.set(e, (e < 4 ? lo[e] : hi[e - 4]) + bias[e]);
   }
   return v;
 }
@@ -89,8 +89,7 @@ struct GatedEpi {
         const int64_t row = w.row(j);
         if (row >= m) continue;
         const float sr = kInt ? s.row[row] : 1.0f;
-        f32x8 g = eight(acc[4 * q][j], acc[4 * q + 1][j], sr, sg), u = eight(acc[4 * q + 2][j], acc[4 * q + 3][j], sr, su);
-        g.lo += bg.lo, g.hi += bg.hi, u.lo += bu.lo, u.hi += bu.hi;
+        f32x8 g = eight(acc[4 * q][j], acc[4 * q + 1][j], sr, sg, bg), u = eight(acc[4 * q + 2][j], acc[4 * q + 3][j], sr, su, bu);
         if (f.pre) {
           T* pre = (T*)f.pre + row * 2 * n + c;
           store8_n<STREAM>(pre, g, cnt);
@@ -123,8 +122,8 @@ struct GatedEpi {
       f32x8 g[2], u[2];
 #pragma unroll
       for (int q = 0; q < 2; ++q) {
-        g[q] = eight(acc[4 * q][j], acc[4 * q + 1][j], sr, sg[q]), u[q] = eight(acc[4 * q + 2][j], acc[4 * q + 3][j], sr, su[q]);
-        g[q].lo += bg[q].lo, g[q].hi += bg[q].hi, u[q].lo += bu[q].lo, u[q].hi += bu[q].hi;
+        g[q] = eight(acc[4 * q][j], acc[4 * q + 1][j], sr, sg[q], bg[q]);
+        u[q] = eight(acc[4 * q + 2][j], acc[4 * q + 3][j], sr, su[q], bu[q]);
       }
       if (f.pre) {
         T* pre = (T*)f.pre + row * 2 * n + c;

@@ -13,41 +13,63 @@ inline int int8_row(int dim) { return FGPU_INT8_ROW(dim); }
 bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
 
 // ---- rounding ------------------------------------------------------------------
-// The quotient is rounded as the real number it is: n = rint of an approximate one, then compared with the borders, x 127
-// against (n +- 1/2) max, in terms that are exact.  Both are scaled by the maximum's power of two first, so that nothing
-// overflows; of float32 operands the products' low parts (t) are kept.  With n right or one beside, d = 127 x - n max is
-// exact, and so is |d| - max / 2 where the two are close.
+// The quotient x 127 / max is rounded as the real number it is.  n, from a product with 127 / max rounded, is the nearest whole
+// number or, beside a border between two, one of both; d = 127 x - n max says which: it is exact (of float32 operands its low
+// part t is kept apart), and n is right unless 2 |d| > max, or 2 |d| = max and n is odd.  Few groups of eight hold a value so
+// near a border (float32: one in 2000; bfloat16, mostly ties with half the maximum: one in 30 to 300): the others take one
+// multiplication, a fused one that adds 1.5 2^23 and so leaves n in the sum's low bits, and two to see that.
 template <class T>
 struct Rounder {
-  float top, per;  // the maximum scaled to [1/2, 1); 127 / top
-  int exp;         // its power of two
-  float scale;     // what q is multiplied by to stand for x
-  bool live;       // not all zeros, nothing infinite or NaN
+  static constexpr float kWhole = 12582912.0f;  // 1.5 2^23
+  float most;   // the largest magnitude, scaled into [1/2, 1) where it lies near an end of the type
+  float per;    // 127 / most
+  float near;   // |d| below it: n is right
+  float scale;  // what q is multiplied by to stand for x
+  int exp;      // the power of two that x is scaled by
   // bits: those of the largest magnitude.  A row that holds something not finite has a NaN scale and zeros.
   __device__ __forceinline__ explicit Rounder(uint32_t bits) {
-    const float most = __uint_as_float(bits);
-    live = bits != 0 && bits < 0x7f800000u;
-    scale = bits < 0x7f800000u ? most / 127.0f : __uint_as_float(0x7fc00000u);
-    exp = __builtin_amdgcn_frexp_expf(most);
-    top = live ? ldexpf(most, -exp) : 1.0f;
-    per = 127.0f / top;
+    const float top = __uint_as_float(bits);
+    const bool live = bits != 0 && bits < 0x7f800000u;
+    scale = bits < 0x7f800000u ? top / 127.0f : __uint_as_float(0x7fc00000u);
+    exp = live && (top < 0x1p-100f || top > 0x1p100f) ? -__builtin_amdgcn_frexp_expf(top) : 0;
+    most = exp ? ldexpf(top, exp) : top;
+    per = live ? 127.0f / most : 0.0f;
+    near = sizeof(T) == 4 ? 0.4999f * most : 0.5f * most;
+    if (!live) most = near = INFINITY;  // every d is far below, and every n of 0 x right, but for what is not finite itself
   }
-  __device__ __forceinline__ int round(float x) const {
-    const float v = ldexpf(x, -exp), h = 127.0f * v;
-    float n = rintf(v * per);
-    const float p = n * top, d = h - p;
-    float over = fabsf(d) - 0.5f * top;
-    if constexpr (sizeof(T) == 4) {
-      const float t = fmaf(127.0f, v, -h) - fmaf(n, top, -p);
-      over += d < 0 ? -t : t;
+  __device__ __forceinline__ u32x2 round8(f32x8 x) const {
+    if (exp) {
+#pragma unroll
+      for (int e = 0; e < 8; ++e) x.set(e, ldexpf(x[e], exp));
     }
-    const int i = (int)n;
-    const bool move = over > 0 || (over == 0 && (i & 1));
-    return live ? i + (move ? (d < 0 ? -1 : 1) : 0) : 0;
-  }
-  __device__ __forceinline__ uint32_t round4(float a, float b, float c, float d) const {
-    return (uint32_t)(round(a) & 255) | (uint32_t)(round(b) & 255) << 8 | (uint32_t)(round(c) & 255) << 16 |
-           (uint32_t)round(d) << 24;
+    float n[8], d[8], far = 0;
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+      n[e] = fmaf(x[e], per, kWhole);
+      d[e] = fmaf(kWhole - n[e], most, 127.0f * x[e]);
+      far = fmaxf(far, fabsf(d[e]));
+    }
+    if (far >= near) {
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        float over = fabsf(d[e]) - 0.5f * most;
+        if constexpr (sizeof(T) == 4) {  // d again, from both parts of both products
+          const float h = 127.0f * x[e], w = n[e] - kWhole, p = w * most, c = h - p;
+          const float t = fmaf(127.0f, x[e], -h) - fmaf(w, most, -p);
+          over = fabsf(c) - 0.5f * most + (c < 0 ? -t : t);
+        }
+        const bool move = over > 0 || (over == 0 && (__float_as_uint(n[e]) & 1));
+        if (move) n[e] += d[e] < 0 ? -1.0f : 1.0f;
+      }
+    }
+    u32x2 out;
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {  // the low bytes
+      const uint32_t a = __builtin_amdgcn_perm(__float_as_uint(n[4 * h + 1]), __float_as_uint(n[4 * h]), 0x0c0c0400u);
+      const uint32_t b = __builtin_amdgcn_perm(__float_as_uint(n[4 * h + 3]), __float_as_uint(n[4 * h + 2]), 0x04000c0cu);
+      out[h] = a | b;
+    }
+    return out;
   }
 };
 __device__ __forceinline__ uint32_t most_bits(uint32_t m, const f32x8& v) {
@@ -96,7 +118,7 @@ __global__ __launch_bounds__(256) void quantize_kernel(const T* x, int64_t rows,
     if (at == 0) scale[r] = k.scale;
     int8_t* to = q + r * width;
     auto put = [&](int c, const f32x8& v) {
-      *reinterpret_cast<u32x2*>(to + c) = u32x2{k.round4(v[0], v[1], v[2], v[3]), k.round4(v[4], v[5], v[6], v[7])};
+      *reinterpret_cast<u32x2*>(to + c) = k.round8(v);
     };
 #pragma unroll
     for (int i = 0; i < kHeld; ++i) {
@@ -150,8 +172,7 @@ struct Int8Epi {
       for (int j = 0; j < G::FM; ++j) {
         const int64_t row = w.row(j);
         if (row >= m) continue;
-        f32x8 v = eight(acc[2 * p][j], acc[2 * p + 1][j], s.row[row], sc);
-        v.lo += bias.lo, v.hi += bias.hi;
+        f32x8 v = eight(acc[2 * p][j], acc[2 * p + 1][j], s.row[row], sc, bias);
         if (ACT != FGPU_ACT_NONE) {
 #pragma unroll
           for (int e = 0; e < 8; ++e) v.set(e, act_value<T>(v[e], ACT));
@@ -238,11 +259,8 @@ __global__ __launch_bounds__(kFewThreads) void few_rows_kernel(FewJob j) {
     const Rounder<T> q(top);
     if (tid < 16) row_scale[tid] = q.scale;
     auto whole = [&](const f32x8 (&v)[2]) {
-      i32x4 r;
-#pragma unroll
-      for (int h = 0; h < 4; ++h)
-        r[h] = (int)q.round4(v[h / 2][h % 2 * 4], v[h / 2][h % 2 * 4 + 1], v[h / 2][h % 2 * 4 + 2], v[h / 2][h % 2 * 4 + 3]);
-      return r;
+      const u32x2 lo = q.round8(v[0]), hi = q.round8(v[1]);
+      return i32x4{(int)lo[0], (int)lo[1], (int)hi[0], (int)hi[1]};
     };
 #pragma unroll
     for (int h = 0; h < kFewHeld; ++h) acc = __builtin_amdgcn_mfma_i32_16x16x64_i8(b[h], whole(a[h]), acc, 0, 0, 0);
@@ -299,6 +317,109 @@ fgpu_status few_rows(const FewJob& j, bool gated, bool quant, hipStream_t s) {
   return FGPU_OK;
 }
 
+// ---- some hundred rows: one launch ----------------------------------------------------
+// A workgroup rounds its 32 rows of x into LDS, whole, and then eight waves form 128 columns (gated: 64 of each half) from there
+// and from the weight as it lies, whose first steps are on the way meanwhile.  Every column of workgroups rounds the rows
+// again: up to one workgroup a CU and 512 k that takes the GPU as long as rounding in a launch of its own (float32 1000 x 385 x
+// 771 9.0 us and 9.3; bfloat16 128 x 512 x 2048 9.9 and 8.2; with 1024 k 12 and 10), and the caller a launch and a workspace
+// less, which is what calls of this size wait for (15 us a call and 10).
+constexpr int kPanelRows = 32, kPanelK = 512, kPanelWaves = 8, kPanelThreads = kPanelWaves * kWave;
+__host__ __device__ constexpr int panel_stride(int ld) { return (ld / 16 | 1) * 16; }  // rows fall on different banks
+
+template <class T, bool GATED>
+__global__ __launch_bounds__(kPanelThreads) void panel_kernel(FewJob j) {
+  __shared__ __attribute__((aligned(16))) char rows[kPanelRows * panel_stride(kPanelK)];
+  __shared__ float row_scale[kPanelRows];
+  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int across = (j.n + (GATED ? 63 : 127)) / (GATED ? 64 : 128);
+  const int m0 = blockIdx.x / across * kPanelRows, n0 = blockIdx.x % across * (GATED ? 64 : 128);
+  const int i = lane & 15, kc = (lane >> 4) * 16, stride = panel_stride(j.ld), steps = (j.ld + kFewStep - 1) / kFewStep;
+  const i32x4 none = {0, 0, 0, 0};
+  const int first = n0 + wave * (GATED ? 8 : 16), col = first + (GATED ? i & 7 : i);
+  const int8_t* wrow = j.w + (int64_t)(GATED && (i & 8) ? col + j.n : col) * j.ld;
+  auto weight = [&](int s) {
+    const int k = s * kFewStep + kc;
+    return col < j.n && k < j.ld ? *reinterpret_cast<const i32x4*>(wrow + k) : none;
+  };
+  constexpr int kAhead = 8;
+  i32x4 b[kAhead];
+#pragma unroll
+  for (int h = 0; h < kAhead; ++h) b[h] = weight(h);
+  {
+    constexpr int G = kPanelThreads / kPanelRows, held = kPanelK / 8 / G;  // 16 lanes a row
+    const int r = tid / G, at = tid % G, row = m0 + r;
+    const T* x = (const T*)j.x + (int64_t)row * j.k;
+    f32x8 v[held];
+    uint32_t most = 0;
+#pragma unroll
+    for (int h = 0; h < held; ++h) {
+      const int c = (at + h * G) * 8;
+      v[h] = row < j.m && c < j.k ? load8_n(x + c, j.k - c) : f32x8{{0, 0, 0, 0}, {0, 0, 0, 0}};
+    }
+#pragma unroll
+    for (int h = 0; h < held; ++h) most = most_bits(most, v[h]);
+    const Rounder<T> q(lanes_max<16>(most));
+    if (at == 0) row_scale[r] = q.scale;
+    char* to = rows + r * stride;
+#pragma unroll
+    for (int h = 0; h < held; ++h) {
+      const int c = (at + h * G) * 8;
+      if (c < j.ld) *reinterpret_cast<u32x2*>(to + c) = q.round8(v[h]);
+    }
+  }
+  __syncthreads();
+  i32x4 acc[2] = {none, none};
+  auto work = [&](int s, const i32x4& w) {
+    const int k = s * kFewStep + kc;
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      const i32x4 a = k < j.ld ? *reinterpret_cast<const i32x4*>(rows + (16 * h + i) * stride + k) : none;
+      acc[h] = __builtin_amdgcn_mfma_i32_16x16x64_i8(w, a, acc[h], 0, 0, 0);
+    }
+  };
+  for (int s = 0; s < steps; s += kAhead) {
+    i32x4 now[kAhead];
+#pragma unroll
+    for (int h = 0; h < kAhead; ++h) now[h] = b[h];
+#pragma unroll
+    for (int h = 0; h < kAhead; ++h) b[h] = weight(s + kAhead + h);
+#pragma unroll
+    for (int h = 0; h < kAhead; ++h) work(s + h, now[h]);  // past the end: zeros
+  }
+#pragma unroll
+  for (int h = 0; h < 2; ++h) {
+    const int m = 16 * h + i, c = first + (lane >> 4) * 4, cnt = j.n - c;
+    const float r = row_scale[m];
+    auto scaled = [&](const i32x4& v, const float* sc) {
+      const f32x4 by = load4_n(sc, cnt);
+      f32x4 o;
+#pragma unroll
+      for (int e = 0; e < 4; ++e) o[e] = (float)v[e] * by[e] * r;
+      return o;
+    };
+    i32x4 other = none;
+    if constexpr (GATED) {
+#pragma unroll
+      for (int e = 0; e < 4; ++e) other[e] = xchg<32>(acc[h][e]);
+    }
+    if (m0 + m >= j.m || cnt <= 0 || (GATED && lane >= 32)) continue;
+    if constexpr (GATED)
+      finish4_gated<T>(j.f, scaled(acc[h], j.s.col + c), scaled(other, j.s.col + j.n + c), m0 + m, j.n, c, cnt);
+    else
+      finish4<T>(j.f, scaled(acc[h], j.s.col + c), (int64_t)(m0 + m) * j.n + c, c, cnt);
+  }
+}
+bool takes_panel(int64_t rows, int k, int n, bool gated) {
+  return k <= kPanelK && (rows + kPanelRows - 1) / kPanelRows * ceil_div(n, gated ? 64 : 128) <= 256;
+}
+template <class T>
+fgpu_status panel(const FewJob& j, bool gated, hipStream_t s) {
+  const int grid = ceil_div(j.m, kPanelRows) * ceil_div(j.n, gated ? 64 : 128);
+  gated ? panel_kernel<T, true><<<grid, kPanelThreads, 0, s>>>(j) : panel_kernel<T, false><<<grid, kPanelThreads, 0, s>>>(j);
+  FGPU_HIP(hipGetLastError());
+  return FGPU_OK;
+}
+
 fgpu_status check_common(int64_t rows, int in_dim, int64_t out, int dtype, int act) {
   FGPU_CHECK(dtype == FGPU_DTYPE_F32 || dtype == FGPU_DTYPE_BF16, FGPU_ERR_ARG, "8-bit linear: unknown dtype");
   FGPU_CHECK(act >= FGPU_ACT_NONE && act <= FGPU_ACT_SILU, FGPU_ERR_ARG, "8-bit linear: unknown activation");
@@ -307,9 +428,9 @@ fgpu_status check_common(int64_t rows, int in_dim, int64_t out, int dtype, int a
              "8-bit linear: more than 2^30 rows or 2^16 dims");
   return FGPU_OK;
 }
-// out: weight rows.
-size_t workspace_bytes_of(int64_t rows, int in_dim, int64_t out, int dtype, bool quant) {
-  if (check_common(rows, in_dim, out, dtype, 0) != FGPU_OK || rows <= kFewRows || !quant) return 0;
+size_t workspace_bytes_of(int64_t rows, int in_dim, int n, bool gated, int dtype, bool quant) {
+  if (check_common(rows, in_dim, gated ? 2 * (int64_t)n : n, dtype, 0) != FGPU_OK || !quant) return 0;
+  if (rows <= kFewRows || takes_panel(rows, in_dim, n, gated)) return 0;
   return carve_bytes<int8_t>((size_t)rows * int8_row(in_dim)) + carve_bytes<float>(rows);
 }
 
@@ -319,6 +440,7 @@ fgpu_status run_layer(const void* x, const float* x_scale, const int8_t* w, cons
   const int ld = int8_row(k), out = gated ? 2 * n : n;
   const bool quant = !x_scale;
   if (rows <= kFewRows) return few_rows<T>({x, w, (int)rows, n, k, ld, {x_scale, w_scale}, f}, gated, quant, s);
+  if (quant && takes_panel(rows, k, n, gated)) return panel<T>({x, w, (int)rows, n, k, ld, {nullptr, w_scale}, f}, gated, s);
   Carve ws(d_ws, ws_bytes);
   if (quant) {
     int8_t* q = ws.take<int8_t>((size_t)rows * ld);
@@ -376,7 +498,7 @@ fgpu_status fgpu_quantize_rows(const void* d_x, int64_t rows, int dim, int dtype
 }
 
 size_t fgpu_linear_int8_workspace_bytes(int64_t rows, int in_dim, int out_dim, int dtype, int quantized_x) {
-  return workspace_bytes_of(rows, in_dim, out_dim, dtype, !quantized_x);
+  return workspace_bytes_of(rows, in_dim, out_dim, false, dtype, !quantized_x);
 }
 fgpu_status fgpu_linear_int8(const void* d_x, const float* d_x_scale, const int8_t* d_w, const float* d_w_scale,
                              const void* d_bias, const void* d_residual, int64_t rows, int in_dim, int out_dim, int dtype,
@@ -386,7 +508,7 @@ fgpu_status fgpu_linear_int8(const void* d_x, const float* d_x_scale, const int8
 }
 
 size_t fgpu_gated_linear_int8_workspace_bytes(int64_t rows, int in_dim, int hidden, int dtype, int quantized_x) {
-  return workspace_bytes_of(rows, in_dim, 2 * (int64_t)hidden, dtype, !quantized_x);
+  return workspace_bytes_of(rows, in_dim, hidden, true, dtype, !quantized_x);
 }
 fgpu_status fgpu_gated_linear_int8(const void* d_x, const float* d_x_scale, const int8_t* d_w, const float* d_w_scale,
                                    const void* d_bias, int64_t rows, int in_dim, int hidden, int dtype, int act, void* d_h,

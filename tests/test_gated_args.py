@@ -54,9 +54,9 @@ ALL = [gated, gated_bwd, quantize, int8, gated_int8, ortho]
     (quantize, dict(dim=0), ARG), (quantize, dict(q=None), ARG), (quantize, dict(scale=None), ARG), (quantize, dict(q=P + 8), ARG),
     (quantize, dict(dim=(1 << 16) + 1), UNSUPPORTED), (quantize, dict(rows=(1 << 30) + 1), UNSUPPORTED),
     (int8, dict(wsc=None), ARG), (int8, dict(y=None), ARG), (int8, dict(n=(1 << 16) + 1), UNSUPPORTED),
-    (int8, dict(rows=1 << 12, wsb=0), WORKSPACE), (int8, dict(rows=1 << 12, ws=None), WORKSPACE),
+    (int8, dict(rows=1 << 12, k=1024, wsb=0), WORKSPACE), (int8, dict(rows=1 << 12, k=1024, ws=None), WORKSPACE),
     (gated_int8, dict(wsc=None), ARG), (gated_int8, dict(h=None), ARG), (gated_int8, dict(n=(1 << 15) + 1), UNSUPPORTED),
-    (gated_int8, dict(n=(1 << 31) - 1), UNSUPPORTED), (gated_int8, dict(rows=1 << 12, wsb=0), WORKSPACE),
+    (gated_int8, dict(n=(1 << 31) - 1), UNSUPPORTED), (gated_int8, dict(rows=1 << 12, k=1024, wsb=0), WORKSPACE),
     (ortho, dict(cols=-1), ARG), (ortho, dict(steps=0), ARG), (ortho, dict(steps=65), ARG), (ortho, dict(eps=-1.0), ARG),
     (ortho, dict(eps=INF), ARG), (ortho, dict(a=INF), ARG), (ortho, dict(b=float("nan")), ARG), (ortho, dict(c=-INF), ARG),
     (ortho, dict(y=None), ARG), (ortho, dict(ws=P + 8), ARG), (ortho, dict(wsb=0), WORKSPACE), (ortho, dict(ws=None), WORKSPACE),
@@ -80,8 +80,8 @@ def test_workspace_sizes():
     for f, size, args in [
             (gated, L.fgpu_gated_linear_workspace_bytes(5000, 1023, 512, BF16), dict(rows=5000, k=1023, n=512, dt=BF16)),
             (gated_bwd, L.fgpu_gated_linear_backward_workspace_bytes(5000, 100, 30, F32), dict(rows=5000, k=100, n=30)),
-            (int8, L.fgpu_linear_int8_workspace_bytes(5000, 100, 30, F32, 0), dict(rows=5000, k=100, n=30)),
-            (gated_int8, L.fgpu_gated_linear_int8_workspace_bytes(5000, 100, 30, BF16, 0), dict(rows=5000, k=100, n=30, dt=BF16)),
+            (int8, L.fgpu_linear_int8_workspace_bytes(5000, 1000, 30, F32, 0), dict(rows=5000, k=1000, n=30)),
+            (gated_int8, L.fgpu_gated_linear_int8_workspace_bytes(5000, 1000, 30, BF16, 0), dict(rows=5000, k=1000, n=30, dt=BF16)),
             (ortho, L.fgpu_orthogonalize_workspace_bytes(1000, 30, F32), dict(rows=1000, cols=30))]:
         assert size > 0 and f(**args, wsb=size - 1) == WORKSPACE
     assert L.fgpu_gated_linear_workspace_bytes(1 << 16, 1024, 4096, BF16) == 0
