@@ -7,6 +7,7 @@
 #include <cmath>
 
 #include "gated.hpp"
+#include "head_direct.hpp"
 
 namespace fgpu {
 namespace {
@@ -174,7 +175,8 @@ Choice choose(int m, int n, int k, bool f32) {
       if (t < us) us = t, c.split = width;
     }
   }
-  if (direct_forward_estimate_us(p) < us) c.direct = true, c.split = 0;
+  const bool one_launch = (int64_t)ceil_div(m, 32) * ceil_div(n, 16) * kDirectThreads < kLaunchThreads;
+  if (one_launch && direct_forward_estimate_us(p) < us) c.direct = true, c.split = 0;
   return c;
 }
 

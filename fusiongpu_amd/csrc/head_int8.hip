@@ -26,16 +26,18 @@ struct Rounder {
   float near;   // |d| below it: n is right
   float scale;  // what q is multiplied by to stand for x
   int exp;      // the power of two that x is scaled by
+  uint32_t keep;  // zero where everything becomes zero
   // bits: those of the largest magnitude.  A row that holds something not finite has a NaN scale and zeros.
   __device__ __forceinline__ explicit Rounder(uint32_t bits) {
     const float top = __uint_as_float(bits);
     const bool live = bits != 0 && bits < 0x7f800000u;
     scale = bits < 0x7f800000u ? top / 127.0f : __uint_as_float(0x7fc00000u);
+    keep = live ? ~0u : 0u;
     exp = live && (top < 0x1p-100f || top > 0x1p100f) ? -__builtin_amdgcn_frexp_expf(top) : 0;
     most = exp ? ldexpf(top, exp) : top;
     per = live ? 127.0f / most : 0.0f;
     near = sizeof(T) == 4 ? 0.4999f * most : 0.5f * most;
-    if (!live) most = near = INFINITY;  // every d is far below, and every n of 0 x right, but for what is not finite itself
+    if (!live) most = near = INFINITY;  // no d is looked at
   }
   __device__ __forceinline__ u32x2 round8(f32x8 x) const {
     if (exp) {
@@ -67,7 +69,7 @@ struct Rounder {
     for (int h = 0; h < 2; ++h) {  // the low bytes
       const uint32_t a = __builtin_amdgcn_perm(__float_as_uint(n[4 * h + 1]), __float_as_uint(n[4 * h]), 0x0c0c0400u);
       const uint32_t b = __builtin_amdgcn_perm(__float_as_uint(n[4 * h + 3]), __float_as_uint(n[4 * h + 2]), 0x04000c0cu);
-      out[h] = a | b;
+      out[h] = (a | b) & keep;
     }
     return out;
   }

@@ -48,6 +48,7 @@ template <class T>
 __global__ __launch_bounds__(256) void norm_parts_kernel(const T* x, int64_t count, double* part) {
   __shared__ double sum[256];
   double v = 0;
+#pragma unroll 4
   for (int64_t i = ((int64_t)blockIdx.x * 256 + threadIdx.x) * 8; i < count; i += (int64_t)gridDim.x * 256 * 8) {
     const f32x8 q = load8_n(x + i, (int)min(count - i, (int64_t)8));
 #pragma unroll
@@ -77,14 +78,22 @@ __global__ __launch_bounds__(256) void start_kernel(const T* x, int64_t rows, in
   const double norm = sqrt(sum[0]) + eps;
   // Something not finite makes everything NaN; nothing but zeros stays zero.
   const double by = !(norm < INFINITY) ? (double)NAN : norm > 0 ? kHeld / norm : 0;
-  const int64_t per = whole8(cols) / 8, total = rows * per;
-  for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < total; i += (int64_t)gridDim.x * 256) {
-    const int64_t r = i / per;
-    const int c = (int)(i - r * per) * 8;
+  // In float32 where the factor is far from the ends of the type.
+  const float by32 = by > 1e-30 && by < 1e30 ? (float)by : 0.0f;
+  const uint32_t per = (uint32_t)(whole8(cols) / 8);
+  const uint64_t total = rows * (uint64_t)per;
+#pragma unroll 2
+  for (uint64_t i = (uint64_t)blockIdx.x * 256 + threadIdx.x; i < total; i += (uint64_t)gridDim.x * 256) {
+    const int64_t r = total < (1ull << 32) ? (uint32_t)i / per : i / per;
+    const int c = (int)(i - r * (uint64_t)per) * 8;
     const f32x8 q = load8_n(x + r * cols + c, cols - c);
     f32x8 o;
+    if (by32 != 0) {
+      o = {q.lo * by32, q.hi * by32};
+    } else {
 #pragma unroll
-    for (int e = 0; e < 8; ++e) o.set(e, c + e < cols ? (float)(q[e] * by) : 0.0f);
+      for (int e = 0; e < 8; ++e) o.set(e, c + e < cols ? (float)(q[e] * by) : 0.0f);
+    }
     put_planes8(out, r * out.ld + c, o);
   }
 }
@@ -491,7 +500,7 @@ fgpu_status run_ortho(const T* x, const Shape& sh, int steps, float a, float b, 
   const int64_t count = (int64_t)sh.rows * sh.cols;
   const int blocks = (int)std::min<int64_t>((count + 2047) / 2048, kNormBlocks);
   norm_parts_kernel<T><<<blocks, 256, 0, s>>>(x, count, norm);
-  start_kernel<T><<<(int)std::min<int64_t>((sh.rows * (whole8(sh.cols) / 8) + 255) / 256, 4096), 256, 0, s>>>(
+  start_kernel<T><<<(int)std::min<int64_t>((sh.rows * (whole8(sh.cols) / 8) + 255) / 256, 1024), 256, 0, s>>>(
       x, sh.rows, sh.cols, norm, blocks, eps, xs[0]);
   FGPU_HIP(hipGetLastError());
   const int n = sh.small;

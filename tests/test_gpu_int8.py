@@ -88,6 +88,8 @@ def test_quantize_not_finite(dt):
     x = rnd(1, 5, 30, dtype=TYPES[dt])
     want, ws = codes(x)
     x[1, 4], x[2, 0], x[3, 29] = math.nan, math.inf, -math.inf
+    if dt == "f32":  # a NaN that carries something in its low bits
+        x.view(torch.int32)[1, 5] = 0x7FC12345
     q, scale = fg.quantize_rows(x)
     assert torch.isnan(scale[1:4]).all() and (q[1:4] == 0).all()
     assert torch.equal(q[[0, 4], :30].cpu().double(), want[[0, 4]]) and torch.equal(scale[[0, 4]].cpu(), ws[[0, 4]])
@@ -135,7 +137,8 @@ def check_layer(m, k, n, dt, act, bias, residual, gated, given, seed=0):
 
 SIZES = [(1, 1, 1), (1, 1024, 4096), (1, 1000, 33), (2, 8, 1030), (16, 100, 17), (16, 4100, 40), (17, 100, 17), (33, 65, 63),
          (64, 64, 64), (127, 15, 129), (300, 513, 257), (257, 2056, 255), (1000, 385, 771), (2050, 1024, 520), (16390, 64, 516),
-         (40000, 24, 40), (3, 30000, 5)]
+         (40000, 24, 40), (3, 30000, 5), (3000, 1040, 1000), (3000, 1040, 2000), (5000, 656, 1030), (5000, 656, 2060),
+         (200, 512, 800), (260, 500, 1000)]
 
 
 @pytest.mark.parametrize("dt", ["f32", "bf16"])
