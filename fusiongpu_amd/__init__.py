@@ -1171,16 +1171,19 @@ def gated_linear_backward(dh, x, weight, pre, act: str = "silu", want=("x", "wei
     return dx, dw, db
 
 
+# The current device's index, without torch's check that it is initialised (a tensor on it says so).
+_device_now = getattr(_torch()._C, "_cuda_getDevice", None) or _torch().cuda.current_device
+
+
 def _stream_here(*tensors):
     """The handle of the current stream, for a call on `tensors`: refuses those of another device than the current one, whose
     stream it is."""
-    cuda = _TORCH.cuda
-    now = cuda.current_device()
+    now = _device_now()
     for t in tensors:
         if t is not None and t.get_device() != now:
             raise ValueError(f"a tensor on {t.device}, but the current device is cuda:{now}: make the call under "
                              "torch.cuda.device(...) of its tensors")
-    return _raw_stream(now) if _raw_stream is not None else cuda.current_stream().cuda_stream
+    return _raw_stream(now) if _raw_stream is not None else _TORCH.cuda.current_stream().cuda_stream
 
 
 @functools.lru_cache(maxsize=1024)

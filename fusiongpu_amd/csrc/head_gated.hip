@@ -96,21 +96,31 @@ __global__ __launch_bounds__(T::threads, 2) void gated_split_kernel(SplitJob32 j
         for (int c = 0; c < 6; ++c) acc[i][q] = OfBf16::mma(b[i][pair_b(c)], a[q][pair_a(c)], acc[i][q]);
   };
   // Behind the barrier of step i its planes are in `cur`, nobody reads `other`, and the values of i + 1 and i + 2 are on the way.
+  // The next step's planes are formed between this one's matrix instructions.
+  auto step = [&](char* cur, char* other, Stage& next, int k) {
+    __syncthreads();
+    work(cur);
+    store(next, other);
+    load(next, k + 3 * B);
+#pragma unroll
+    for (int i = 0; i < T::FM * T::FN * 6; ++i) {
+      __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);  // a matrix instruction
+      __builtin_amdgcn_sched_group_barrier(0x002, 4, 0);  // and four others
+    }
+  };
   Stage t0, t1;
   load(t0, 0);
   load(t1, B);
   store(t0, s0);
   load(t0, 2 * B);
-  for (int k = 0; k < j.k; k += 2 * B) {
+  int k = 0;
+  for (; k + B < j.k; k += 2 * B) {
+    step(s0, s1, t1, k);
+    step(s1, s0, t0, k + B);
+  }
+  if (k < j.k) {
     __syncthreads();
     work(s0);
-    if (k + B >= j.k) break;
-    store(t1, s1);
-    load(t1, k + 3 * B);
-    __syncthreads();
-    work(s1);
-    store(t0, s0);
-    load(t0, k + 4 * B);
   }
   const GemmWave<T> w{m0, n0, tm, tn, 0, wm, wn, lane, s1};
   epi.template finish<T>(acc, w, s1, typename GatedEpi<float, ACT>::template Side<T>{});
@@ -137,7 +147,7 @@ fgpu_status run_split(SplitJob32 j, const Finish& f, hipStream_t s) {
 // and of each of several.
 double split_us(int m, int n, int k, int width) {
   const int64_t each = ceil_div((int64_t)ceil_div(m, 64) * ceil_div(n, width / 2), 256);
-  const double alone = width == 64 ? 0.72 : 1.08, shared = width == 64 ? 0.56 : 0.88;
+  const double alone = width == 64 ? 0.66 : 1.12, shared = width == 64 ? 0.54 : 0.88;
   return 3.3 + ceil_div(k, kPlanesBK) * (each == 1 ? alone : each * shared);
 }
 
@@ -153,7 +163,7 @@ bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 
 
 // Which kernel a forward call takes, by estimates: that of few tiles, tiles whose planes are formed on the way (float32), or tiles
 // of operands as they are or packed (a launch more).  us, few / on the way / packed: float32 1000 x 771 x 385 (rows, hidden, in)
-// - / 18.8 / 25.9, 2000 x 771 x 385 - / 26.6 / 42.7, 300 x 771 x 1024 20.6 / 26.7 / -, 4000 x 2048 x 1024 - / 202 / 167.
+// - / 17.4 / 25.9, 2000 x 771 x 385 - / 26.6 / 42.7, 300 x 771 x 1024 20.6 / 26.7 / -, 4000 x 2048 x 1024 - / 202 / 167.
 struct Choice {
   bool direct = false;
   int split = 0;  // the width of its tiles

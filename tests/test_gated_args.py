@@ -100,7 +100,7 @@ def host(monkeypatch):
                  "fgpu_gated_linear_int8", "fgpu_orthogonalize"):
         monkeypatch.setattr(fg.lib, name, no_call)
     monkeypatch.setattr(torch.Tensor, "is_cuda", True)
-    monkeypatch.setattr(torch.cuda, "current_device", lambda: -1)
+    monkeypatch.setattr(fg, "_device_now", lambda: -1)
     monkeypatch.setattr(fg, "_stream", lambda: None)
 
 
@@ -149,7 +149,7 @@ def test_python_refusals(host, call, error):
 
 
 def test_tensors_of_another_device_are_refused(host, monkeypatch):
-    monkeypatch.setattr(torch.cuda, "current_device", lambda: 1)
+    monkeypatch.setattr(fg, "_device_now", lambda: 1)
     w8, s = t(4, 16, dtype=I8), t(4)
     for call in (lambda: fg.gated_linear(t(2, 8), t(4, 8)), lambda: fg.gated_linear_backward(t(2, 2), t(2, 8), t(4, 8), t(2, 4)),
                  lambda: fg.quantize_rows(t(2, 8)), lambda: fg.linear_int8(t(2, 8), w8, s),
