@@ -147,13 +147,11 @@ template <int PAIRS, class Num, class T, int ACT>
 fgpu_status run_gated(const GemmArgs& g, int tile, const GatedEpi<T, ACT>& e, hipStream_t s) {
   const int grid = g.tiles_m * g.tiles_n;
   using E = GatedEpi<T, ACT>;
-  if (tile == 256) {
-    gemm_kernel<GatedTile256, true, true, PAIRS, E, Num, kGated><<<grid, GatedTile256::threads, 0, s>>>(g, e);
-  } else if (tile == 64) {
-    gemm_kernel<GatedTile64, true, true, PAIRS, E, Num, kGated><<<grid, GatedTile64::threads, 0, s>>>(g, e);
-  } else if constexpr (PAIRS == 1) {
-    gemm_kernel<GatedTile128, true, true, PAIRS, E, Num, kGated><<<grid, GatedTile128::threads, 0, s>>>(g, e);
+  if constexpr (PAIRS == 1) {
+    if (tile == 64) gemm_kernel<GatedTile64, true, true, PAIRS, E, Num, kGated><<<grid, GatedTile64::threads, 0, s>>>(g, e);
+    if (tile == 128) gemm_kernel<GatedTile128, true, true, PAIRS, E, Num, kGated><<<grid, GatedTile128::threads, 0, s>>>(g, e);
   }
+  if (tile == 256) gemm_kernel<GatedTile256, true, true, PAIRS, E, Num, kGated><<<grid, GatedTile256::threads, 0, s>>>(g, e);
   FGPU_HIP(hipGetLastError());
   return FGPU_OK;
 }

@@ -34,8 +34,11 @@ struct Eight {
 };
 template <class T, int ACT>
 __global__ __launch_bounds__(T::threads, 2) void gated_split_kernel(SplitJob32 j, GatedEpi<float, ACT> epi) {
-  constexpr int B = kPlanesBK, pa = T::BM * B * 2, pb = T::BN * B * 2, kb = T::BN * 4 / T::threads;
-  static_assert(T::BM * 4 == T::threads && kb * T::threads == T::BN * 4, "whole chunks a thread");
+  // Chunks of eight values: a thread takes one of each operand, or two of one; of fewer chunks than threads, the first waves.
+  constexpr int B = kPlanesBK, pa = T::BM * B * 2, pb = T::BN * B * 2;
+  constexpr int ka = (T::BM * 4 + T::threads - 1) / T::threads, kb = (T::BN * 4 + T::threads - 1) / T::threads;
+  constexpr int ta = T::BM * 4 < T::threads ? T::BM * 4 : T::threads, tb = T::BN * 4 < T::threads ? T::BN * 4 : T::threads;
+  static_assert(ka * ta == T::BM * 4 && kb * tb == T::BN * 4, "whole chunks a thread");
   __shared__ __attribute__((aligned(1024))) char s0[3 * (pa + pb)];
   __shared__ __attribute__((aligned(1024))) char s1[3 * (pa + pb)];
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
@@ -50,14 +53,19 @@ __global__ __launch_bounds__(T::threads, 2) void gated_split_kernel(SplitJob32 j
   ra.init(lane, wm * (T::BM / T::WM));
   rb.init(lane, wn * (T::BN / T::WN));
   struct Stage {
-    Eight a, b[kb];
+    Eight a[ka], b[kb];
   };
+  const bool has_a = ta == T::threads || wave < ta / kWave, has_b = tb == T::threads || wave < tb / kWave;
   auto load = [&](Stage& t, int k) {
-    t.a.load(j.x, m0 + row, m0 + row < j.m, k + chunk * 8, j.k);
+#pragma unroll
+    for (int i = 0; i < ka; ++i) {
+      const int r = row + i * (ta / 4);
+      t.a[i].load(j.x, m0 + r, has_a && m0 + r < j.m, k + chunk * 8, j.k);
+    }
 #pragma unroll
     for (int i = 0; i < kb; ++i) {
-      const int r = row + i * (T::threads / 4), h = n0 + (r >> 6) * 32 + (r & 31);
-      t.b[i].load(j.w, (r & 32) ? (int64_t)h + j.n : h, h < j.n, k + chunk * 8, j.k);
+      const int r = row + i * (tb / 4), h = n0 + (r >> 6) * 32 + (r & 31);
+      t.b[i].load(j.w, (r & 32) ? (int64_t)h + j.n : h, has_b && h < j.n, k + chunk * 8, j.k);
     }
   };
   auto put = [&](char* at, int plane, const Eight& e) {
@@ -67,11 +75,15 @@ __global__ __launch_bounds__(T::threads, 2) void gated_split_kernel(SplitJob32 j
     for (int q = 0; q < 3; ++q) *reinterpret_cast<bf16x8*>(at + q * plane) = p[q];
   };
   auto store = [&](const Stage& t, char* s) {
-    put(s + row * (B * 2) + (chunk ^ tile_swizzle<true, false, 4>(row)) * 16, pa, t.a);
+#pragma unroll
+    for (int i = 0; i < ka; ++i) {
+      const int r = row + i * (ta / 4);
+      if (has_a) put(s + r * (B * 2) + (chunk ^ tile_swizzle<true, false, 4>(r)) * 16, pa, t.a[i]);
+    }
 #pragma unroll
     for (int i = 0; i < kb; ++i) {
-      const int r = row + i * (T::threads / 4);
-      put(s + 3 * pa + r * (B * 2) + (chunk ^ tile_swizzle<true, true, 4>(r)) * 16, pb, t.b[i]);
+      const int r = row + i * (tb / 4);
+      if (has_b) put(s + 3 * pa + r * (B * 2) + (chunk ^ tile_swizzle<true, true, 4>(r)) * 16, pb, t.b[i]);
     }
   };
   f32x4 acc[T::FN][T::FM];
@@ -125,7 +137,7 @@ __global__ __launch_bounds__(T::threads, 2) void gated_split_kernel(SplitJob32 j
   const GemmWave<T> w{m0, n0, tm, tn, 0, wm, wn, lane, s1};
   epi.template finish<T>(acc, w, s1, typename GatedEpi<float, ACT>::template Side<T>{});
 }
-using WideSplitTile = GemmTile<64, 128, 2, 2>;
+using WideSplitTile = GemmTile<64, 128, 4, 2>;
 template <class T>
 fgpu_status run_split(SplitJob32 j, const Finish& f, hipStream_t s) {
   j.tiles_n = ceil_div(j.n, T::BN / 2);
@@ -147,7 +159,7 @@ fgpu_status run_split(SplitJob32 j, const Finish& f, hipStream_t s) {
 // and of each of several.
 double split_us(int m, int n, int k, int width) {
   const int64_t each = ceil_div((int64_t)ceil_div(m, 64) * ceil_div(n, width / 2), 256);
-  const double alone = width == 64 ? 0.66 : 1.12, shared = width == 64 ? 0.54 : 0.88;
+  const double alone = width == 64 ? 0.66 : 0.98, shared = width == 64 ? 0.54 : 0.86;
   return 3.3 + ceil_div(k, kPlanesBK) * (each == 1 ? alone : each * shared);
 }
 
@@ -163,7 +175,7 @@ bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 
 
 // Which kernel a forward call takes, by estimates: that of few tiles, tiles whose planes are formed on the way (float32), or tiles
 // of operands as they are or packed (a launch more).  us, few / on the way / packed: float32 1000 x 771 x 385 (rows, hidden, in)
-// - / 17.4 / 25.9, 2000 x 771 x 385 - / 26.6 / 42.7, 300 x 771 x 1024 20.6 / 26.7 / -, 4000 x 2048 x 1024 - / 202 / 167.
+// - / 17.2 / 25.9, 2000 x 771 x 385 - / 25.9 / 42.7, 300 x 771 x 1024 20.6 / 23.9 / -, 4000 x 2048 x 1024 - / 197 / 167.
 struct Choice {
   bool direct = false;
   int split = 0;  // the width of its tiles
@@ -172,11 +184,7 @@ struct Choice {
 Choice choose(int m, int n, int k, bool f32) {
   const Product p{m, 2 * n, k, f32};
   Choice c;
-  c.plan = plan_product(p, false, f32 ? 256 : 0);
-  if (f32) {  // packed tiles of 128 are faster nowhere
-    const Plan q = plan_product(p, false, 64);
-    if (!c.plan.tile || (q.tile && q.us < c.plan.us)) c.plan = q;
-  }
+  c.plan = plan_product(p, false, f32 ? 256 : 0);  // smaller packed tiles of float32 are slower than those formed on the way
   double us = c.plan.tile ? c.plan.us : INFINITY;
   if (needs_pack(k, f32)) us += 5.7 + ((double)p.m + p.n) * k * (f32 ? 10 : 4) / 4e6;
   if (f32 && (int64_t)ceil_div(m, 64) * ceil_div(n, 32) * GatedTile64::threads < kLaunchThreads) {

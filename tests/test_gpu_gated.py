@@ -98,7 +98,7 @@ def test_every_tile(act, dt):
         seen.add(fg.lib.fgpu_gated_linear_tile(m, k, n, int(dt == "bf16")))
         check_gated(m, k, n, dt, act, True, True, seed=m)
     split = 2048  # planes formed on the way: 64 and 128 wide
-    assert seen >= ({0, 64, 256, split + 64, split + 128} if dt == "f32" else {0, 64, 128, 256}), seen
+    assert seen >= ({0, 256, split + 64, split + 128} if dt == "f32" else {0, 64, 128, 256}), seen
 
 
 @pytest.mark.parametrize("dt", ["f32", "bf16"])
