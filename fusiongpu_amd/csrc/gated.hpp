@@ -28,9 +28,10 @@ __device__ __forceinline__ f32x8 eight(const A& lo, const A& hi, float row, cons
   return v;
 }
 
-// 64 columns of 16 rows in bfloat16, of which a lane holds eight from 8 (lane / 16) on and the eight 32 further (a and b) of row
-// lane % 16, as 128 bytes of eight rows a store: lanes eight rows apart swap halves.  16 rows of 64 bytes each, half a line, write
-// a good third slower (65536 x 4096 with both factors kept, k 64 472 -> 333 us, k 1024 1120 -> 1080).  rows: how many of the 16.
+// 64 columns of 16 rows in bfloat16, of which a lane holds eight from 8 (lane / 16) on and the eight 32 further (a and b) of
+// row lane % 16, as 128 bytes of eight rows a store: lanes eight rows apart swap halves.  16 rows of 64 bytes each, half a
+// line, write a good third slower (65536 x 4096 with both factors kept, k 64 472 -> 333 us, k 1024 1120 -> 1080).  rows: how
+// many of the 16.
 template <bool STREAM>
 __device__ __forceinline__ void store_lines(bf16* p, int64_t ld, int lane, int rows, const f32x8& a, const f32x8& b) {
   typedef uint32_t u32x4u __attribute__((ext_vector_type(4), aligned(2)));
@@ -89,7 +90,8 @@ struct GatedEpi {
         const int64_t row = w.row(j);
         if (row >= m) continue;
         const float sr = kInt ? s.row[row] : 1.0f;
-        f32x8 g = eight(acc[4 * q][j], acc[4 * q + 1][j], sr, sg, bg), u = eight(acc[4 * q + 2][j], acc[4 * q + 3][j], sr, su, bu);
+        const f32x8 g = eight(acc[4 * q][j], acc[4 * q + 1][j], sr, sg, bg);
+        f32x8 u = eight(acc[4 * q + 2][j], acc[4 * q + 3][j], sr, su, bu);
         if (f.pre) {
           T* pre = (T*)f.pre + row * 2 * n + c;
           store8_n<STREAM>(pre, g, cnt);

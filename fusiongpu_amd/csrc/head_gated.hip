@@ -2,7 +2,14 @@
 //
 // Both projections are one product against the stacked weight [Wg; Wu]: a tile's B operand takes 32 rows of Wg and then the
 // 32 of Wu that belong to the same hidden columns (GatedTileLoad), so a lane's accumulators hold g and u of the same
-// columns and act(g) u is formed before anything is stored.
+// columns and act(g) u is formed before anything is stored.  The gradients are those of one linear layer of 2 hidden columns
+// once dz = [dh u act'(g) | dh act(g)] is there, which a launch of its own forms with its column sums (head_prep.hip).
+//
+// 65536 x 1024 -> 4096 in bfloat16 with both factors kept takes 1.07 ms (1.03 PFLOP/s): 0.79 of matrix instructions, then an
+// epilogue of 1.6 GB of stores a tile that nothing overlaps, as a 256 x 256 tile fills its CU (two workgroups of 128 x 128 a
+// CU 1.15 ms, of 256 x 128 with k in steps of 32 through three buffers 1.17 to 1.23, starts set apart no gain).  Its
+// gradients over 16384 rows 0.57 ms: dz 0.12 (670 MB, 5.6 TB/s), two products at 1.2 PFLOP/s.  One row 4.8 us, a launch and
+// two rounds of loads (eight columns of each half a workgroup, so that 2048 hidden ones are a workgroup a CU).
 #include <algorithm>
 #include <cmath>
 
@@ -15,9 +22,11 @@ namespace {
 constexpr int kMaxHidden = FGPU_HEAD_MAX_DIM / 2;
 
 // ---- float32, planes formed on the way to LDS -----------------------------------------
-// Mid-size float32 layers: a launch that copies both operands into planes first costs as much as a third of the product, and what
-// it wrote comes back through other XCDs' caches.  Here a thread loads eight values of a row as they lie (any alignment),
-// two steps ahead, splits them in registers and writes the three planes; each value is split once a tile instead of once.
+// Mid-size float32 layers: a launch that copies both operands into planes first costs as much as a third of the product,
+// and what it wrote comes back through other XCDs' caches.  Here a thread loads eight values of a row as they lie (any
+// alignment), two steps ahead, splits them in registers and writes the three planes; each value is split once a tile
+// instead of once.  1000 x 385 -> 771: 16.5 us, thirteen steps of 0.95 us: LDS, conversions and matrix instructions of a
+// step take 0.5, 0.3 and 0.3 and overlap little behind its one barrier.
 struct SplitJob32 {
   const float* x;
   const float* w;
@@ -107,8 +116,8 @@ __global__ __launch_bounds__(T::threads, 2) void gated_split_kernel(SplitJob32 j
 #pragma unroll
         for (int c = 0; c < 6; ++c) acc[i][q] = OfBf16::mma(b[i][pair_b(c)], a[q][pair_a(c)], acc[i][q]);
   };
-  // Behind the barrier of step i its planes are in `cur`, nobody reads `other`, and the values of i + 1 and i + 2 are on the way.
-  // The next step's planes are formed between this one's matrix instructions.
+  // Behind the barrier of step i its planes are in `cur`, nobody reads `other`, and the values of i + 1 and i + 2 are on the
+  // way. The next step's planes are formed between this one's matrix instructions.
   auto step = [&](char* cur, char* other, Stage& next, int k) {
     __syncthreads();
     work(cur);
@@ -143,7 +152,8 @@ fgpu_status run_split(SplitJob32 j, const Finish& f, hipStream_t s) {
   j.tiles_n = ceil_div(j.n, T::BN / 2);
   auto go = [&](auto act) {
     constexpr int ACT = decltype(act)::value;
-    gated_split_kernel<T, ACT><<<ceil_div(j.m, T::BM) * j.tiles_n, T::threads, 0, s>>>(j, GatedEpi<float, ACT>{f, {}, j.m, j.n});
+    const GatedEpi<float, ACT> epi{f, {}, j.m, j.n};
+    gated_split_kernel<T, ACT><<<ceil_div(j.m, T::BM) * j.tiles_n, T::threads, 0, s>>>(j, epi);
   };
   using std::integral_constant;
   switch (f.act) {
@@ -155,8 +165,8 @@ fgpu_status run_split(SplitJob32 j, const Finish& f, hipStream_t s) {
   FGPU_HIP(hipGetLastError());
   return FGPU_OK;
 }
-// Microseconds, fitted over 100 to 8000 rows, 96 to 2048 hidden and 96 to 2048 k: a step of 32 k of a workgroup alone on its CU,
-// and of each of several.
+// Microseconds, fitted over 100 to 8000 rows, 96 to 2048 hidden and 96 to 2048 k: a step of 32 k of a workgroup alone on its
+// CU, and of each of several.
 double split_us(int m, int n, int k, int width) {
   const int64_t each = ceil_div((int64_t)ceil_div(m, 64) * ceil_div(n, width / 2), 256);
   const double alone = width == 64 ? 0.66 : 0.98, shared = width == 64 ? 0.54 : 0.86;
@@ -173,9 +183,10 @@ fgpu_status check_common(int64_t rows, int in_dim, int hidden, int dtype, int ac
 }
 bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
 
-// Which kernel a forward call takes, by estimates: that of few tiles, tiles whose planes are formed on the way (float32), or tiles
-// of operands as they are or packed (a launch more).  us, few / on the way / packed: float32 1000 x 771 x 385 (rows, hidden, in)
-// - / 17.2 / 25.9, 2000 x 771 x 385 - / 25.9 / 42.7, 300 x 771 x 1024 20.6 / 23.9 / -, 4000 x 2048 x 1024 - / 197 / 167.
+// Which kernel a forward call takes, by estimates: that of few tiles, tiles whose planes are formed on the way (float32), or
+// tiles of operands as they are or packed (a launch more).  us, few / on the way / packed: float32 1000 x 771 x 385 (rows,
+// hidden, in) - / 17.2 / 25.9, 2000 x 771 x 385 - / 25.9 / 42.7, 300 x 771 x 1024 20.6 / 23.9 / -, 4000 x 2048 x 1024 - / 197
+// / 167.
 struct Choice {
   bool direct = false;
   int split = 0;  // the width of its tiles
@@ -235,9 +246,8 @@ fgpu_status fgpu_gated_linear(const void* d_x, const void* d_w, const void* d_bi
   Finish f;
   f.bias = d_bias, f.out = d_h, f.pre = d_pre, f.act = act;
   if (c.direct) {
-    DirectJob j{{d_x, in_dim, rows * in_dim, nullptr}, {d_w, in_dim, (int64_t)2 * hidden * in_dim, nullptr}, m, hidden, in_dim, 0, f,
-                nullptr};
-    j.b.up = hidden;
+    const DirectOperand x{d_x, in_dim, rows * in_dim, nullptr}, w{d_w, in_dim, (int64_t)2 * hidden * in_dim, nullptr, hidden};
+    const DirectJob j{x, w, m, hidden, in_dim, 0, f, nullptr};
     return launch_direct_gated(j, f32, s);
   }
   if (c.split) {

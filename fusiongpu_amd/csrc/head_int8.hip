@@ -2,6 +2,11 @@
 //
 // A row x becomes the whole numbers q = x 127 / max|x| to the nearest, ties to even, and the scale max|x| / 127: products
 // of two such rows are exact in 32 bits (up to 2^16 dims), so a layer's only error is the rounding of its operands.
+//
+// Rounding is bound by HBM: 100003 x 1024 in bfloat16 67 us (307 MB, 4.6 TB/s).  The gated layer on 65536 x 1024 -> 4096
+// takes 0.60 to 0.62 ms, 0.04 of them rounding (the product 1.9 POP/s; the library's plain product of 8192^3 2.4): eight
+// steps of 128 k a tile, then an epilogue of two conversions, four products, an exponential and a reciprocal an element that
+// nothing overlaps. One row x 1024 -> 4096: 5.4 us, a launch, the row's maximum and a round of loads.
 #include <algorithm>
 
 #include "gated.hpp"
@@ -312,16 +317,18 @@ template <class T>
 fgpu_status few_rows(const FewJob& j, bool gated, bool quant, hipStream_t s) {
   const int grid = ceil_div(j.n, gated ? 8 : 16);
   if (gated)
-    quant ? few_rows_kernel<T, true, true><<<grid, kFewThreads, 0, s>>>(j) : few_rows_kernel<T, true, false><<<grid, kFewThreads, 0, s>>>(j);
+    quant ? few_rows_kernel<T, true, true><<<grid, kFewThreads, 0, s>>>(j)
+          : few_rows_kernel<T, true, false><<<grid, kFewThreads, 0, s>>>(j);
   else
-    quant ? few_rows_kernel<T, false, true><<<grid, kFewThreads, 0, s>>>(j) : few_rows_kernel<T, false, false><<<grid, kFewThreads, 0, s>>>(j);
+    quant ? few_rows_kernel<T, false, true><<<grid, kFewThreads, 0, s>>>(j)
+          : few_rows_kernel<T, false, false><<<grid, kFewThreads, 0, s>>>(j);
   FGPU_HIP(hipGetLastError());
   return FGPU_OK;
 }
 
 // ---- some hundred rows: one launch ----------------------------------------------------
-// A workgroup rounds its 32 rows of x into LDS, whole, and then eight waves form 128 columns (gated: 64 of each half) from there
-// and from the weight as it lies, whose first steps are on the way meanwhile.  Every column of workgroups rounds the rows
+// A workgroup rounds its 32 rows of x into LDS, whole, and then eight waves form 128 columns (gated: 64 of each half) from
+// there and from the weight as it lies, whose first steps are on the way meanwhile.  Every column of workgroups rounds the rows
 // again: up to one workgroup a CU and 512 k that takes the GPU as long as rounding in a launch of its own (float32 1000 x 385 x
 // 771 9.0 us and 9.3; bfloat16 128 x 512 x 2048 9.9 and 8.2; with 1024 k 12 and 10), and the caller a launch and a workspace
 // less, which is what calls of this size wait for (15 us a call and 10).
@@ -480,7 +487,8 @@ fgpu_status layer(const void* d_x, const float* d_x_scale, const void* d_w, cons
   f.bias = d_bias, f.residual = d_residual, f.out = d_y, f.act = act;
   const int8_t* w = (const int8_t*)d_w;
   hipStream_t s = as_stream(stream);
-  if (dtype == FGPU_DTYPE_F32) return run_layer<float>(d_x, d_x_scale, w, d_w_scale, rows, in_dim, n, gated, f, d_ws, ws_bytes, s);
+  if (dtype == FGPU_DTYPE_F32)
+    return run_layer<float>(d_x, d_x_scale, w, d_w_scale, rows, in_dim, n, gated, f, d_ws, ws_bytes, s);
   return run_layer<bf16>(d_x, d_x_scale, w, d_w_scale, rows, in_dim, n, gated, f, d_ws, ws_bytes, s);
 }
 

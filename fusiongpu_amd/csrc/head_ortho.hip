@@ -7,6 +7,12 @@
 // lies above 2^-25 of one, and all of them stay below 2^6 while the singular values stay below about two.  The steps
 // multiply a small singular value by up to a each, and with it whatever a rounding leaves in its directions, so X may not
 // be rounded to one plane of 8 or 11 bits between them.
+//
+// 8192 x 1024 in bfloat16, five steps, takes 0.38 ms: A 19 us a step as seven parts of its triangle (strided operands, 18
+// steps of k a workgroup) and 7 to join them, P 12 or 15, X' 31 in one plane (17 of matrix instructions, then 64 MB of X read
+// and written, which a product of one round of workgroups cannot overlap; reading X before the products in half of them gains
+// nothing) and 58 in two (three products, 1.25 PFLOP/s of them), norm and start 23.  128 x 771 in float32 72 us: seventeen
+// launches, of which none takes under 3 us: A 5.2 (one launch, k over sixteen waves; in parts 8.3), P 3.3, X' 3.5.
 #include <algorithm>
 #include <cmath>
 
@@ -64,18 +70,14 @@ __global__ __launch_bounds__(256) void norm_parts_kernel(const T* x, int64_t cou
 }
 
 template <class T>
-__global__ __launch_bounds__(256) void start_kernel(const T* x, int64_t rows, int cols, const double* part, int parts, float eps,
-                                                    Planes out) {
-  __shared__ double sum[256];
-  double v = 0;
-  for (int i = threadIdx.x; i < parts; i += 256) v += part[i];
-  sum[threadIdx.x] = v;
-  __syncthreads();
-  for (int h = 128; h > 0; h >>= 1) {
-    if ((int)threadIdx.x < h) sum[threadIdx.x] += sum[threadIdx.x + h];
-    __syncthreads();
-  }
-  const double norm = sqrt(sum[0]) + eps;
+__global__ __launch_bounds__(256) void start_kernel(const T* x, int64_t rows, int cols, const double* part, int parts,
+                                                    float eps, Planes out) {
+  double v = 0;  // each wave adds all parts, in the same order
+#pragma unroll 8
+  for (int i = threadIdx.x & 63; i < kNormBlocks; i += kWave) v += i < parts ? part[i] : 0;
+#pragma unroll
+  for (int h = 32; h > 0; h >>= 1) v += __shfl_xor(v, h, kWave);
+  const double norm = sqrt(v) + eps;
   // Something not finite makes everything NaN; nothing but zeros stays zero.
   const double by = !(norm < INFINITY) ? (double)NAN : norm > 0 ? kHeld / norm : 0;
   // In float32 where the factor is far from the ends of the type.
@@ -247,7 +249,8 @@ struct FewRead {
 #pragma unroll
       for (int p = 0; p < P; ++p)
 #pragma unroll
-        for (int i = 0; i < F; ++i) *reinterpret_cast<bf16x8*>(lds + p * kFewBK * row_bytes + (lane + kWave * i) * 16) = r[p][i];
+        for (int i = 0; i < F; ++i)
+          *reinterpret_cast<bf16x8*>(lds + p * kFewBK * row_bytes + (lane + kWave * i) * 16) = r[p][i];
       wave_lds_order();
       const int l = lane & 15, g = lane >> 4;
 #pragma unroll
@@ -289,7 +292,8 @@ __global__ __launch_bounds__(kFewWaves * kWave) void few_tiles_kernel(Planes a, 
       for (int i = 0; i < 2; ++i)
 #pragma unroll
         for (int q = 0; q < PAIRS; ++q)
-          acc[i][j] = OfHalf::mma(fb[i][PAIRS == 1 ? 0 : pair_b<PAIRS>(q)], fa[j][PAIRS == 1 ? 0 : pair_a<PAIRS>(q)], acc[i][j]);
+          acc[i][j] = OfHalf::mma(fb[i][PAIRS == 1 ? 0 : pair_b<PAIRS>(q)], fa[j][PAIRS == 1 ? 0 : pair_a<PAIRS>(q)],
+                                  acc[i][j]);
   };
   for (int s = s0; s < s1; s += 2) {  // two steps' loads in flight
     RA a0, a1;
@@ -373,7 +377,8 @@ struct SymmetricCut {
   Cut whole, part;
   bool joined;
   size_t part_bytes(int n) const {
-    return joined ? carve_bytes<float>((size_t)part.splits * triangle_tiles(ceil_div(n, part.tile)) * part.tile * part.tile) : 0;
+    const size_t tiles = triangle_tiles(ceil_div(n, part.tile));
+    return joined ? carve_bytes<float>(part.splits * tiles * part.tile * part.tile) : 0;
   }
 };
 SymmetricCut cut_symmetric(int n, int k, int pairs, bool strided) {
@@ -385,7 +390,8 @@ SymmetricCut cut_symmetric(int n, int k, int pairs, bool strided) {
       if (splits > 1 && (splits > ceil_div(k, 2 * kGemmBK) || tiles * splits > 2048)) break;
       Cut q{tile, splits, ceil_div(ceil_div(k, kGemmBK), splits) * kGemmBK};
       if (ceil_div(k, q.k_per_split) != splits) continue;
-      q.us = cut_us(q, pairs, strided, tiles, tile == 256 ? 6 : tile == 128 ? 3.5 : 2.5) + 4 + tiles * splits * tile * tile * 8.0 / 5e6;
+      q.us = cut_us(q, pairs, strided, tiles, tile == 256 ? 6 : tile == 128 ? 3.5 : 2.5);
+      q.us += 4 + tiles * splits * tile * tile * 8.0 / 5e6;  // the join
       if (!c.part.tile || q.us < c.part.us) c.part = q;
     }
   }
@@ -411,9 +417,12 @@ fgpu_status run_whole(const Planes& a, const Planes& b, int k, const OrthoFinish
       constexpr int W = decltype(waves)::value, FM = decltype(fm)::value;
       few_tiles_kernel<T, PAIRS, AKC, BKC, W, FM><<<ceil_div(f.m, 16 * FM) * across, W * kWave, 0, s>>>(a, b, k, f);
     };
-    using std::integral_constant;
-    if (many) half ? go(integral_constant<int, 16>{}, integral_constant<int, 1>{}) : go(integral_constant<int, 16>{}, integral_constant<int, 2>{});
-    else half ? go(integral_constant<int, 8>{}, integral_constant<int, 1>{}) : go(integral_constant<int, 8>{}, integral_constant<int, 2>{});
+    const std::integral_constant<int, 1> w1{};
+    const std::integral_constant<int, 2> w2{};
+    const std::integral_constant<int, 8> w8{};
+    const std::integral_constant<int, 16> w16{};
+    if (many) half ? go(w16, w1) : go(w16, w2);
+    else half ? go(w8, w1) : go(w8, w2);
     FGPU_HIP(hipGetLastError());
     return FGPU_OK;
   }
@@ -435,12 +444,12 @@ fgpu_status run_symmetric(const Planes& a, int k, const OrthoFinish& f, float* p
   return FGPU_OK;
 }
 
-// How a step forms a X + P X.  In two planes as (a I + P) X, in one with X added apart, from both of its planes: a X + P X, or,
-// near the end, X + (P + (a - 1) I) X, whose second factor is small in the directions whose singular values have arrived.
+// How a step forms a X + P X.  In two planes as (a I + P) X, in one with X added apart, from both of its planes: a X + P X,
+// or, near the end, X + (P + (a - 1) I) X, whose second factor is small in the directions whose singular values have arrived.
 //
 // Of bfloat16 updates A takes one plane of X, and the first two and the last two steps one plane in the other products too:
-// what the first roundings leave lies in the directions of large singular values, which the later steps do not multiply,
-// and the last ones' is little, as said.  Against 64 bits (64 to 512 rows; singular values even, of normal numbers, as i^-1/2 to
+// what the first roundings leave lies in the directions of large singular values, which the later steps do not multiply, and
+// the last ones' is little, as said.  Against 64 bits (64 to 512 rows; singular values even, of normal numbers, as i^-1/2 to
 // i^-2; four to eight steps) the result is then off by at most 1.4e-3 of its norm, mostly below 7e-4, before it is rounded to
 // bfloat16 (1.7e-3); with one plane in every product and P as it is 2.7e-3, with X in one plane as well up to 8e-3.  Of more
 // steps A's rounding leaves up to 1.9e-3, and coefficients larger than the usual ones more than that: those take two.
@@ -465,7 +474,8 @@ struct Shape {
   size_t part_bytes() const {
     size_t b = 0;
     for (int pairs : {1, 3})
-      b = std::max({b, cut_symmetric(small, large, pairs, tall).part_bytes(small), cut_symmetric(small, small, pairs, false).part_bytes(small)});
+      b = std::max({b, cut_symmetric(small, large, pairs, tall).part_bytes(small),
+                    cut_symmetric(small, small, pairs, false).part_bytes(small)});
     return b;
   }
 };
@@ -474,24 +484,28 @@ Planes planes_at(void* p, int rows, int cols) { return {(uint16_t*)p, packed_ld(
 fgpu_status check_common(int64_t rows, int64_t cols, int dtype) {
   FGPU_CHECK(dtype == FGPU_DTYPE_F32 || dtype == FGPU_DTYPE_BF16, FGPU_ERR_ARG, "orthogonalize: unknown dtype");
   FGPU_CHECK(rows >= 0 && cols >= 0, FGPU_ERR_ARG, "orthogonalize: rows and cols >= 0");
-  FGPU_CHECK(rows <= FGPU_HEAD_MAX_DIM && cols <= FGPU_HEAD_MAX_DIM, FGPU_ERR_UNSUPPORTED, "orthogonalize: more than 2^16 rows or columns");
+  FGPU_CHECK(rows <= FGPU_HEAD_MAX_DIM && cols <= FGPU_HEAD_MAX_DIM, FGPU_ERR_UNSUPPORTED,
+             "orthogonalize: more than 2^16 rows or columns");
   return FGPU_OK;
 }
 
 template <class T, int PAIRS>
 fgpu_status gram(const Planes& x, const Shape& sh, const OrthoFinish& f, float* part, hipStream_t s) {
-  return sh.tall ? run_symmetric<T, PAIRS, false>(x, sh.large, f, part, s) : run_symmetric<T, PAIRS, true>(x, sh.large, f, part, s);
+  if (sh.tall) return run_symmetric<T, PAIRS, false>(x, sh.large, f, part, s);
+  return run_symmetric<T, PAIRS, true>(x, sh.large, f, part, s);
 }
 template <class T, int PAIRS>
 fgpu_status step(const Planes& x, const Planes& p, const Shape& sh, const OrthoFinish& f, hipStream_t s) {
   const Cut q = cut_product(f.m, f.n, sh.small, PAIRS, sh.tall ? 0 : 1);
-  return sh.tall ? run_whole<T, PAIRS, true, true>(x, p, sh.small, f, q, s) : run_whole<T, PAIRS, true, false>(p, x, sh.small, f, q, s);
+  if (sh.tall) return run_whole<T, PAIRS, true, true>(x, p, sh.small, f, q, s);
+  return run_whole<T, PAIRS, true, false>(p, x, sh.small, f, q, s);
 }
 
 template <class T>
 fgpu_status run_ortho(const T* x, const Shape& sh, int steps, float a, float b, float c, float eps, T* out, Carve& ws,
                       hipStream_t s) {
-  Planes xs[2] = {planes_at(ws.take<char>(sh.x_bytes()), sh.rows, sh.cols), planes_at(ws.take<char>(sh.x_bytes()), sh.rows, sh.cols)};
+  Planes xs[2];
+  for (Planes& x2 : xs) x2 = planes_at(ws.take<char>(sh.x_bytes()), sh.rows, sh.cols);
   const Planes ga = planes_at(ws.take<char>(sh.a_bytes()), sh.small, sh.small);
   const Planes gp = planes_at(ws.take<char>(sh.a_bytes()), sh.small, sh.small);
   float* part = (float*)ws.take<char>(sh.part_bytes());
@@ -540,7 +554,8 @@ fgpu_status fgpu_orthogonalize(const void* d_x, int64_t rows, int64_t cols, int 
                                float eps, void* d_y, void* d_workspace, size_t workspace_bytes, void* stream) {
   FGPU_TRY(check_common(rows, cols, dtype));
   FGPU_CHECK(steps >= 1 && steps <= FGPU_ORTHO_MAX_STEPS, FGPU_ERR_ARG, "orthogonalize: 1 to 64 steps");
-  FGPU_CHECK(std::isfinite(a) && std::isfinite(b) && std::isfinite(c), FGPU_ERR_ARG, "orthogonalize: coefficients must be finite");
+  FGPU_CHECK(std::isfinite(a) && std::isfinite(b) && std::isfinite(c), FGPU_ERR_ARG,
+             "orthogonalize: coefficients must be finite");
   FGPU_CHECK(eps >= 0 && std::isfinite(eps), FGPU_ERR_ARG, "orthogonalize: eps >= 0");
   if (rows == 0 || cols == 0) return FGPU_OK;
   FGPU_CHECK(d_x && d_y, FGPU_ERR_ARG, "orthogonalize: null input or output");

@@ -1,8 +1,8 @@
 // mfma_gemm.hpp -- the matrix-product core of the query head's operators (head_linear.hip, head_gated.hip, head_int8.hip,
 // head_ortho.hip, head_loss.hip).
 //
-// D[m][n] = sum_k A(m, k) B(n, k) on MFMA, bf16 with float32 accumulators unless said otherwise (OfHalf, OfInt8).  Each operand is read either with k contiguous
-// (rows of k) or with k strided (rows of m or n, one row a k), so the forward product x W^T and both gradients dz W and
+// D[m][n] = sum_k A(m, k) B(n, k) on MFMA, bf16 with float32 accumulators unless said otherwise (OfHalf, OfInt8).  Each
+// operand is read either with k contiguous (rows of k) or with k strided (rows of m or n, one row a k), so the forward product x W^T and both gradients dz W and
 // dz^T x come from one kernel without a transposed copy.  float32 operands are held as three bf16 planes (split2
 // below) and the k loop walks the six plane pairs that are more than 2^-22 of the whole.
 #pragma once
@@ -437,7 +437,8 @@ struct GemmWave {
 // acc[f][j]: a lane holds columns col(p) .. col(p) + 7 of row(j) in acc[2 p][j] and acc[2 p + 1][j].
 
 template <class T, bool BKC, int FORM, int BK = kGemmBK>
-using GemmLoadB = std::conditional_t<FORM == kGated, GatedTileLoad<T::BN, T::threads, BK>, TileLoad<T::BN, T::threads, BKC, true, BK>>;
+using GemmLoadB = std::conditional_t<FORM == kGated, GatedTileLoad<T::BN, T::threads, BK>,
+                                     TileLoad<T::BN, T::threads, BKC, true, BK>>;
 
 // One workgroup a tile.  Of a k step's 64, the fragments of one half are read while the other half's products run, so the
 // LDS's latency passes behind the matrix instructions; the step's only barrier lies between its halves, when every wave

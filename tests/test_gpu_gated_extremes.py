@@ -118,3 +118,22 @@ def test_coefficients_that_diverge(dt, steps):
     """(4, -6, 3) sends singular values past 64 before the fifth step (1.38, 1.56, 4.2, 3.5e3, ...): nothing finite comes back."""
     y = fg.orthogonalize(rnd(1, 60, 90, dtype=dt), steps=steps, coefficients=(4.0, -6.0, 3.0))
     assert not torch.isfinite(y).any()
+
+
+@pytest.mark.parametrize("dt", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("m,n", [(2110, 1317), (2300, 3100), (4351, 4049), (4004, 6054), (7300, 5606)])
+def test_large_orthogonalisations(m, n, dt):
+    """Every tile, whole products and joined triangles.  The bound of the operator's own tests: for each step 16 (2^-22 + 3
+    sqrt(k) u) |X_i| 3.4445^(steps left), and of bfloat16 2.8e-3 of the result's norm as above."""
+    x = rnd(m, m, n, dtype=dt)
+    y = fg.orthogonalize(x).double()
+    z = x.double()
+    z = z / (z.norm() + 1e-7)
+    if m > n:
+        z, y = z.t().contiguous(), y.t()
+    bound = 0.0
+    for i in range(5):
+        bound += 16 * (2.0**-22 + 3 * max(m, n)**0.5 * U) * z.norm().item() * 3.4445**(4 - i)
+        g = z @ z.t().contiguous()
+        z = 3.4445 * z + (-4.7750 * g + 2.0315 * (g @ g)) @ z
+    assert (y - z).norm() <= (bound + U * z.norm() if dt is torch.float32 else 2.8e-3 * z.norm())
