@@ -104,20 +104,23 @@ __device__ __forceinline__ void put8_n(uint16_t* d, int64_t plane, const f32x8& 
   }
 }
 
-// The same of a gated layer: a thread eight hidden columns, both halves of dz.
+// The same of a gated layer: a thread eight hidden columns, both halves of dz; of narrow layers a wave two, four or eight rows
+// at once (4099 x 96 in float32, the sums alone: 8.1 -> 5.4 us).
 template <class T>
 __device__ __forceinline__ void make_gated_dz(const DzJob& j, int block) {
   __shared__ float sum[2][3][512];
   const int across = (j.cols + 2 * kDzCols - 1) / (2 * kDzCols), chunk = block / across;
   const int lane = threadIdx.x & 63, w = threadIdx.x >> 6;
-  const int c = block % across * 2 * kDzCols + lane * 8, cnt = min(j.cols - c, 8);
+  const int log_wide = j.cols > 256 ? 6 : j.cols > 128 ? 5 : j.cols > 64 ? 4 : 3, wide = 1 << log_wide;  // lanes of a row
+  const int c = block % across * 2 * kDzCols + (lane & (wide - 1)) * 8, cnt = min(j.cols - c, 8);
   const int per = (j.rows + j.chunks - 1) / j.chunks, r0 = chunk * per, r1 = min(j.rows, r0 + per);
+  const int first = r0 + ((w * kWave + lane) >> log_wide), next = 256 >> log_wide;
   uint16_t* dst = const_cast<uint16_t*>(j.dst.p);
   f32x8 ag{{0, 0, 0, 0}, {0, 0, 0, 0}}, au = ag;
   if (cnt > 0) {
     const int pad = c + 8 >= j.cols ? (int)whole8(2 * j.cols) - 2 * j.cols : 0;  // zeros behind the row
 #pragma unroll 2
-    for (int r = r0 + w; r < r1; r += 4) {
+    for (int r = first; r < r1; r += next) {
       const T* pre = (const T*)j.pre + (int64_t)r * 2 * j.cols + c;
       const f32x8 d = load8_n((const T*)j.dy + (int64_t)r * j.cols + c, cnt);
       const f32x8 g = load8_n(pre, cnt), u = load8_n(pre + j.cols, cnt);
@@ -140,12 +143,19 @@ __device__ __forceinline__ void make_gated_dz(const DzJob& j, int block) {
     }
   }
   if (!j.part) return;
+  for (int h = wide; h < kWave; h *= 2) {  // a wave's rows
+#pragma unroll
+    for (int k = 0; k < 8; ++k) {
+      ag.set(k, ag[k] + __shfl_xor(ag[k], h, kWave));
+      au.set(k, au[k] + __shfl_xor(au[k], h, kWave));
+    }
+  }
   if (w) {
 #pragma unroll
     for (int k = 0; k < 8; ++k) sum[0][w - 1][lane + 64 * k] = ag[k], sum[1][w - 1][lane + 64 * k] = au[k];
   }
   __syncthreads();
-  if (w || cnt <= 0) return;
+  if (w || cnt <= 0 || lane >= wide) return;
   float* d = j.part + (int64_t)chunk * 2 * j.cols + c;
 #pragma unroll
   for (int k = 0; k < 8; ++k) {

@@ -127,6 +127,16 @@ def check_grads(dh, x, w, pre, act, dt, dx, dw, db):
 
 
 @pytest.mark.parametrize("dt", ["f32", "bf16"])
+@pytest.mark.parametrize("n", [7, 8, 63, 64, 65, 127, 128, 129, 200, 255, 256, 257])
+def test_backward_of_narrow_layers(n, dt):
+    """Every count of rows a wave takes at once, of rows that do not divide by it."""
+    t = TYPES[dt]
+    dh, x, w = rnd(1, 715, n, dtype=t), rnd(2, 715, 41, dtype=t), rnd(3, 2 * n, 41, scale=0.2, dtype=t)
+    pre = rnd(4, 715, 2 * n, dtype=t)
+    check_grads(dh, x, w, pre, "silu", dt, *fg.gated_linear_backward(dh, x, w, pre, act="silu"))
+
+
+@pytest.mark.parametrize("dt", ["f32", "bf16"])
 @pytest.mark.parametrize("act", ACTS)
 def test_backward_activations(act, dt):
     t = TYPES[dt]
