@@ -34,17 +34,38 @@ __device__ __forceinline__ bool loss_row_live(const LossRows& r, int m) {
   return !(r.bias && r.bias[t] <= FGPU_MASK_BIAS);
 }
 
-// One thread four columns of a row, the workgroups of the job in turn.
+// Eight elements of an operand's row at any address, the first n of them.
+template <class T>
+__device__ __forceinline__ void put8_n(uint16_t* d, int64_t plane, const f32x8& v, int n) {
+  bf16x8 p[Frag<T>::planes];
+  if constexpr (sizeof(T) == 2) p[0] = to_bf16x8(v);
+  else split8(v, p[0], p[1], p[2]);
+#pragma unroll
+  for (int q = 0; q < Frag<T>::planes; ++q) {
+    bf16* at = (bf16*)d + q * plane;
+    if (n >= 8) {
+      *reinterpret_cast<bf16x8u*>(at) = p[q];
+    } else {
+#pragma unroll
+      for (int e = 0; e < 7; ++e)
+        if (e < n) at[e] = p[q][e];
+    }
+  }
+}
+
+// One thread eight columns of a row, the workgroups of the job in turn.
 template <class T>
 __device__ __forceinline__ void copy_rows(const CopyJob& j, const LossRows& loss, int block, int blocks) {
   uint16_t* dst = const_cast<uint16_t*>(j.dst.p);
-  const int64_t per = whole8(j.cols) / 4, total = j.rows * per;
-  for (int64_t i = (int64_t)block * 256 + threadIdx.x; i < total; i += (int64_t)blocks * 256) {
-    const int64_t r = i / per, c = (i - r * per) * 4;
-    f32x4 v = {0, 0, 0, 0};
+  const uint32_t per = (uint32_t)(whole8(j.cols) / 8);
+  const uint64_t total = j.rows * (uint64_t)per;
+  for (uint64_t i = (uint64_t)block * 256 + threadIdx.x; i < total; i += (uint64_t)blocks * 256) {
+    const int64_t r = total < (1ull << 32) ? (uint32_t)i / per : i / per;  // a 64-bit division takes some hundred cycles
+    const int c = (int)(i - r * (uint64_t)per) * 8;
+    f32x8 v{{0, 0, 0, 0}, {0, 0, 0, 0}};
     const bool zero = (j.row_bias && j.row_bias[r] <= FGPU_MASK_BIAS) || (j.loss_rows && !loss_row_live(loss, (int)r));
-    if (c < j.cols && !zero) v = load4_n((const T*)j.src + r * j.cols + c, (int)min(j.cols - c, (int64_t)4));
-    put4<T>(dst + r * j.dst.ld + c, j.dst.plane, v);
+    if (c < j.cols && !zero) v = load8_n((const T*)j.src + r * j.cols + c, (int)min((int64_t)j.cols - c, (int64_t)8));
+    put8_n<T>(dst + r * j.dst.ld + c, j.dst.plane, v, 8);
   }
 }
 
@@ -82,25 +103,6 @@ __device__ __forceinline__ void make_dz(const DzJob& j, int block) {
   if (w == 0 && cnt > 0) {
     for (int k = 1; k < 4; ++k) acc += sum[k][lane];
     for (int k = 0; k < min(cnt, 4); ++k) j.part[(int64_t)chunk * j.cols + c + k] = acc[k];
-  }
-}
-
-// Eight elements of an operand's row at any address, the first n of them.
-template <class T>
-__device__ __forceinline__ void put8_n(uint16_t* d, int64_t plane, const f32x8& v, int n) {
-  bf16x8 p[Frag<T>::planes];
-  if constexpr (sizeof(T) == 2) p[0] = to_bf16x8(v);
-  else split8(v, p[0], p[1], p[2]);
-#pragma unroll
-  for (int q = 0; q < Frag<T>::planes; ++q) {
-    bf16* at = (bf16*)d + q * plane;
-    if (n >= 8) {
-      *reinterpret_cast<bf16x8u*>(at) = p[q];
-    } else {
-#pragma unroll
-      for (int e = 0; e < 7; ++e)
-        if (e < n) at[e] = p[q][e];
-    }
   }
 }
 
@@ -207,7 +209,7 @@ int dz_chunks(int rows, int cols) {
 
 fgpu_status launch_prep(const Prep& p, bool f32, hipStream_t s) {
   auto copy_blocks = [](const CopyJob& j) {
-    return j.src ? (int)std::min<int64_t>(ceil_div(j.rows * (whole8(j.cols) / 4), 256), 8192) : 0;
+    return j.src ? (int)std::min<int64_t>(ceil_div(j.rows * (whole8(j.cols) / 8), 256), 8192) : 0;
   };
   Blocks n{0, copy_blocks(p.copy[0]), copy_blocks(p.copy[1]), 0, 0};
   if (p.dz.dy) n.dz = ceil_div(p.dz.cols, p.dz.gated ? 2 * kDzCols : kDzCols) * p.dz.chunks;
