@@ -305,7 +305,7 @@ __global__ __launch_bounds__(kFewThreads) void few_rows_kernel(FewJob j) {
     const float r = row_scale[m];
     f32x4 o;
 #pragma unroll
-    for (int e = 0; e < 4; ++e) o[e] = (float)v[e] * r * by[e];
+    for (int e = 0; e < 4; ++e) o[e] = (float)v[e] * by[e] * r;
     return o;
   };
   if constexpr (GATED)
