@@ -11,8 +11,8 @@
 // 8192 x 1024 in bfloat16, five steps, takes 0.38 ms: A 19 us a step as seven parts of its triangle (strided operands, 18
 // steps of k a workgroup) and 7 to join them, P 12 or 15, X' 31 in one plane (17 of matrix instructions, then 64 MB of X read
 // and written, which a product of one round of workgroups cannot overlap; reading X before the products in half of them gains
-// nothing) and 58 in two (three products, 1.25 PFLOP/s of them), norm and start 23.  128 x 771 in float32 72 us: seventeen
-// launches, of which none takes under 3 us: A 5.2 (one launch, k over sixteen waves; in parts 8.3), P 3.3, X' 3.5.
+// nothing) and 58 in two (three products, 1.25 PFLOP/s of them), norm and start 23.  128 x 771 in float32 70 us: twelve
+// launches, of a step A (one launch, k over sixteen waves; in parts 8.3), then P and X'.
 #include <algorithm>
 #include <cmath>
 
@@ -326,6 +326,97 @@ __global__ __launch_bounds__(kFewWaves * kWave) void few_tiles_kernel(Planes a, 
   if (row < f.m && col < ((f.n + 7) & ~7)) f.put<T>(v, row, col);
 }
 
+// A step's P and its product with X in one launch, of short sides: a workgroup of eight waves forms the rows of P that its
+// 16 x 32 of the result need (P is symmetric: 16 of them where X is wide, 32 where it is tall) into LDS, a wave 16 x 32 with
+// all its loads in flight at once, and then each wave takes one step of k of the product, whose part of X is on the way
+// meanwhile.  Every workgroup of a row (column) forms the same rows of P: it pays while there are CUs for all and a wave's
+// part is one round of loads.  us of five steps in float32, one launch / two: 64 x 256 48 / 58, 128 x 771 70 / 74, 1300 x 96
+// 77 / 83, but 771 x 128 84 / 74, 192 x 500 81 / 71.
+constexpr int kBothWide = 128, kBothTall = 96;
+constexpr int kBothWaves = 8, kBothSteps = kBothWide / kFewBK, kBothStride = kBothWide + 8;  // rows fall on different banks
+template <class T, int PP, int PAIRS, bool TALL>
+__global__ __launch_bounds__(kBothWaves * kWave) void both_kernel(Planes a, OrthoFinish fp, Planes x, OrthoFinish f) {
+  using RX = FewRead<PAIRS, TALL, !TALL, TALL ? 1 : 2>;
+  constexpr int P = planes_of(PAIRS), kRows = TALL ? 32 : 16;
+  constexpr int stage = kBothWaves * RX::lds_bytes, joined = kBothWaves * 2 * kWave * 16;
+  __shared__ __attribute__((aligned(1024))) char lds[stage > joined ? stage : joined];
+  __shared__ __attribute__((aligned(16))) uint16_t strip[P][kRows][kBothStride];
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), l = lane & 15;
+  const int across = (f.n + 31) / 32, m0 = blockIdx.x / across * 16, n0 = blockIdx.x % across * 32;
+  const int n = fp.n, n8 = (n + 7) & ~7, steps = (n + kFewBK - 1) / kFewBK, p0 = TALL ? n0 : m0;
+  const bool mine = wave < steps;
+  RX rx;
+  if (mine) rx.load(x, TALL ? m0 : n0, TALL ? f.m : f.n, wave * kFewBK, n, lane);
+  static_assert(kBothTall / kFewBK * 2 <= kBothWaves && kBothSteps <= kBothWaves, "a part of P a wave, a step a wave");
+  if (wave < steps * (kRows / 16)) {
+    const int r = wave % (kRows / 16) * 16, c0 = wave / (kRows / 16) * 32;
+    f32x4 acc[2] = {{0, 0, 0, 0}, {0, 0, 0, 0}};
+    FewRead<PP, true, false, 1> ra[kBothSteps];
+    FewRead<PP, true, true> rb[kBothSteps];
+#pragma unroll
+    for (int h = 0; h < kBothSteps; ++h) {  // past the end: zeros
+      ra[h].load(a, p0 + r, n, h * kFewBK, n, lane);
+      rb[h].load(a, c0, n, h * kFewBK, n, lane);
+    }
+#pragma unroll
+    for (int h = 0; h < kBothSteps; ++h)
+#pragma unroll
+      for (int i = 0; i < 2; ++i)
+#pragma unroll
+        for (int q = 0; q < PP; ++q)
+          acc[i] = OfHalf::mma(rb[h].r[PP == 1 ? 0 : pair_b<PP>(q)][i], ra[h].r[PP == 1 ? 0 : pair_a<PP>(q)][0], acc[i]);
+    const int row = p0 + r + l, col = c0 + 8 * (lane >> 4);
+    f32x8 v{{0, 0, 0, 0}, {0, 0, 0, 0}};
+    if (row < n && col < n8) v = fp.value(f32x8{acc[0], acc[1]}, row, col, true);
+#pragma unroll
+    for (int q = 0; q < P; ++q) {
+      f16x8 h;
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        h[e] = (_Float16)v[e];
+        if (q + 1 < P) v.set(e, v[e] - (float)h[e]);
+      }
+      *reinterpret_cast<f16x8*>(&strip[q][r + l][col]) = h;
+    }
+  }
+  __syncthreads();
+  f32x4 acc[2] = {{0, 0, 0, 0}, {0, 0, 0, 0}};
+  if (mine) {
+    constexpr int FX = TALL ? 1 : 2, FP = TALL ? 2 : 1;
+    bf16x8 fx[FX][P], pf[FP][P];
+    rx.frags(fx, lds + wave * RX::lds_bytes, lane);
+#pragma unroll
+    for (int q = 0; q < P; ++q)
+#pragma unroll
+      for (int i = 0; i < FP; ++i)
+        pf[i][q] = *reinterpret_cast<const bf16x8*>(
+            &strip[q][TALL ? 8 * (l >> 2) + 4 * i + (l & 3) : l][wave * kFewBK + 8 * (lane >> 4)]);
+#pragma unroll
+    for (int i = 0; i < 2; ++i)
+#pragma unroll
+      for (int q = 0; q < PAIRS; ++q) {
+        const int qa = PAIRS == 1 ? 0 : pair_a<PAIRS>(q), qb = PAIRS == 1 ? 0 : pair_b<PAIRS>(q);
+        if constexpr (TALL) acc[i] = OfHalf::mma(pf[i][qb], fx[0][qa], acc[i]);
+        else acc[i] = OfHalf::mma(fx[i][qb], pf[0][qa], acc[i]);
+      }
+  }
+  __syncthreads();
+  f32x4* join = reinterpret_cast<f32x4*>(lds);  // [wave][column fragment][lane]
+  if (mine) join[wave * 2 * kWave + lane] = acc[0], join[(wave * 2 + 1) * kWave + lane] = acc[1];
+  __syncthreads();
+  if (wave) return;
+  const int row = m0 + l, col = n0 + 8 * (lane >> 4);
+  f32x8 v{acc[0], acc[1]};
+#pragma unroll
+  for (int w = 1; w < kBothSteps; ++w) {
+    if (w < steps) v.lo += join[w * 2 * kWave + lane], v.hi += join[(w * 2 + 1) * kWave + lane];
+  }
+  if (row < f.m && col < ((f.n + 7) & ~7)) f.put<T>(v, row, col);
+}
+bool takes_both(int rows, int cols) {
+  return std::min(rows, cols) <= (rows > cols ? kBothTall : kBothWide) && (int64_t)ceil_div(rows, 16) * ceil_div(cols, 32) <= 256;
+}
+
 // ---- how a product is cut ------------------------------------------------------------
 // Microseconds, fitted over sides of 64 to 4096 and k to 8192: a step of k (64 of one plane, 32 of two) of a workgroup while
 // it has its CU to itself, for each of those that share one, and how many do; both operands k contiguous (a strided one takes
@@ -501,6 +592,15 @@ fgpu_status step(const Planes& x, const Planes& p, const Shape& sh, const OrthoF
   return run_whole<T, PAIRS, true, false>(p, x, sh.small, f, q, s);
 }
 
+template <class T, int PP, int PAIRS>
+fgpu_status both(const Planes& a, const OrthoFinish& fp, const Planes& x, const Shape& sh, const OrthoFinish& f, hipStream_t s) {
+  const int grid = ceil_div(f.m, 16) * ceil_div(f.n, 32);
+  if (sh.tall) both_kernel<T, PP, PAIRS, true><<<grid, kBothWaves * kWave, 0, s>>>(a, fp, x, f);
+  else both_kernel<T, PP, PAIRS, false><<<grid, kBothWaves * kWave, 0, s>>>(a, fp, x, f);
+  FGPU_HIP(hipGetLastError());
+  return FGPU_OK;
+}
+
 template <class T>
 fgpu_status run_ortho(const T* x, const Shape& sh, int steps, float a, float b, float c, float eps, T* out, Carve& ws,
                       hipStream_t s) {
@@ -531,6 +631,15 @@ fgpu_status run_ortho(const T* x, const Shape& sh, int steps, float a, float b, 
     if (last) fx.out = out, fx.alpha /= kHeld, fx.beta /= kHeld;
     FGPU_TRY((m.gram == 1 ? gram<T, 1>(from, sh, fa, part, s) : gram<T, 3>(from, sh, fa, part, s)));
     const bool early = m.rest == 1 && !m.near_one;
+    if (takes_both(sh.rows, sh.cols)) {
+      if constexpr (sizeof(T) == 4) {
+        FGPU_TRY((both<T, 3, 3>(ga, fp, from, sh, fx, s)));
+      } else {
+        FGPU_TRY((early ? both<T, 1, 1>(ga, fp, from, sh, fx, s) : m.rest == 1 ? both<T, 3, 1>(ga, fp, from, sh, fx, s)
+                                                                               : both<T, 3, 3>(ga, fp, from, sh, fx, s)));
+      }
+      continue;
+    }
     FGPU_TRY((early ? run_symmetric<T, 1, true>(ga, n, fp, part, s) : run_symmetric<T, 3, true>(ga, n, fp, part, s)));
     FGPU_TRY((m.rest == 1 ? step<T, 1>(from, gp, sh, fx, s) : step<T, 3>(from, gp, sh, fx, s)));
   }

@@ -64,6 +64,16 @@ def test_orthogonalize(m, n, dt):
     check(rnd(m + n, m, n, scale=1e-3, dtype=TYPES[dt]), dt=dt)
 
 
+# A step in two launches and in three, of sides around both bounds and the waves' parts; rows of planes apart and not.
+@pytest.mark.parametrize("dt", ["f32", "bf16"])
+@pytest.mark.parametrize("m,n", [(1, 8192), (8192, 1), (16, 8193), (31, 100), (32, 33), (97, 97), (96, 97), (97, 96), (101, 96),
+                                 (127, 1024), (128, 128), (128, 1025), (129, 200), (200, 129), (65, 1600), (1600, 65), (64, 2048),
+                                 (256, 1024), (1024, 256), (256, 1032), (192, 192)])
+@pytest.mark.parametrize("steps", [1, 3, 5])
+def test_few_launches(m, n, dt, steps):
+    check(rnd(m * n + steps, m, n, dtype=torch.float32 if dt == "f32" else torch.bfloat16), steps=steps, dt=dt)
+
+
 @pytest.mark.parametrize("dt", ["f32", "bf16"])
 @pytest.mark.parametrize("m,n", [(96, 400), (400, 96), (256, 256)])
 @pytest.mark.parametrize("power", [0.5, 1.0, 2.0])
