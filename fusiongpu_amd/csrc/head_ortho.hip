@@ -11,8 +11,8 @@
 // 8192 x 1024 in bfloat16, five steps, takes 0.38 ms: A 19 us a step as seven parts of its triangle (strided operands, 18
 // steps of k a workgroup) and 7 to join them, P 12 or 15, X' 31 in one plane (17 of matrix instructions, then 64 MB of X read
 // and written, which a product of one round of workgroups cannot overlap; reading X before the products in half of them gains
-// nothing) and 58 in two (three products, 1.25 PFLOP/s of them), norm and start 23.  128 x 771 in float32 70 us: twelve
-// launches, of a step A (one launch, k over sixteen waves; in parts 8.3), then P and X'.
+// nothing) and 58 in two (three products, 1.25 PFLOP/s of them), norm and start 23.  128 x 771 in float32 65 us: twelve
+// launches, a step's two 6 each: A (k over sixteen waves; in parts 8.3), then P and X'.
 #include <algorithm>
 #include <cmath>
 
@@ -331,7 +331,7 @@ __global__ __launch_bounds__(kFewWaves * kWave) void few_tiles_kernel(Planes a, 
 // all its loads in flight at once, and then each wave takes one step of k of the product, whose part of X is on the way
 // meanwhile.  Every workgroup of a row (column) forms the same rows of P: it pays while there are CUs for all and a wave's
 // part is one round of loads.  us of five steps in float32, one launch / two: 64 x 256 48 / 58, 128 x 771 70 / 74, 1300 x 96
-// 77 / 83, but 771 x 128 84 / 74, 192 x 500 81 / 71.
+// 76 / 82, but 771 x 128 84 / 74, 192 x 500 81 / 71.
 constexpr int kBothWide = 128, kBothTall = 96;
 constexpr int kBothWaves = 8, kBothSteps = kBothWide / kFewBK, kBothStride = kBothWide + 8;  // rows fall on different banks
 template <class T, int PP, int PAIRS, bool TALL>
@@ -560,8 +560,17 @@ struct Shape {
   int rows, cols, small, large;
   bool tall;
   Shape(int r, int c) : rows(r), cols(c), small(std::min(r, c)), large(std::max(r, c)), tall(r > c) {}
-  size_t x_bytes() const { return carve_bytes<uint16_t>((size_t)rows * packed_ld(cols) * 2); }
-  size_t a_bytes() const { return carve_bytes<uint16_t>((size_t)small * packed_ld(small) * 2); }
+  // Where the kernels of few tiles work, rows a multiple of 128 bytes apart lie 16 bytes further: their loads take 64 bytes of
+  // sixteen rows at once (us, float32, apart / not: 128 x 771 65 / 70, 128 x 1024 72 / 81, 512 x 256 70 / 75; X's rows of tall
+  // matrices 75 / 70, and larger tiles take whole lines: 2048 x 1024 345 / 281).
+  int64_t apart(int c, bool more) const {
+    const int64_t ld = packed_ld(c);
+    return ld + (more && ld % 64 == 0 && small <= 256 && large <= 1024 ? 8 : 0);
+  }
+  int64_t x_ld() const { return apart(cols, !tall); }
+  int64_t a_ld() const { return apart(small, true); }
+  size_t x_bytes() const { return carve_bytes<uint16_t>((size_t)rows * x_ld() * 2); }
+  size_t a_bytes() const { return carve_bytes<uint16_t>((size_t)small * a_ld() * 2); }
   size_t part_bytes() const {
     size_t b = 0;
     for (int pairs : {1, 3})
@@ -570,7 +579,7 @@ struct Shape {
     return b;
   }
 };
-Planes planes_at(void* p, int rows, int cols) { return {(uint16_t*)p, packed_ld(cols), rows * packed_ld(cols)}; }
+Planes planes_at(void* p, int rows, int64_t ld) { return {(uint16_t*)p, ld, rows * ld}; }
 
 fgpu_status check_common(int64_t rows, int64_t cols, int dtype) {
   FGPU_CHECK(dtype == FGPU_DTYPE_F32 || dtype == FGPU_DTYPE_BF16, FGPU_ERR_ARG, "orthogonalize: unknown dtype");
@@ -605,9 +614,9 @@ template <class T>
 fgpu_status run_ortho(const T* x, const Shape& sh, int steps, float a, float b, float c, float eps, T* out, Carve& ws,
                       hipStream_t s) {
   Planes xs[2];
-  for (Planes& x2 : xs) x2 = planes_at(ws.take<char>(sh.x_bytes()), sh.rows, sh.cols);
-  const Planes ga = planes_at(ws.take<char>(sh.a_bytes()), sh.small, sh.small);
-  const Planes gp = planes_at(ws.take<char>(sh.a_bytes()), sh.small, sh.small);
+  for (Planes& x2 : xs) x2 = planes_at(ws.take<char>(sh.x_bytes()), sh.rows, sh.x_ld());
+  const Planes ga = planes_at(ws.take<char>(sh.a_bytes()), sh.small, sh.a_ld());
+  const Planes gp = planes_at(ws.take<char>(sh.a_bytes()), sh.small, sh.a_ld());
   float* part = (float*)ws.take<char>(sh.part_bytes());
   double* norm = ws.take<double>(kNormBlocks);
   FGPU_CHECK(ws.held(), FGPU_ERR_WORKSPACE, "orthogonalize: workspace smaller than fgpu_orthogonalize_workspace_bytes");
