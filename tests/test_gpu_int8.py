@@ -256,3 +256,19 @@ def test_same_bits_on_another_stream_and_replayed(dt, m):
         torch.cuda.synchronize()
         got = [o.clone() for o in out]
         assert all(torch.equal(p, q) for p, q in zip(got, every()))
+
+
+@pytest.mark.parametrize("dt", ["f32", "bf16"])
+@pytest.mark.parametrize("m,k,n", [(700, 600, 200), (2049, 640, 1111), (6000, 528, 2120), (9001, 1040, 2304)])
+def test_residual_in_place_of_every_tile(m, k, n, dt):
+    """Rows and columns that end inside a tile and inside a wave's 64 columns, the residual where the result goes."""
+    t = TYPES[dt]
+    x, r, b = rnd(1, m, k, dtype=t), rnd(2, m, n, dtype=t), rnd(4, n, dtype=t)
+    q, s = fg.quantize_rows(rnd(3, n, k, scale=1 / math.sqrt(k)))
+    check_layer(m, k, n, dt, "gelu", True, True, False, False)
+    want = fg.linear_int8(x, q, s, b, r, act="gelu")
+    hold = torch.full((m * n + 64,), 7.0, dtype=t, device="cuda")
+    y = hold[32:32 + m * n].view(m, n)
+    y.copy_(r)
+    assert torch.equal(fg.linear_int8(x, q, s, b, y, act="gelu", out=y), want)
+    assert (hold[:32] == 7).all() and (hold[-32:] == 7).all()
