@@ -228,11 +228,14 @@ int products_tile(const Product* p, int count, int which);  // the width of its 
 // An array as an operand: itself where its rows can be read as they are (bf16, cols % 8 == 0), otherwise a copy with
 // rows of packed_ld(cols) elements, float32 as three planes.
 __host__ __device__ inline int64_t whole8(int64_t cols) { return (cols + 7) / 8 * 8; }
-// Rows a multiple of 4 KB apart fall on the same memory channels: 128 bytes more between them (the score gradient of 8192 x
-// 65536 with its two products at 768 dims 2.73 -> 2.52 ms; float32 4096 x 2048 x 2048 forward 295 -> 279 us; 16384 x 1024 x
-// 4096 bf16 backward 343 -> 343).
+// Rows begin on whole lines of 128 bytes, of which a tile's step takes one a row, where short rows' longer copies do not
+// cost more than that gives (float32 gradients of a gated layer 8192 x 1000 x 1500 995 -> 767 us, 20000 x 300 x 600 355 ->
+// 297, 8192 x 200 x 1030 218 -> 190, but 65536 x 72 x 100 119 -> 145; of a linear one 65536 x 385 x 771 1086 -> 851).  Rows a
+// multiple of 4 KB apart fall on the same memory channels: 128 bytes more between them (the score gradient of 8192 x 65536
+// with its two products at 768 dims 2.73 -> 2.52 ms; float32 4096 x 2048 x 2048 forward 295 -> 279 us; 16384 x 1024 x 4096
+// bf16 backward 343 -> 343).
 inline int64_t packed_ld(int64_t cols) {
-  const int64_t ld = whole8(cols);
+  const int64_t ld = cols > 128 ? (cols + 63) / 64 * 64 : whole8(cols);
   return ld % 2048 ? ld : ld + 64;
 }
 inline bool needs_pack(int64_t cols, bool f32) { return f32 || cols % 8 != 0; }

@@ -560,12 +560,13 @@ struct Shape {
   int rows, cols, small, large;
   bool tall;
   Shape(int r, int c) : rows(r), cols(c), small(std::min(r, c)), large(std::max(r, c)), tall(r > c) {}
-  // Where the kernels of few tiles work, rows a multiple of 128 bytes apart lie 16 bytes further: their loads take 64 bytes of
-  // sixteen rows at once (us, float32, apart / not: 128 x 771 65 / 70, 128 x 1024 72 / 81, 512 x 256 70 / 75; X's rows of tall
-  // matrices 75 / 70, and larger tiles take whole lines: 2048 x 1024 345 / 281).
+  // Where the kernels of few tiles work rows lie close, but those a multiple of 128 bytes apart 16 bytes further: their loads
+  // take 64 bytes of sixteen rows at once (us, float32, apart / not: 128 x 771 65 / 70, 128 x 1024 72 / 81, 512 x 256 70 / 75,
+  // 257 x 700 83 / 92, 500 x 700 130 / 139; X's rows of tall matrices 75 / 70).  Larger tiles take whole lines (2048 x 1024
+  // 345 / 281).
   int64_t apart(int c, bool more) const {
-    const int64_t ld = packed_ld(c);
-    return ld + (more && ld % 64 == 0 && small <= 256 && large <= 1024 ? 8 : 0);
+    if (small > 512 || large > 1024) return packed_ld(c);
+    return whole8(c) + (more && whole8(c) % 64 == 0 ? 8 : 0);
   }
   int64_t x_ld() const { return apart(cols, !tall); }
   int64_t a_ld() const { return apart(small, true); }
