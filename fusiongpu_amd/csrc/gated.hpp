@@ -28,14 +28,13 @@ __device__ __forceinline__ f32x8 eight(const A& lo, const A& hi, float row, cons
   return v;
 }
 
-// 64 columns of 16 rows in bfloat16, of which a lane holds eight from 8 (lane / 16) on and the eight 32 further (a and b) of
+// 64 columns of 16 rows of 16 bits each, of which a lane holds eight from 8 (lane / 16) on and the eight 32 further (a and b) of
 // row lane % 16, as 128 bytes of eight rows a store: lanes eight rows apart swap halves.  16 rows of 64 bytes each, half a
 // line, write a good third slower (65536 x 4096 with both factors kept, k 64 472 -> 333 us, k 1024 1120 -> 1080).  rows: how
 // many of the 16.
 template <bool STREAM>
-__device__ __forceinline__ void store_lines(bf16* p, int64_t ld, int lane, int rows, const f32x8& a, const f32x8& b) {
+__device__ __forceinline__ void store_lines(uint16_t* p, int64_t ld, int lane, int rows, const u32x4& x, const u32x4& y) {
   typedef uint32_t u32x4u __attribute__((ext_vector_type(4), aligned(2)));
-  const u32x4 x = __builtin_bit_cast(u32x4, to_bf16x8(a)), y = __builtin_bit_cast(u32x4, to_bf16x8(b));
   const bool upper = (lane & 8) == 0;
   u32x4 first, second;
 #pragma unroll
@@ -53,6 +52,11 @@ __device__ __forceinline__ void store_lines(bf16* p, int64_t ld, int lane, int r
     if (row < rows) *at = first;
     if (row + 8 < rows) *next = second;
   }
+}
+template <bool STREAM>
+__device__ __forceinline__ void store_lines(bf16* p, int64_t ld, int lane, int rows, const f32x8& a, const f32x8& b) {
+  store_lines<STREAM>((uint16_t*)p, ld, lane, rows, __builtin_bit_cast(u32x4, to_bf16x8(a)),
+                      __builtin_bit_cast(u32x4, to_bf16x8(b)));
 }
 
 template <class T, int ACT>

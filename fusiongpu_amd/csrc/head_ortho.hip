@@ -8,8 +8,8 @@
 // multiply a small singular value by up to a each, and with it whatever a rounding leaves in its directions, so X may not
 // be rounded to one plane of 8 or 11 bits between them.
 //
-// 8192 x 1024 in bfloat16, five steps, takes 0.38 ms: A 19 us a step as seven parts of its triangle (strided operands, 18
-// steps of k a workgroup) and 7 to join them, P 12 or 15, X' 31 in one plane (17 of matrix instructions, then 64 MB of X read
+// 8192 x 1024 in bfloat16, five steps, takes 0.37 ms: A 19 us a step as seven parts of its triangle (strided operands, 18
+// steps of k a workgroup) and 7 to join them, P 12 or 15, X' 29 in one plane (17 of matrix instructions, then 64 MB of X read
 // and written, which a product of one round of workgroups cannot overlap; reading X before the products in half of them gains
 // nothing) and 58 in two (three products, 1.25 PFLOP/s of them), norm and start 23.  128 x 771 in float32 65 us: twelve
 // launches, a step's two 6 each: A (k over sixteen waves; in parts 8.3), then P and X'.
@@ -38,13 +38,16 @@ __device__ __forceinline__ f32x8 planes8(const Planes& a, int64_t at) {
   for (int e = 0; e < 8; ++e) v.set(e, (float)h[e] + (float)l[e]);
   return v;
 }
-__device__ __forceinline__ void put_planes8(const Planes& a, int64_t at, const f32x8& v) {
-  f16x8 h, l;
+__device__ __forceinline__ void to_planes(const f32x8& v, f16x8& h, f16x8& l) {
 #pragma unroll
   for (int e = 0; e < 8; ++e) {
     h[e] = (_Float16)v[e];
     l[e] = (_Float16)(v[e] - (float)h[e]);
   }
+}
+__device__ __forceinline__ void put_planes8(const Planes& a, int64_t at, const f32x8& v) {
+  f16x8 h, l;
+  to_planes(v, h, l);
   *reinterpret_cast<f16x8*>(a.p + at) = h;
   *reinterpret_cast<f16x8*>(a.p + a.plane + at) = l;
 }
@@ -138,6 +141,9 @@ struct OrthoEpi {
   template <class G>
   __device__ __forceinline__ void finish(f32x4 (&acc)[G::FN][G::FM], const GemmWave<G>& w, char*, const Side<G>&) const {
     const int n8 = (f.n + 7) & ~7;
+    if constexpr (G::FN == 4) {
+      if (w.first_col() + 64 <= f.n && (sizeof(T) == 2 || !f.out)) return lines(acc, w);
+    }
 #pragma unroll
     for (int p = 0; p < G::FN / 2; ++p) {
       const int col = w.col(p);
@@ -147,6 +153,31 @@ struct OrthoEpi {
         const int64_t row = w.row(j);
         if (row < f.m) f.put<T>(f32x8{acc[2 * p][j], acc[2 * p + 1][j]}, row, col);
       }
+    }
+  }
+  // The same where a wave's 64 columns all lie inside: whole lines a store (8192 x 1024 in bfloat16 378 -> 369 us).
+  template <class G>
+  __device__ __forceinline__ void lines(f32x4 (&acc)[G::FN][G::FM], const GemmWave<G>& w) const {
+#pragma unroll
+    for (int j = 0; j < G::FM; ++j) {
+      const int64_t row = w.m0 + (w.wm * G::FM + j) * 16, mine = row + (w.lane & 15);
+      const int inside = (int)min((int64_t)16, f.m - row);
+      if (inside <= 0) break;
+      f32x8 v[2];
+#pragma unroll
+      for (int p = 0; p < 2; ++p)
+        v[p] = f.value(f32x8{acc[2 * p][j], acc[2 * p + 1][j]}, mine, w.col(p), mine < f.m);
+      if (sizeof(T) == 2 && f.out) {
+        store_lines<false>((bf16*)f.out + row * f.n + w.first_col(), f.n, w.lane, inside, v[0], v[1]);
+        continue;
+      }
+      f16x8 h[2], l[2];
+#pragma unroll
+      for (int p = 0; p < 2; ++p) to_planes(v[p], h[p], l[p]);
+      uint16_t* at = f.to.p + row * f.to.ld + w.first_col();
+      store_lines<false>(at, f.to.ld, w.lane, inside, __builtin_bit_cast(u32x4, h[0]), __builtin_bit_cast(u32x4, h[1]));
+      store_lines<false>(at + f.to.plane, f.to.ld, w.lane, inside, __builtin_bit_cast(u32x4, l[0]),
+                         __builtin_bit_cast(u32x4, l[1]));
     }
   }
 };
@@ -414,7 +445,8 @@ __global__ __launch_bounds__(kBothWaves * kWave) void both_kernel(Planes a, Orth
   if (row < f.m && col < ((f.n + 7) & ~7)) f.put<T>(v, row, col);
 }
 bool takes_both(int rows, int cols) {
-  return std::min(rows, cols) <= (rows > cols ? kBothTall : kBothWide) && (int64_t)ceil_div(rows, 16) * ceil_div(cols, 32) <= 256;
+  const int side = std::min(rows, cols), most = rows > cols ? kBothTall : kBothWide;
+  return side <= most && (int64_t)ceil_div(rows, 16) * ceil_div(cols, 32) <= 256;
 }
 
 // ---- how a product is cut ------------------------------------------------------------
@@ -603,7 +635,8 @@ fgpu_status step(const Planes& x, const Planes& p, const Shape& sh, const OrthoF
 }
 
 template <class T, int PP, int PAIRS>
-fgpu_status both(const Planes& a, const OrthoFinish& fp, const Planes& x, const Shape& sh, const OrthoFinish& f, hipStream_t s) {
+fgpu_status both(const Planes& a, const OrthoFinish& fp, const Planes& x, const Shape& sh, const OrthoFinish& f,
+                 hipStream_t s) {
   const int grid = ceil_div(f.m, 16) * ceil_div(f.n, 32);
   if (sh.tall) both_kernel<T, PP, PAIRS, true><<<grid, kBothWaves * kWave, 0, s>>>(a, fp, x, f);
   else both_kernel<T, PP, PAIRS, false><<<grid, kBothWaves * kWave, 0, s>>>(a, fp, x, f);

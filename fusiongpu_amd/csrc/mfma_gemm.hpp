@@ -2,9 +2,9 @@
 // head_ortho.hip, head_loss.hip).
 //
 // D[m][n] = sum_k A(m, k) B(n, k) on MFMA, bf16 with float32 accumulators unless said otherwise (OfHalf, OfInt8).  Each
-// operand is read either with k contiguous (rows of k) or with k strided (rows of m or n, one row a k), so the forward product x W^T and both gradients dz W and
-// dz^T x come from one kernel without a transposed copy.  float32 operands are held as three bf16 planes (split2
-// below) and the k loop walks the six plane pairs that are more than 2^-22 of the whole.
+// operand is read either with k contiguous (rows of k) or with k strided (rows of m or n, one row a k), so the forward
+// product x W^T and both gradients dz W and dz^T x come from one kernel without a transposed copy.  float32 operands are
+// held as three bf16 planes (split2 below) and the k loop walks the six plane pairs that are more than 2^-22 of the whole.
 #pragma once
 
 #include <type_traits>

@@ -178,7 +178,8 @@ def demo(n=20000, dim=128, in_dim=768, hidden=1024, steps=300, batch=2048, seed=
             log(f"step {s + 1}: loss {loss.item():.3f}")
     after = recall()
     if log:
-        log(f"recall@1 of the searched index: {before:.3f} before, {after:.3f} after, {recall(head.int8()):.3f} with 8-bit weights")
+        log(f"recall@1 of the searched index: {before:.3f} before, {after:.3f} after, "
+            f"{recall(head.int8()):.3f} with 8-bit weights")
     index.close()
     return before, after
 
