@@ -185,7 +185,7 @@ __device__ __forceinline__ void clear_candidates(const LossRows& r, int block, i
 struct Blocks {
   int dz, copy0, copy1, loss, clear;
 };
-// GATED: a kernel of its own, as both forms' registers and LDS in one leave the plain one fewer waves (16384 x 4096 in bfloat16,
+// GATED: a kernel of its own, as the registers and LDS of both forms leave the plain one fewer waves (16384 x 4096 in bfloat16,
 // the sums alone 57 us and 83).
 template <class T, bool GATED>
 __global__ __launch_bounds__(256) void prep_kernel(Prep p, Blocks n) {
