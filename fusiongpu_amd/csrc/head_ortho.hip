@@ -1,18 +1,18 @@
 // head_ortho.hip -- an update with its singular values drawn to one, by Newton-Schulz products.
 //
 // X_0 = x / (|x| + eps) in the Frobenius norm; each step forms the products of the shorter side, A = X X^T (or X^T X),
-// P = b A + c A^2, and X <- a X + P X (or X P): every singular value s becomes a s + b s^3 + c s^5, the vectors stay.
+// P = a I + b A + c A^2, and X <- P X (or X P): every singular value s becomes a s + b s^3 + c s^5, the vectors stay.
 //
 // Between the products X, A and P are held as two float16 planes, 2^10 times their value: h + l is good to 2^-23 of what
 // lies above 2^-25 of one, and all of them stay below 2^6 while the singular values stay below about two.  The steps
-// multiply a small singular value by up to a each, and with it whatever a rounding leaves in its directions, so X may not
-// be rounded to one plane of 8 or 11 bits between them.
+// multiply a small singular value by up to a each, and with it whatever a rounding leaves in its directions, so none of them
+// may be rounded to one plane of 8 or 11 bits, of bfloat16 updates either: one plane in A, and in P and X' of the first and last
+// two steps, took 8192 x 1024 from 550 to 370 us and put results up to 9e-3 of their norm off at five steps and 1.8e-2 at eight
+// (updates of few rows that are not zero; sparse ones 5e-3, of low rank 2e-3), where two planes leave at most 6e-5.
 //
-// 8192 x 1024 in bfloat16, five steps, takes 0.37 ms: A 19 us a step as seven parts of its triangle (strided operands, 18
-// steps of k a workgroup) and 7 to join them, P 12 or 15, X' 29 in one plane (17 of matrix instructions, then 64 MB of X read
-// and written, which a product of one round of workgroups cannot overlap; reading X before the products in half of them gains
-// nothing) and 58 in two (three products, 1.25 PFLOP/s of them), norm and start 23.  128 x 771 in float32 65 us: twelve
-// launches, a step's two 6 each: A (k over sixteen waves; in parts 8.3), then P and X'.
+// 8192 x 1024, five steps, takes 0.55 ms in either type; traced, A 40 us a step as thirteen parts of its triangle (strided
+// operands) and 8 to join them, P 16, X' 62 (three products, 0.83 PFLOP/s of them), norm and start 19.  128 x 771 in float32
+// 66 us: twelve launches, a step's two 6 each: A (k over sixteen waves; in parts 8.3), then P and X'.
 #include <algorithm>
 #include <cmath>
 
@@ -23,6 +23,7 @@ namespace {
 
 constexpr float kHeld = 1024.0f;  // what planes hold of a value of one
 constexpr int kNormBlocks = 512;
+constexpr int kPairs = 3, kPlanes = planes_of(kPairs);  // plane products of a product
 
 bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
 
@@ -155,7 +156,7 @@ struct OrthoEpi {
       }
     }
   }
-  // The same where a wave's 64 columns all lie inside: whole lines a store (8192 x 1024 in bfloat16 378 -> 369 us).
+  // The same where a wave's 64 columns all lie inside: whole lines a store.
   template <class G>
   __device__ __forceinline__ void lines(f32x4 (&acc)[G::FN][G::FM], const GemmWave<G>& w) const {
 #pragma unroll
@@ -245,9 +246,9 @@ __global__ __launch_bounds__(256) void triangle_join_kernel(OrthoFinish f, const
 // ends are zeros), as in head_direct.hpp; the partial tiles meet in LDS.  One launch, no parts in memory.
 constexpr int kFewTile = 32, kFewBK = 32;
 inline int few_waves(int k) { return k > 512 ? 16 : 8; }
-template <int PAIRS, bool KC, bool ISB, int F = 2>
+template <bool KC, bool ISB, int F = 2>
 struct FewRead {
-  static constexpr int P = planes_of(PAIRS), lds_bytes = KC ? 0 : P * kFewBK * F * 32;
+  static constexpr int P = kPlanes, lds_bytes = KC ? 0 : P * kFewBK * F * 32;
   bf16x8 r[P][F];
   __device__ __forceinline__ void load(const Planes& o, int r0, int nr, int k0, int nk, int lane) {
 #pragma unroll
@@ -298,10 +299,10 @@ struct FewRead {
     }
   }
 };
-template <class T, int PAIRS, bool AKC, bool BKC, int kFewWaves, int FM>
+template <class T, bool AKC, bool BKC, int kFewWaves, int FM>
 __global__ __launch_bounds__(kFewWaves * kWave) void few_tiles_kernel(Planes a, Planes b, int k, OrthoFinish f) {
-  using RA = FewRead<PAIRS, AKC, false, FM>;
-  using RB = FewRead<PAIRS, BKC, true>;
+  using RA = FewRead<AKC, false, FM>;
+  using RB = FewRead<BKC, true>;
   constexpr int stage = kFewWaves * (RA::lds_bytes + RB::lds_bytes), joined = kFewWaves * FM * 2 * kWave * 16;
   __shared__ __attribute__((aligned(1024))) char lds[stage > joined ? stage : joined];
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
@@ -322,9 +323,8 @@ __global__ __launch_bounds__(kFewWaves * kWave) void few_tiles_kernel(Planes a, 
 #pragma unroll
       for (int i = 0; i < 2; ++i)
 #pragma unroll
-        for (int q = 0; q < PAIRS; ++q)
-          acc[i][j] = OfHalf::mma(fb[i][PAIRS == 1 ? 0 : pair_b<PAIRS>(q)], fa[j][PAIRS == 1 ? 0 : pair_a<PAIRS>(q)],
-                                  acc[i][j]);
+        for (int q = 0; q < kPairs; ++q)
+          acc[i][j] = OfHalf::mma(fb[i][pair_b<kPairs>(q)], fa[j][pair_a<kPairs>(q)], acc[i][j]);
   };
   for (int s = s0; s < s1; s += 2) {  // two steps' loads in flight
     RA a0, a1;
@@ -365,10 +365,10 @@ __global__ __launch_bounds__(kFewWaves * kWave) void few_tiles_kernel(Planes a, 
 // 76 / 82, but 771 x 128 84 / 74, 192 x 500 81 / 71.
 constexpr int kBothWide = 128, kBothTall = 96;
 constexpr int kBothWaves = 8, kBothSteps = kBothWide / kFewBK, kBothStride = kBothWide + 8;  // rows fall on different banks
-template <class T, int PP, int PAIRS, bool TALL>
+template <class T, bool TALL>
 __global__ __launch_bounds__(kBothWaves * kWave) void both_kernel(Planes a, OrthoFinish fp, Planes x, OrthoFinish f) {
-  using RX = FewRead<PAIRS, TALL, !TALL, TALL ? 1 : 2>;
-  constexpr int P = planes_of(PAIRS), kRows = TALL ? 32 : 16;
+  using RX = FewRead<TALL, !TALL, TALL ? 1 : 2>;
+  constexpr int P = kPlanes, kRows = TALL ? 32 : 16;
   constexpr int stage = kBothWaves * RX::lds_bytes, joined = kBothWaves * 2 * kWave * 16;
   __shared__ __attribute__((aligned(1024))) char lds[stage > joined ? stage : joined];
   __shared__ __attribute__((aligned(16))) uint16_t strip[P][kRows][kBothStride];
@@ -382,8 +382,8 @@ __global__ __launch_bounds__(kBothWaves * kWave) void both_kernel(Planes a, Orth
   if (wave < steps * (kRows / 16)) {
     const int r = wave % (kRows / 16) * 16, c0 = wave / (kRows / 16) * 32;
     f32x4 acc[2] = {{0, 0, 0, 0}, {0, 0, 0, 0}};
-    FewRead<PP, true, false, 1> ra[kBothSteps];
-    FewRead<PP, true, true> rb[kBothSteps];
+    FewRead<true, false, 1> ra[kBothSteps];
+    FewRead<true, true> rb[kBothSteps];
 #pragma unroll
     for (int h = 0; h < kBothSteps; ++h) {  // past the end: zeros
       ra[h].load(a, p0 + r, n, h * kFewBK, n, lane);
@@ -394,21 +394,14 @@ __global__ __launch_bounds__(kBothWaves * kWave) void both_kernel(Planes a, Orth
 #pragma unroll
       for (int i = 0; i < 2; ++i)
 #pragma unroll
-        for (int q = 0; q < PP; ++q)
-          acc[i] = OfHalf::mma(rb[h].r[PP == 1 ? 0 : pair_b<PP>(q)][i], ra[h].r[PP == 1 ? 0 : pair_a<PP>(q)][0], acc[i]);
+        for (int q = 0; q < kPairs; ++q) acc[i] = OfHalf::mma(rb[h].r[pair_b<kPairs>(q)][i], ra[h].r[pair_a<kPairs>(q)][0], acc[i]);
     const int row = p0 + r + l, col = c0 + 8 * (lane >> 4);
     f32x8 v{{0, 0, 0, 0}, {0, 0, 0, 0}};
     if (row < n && col < n8) v = fp.value(f32x8{acc[0], acc[1]}, row, col, true);
-#pragma unroll
-    for (int q = 0; q < P; ++q) {
-      f16x8 h;
-#pragma unroll
-      for (int e = 0; e < 8; ++e) {
-        h[e] = (_Float16)v[e];
-        if (q + 1 < P) v.set(e, v[e] - (float)h[e]);
-      }
-      *reinterpret_cast<f16x8*>(&strip[q][r + l][col]) = h;
-    }
+    f16x8 h, lo;
+    to_planes(v, h, lo);
+    *reinterpret_cast<f16x8*>(&strip[0][r + l][col]) = h;
+    *reinterpret_cast<f16x8*>(&strip[1][r + l][col]) = lo;
   }
   __syncthreads();
   f32x4 acc[2] = {{0, 0, 0, 0}, {0, 0, 0, 0}};
@@ -425,8 +418,8 @@ __global__ __launch_bounds__(kBothWaves * kWave) void both_kernel(Planes a, Orth
 #pragma unroll
     for (int i = 0; i < 2; ++i)
 #pragma unroll
-      for (int q = 0; q < PAIRS; ++q) {
-        const int qa = PAIRS == 1 ? 0 : pair_a<PAIRS>(q), qb = PAIRS == 1 ? 0 : pair_b<PAIRS>(q);
+      for (int q = 0; q < kPairs; ++q) {
+        const int qa = pair_a<kPairs>(q), qb = pair_b<kPairs>(q);
         if constexpr (TALL) acc[i] = OfHalf::mma(pf[i][qb], fx[0][qa], acc[i]);
         else acc[i] = OfHalf::mma(fx[i][qb], pf[0][qa], acc[i]);
       }
@@ -450,24 +443,23 @@ bool takes_both(int rows, int cols) {
 }
 
 // ---- how a product is cut ------------------------------------------------------------
-// Microseconds, fitted over sides of 64 to 4096 and k to 8192: a step of k (64 of one plane, 32 of two) of a workgroup while
+// Microseconds, fitted over sides of 64 to 4096 and k to 8192: a step of 32 k of a workgroup while
 // it has its CU to itself, for each of those that share one, and how many do; both operands k contiguous (a strided one takes
 // 1.3 times as long).
 struct StepTime {
   double alone, shared;
   int most;
 };
-StepTime step_time(int tile, int pairs) {
-  if (pairs == 1) return tile == 256 ? StepTime{1.5, 1.5, 1} : tile == 128 ? StepTime{0.6, 0.43, 2} : StepTime{0.3, 0.2, 5};
+StepTime step_time(int tile) {
   return tile == 256 ? StepTime{2.0, 2.0, 1} : tile == 128 ? StepTime{0.75, 0.6, 2} : StepTime{0.26, 0.2, 3};
 }
 struct Cut {
   int tile = 0, splits = 1, k_per_split = 0;
   double us = 0;
 };
-double cut_us(const Cut& q, int pairs, bool strided, int64_t tiles, double fixed) {
-  const StepTime t = step_time(q.tile, pairs);
-  const int steps = ceil_div(q.k_per_split, pairs == 1 ? kGemmBK : kPlanesBK), round = 256 * t.most;
+double cut_us(const Cut& q, bool strided, int64_t tiles, double fixed) {
+  const StepTime t = step_time(q.tile);
+  const int steps = ceil_div(q.k_per_split, kPlanesBK), round = 256 * t.most;
   const double k = steps * (strided ? 1.3 : 1.0);
   const int64_t wgs = tiles * q.splits, full = wgs / round, rest = wgs % round;
   double us = full * (k * std::max(t.alone, t.most * t.shared) + fixed);
@@ -475,22 +467,22 @@ double cut_us(const Cut& q, int pairs, bool strided, int64_t tiles, double fixed
   return us;
 }
 // The kernel of few tiles, whose waves take their steps one after the other; strided: how many operands are.
-double few_us(int m, int n, int k, int pairs, int strided) {
+double few_us(int m, int n, int k, int strided) {
   const int steps = ceil_div(ceil_div(k, kFewBK), few_waves(k));
   const double all = (double)ceil_div(m, kFewTile) * ceil_div(n, kFewTile) * steps / 256;
   const double more = few_waves(k) == 16 ? 1.75 : 1;
   const double half = ceil_div(m, 16) * (int64_t)ceil_div(n, kFewTile) <= 256 ? 0.7 : 1;
   const double alone = (strided == 2 ? 0.42 : strided ? 0.5 : 0.6) * more * half;
   const double shared = (strided == 2 ? 0.65 : strided ? 0.83 : 1.09) * more;
-  return 2.6 + std::max(steps * alone, all * shared) * (pairs == 1 ? 1 : 1.9);
+  return 2.6 + std::max(steps * alone, all * shared) * 1.9;
 }
 // A product of m x n over k, whole: tile 32 for the kernel of few tiles.
-Cut cut_product(int m, int n, int k, int pairs, int strided) {
-  Cut best{kFewTile, 1, 0, few_us(m, n, k, pairs, strided)};
+Cut cut_product(int m, int n, int k, int strided) {
+  Cut best{kFewTile, 1, 0, few_us(m, n, k, strided)};
   for (int tile : {256, 128, 64}) {
     const int64_t tiles = (int64_t)ceil_div(m, tile) * ceil_div(n, tile);
     Cut q{tile, 1, ceil_div(k, kGemmBK) * kGemmBK};
-    q.us = cut_us(q, pairs, strided == 2, tiles, tile == 256 ? 9 : tile == 128 ? 5 : 3);
+    q.us = cut_us(q, strided == 2, tiles, tile == 256 ? 9 : tile == 128 ? 5 : 3);
     if (q.us < best.us) best = q;
   }
   return best;
@@ -504,16 +496,16 @@ struct SymmetricCut {
     return joined ? carve_bytes<float>(part.splits * tiles * part.tile * part.tile) : 0;
   }
 };
-SymmetricCut cut_symmetric(int n, int k, int pairs, bool strided) {
+SymmetricCut cut_symmetric(int n, int k, bool strided) {
   SymmetricCut c;
-  c.whole = cut_product(n, n, k, pairs, strided ? 2 : 0);
+  c.whole = cut_product(n, n, k, strided ? 2 : 0);
   for (int tile : {256, 128, 64}) {
     const int64_t tiles = triangle_tiles(ceil_div(n, tile));
     for (int splits = 1; splits <= 64; ++splits) {
       if (splits > 1 && (splits > ceil_div(k, 2 * kGemmBK) || tiles * splits > 2048)) break;
       Cut q{tile, splits, ceil_div(ceil_div(k, kGemmBK), splits) * kGemmBK};
       if (ceil_div(k, q.k_per_split) != splits) continue;
-      q.us = cut_us(q, pairs, strided, tiles, tile == 256 ? 6 : tile == 128 ? 3.5 : 2.5);
+      q.us = cut_us(q, strided, tiles, tile == 256 ? 6 : tile == 128 ? 3.5 : 2.5);
       q.us += 4 + tiles * splits * tile * tile * 8.0 / 5e6;  // the join
       if (!c.part.tile || q.us < c.part.us) c.part = q;
     }
@@ -522,15 +514,15 @@ SymmetricCut cut_symmetric(int n, int k, int pairs, bool strided) {
   return c;
 }
 
-template <int PAIRS, bool AKC, bool BKC, int FORM, class E>
+template <bool AKC, bool BKC, int FORM, class E>
 fgpu_status run_cut(const GemmArgs& g, int tile, int grid, const E& e, hipStream_t s) {
-  if (tile == 256) gemm_kernel<Tile256, AKC, BKC, PAIRS, E, OfHalf, FORM><<<grid, Tile256::threads, 0, s>>>(g, e);
-  else if (tile == 128) gemm_kernel<Tile128, AKC, BKC, PAIRS, E, OfHalf, FORM><<<grid, Tile128::threads, 0, s>>>(g, e);
-  else gemm_kernel<Tile64, AKC, BKC, PAIRS, E, OfHalf, FORM><<<grid, Tile64::threads, 0, s>>>(g, e);
+  if (tile == 256) gemm_kernel<Tile256, AKC, BKC, kPairs, E, OfHalf, FORM><<<grid, Tile256::threads, 0, s>>>(g, e);
+  else if (tile == 128) gemm_kernel<Tile128, AKC, BKC, kPairs, E, OfHalf, FORM><<<grid, Tile128::threads, 0, s>>>(g, e);
+  else gemm_kernel<Tile64, AKC, BKC, kPairs, E, OfHalf, FORM><<<grid, Tile64::threads, 0, s>>>(g, e);
   FGPU_HIP(hipGetLastError());
   return FGPU_OK;
 }
-template <class T, int PAIRS, bool AKC, bool BKC>
+template <class T, bool AKC, bool BKC>
 fgpu_status run_whole(const Planes& a, const Planes& b, int k, const OrthoFinish& f, const Cut& q, hipStream_t s) {
   if (q.tile == kFewTile) {
     // Half the rows a workgroup while that leaves CUs without one.
@@ -538,7 +530,7 @@ fgpu_status run_whole(const Planes& a, const Planes& b, int k, const OrthoFinish
     const bool half = ceil_div(f.m, 16) * across <= 256, many = few_waves(k) == 16;
     auto go = [&](auto waves, auto fm) {
       constexpr int W = decltype(waves)::value, FM = decltype(fm)::value;
-      few_tiles_kernel<T, PAIRS, AKC, BKC, W, FM><<<ceil_div(f.m, 16 * FM) * across, W * kWave, 0, s>>>(a, b, k, f);
+      few_tiles_kernel<T, AKC, BKC, W, FM><<<ceil_div(f.m, 16 * FM) * across, W * kWave, 0, s>>>(a, b, k, f);
     };
     const std::integral_constant<int, 1> w1{};
     const std::integral_constant<int, 2> w2{};
@@ -551,41 +543,20 @@ fgpu_status run_whole(const Planes& a, const Planes& b, int k, const OrthoFinish
   }
   const GemmArgs g{{a.p, a.ld, a.plane}, {b.p, b.ld, b.plane}, f.m, f.n, k, ceil_div(f.m, q.tile), ceil_div(f.n, q.tile), 1,
                    q.k_per_split};
-  return run_cut<PAIRS, AKC, BKC, kPlain>(g, q.tile, g.tiles_m * g.tiles_n, OrthoEpi<T>{f}, s);
+  return run_cut<AKC, BKC, kPlain>(g, q.tile, g.tiles_m * g.tiles_n, OrthoEpi<T>{f}, s);
 }
 // a a^T of n rows (KC: k contiguous).
-template <class T, int PAIRS, bool KC>
+template <class T, bool KC>
 fgpu_status run_symmetric(const Planes& a, int k, const OrthoFinish& f, float* part, hipStream_t s) {
-  const SymmetricCut c = cut_symmetric(f.n, k, PAIRS, !KC);
-  if (!c.joined) return run_whole<T, PAIRS, KC, KC>(a, a, k, f, c.whole, s);
+  const SymmetricCut c = cut_symmetric(f.n, k, !KC);
+  if (!c.joined) return run_whole<T, KC, KC>(a, a, k, f, c.whole, s);
   const Cut& q = c.part;
   const int t = ceil_div(f.n, q.tile), tiles = triangle_tiles(t);
   const GemmArgs g{{a.p, a.ld, a.plane}, {a.p, a.ld, a.plane}, f.n, f.n, k, t, t, q.splits, q.k_per_split};
-  FGPU_TRY((run_cut<PAIRS, KC, KC, kTriangle>(g, q.tile, tiles * q.splits, TriangleEpi{part, tiles}, s)));
+  FGPU_TRY((run_cut<KC, KC, kTriangle>(g, q.tile, tiles * q.splits, TriangleEpi{part, tiles}, s)));
   triangle_join_kernel<<<tiles * (q.tile / 64) * (q.tile / 64), 256, 0, s>>>(f, part, q.splits, tiles, q.tile);
   FGPU_HIP(hipGetLastError());
   return FGPU_OK;
-}
-
-// How a step forms a X + P X.  In two planes as (a I + P) X, in one with X added apart, from both of its planes: a X + P X,
-// or, near the end, X + (P + (a - 1) I) X, whose second factor is small in the directions whose singular values have arrived.
-//
-// Of bfloat16 updates A takes one plane of X, and the first two and the last two steps one plane in the other products too:
-// what the first roundings leave lies in the directions of large singular values, which the later steps do not multiply, and
-// the last ones' is little, as said.  Against 64 bits (64 to 512 rows; singular values even, of normal numbers, as i^-1/2 to
-// i^-2; four to eight steps) the result is then off by at most 1.4e-3 of its norm, mostly below 7e-4, before it is rounded to
-// bfloat16 (1.7e-3); with one plane in every product and P as it is 2.7e-3, with X in one plane as well up to 8e-3.  Of more
-// steps A's rounding leaves up to 1.9e-3, and coefficients larger than the usual ones more than that: those take two.
-struct Form {
-  int gram, rest;  // plane products of A, of the product with P; P itself takes three but in the first two steps
-  bool apart, near_one;
-};
-Form form_of(bool f32, int i, int steps, float a, float b, float c) {
-  if (f32 || std::fabs(a) + std::fabs(b) + std::fabs(c) > 10.5f) return {3, 3, false, false};
-  const int gram = steps <= 8 ? 1 : 3;
-  if (i < 2) return {gram, 1, true, false};
-  if (i >= steps - 2) return {gram, 1, true, true};
-  return {gram, 3, false, false};
 }
 
 struct Shape {
@@ -605,11 +576,8 @@ struct Shape {
   size_t x_bytes() const { return carve_bytes<uint16_t>((size_t)rows * x_ld() * 2); }
   size_t a_bytes() const { return carve_bytes<uint16_t>((size_t)small * a_ld() * 2); }
   size_t part_bytes() const {
-    size_t b = 0;
-    for (int pairs : {1, 3})
-      b = std::max({b, cut_symmetric(small, large, pairs, tall).part_bytes(small),
-                    cut_symmetric(small, small, pairs, false).part_bytes(small)});
-    return b;
+    return std::max(cut_symmetric(small, large, tall).part_bytes(small),
+                    cut_symmetric(small, small, false).part_bytes(small));
   }
 };
 Planes planes_at(void* p, int rows, int64_t ld) { return {(uint16_t*)p, ld, rows * ld}; }
@@ -622,24 +590,24 @@ fgpu_status check_common(int64_t rows, int64_t cols, int dtype) {
   return FGPU_OK;
 }
 
-template <class T, int PAIRS>
+// A = X X^T, P = b A + c A^2 + a I and P X (of tall X: X^T X and X P).
+template <class T>
 fgpu_status gram(const Planes& x, const Shape& sh, const OrthoFinish& f, float* part, hipStream_t s) {
-  if (sh.tall) return run_symmetric<T, PAIRS, false>(x, sh.large, f, part, s);
-  return run_symmetric<T, PAIRS, true>(x, sh.large, f, part, s);
+  if (sh.tall) return run_symmetric<T, false>(x, sh.large, f, part, s);
+  return run_symmetric<T, true>(x, sh.large, f, part, s);
 }
-template <class T, int PAIRS>
+template <class T>
 fgpu_status step(const Planes& x, const Planes& p, const Shape& sh, const OrthoFinish& f, hipStream_t s) {
-  const Cut q = cut_product(f.m, f.n, sh.small, PAIRS, sh.tall ? 0 : 1);
-  if (sh.tall) return run_whole<T, PAIRS, true, true>(x, p, sh.small, f, q, s);
-  return run_whole<T, PAIRS, true, false>(p, x, sh.small, f, q, s);
+  const Cut q = cut_product(f.m, f.n, sh.small, sh.tall ? 0 : 1);
+  if (sh.tall) return run_whole<T, true, true>(x, p, sh.small, f, q, s);
+  return run_whole<T, true, false>(p, x, sh.small, f, q, s);
 }
-
-template <class T, int PP, int PAIRS>
+template <class T>
 fgpu_status both(const Planes& a, const OrthoFinish& fp, const Planes& x, const Shape& sh, const OrthoFinish& f,
                  hipStream_t s) {
   const int grid = ceil_div(f.m, 16) * ceil_div(f.n, 32);
-  if (sh.tall) both_kernel<T, PP, PAIRS, true><<<grid, kBothWaves * kWave, 0, s>>>(a, fp, x, f);
-  else both_kernel<T, PP, PAIRS, false><<<grid, kBothWaves * kWave, 0, s>>>(a, fp, x, f);
+  if (sh.tall) both_kernel<T, true><<<grid, kBothWaves * kWave, 0, s>>>(a, fp, x, f);
+  else both_kernel<T, false><<<grid, kBothWaves * kWave, 0, s>>>(a, fp, x, f);
   FGPU_HIP(hipGetLastError());
   return FGPU_OK;
 }
@@ -663,28 +631,18 @@ fgpu_status run_ortho(const T* x, const Shape& sh, int steps, float a, float b, 
   const int n = sh.small;
   for (int i = 0; i < steps; ++i) {
     const Planes &from = xs[i & 1], &to = xs[i + 1 & 1];
-    const bool last = i + 1 == steps;
-    const Form m = form_of(sizeof(T) == 4, i, steps, a, b, c);
     OrthoFinish fa, fp, fx;
     fa.alpha = 1 / kHeld, fa.to = ga, fa.m = fa.n = n;
-    fp.alpha = c / kHeld, fp.beta = b, fp.c = ga, fp.to = gp, fp.m = fp.n = n;
-    fp.diagonal = kHeld * (!m.apart ? a : m.near_one ? a - 1 : 0);
+    fp.alpha = c / kHeld, fp.beta = b, fp.c = ga, fp.diagonal = kHeld * a, fp.to = gp, fp.m = fp.n = n;
     fx.alpha = 1 / kHeld, fx.to = to, fx.m = sh.rows, fx.n = sh.cols;
-    if (m.apart) fx.beta = m.near_one ? 1 : a, fx.c = from;
-    if (last) fx.out = out, fx.alpha /= kHeld, fx.beta /= kHeld;
-    FGPU_TRY((m.gram == 1 ? gram<T, 1>(from, sh, fa, part, s) : gram<T, 3>(from, sh, fa, part, s)));
-    const bool early = m.rest == 1 && !m.near_one;
+    if (i + 1 == steps) fx.out = out, fx.alpha /= kHeld;
+    FGPU_TRY(gram<T>(from, sh, fa, part, s));
     if (takes_both(sh.rows, sh.cols)) {
-      if constexpr (sizeof(T) == 4) {
-        FGPU_TRY((both<T, 3, 3>(ga, fp, from, sh, fx, s)));
-      } else {
-        FGPU_TRY((early ? both<T, 1, 1>(ga, fp, from, sh, fx, s) : m.rest == 1 ? both<T, 3, 1>(ga, fp, from, sh, fx, s)
-                                                                               : both<T, 3, 3>(ga, fp, from, sh, fx, s)));
-      }
-      continue;
+      FGPU_TRY(both<T>(ga, fp, from, sh, fx, s));
+    } else {
+      FGPU_TRY((run_symmetric<T, true>(ga, n, fp, part, s)));
+      FGPU_TRY(step<T>(from, gp, sh, fx, s));
     }
-    FGPU_TRY((early ? run_symmetric<T, 1, true>(ga, n, fp, part, s) : run_symmetric<T, 3, true>(ga, n, fp, part, s)));
-    FGPU_TRY((m.rest == 1 ? step<T, 1>(from, gp, sh, fx, s) : step<T, 3>(from, gp, sh, fx, s)));
   }
   return FGPU_OK;
 }

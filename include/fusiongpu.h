@@ -702,13 +702,11 @@ fgpu_status fgpu_gated_linear_int8(const void* d_x, const float* d_x_scale, cons
  * + c A^2) X with A = X X^T (of more rows than columns, the same from the other
  * side): each singular value s becomes a s + b s^3 + c s^5.  y = X.  A matrix of
  * zeros stays zero; something not finite makes all of y NaN.  Between the
- * products X, A and b A + c A^2 are held to 2^-23 of their value and 2^-35 of
- * one, and must stay below 64 in magnitude (coefficients that keep the singular
- * values below about two do; past it y is NaN).  float32 products take all of that; of bfloat16
- * matrices, up to 8 steps and |a| + |b| + |c| <= 10.5, several take operands
- * rounded to 2^-12, which puts y up to 1.4e-3 of its norm off, mostly half of
- * that, beside its own rounding's 1.7e-3 (head_ortho.hip says which).  rows and
- * cols up to 2^16; d_y may be d_x; d_x and d_y need their element's alignment. */
+ * products X, A and a I + b A + c A^2 are held to 2^-23 of their value and 2^-35
+ * of one, and must stay below 64 in magnitude (coefficients that keep the
+ * singular values below about two do; past it y is NaN).  Of a bfloat16 matrix y
+ * is what the same numbers in float32 give, rounded once.  rows and cols up to
+ * 2^16; d_y may be d_x; d_x and d_y need their element's alignment. */
 #define FGPU_ORTHO_MAX_STEPS 64
 size_t fgpu_orthogonalize_workspace_bytes(int64_t rows, int64_t cols, int dtype);
 fgpu_status fgpu_orthogonalize(const void* d_x, int64_t rows, int64_t cols, int dtype, int steps, float a, float b, float c,
