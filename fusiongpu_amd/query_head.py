@@ -132,7 +132,8 @@ class Int8QueryHead(_Searches):
 
     def __init__(self, head: QueryHead):
         self.dtype, self.skip, self.gated = head.dtype, head.skip, head.gated
-        self._c = {n: p.to(head.dtype) for n, p in head.params.items() if p.dim() == 1}
+        # copies, in float32 too: the head's next step writes its parameters in place
+        self._c = {n: p.to(head.dtype, copy=True) for n, p in head.params.items() if p.dim() == 1}
         self._w = {n: fg.quantize_rows(p) for n, p in head.params.items() if p.dim() == 2}
 
     def __call__(self, x, stream=None):
