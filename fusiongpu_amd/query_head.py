@@ -106,18 +106,19 @@ class QueryHead(_Searches):
                    eps: float = 1e-8, matrix_lr: float | None = None):
         """One step on the contrastive loss; returns the mean loss before it (a device scalar).  Adam; with matrix_lr the two
         weights move instead by their momentum with its singular values drawn to one, matrix_lr sqrt(max(1, rows / cols))
-        times it."""
+        times it (a gated head's w1 as the one matrix that it is, both projections' rows together).  Steps with and without
+        it may follow one another: Adam's moments take in every step's gradients."""
         mean, grads = self.loss(x, candidates, targets, scale, ids)
         self.steps += 1
         rate = lr * math.sqrt(1 - betas[1]**self.steps) / (1 - betas[0]**self.steps)
         for n in self.NAMES:
             g, p, (m, v) = grads[n].float(), self.params[n], self._moments[n]
             m.lerp_(g, 1 - betas[0])
+            v.lerp_(g * g, 1 - betas[1])  # of the weights too: a later step may be without matrix_lr
             if matrix_lr is not None and p.dim() == 2:
                 p -= matrix_lr * max(1, p.shape[0] / p.shape[1])**0.5 * fg.orthogonalize(m.to(self.dtype)).float()
-                continue
-            v.lerp_(g * g, 1 - betas[1])
-            p -= rate * m / (v.sqrt() + eps)
+            else:
+                p -= rate * m / (v.sqrt() + eps)
         self._cast()
         return mean
 
