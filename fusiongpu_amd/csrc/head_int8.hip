@@ -249,6 +249,29 @@ struct FewJob {
 };
 constexpr int kFewWaves = 8, kFewThreads = kFewWaves * kWave, kFewRows = 16, kFewHeld = 2;
 constexpr int kFewStep = 64;
+// Four columns of a row with their scales and bias, in the steps of the tiles' epilogues (`eight`): a row's bits are the same
+// whichever kernel its batch takes.
+struct Four {
+  f32x4 by = {0, 0, 0, 0}, bias = {0, 0, 0, 0};
+  template <class T>
+  __device__ __forceinline__ void load(const FewJob& j, int at, int cnt) {
+    by = load4_n(j.s.col + at, cnt);
+    if (j.f.bias) bias = load4_n((const T*)j.f.bias + at, cnt);
+  }
+  __device__ __forceinline__ f32x4 of(const i32x4& v, float row) const {
+    f32x4 o;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) o[e] = fmaf((float)v[e] * by[e], row, bias[e]);
+    return o;
+  }
+};
+// The rest of the epilogue, g and u (or the only one, g) scaled and with their bias.
+template <class T, bool GATED>
+__device__ __forceinline__ void finish_four(Finish f, const f32x4& g, const f32x4& u, int64_t row, int n, int col, int cnt) {
+  f.bias = nullptr;
+  if constexpr (GATED) finish4_gated<T>(f, g, u, row, n, col, cnt);
+  else finish4<T>(f, g, row * n + col, col, cnt);
+}
 
 template <class T, bool GATED, bool QUANT>
 __global__ __launch_bounds__(kFewThreads) void few_rows_kernel(FewJob j) {
@@ -322,29 +345,24 @@ __global__ __launch_bounds__(kFewThreads) void few_rows_kernel(FewJob j) {
       acc = __builtin_amdgcn_mfma_i32_16x16x64_i8(weight(s), value(s), acc, 0, 0, 0);
   }
   join[wave][lane] = acc;
-  __syncthreads();
   // A thread four columns of a row (gated: of both halves, from the lanes 32 apart).
-  if (tid >= (GATED ? 32 : 64) || (lane & 15) >= j.m) return;
   const int m = lane & 15, c = n0 + (lane >> 4) * 4, cnt = j.n - c;
-  if (cnt <= 0) return;
+  const bool mine = tid < (GATED ? 32 : 64) && m < j.m && cnt > 0;
+  Four g4, u4;
+  if (mine) {  // on the way while the waves meet
+    g4.load<T>(j, c, cnt);
+    if (GATED) u4.load<T>(j, j.n + c, cnt);
+  }
+  __syncthreads();
+  if (!mine) return;
   auto sum = [&](int l) {
     i32x4 v = join[0][l];
 #pragma unroll
     for (int w = 1; w < kFewWaves; ++w) v += join[w][l];
     return v;
   };
-  auto scaled = [&](const i32x4& v, const float* sc) {
-    const f32x4 by = load4_n(sc, cnt);
-    const float r = row_scale[m];
-    f32x4 o;
-#pragma unroll
-    for (int e = 0; e < 4; ++e) o[e] = (float)v[e] * by[e] * r;
-    return o;
-  };
-  if constexpr (GATED)
-    finish4_gated<T>(j.f, scaled(sum(lane), j.s.col + c), scaled(sum(lane + 32), j.s.col + j.n + c), m, j.n, c, cnt);
-  else
-    finish4<T>(j.f, scaled(sum(lane), j.s.col + c), (int64_t)m * j.n + c, c, cnt);
+  const f32x4 g = g4.of(sum(lane), row_scale[m]), u = GATED ? u4.of(sum(lane + 32), row_scale[m]) : g;
+  finish_four<T, GATED>(j.f, g, u, m, j.n, c, cnt);
 }
 template <class T>
 fgpu_status few_rows(const FewJob& j, bool gated, bool quant, hipStream_t s) {
@@ -428,27 +446,23 @@ __global__ __launch_bounds__(kPanelThreads) void panel_kernel(FewJob j) {
 #pragma unroll
     for (int h = 0; h < kAhead; ++h) work(s + h, now[h]);  // past the end: zeros
   }
+  const int c = first + (lane >> 4) * 4, cnt = j.n - c;
+  Four g4, u4;
+  if (cnt > 0 && !(GATED && lane >= 32)) {
+    g4.load<T>(j, c, cnt);
+    if (GATED) u4.load<T>(j, j.n + c, cnt);
+  }
 #pragma unroll
   for (int h = 0; h < 2; ++h) {
-    const int m = 16 * h + i, c = first + (lane >> 4) * 4, cnt = j.n - c;
-    const float r = row_scale[m];
-    auto scaled = [&](const i32x4& v, const float* sc) {
-      const f32x4 by = load4_n(sc, cnt);
-      f32x4 o;
-#pragma unroll
-      for (int e = 0; e < 4; ++e) o[e] = (float)v[e] * by[e] * r;
-      return o;
-    };
+    const int m = 16 * h + i;
     i32x4 other = none;
     if constexpr (GATED) {
 #pragma unroll
       for (int e = 0; e < 4; ++e) other[e] = xchg<32>(acc[h][e]);
     }
     if (m0 + m >= j.m || cnt <= 0 || (GATED && lane >= 32)) continue;
-    if constexpr (GATED)
-      finish4_gated<T>(j.f, scaled(acc[h], j.s.col + c), scaled(other, j.s.col + j.n + c), m0 + m, j.n, c, cnt);
-    else
-      finish4<T>(j.f, scaled(acc[h], j.s.col + c), (int64_t)(m0 + m) * j.n + c, c, cnt);
+    const f32x4 g = g4.of(acc[h], row_scale[m]), u = GATED ? u4.of(other, row_scale[m]) : g;
+    finish_four<T, GATED>(j.f, g, u, m0 + m, j.n, c, cnt);
   }
 }
 bool takes_panel(int64_t rows, int k, int n, bool gated) {

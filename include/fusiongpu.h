@@ -685,7 +685,8 @@ fgpu_status fgpu_quantize_rows(const void* d_x, int64_t rows, int dim, int dtype
  * as above inside the call, or held so already: [rows][FGPU_INT8_ROW(in_dim)]
  * with d_x_scale [rows] (behind the values, x's or w's bytes are zeros).  z =
  * x_scale w_scale sum q_x q_w + bias, the sum exact in 32 bits; bias, residual
- * and y are of `dtype`.  d_residual may be d_y itself. */
+ * and y are of `dtype`.  A row's result is the same to the bit in any batch, and
+ * whether the call rounds x or gets it rounded.  d_residual may be d_y itself. */
 size_t fgpu_linear_int8_workspace_bytes(int64_t rows, int in_dim, int out_dim, int dtype, int quantized_x);
 fgpu_status fgpu_linear_int8(const void* d_x, const float* d_x_scale, const int8_t* d_w, const float* d_w_scale,
                              const void* d_bias, const void* d_residual, int64_t rows, int in_dim, int out_dim, int dtype,
