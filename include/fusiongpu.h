@@ -705,7 +705,9 @@ fgpu_status fgpu_gated_linear_int8(const void* d_x, const float* d_x_scale, cons
  * zeros stays zero; something not finite makes all of y NaN.  Between the
  * products X, A and a I + b A + c A^2 are held to 2^-23 of their value and 2^-35
  * of one, and must stay below 64 in magnitude (coefficients that keep the
- * singular values below about two do; past it y is NaN).  Of a bfloat16 matrix y
+ * singular values below about two do).  What passes it makes all of y NaN, or,
+ * where that is a I + b A + c A^2 of the last step, the rows (of more rows than
+ * columns, the columns) of y that it multiplies.  Of a bfloat16 matrix y
  * is what the same numbers in float32 give, rounded once.  rows and cols up to
  * 2^16; d_y may be d_x; d_x and d_y need their element's alignment. */
 #define FGPU_ORTHO_MAX_STEPS 64
