@@ -145,6 +145,7 @@ _SIGS = {
     "fgpu_gated_linear_int8_workspace_bytes": (_sz, [_i64, _i32, _i32, _i32, _i32]),
     "fgpu_gated_linear_int8": (_i32, [_vp, _vp, _vp, _vp, _vp, _i64, _i32, _i32, _i32, _i32, _vp, _vp, _sz, _vp]),
     "fgpu_orthogonalize_workspace_bytes": (_sz, [_i64, _i64, _i32]),
+    "fgpu_orthogonalize_tile": (_i32, [_i64, _i64, _i32]),
     "fgpu_orthogonalize": (_i32, [_vp, _i64, _i64, _i32, _i32, _f32, _f32, _f32, _f32, _vp, _vp, _sz, _vp]),
     "fgpu_layer_norm": (_i32, [_vp, _vp, _vp, _i64, _i32, _i32, _f32, _vp, _vp, _vp, _vp]),
     "fgpu_layer_norm_backward_workspace_bytes": (_sz, [_i64, _i32, _i32]),

@@ -246,6 +246,8 @@ __global__ __launch_bounds__(256) void triangle_join_kernel(OrthoFinish f, const
 // ends are zeros), as in head_direct.hpp; the partial tiles meet in LDS.  One launch, no parts in memory.
 constexpr int kFewTile = 32, kFewBK = 32;
 inline int few_waves(int k) { return k > 512 ? 16 : 8; }
+// Half the rows a workgroup while that leaves CUs without one.
+inline bool few_half(int m, int n) { return (int64_t)ceil_div(m, 16) * ceil_div(n, kFewTile) <= 256; }
 template <bool KC, bool ISB, int F = 2>
 struct FewRead {
   static constexpr int P = kPlanes, lds_bytes = KC ? 0 : P * kFewBK * F * 32;
@@ -471,7 +473,7 @@ double few_us(int m, int n, int k, int strided) {
   const int steps = ceil_div(ceil_div(k, kFewBK), few_waves(k));
   const double all = (double)ceil_div(m, kFewTile) * ceil_div(n, kFewTile) * steps / 256;
   const double more = few_waves(k) == 16 ? 1.75 : 1;
-  const double half = ceil_div(m, 16) * (int64_t)ceil_div(n, kFewTile) <= 256 ? 0.7 : 1;
+  const double half = few_half(m, n) ? 0.7 : 1;
   const double alone = (strided == 2 ? 0.42 : strided ? 0.5 : 0.6) * more * half;
   const double shared = (strided == 2 ? 0.65 : strided ? 0.83 : 1.09) * more;
   return 2.6 + std::max(steps * alone, all * shared) * 1.9;
@@ -525,9 +527,8 @@ fgpu_status run_cut(const GemmArgs& g, int tile, int grid, const E& e, hipStream
 template <class T, bool AKC, bool BKC>
 fgpu_status run_whole(const Planes& a, const Planes& b, int k, const OrthoFinish& f, const Cut& q, hipStream_t s) {
   if (q.tile == kFewTile) {
-    // Half the rows a workgroup while that leaves CUs without one.
     const int across = ceil_div(f.n, kFewTile);
-    const bool half = ceil_div(f.m, 16) * across <= 256, many = few_waves(k) == 16;
+    const bool half = few_half(f.m, f.n), many = few_waves(k) == 16;
     auto go = [&](auto waves, auto fm) {
       constexpr int W = decltype(waves)::value, FM = decltype(fm)::value;
       few_tiles_kernel<T, AKC, BKC, W, FM><<<ceil_div(f.m, 16 * FM) * across, W * kWave, 0, s>>>(a, b, k, f);
@@ -658,6 +659,17 @@ size_t fgpu_orthogonalize_workspace_bytes(int64_t rows, int64_t cols, int dtype)
   if (check_common(rows, cols, dtype) != FGPU_OK || rows == 0 || cols == 0) return 0;
   const Shape sh((int)rows, (int)cols);
   return 2 * (sh.x_bytes() + sh.a_bytes()) + sh.part_bytes() + carve_bytes<double>(kNormBlocks);
+}
+
+int fgpu_orthogonalize_tile(int64_t rows, int64_t cols, int product) {
+  if (check_common(rows, cols, FGPU_DTYPE_F32) != FGPU_OK || rows == 0 || cols == 0 || product < 0 || product > 2) return -1;
+  const Shape sh((int)rows, (int)cols);
+  auto whole = [](const Cut& q, int m, int n) { return q.tile == kFewTile && few_half(m, n) ? 16 : q.tile; };
+  if (product && takes_both(sh.rows, sh.cols)) return 0;
+  if (product == 2) return whole(cut_product(sh.rows, sh.cols, sh.small, sh.tall ? 0 : 1), sh.rows, sh.cols);
+  const SymmetricCut c = product ? cut_symmetric(sh.small, sh.small, false) : cut_symmetric(sh.small, sh.large, sh.tall);
+  if (!c.joined) return whole(c.whole, sh.small, sh.small);
+  return c.part.tile + FGPU_TILE_TRIANGLE + (c.part.splits > 1 ? FGPU_TILE_PARTS : 0);
 }
 
 fgpu_status fgpu_orthogonalize(const void* d_x, int64_t rows, int64_t cols, int dtype, int steps, float a, float b, float c,

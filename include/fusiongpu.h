@@ -712,6 +712,14 @@ fgpu_status fgpu_gated_linear_int8(const void* d_x, const float* d_x_scale, cons
  * 2^16; d_y may be d_x; d_x and d_y need their element's alignment. */
 #define FGPU_ORTHO_MAX_STEPS 64
 size_t fgpu_orthogonalize_workspace_bytes(int64_t rows, int64_t cols, int dtype);
+/* Which kernel a product of a step takes: 0 is A, 1 is a I + b A + c A^2, 2 the
+ * product with X.  The width of its tiles, 16 or 32 rows of them where a
+ * workgroup's waves share k; plus FGPU_TILE_TRIANGLE where the tiles on and below
+ * the diagonal are formed and joined, and FGPU_TILE_PARTS where those come in
+ * parts of k; 0 where one launch forms 1 and 2; -1 for what is refused. */
+#define FGPU_TILE_TRIANGLE 4096
+#define FGPU_TILE_PARTS 8192
+int fgpu_orthogonalize_tile(int64_t rows, int64_t cols, int product);
 fgpu_status fgpu_orthogonalize(const void* d_x, int64_t rows, int64_t cols, int dtype, int steps, float a, float b, float c,
                                float eps, void* d_y, void* d_workspace, size_t workspace_bytes, void* stream);
 
