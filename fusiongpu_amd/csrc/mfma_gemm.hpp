@@ -187,7 +187,8 @@ struct OfHalf {
     return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(f16x8, n), __builtin_bit_cast(f16x8, m), c, 0, 0, 0);
   }
 };
-// Two 8-bit integers a unit: k counts pairs, and sums are exact up to 2^17 products.
+// Two 8-bit integers a unit: k counts pairs.  2^16 products of -128 and -128 are 2^30, which an accumulator holds;
+// 2^17 would be 2^31.
 struct OfInt8 {
   using Acc = i32x4;
   static __device__ __forceinline__ Acc mma(const bf16x8& n, const bf16x8& m, Acc c) {
