@@ -184,14 +184,14 @@ struct Product {
   int m, n, k;
   bool f32;
   bool chunked = false;
-  int pairs = 0;  // plane products of a step of k, 0: six of float32, one of bf16
 };
-// How a product is cut: tiles of `tile` squared, k in `splits` parts; tile 0: no cut is one launch.
+// How a product is cut: tiles of `tile` squared, k in `splits` parts.
 struct Plan {
   int tile, tiles_m, tiles_n, splits, k_per_split;
   double us;
 };
-Plan plan_product(const Product& p, bool may_split, int only_tile = 0);
+// In one part; tile 0: no cut is one launch.
+Plan plan_whole(const Product& p, int only_tile = 0);
 // One product and where its result goes.
 struct ProductJob {
   Product p;

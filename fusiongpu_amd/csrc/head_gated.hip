@@ -195,7 +195,7 @@ struct Choice {
 Choice choose(int m, int n, int k, bool f32) {
   const Product p{m, 2 * n, k, f32};
   Choice c;
-  c.plan = plan_product(p, false, f32 ? 256 : 0);  // smaller packed tiles of float32 are slower than those formed on the way
+  c.plan = plan_whole(p, f32 ? 256 : 0);  // smaller packed tiles of float32 are slower than those formed on the way
   double us = c.plan.tile ? c.plan.us : INFINITY;
   if (needs_pack(k, f32)) us += 5.7 + ((double)p.m + p.n) * k * (f32 ? 10 : 4) / 4e6;
   if (f32 && (int64_t)ceil_div(m, 64) * ceil_div(n, 32) * GatedTile64::threads < kLaunchThreads) {

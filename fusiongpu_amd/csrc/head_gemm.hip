@@ -237,7 +237,7 @@ Plan plan_at(const Product& p, int tile, int splits) {
   const double fixed = tile == 256 ? 8 : tile == 128 ? 4 : 3;
   const int most = tile == 256 ? 1 : tile == 128 ? 2 : p.f32 ? 3 : 5;
   const int64_t wgs = (int64_t)q.tiles_m * q.tiles_n * q.splits, full = wgs / (256 * most), rest = wgs % (256 * most);
-  const double k = (double)per * (p.pairs ? p.pairs : p.f32 ? 6 : 1);
+  const double k = (double)per * (p.f32 ? 6 : 1);
   q.us = full * (k * std::max(alone, most * shared) + fixed);
   if (rest) q.us += k * std::max(alone, ceil_div(rest, 256) * shared) + fixed;
   if (q.splits > 1) q.us += 3 + 8.0 * q.splits * p.m * ((p.n + 3) & ~3) / 6e6;
@@ -366,7 +366,7 @@ fgpu_status launch_join(const SplitJob& a, const SplitJob& b, const ColumnSum* s
   return FGPU_OK;
 }
 
-Plan plan_product(const Product& p, bool may_split, int only_tile) { return plan_of(p, only_tile, may_split); }
+Plan plan_whole(const Product& p, int only_tile) { return plan_of(p, only_tile, false); }
 
 size_t products_workspace_bytes(const Product* p, int count) {
   Plan q[2];

@@ -507,7 +507,7 @@ fgpu_status run_layer(const void* x, const float* x_scale, const int8_t* w, cons
   }
   // Operands in units of two integers.
   const Product p{(int)rows, out, ld / 2, false};
-  const Plan q = plan_product(p, false);
+  const Plan q = plan_whole(p);
   FGPU_CHECK(q.tile, FGPU_ERR_UNSUPPORTED, "8-bit linear: more tiles than one launch takes (2^39 results)");
   const GemmOperand a{(const uint16_t*)x, ld / 2, 0}, b{(const uint16_t*)w, ld / 2, 0};
   const Scales sc{x_scale, w_scale};

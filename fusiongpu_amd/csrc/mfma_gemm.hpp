@@ -329,24 +329,24 @@ struct TileLoad {
 
 // The same for the B operand of a gated product, k contiguous: of each 64 rows of the tile the first half are rows of B, the
 // second half the ones `up` elements further on that their products go with.  A wave's lanes fill rows of one half.
-template <int R, int NT, int BK = kGemmBK>
-struct GatedTileLoad : TileLoad<R, NT, true, true, BK> {
-  using Base = TileLoad<R, NT, true, true, BK>;
+template <int R, int NT>
+struct GatedTileLoad : TileLoad<R, NT, true, true> {
+  using Base = TileLoad<R, NT, true, true>;
   static constexpr int wave_rows = kWave * 16 / Base::row_bytes;
   __device__ void init(int64_t ld, int tid) {
     Base::init(ld, tid);
     this->voff -= (uint32_t)((int64_t)(tid / kWave * wave_rows) * ld * 2);  // from the wave's first row
   }
   __device__ __forceinline__ void issue(const GemmOperand& o, int64_t up, int plane, int r0, int nr, int k0, int nk,
-                                        lds_char* lds, int wave, bool live = true) const {
+                                        lds_char* lds, int wave) const {
     const uint16_t* base = o.p + plane * o.plane + (int64_t)r0 * o.ld + k0;
-    const int64_t last = (int64_t)(min(nr - r0, R / 2) - 1) * o.ld + min(((nk + 7) & ~7) - k0, BK);
+    const int64_t last = (int64_t)(min(nr - r0, R / 2) - 1) * o.ld + min(((nk + 7) & ~7) - k0, kGemmBK);
     const uint32_t off = this->kc >= nk - k0 ? 0x80000000u : this->voff;
 #pragma unroll
     for (int i = 0; i < Base::loads; ++i) {
       const int row = i * Base::rows_a_load + wave * wave_rows;  // of the tile, the wave's first
       auto rsrc = __builtin_amdgcn_make_buffer_rsrc(const_cast<uint16_t*>(base + (row & 32 ? up : 0)), 0,
-                                                    live ? (int)(last * 2) : 0, 0x00027000);
+                                                    (int)(last * 2), 0x00027000);
       const uint32_t at = (uint32_t)((row >> 6) * 32 + (row & 31)) * (uint32_t)(o.ld * 2);
       __builtin_amdgcn_raw_ptr_buffer_load_lds(rsrc, (lds_void*)(lds + i * (NT * 16) + wave * (kWave * 16)), 16, off + at, 0,
                                                0, 0);
@@ -437,9 +437,8 @@ struct GemmWave {
 };
 // acc[f][j]: a lane holds columns col(p) .. col(p) + 7 of row(j) in acc[2 p][j] and acc[2 p + 1][j].
 
-template <class T, bool BKC, int FORM, int BK = kGemmBK>
-using GemmLoadB = std::conditional_t<FORM == kGated, GatedTileLoad<T::BN, T::threads, BK>,
-                                     TileLoad<T::BN, T::threads, BKC, true, BK>>;
+template <class T, bool BKC, int FORM>
+using GemmLoadB = std::conditional_t<FORM == kGated, GatedTileLoad<T::BN, T::threads>, TileLoad<T::BN, T::threads, BKC, true>>;
 
 // One workgroup a tile.  Of a k step's 64, the fragments of one half are read while the other half's products run, so the
 // LDS's latency passes behind the matrix instructions; the step's only barrier lies between its halves, when every wave
@@ -467,14 +466,14 @@ constexpr int gemm_stage() {
 template <class T, int PAIRS, bool KC>
 constexpr int gemm_third() { return gemm_planes<T, PAIRS>() && KC && T::BM == 64 ? gemm_stage<T, PAIRS>() : 16; }
 
-template <class T, bool AKC, bool BKC, int PAIRS, class Num, int FORM, class Acc>
+template <class T, bool AKC, bool BKC, int PAIRS, class Num, class Acc>
 __device__ __forceinline__ void planes_products(const GemmArgs& g, Acc& acc, int m0, int n0, int kbeg, int kend, int wm, int wn,
                                                 char (&s0)[gemm_stage<T, PAIRS>()], char (&s1)[gemm_stage<T, PAIRS>()],
                                                 char (&s2)[gemm_third<T, PAIRS, AKC && BKC>()]) {
   constexpr int P = planes_of(PAIRS);
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   TileLoad<T::BM, T::threads, AKC, false, kPlanesBK> la;
-  GemmLoadB<T, BKC, FORM, kPlanesBK> lb;
+  TileLoad<T::BN, T::threads, BKC, true, kPlanesBK> lb;
   la.init(g.a.ld, tid);
   lb.init(g.b.ld, tid);
   TileRead<T::BM, AKC, false, kPlanesBK> ra;
@@ -492,8 +491,7 @@ __device__ __forceinline__ void planes_products(const GemmArgs& g, Acc& acc, int
 #pragma unroll
     for (int p = 0; p < P; ++p) {
       la.issue(g.a, p, m0, g.m, k, g.k, (lds_char*)s + p * pa, wave, live);
-      if constexpr (FORM == kGated) lb.issue(g.b, g.up, p, n0, g.n, k, g.k, (lds_char*)s + P * pa + p * pb, wave, live);
-      else lb.issue(g.b, p, n0, g.n, k, g.k, (lds_char*)s + P * pa + p * pb, wave, live);
+      lb.issue(g.b, p, n0, g.n, k, g.k, (lds_char*)s + P * pa + p * pb, wave, live);
     }
   };
   auto work = [&](char* s) {
@@ -569,8 +567,9 @@ __device__ __forceinline__ void gemm_tile(const GemmArgs& g, const Epi& epi, int
     for (int j = 0; j < T::FM; ++j) acc[i][j] = typename Num::Acc{0, 0, 0, 0};
   typename Epi::template Side<T> side;
   if constexpr (gemm_planes<T, PAIRS>()) {
+    static_assert(FORM != kGated, "both factors' columns: through GemmLoadB");
     side.fetch(epi, m0, n0, tid);
-    planes_products<T, AKC, BKC, PAIRS, Num, FORM>(g, acc, m0, n0, kbeg, kend, wm, wn, s0, s1, s2);
+    planes_products<T, AKC, BKC, PAIRS, Num>(g, acc, m0, n0, kbeg, kend, wm, wn, s0, s1, s2);
   } else {
     const int steps = max(0, (kend - kbeg + kGemmBK - 1) / kGemmBK) * PAIRS;
 
