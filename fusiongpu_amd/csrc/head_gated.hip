@@ -5,10 +5,11 @@
 // columns and act(g) u is formed before anything is stored.  The gradients are those of one linear layer of 2 hidden columns
 // once dz = [dh u act'(g) | dh act(g)] is there, which a launch of its own forms with its column sums (head_prep.hip).
 //
-// 65536 x 1024 -> 4096 in bfloat16 with both factors kept takes 1.07 ms (1.03 PFLOP/s): 0.79 of matrix instructions, then an
-// epilogue of 1.6 GB of stores a tile that nothing overlaps, as a 256 x 256 tile fills its CU (two workgroups of 128 x 128 a
-// CU 1.15 ms, of 256 x 128 with k in steps of 32 through three buffers 1.17 to 1.23, starts set apart no gain).  Its
-// gradients over 16384 rows 0.57 ms: dz 0.12 (670 MB, 5.6 TB/s), two products at 1.2 PFLOP/s.  One row 4.8 us, a launch and
+// 65536 x 1024 -> 4096 in bfloat16 with both factors kept takes 1.06 to 1.10 ms (1.0 PFLOP/s), the matrix units busy 46 % of
+// its cycles: sixteen steps of k, then an epilogue with its part of 1.6 GB of stores that nothing overlaps, as a 256 x 256 tile
+// fills its CU (two workgroups of 128 x 128 a CU 1.15 ms, of 256 x 128 with k in steps of 32 through three buffers 1.17 to
+// 1.23, starts set apart no gain).  Its gradients over 16384 rows 0.57 to 0.59 ms: dz 0.13 (670 MB, 5.0 TB/s), two products at
+// 1.2 PFLOP/s (the matrix units busy 55 %).  One row 4.8 us, a launch and
 // two rounds of loads (eight columns of each half a workgroup, so that 2048 hidden ones are a workgroup a CU).
 #include <algorithm>
 #include <cmath>
@@ -25,7 +26,7 @@ constexpr int kMaxHidden = FGPU_HEAD_MAX_DIM / 2;
 // Mid-size float32 layers: a launch that copies both operands into planes first costs as much as a third of the product,
 // and what it wrote comes back through other XCDs' caches.  Here a thread loads eight values of a row as they lie (any
 // alignment), two steps ahead, splits them in registers and writes the three planes; each value is split once a tile
-// instead of once.  1000 x 385 -> 771: 16.5 us, thirteen steps of 0.95 us: LDS, conversions and matrix instructions of a
+// instead of once.  1000 x 385 -> 771: 17.0 us, thirteen steps of 0.95 us: LDS, conversions and matrix instructions of a
 // step take 0.5, 0.3 and 0.3 and overlap little behind its one barrier.
 struct SplitJob32 {
   const float* x;

@@ -10,9 +10,10 @@
 // two steps, took 8192 x 1024 from 550 to 370 us and put results up to 9e-3 of their norm off at five steps and 1.8e-2 at eight
 // (updates of few rows that are not zero; sparse ones 5e-3, of low rank 2e-3), where two planes leave at most 6e-5.
 //
-// 8192 x 1024, five steps, takes 0.55 ms in either type; traced, A 40 us a step as thirteen parts of its triangle (strided
-// operands) and 8 to join them, P 16, X' 62 (three products, 0.83 PFLOP/s of them), norm and start 19.  128 x 771 in float32
-// 66 us: twelve launches, a step's two 6 each: A (k over sixteen waves; in parts 8.3), then P and X'.
+// 8192 x 1024, five steps, takes 0.55 to 0.57 ms in either type; traced, A 36 to 41 us a step as thirteen parts of its triangle
+// (strided operands, the matrix units busy 30 %) and 8 to join them, P 16, X' 57 to 65 (three products, 0.8 to 0.9 PFLOP/s of
+// them, the matrix units busy 38 %), norm and start 19.  128 x 771 in float32 65 us: twelve launches, a step's two 6 each: A (k
+// over sixteen waves; in parts 8.3), then P and X'.
 #include <algorithm>
 #include <cmath>
 

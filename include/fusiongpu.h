@@ -684,7 +684,8 @@ fgpu_status fgpu_quantize_rows(const void* d_x, int64_t rows, int dim, int dtype
  * d_w_scale [out_dim].  x is of `dtype` (d_x_scale NULL) and rounded row by row
  * as above inside the call, or held so already: [rows][FGPU_INT8_ROW(in_dim)]
  * with d_x_scale [rows] (behind the values, x's or w's bytes are zeros).  z =
- * x_scale w_scale sum q_x q_w + bias, the sum exact in 32 bits; bias, residual
+ * ((sum q_x q_w) w_scale) x_scale + bias, the sum exact in 32 bits and what follows
+ * in float32, in that order; bias, residual
  * and y are of `dtype`.  A row's result is the same to the bit in any batch, and
  * whether the call rounds x or gets it rounded.  d_residual may be d_y itself. */
 size_t fgpu_linear_int8_workspace_bytes(int64_t rows, int in_dim, int out_dim, int dtype, int quantized_x);
