@@ -233,10 +233,9 @@ __host__ __device__ inline int64_t whole8(int64_t cols) { return (cols + 7) / 8 
 // 297, 8192 x 200 x 1030 218 -> 190, but 65536 x 72 x 100 119 -> 145; of a linear one 65536 x 385 x 771 1086 -> 851).  Rows of
 // 130 to 180, padded by up to half, still gain (float32: 65536 x 130 -> 256 70 -> 64, 8192 x 180 -> 1024 39 -> 35, gradients 77
 // -> 75 and 78 -> 76, a loss's over 30000 x 130 to 180 630 to 650 -> 580) but for gradients of very many rows and few columns
-// (65536 x 130 -> 130 137 -> 152, -> 256 165 -> 170).  Rows a
-// multiple of 4 KB apart fall on the same memory channels: 128 bytes more between them (the score gradient of 8192 x 65536
-// with its two products at 768 dims 2.73 -> 2.52 ms; float32 4096 x 2048 x 2048 forward 295 -> 279 us; 16384 x 1024 x 4096
-// bf16 backward 343 -> 343).
+// (65536 x 130 -> 130 137 -> 152, -> 256 165 -> 170).  Rows a multiple of 4 KB apart fall on the same memory channels:
+// 128 bytes more between them (the score gradient of 8192 x 65536 with its two products at 768 dims 2.73 -> 2.52 ms; float32
+// 4096 x 2048 x 2048 forward 295 -> 279 us; 16384 x 1024 x 4096 bf16 backward 343 -> 343).
 inline int64_t packed_ld(int64_t cols) {
   const int64_t ld = cols > 128 ? (cols + 63) / 64 * 64 : whole8(cols);
   return ld % 2048 ? ld : ld + 64;

@@ -9,8 +9,8 @@
 // its cycles: sixteen steps of k, then an epilogue with its part of 1.6 GB of stores that nothing overlaps, as a 256 x 256 tile
 // fills its CU (two workgroups of 128 x 128 a CU 1.15 ms, of 256 x 128 with k in steps of 32 through three buffers 1.17 to
 // 1.23, starts set apart no gain).  Its gradients over 16384 rows 0.57 to 0.59 ms: dz 0.13 (670 MB, 5.0 TB/s), two products at
-// 1.2 PFLOP/s (the matrix units busy 55 %).  One row 4.8 us, a launch and
-// two rounds of loads (eight columns of each half a workgroup, so that 2048 hidden ones are a workgroup a CU).
+// 1.2 PFLOP/s (the matrix units busy 55 %).  One row 4.8 us, a launch and two rounds of loads (eight columns of each half a
+// workgroup, so that 2048 hidden ones are a workgroup a CU).
 #include <algorithm>
 #include <cmath>
 

@@ -6,7 +6,8 @@
 // Rounding is bound by HBM: 100003 x 1024 in bfloat16 67 us (307 MB, 4.6 TB/s).  The gated layer on 65536 x 1024 -> 4096
 // takes 0.62 to 0.65 ms, 0.05 of them rounding (the product 1.9 POP/s, the matrix units busy 39 % of its cycles; the library's
 // plain product of 8192^3 2.4): eight steps of 128 k a tile, then an epilogue of two conversions, four products, an exponential
-// and a reciprocal an element that nothing overlaps.  One row x 1024 -> 4096: 5.2 us, a launch, the row's maximum and a round of loads.
+// and a reciprocal an element that nothing overlaps.  One row x 1024 -> 4096: 5.2 us, a launch, the row's
+// maximum and a round of loads.
 #include <algorithm>
 
 #include "gated.hpp"

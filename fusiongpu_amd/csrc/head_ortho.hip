@@ -397,7 +397,8 @@ __global__ __launch_bounds__(kBothWaves * kWave) void both_kernel(Planes a, Orth
 #pragma unroll
       for (int i = 0; i < 2; ++i)
 #pragma unroll
-        for (int q = 0; q < kPairs; ++q) acc[i] = OfHalf::mma(rb[h].r[pair_b<kPairs>(q)][i], ra[h].r[pair_a<kPairs>(q)][0], acc[i]);
+        for (int q = 0; q < kPairs; ++q)
+          acc[i] = OfHalf::mma(rb[h].r[pair_b<kPairs>(q)][i], ra[h].r[pair_a<kPairs>(q)][0], acc[i]);
     const int row = p0 + r + l, col = c0 + 8 * (lane >> 4);
     f32x8 v{{0, 0, 0, 0}, {0, 0, 0, 0}};
     if (row < n && col < n8) v = fp.value(f32x8{acc[0], acc[1]}, row, col, true);

@@ -37,7 +37,8 @@ def one_a_row(m, k, seed):
     return x, at
 
 
-FORWARD = [(70, 200, 100), (300, 77, 260), (1500, 200, 999), (960, 643, 577), (5000, 600, 2050), (4555, 291, 1556), (4000, 1024, 2048)]
+FORWARD = [(70, 200, 100), (300, 77, 260), (1500, 200, 999), (960, 643, 577), (5000, 600, 2050), (4555, 291, 1556),
+           (4000, 1024, 2048)]
 
 
 @pytest.mark.parametrize("m,k,n", FORWARD)

@@ -1,5 +1,5 @@
-"""Which kernels the orthogonalisation's products take, on the CPU: the sizes that are tested against 64 bits take all of them, and
-the bound of those tests would show a lost plane."""
+"""Which kernels the orthogonalisation's products take, on the CPU: the sizes that are tested against 64 bits take all of them,
+and the bound of those tests would show a lost plane."""
 import pytest
 
 torch = pytest.importorskip("torch")
